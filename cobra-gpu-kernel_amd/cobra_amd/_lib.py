@@ -15,11 +15,14 @@ from typing import Optional
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcobra_amd.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 F16 = 0
 F32 = 1
 BF16 = 2
+# Codes of the key/value cache (COBRA_CACHE_* in include/cobra_amd.h).
+CACHE_E4M3 = 0
+CACHE_I8 = 1
 PLAN_FUSED = 0
 PLAN_STAGED = 1
 PLAN_PADDED = 2
@@ -59,6 +62,21 @@ SIGNATURES = {
     ),
     "cobra_mask_bits": (_c_int, [_vp, _vp, _c_i64, _c_i64, _vp]),
     "cobra_attn_fwd": (_c_int, [_vp, _vp, _c_int, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _vp]),
+    "cobra_cache_width": (_c_int, [_c_i64]),
+    "cobra_cache_reserve": (
+        _c_int, [_vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp],
+    ),
+    "cobra_cache_trim": (_c_int, [_vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "cobra_cache_append": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp],
+    ),
+    "cobra_cache_attn_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "cobra_cache_attn_fwd": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _vp],
+    ),
     "cobra_qkv_attn_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "cobra_qkv_attn_fwd": (
         _c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _vp],

@@ -54,6 +54,7 @@ FILE_FLAGS = {
     "layer_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=8",
                         "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "cache_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -445,6 +445,246 @@ def attn(
     return out
 
 
+_CACHE = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_I8}
+CACHE_BLOCKS = (16, 32, 64, 128)
+
+
+def cache_width(head_dim: int) -> int:
+    """Columns of a cached key or value row: head_dim (a multiple of 8, at most 256) rounded up
+    to 32, 64, 96, 128, 192 or 256."""
+    w = _lib.lib().cobra_cache_width(head_dim)
+    if w < 0:
+        raise ValueError(f"the cache takes head_dim in multiples of 8 up to 256, got {head_dim}")
+    return w
+
+
+def _same_dev(dev: torch.device, **tensors: torch.Tensor) -> None:
+    for what, t in tensors.items():
+        _dev(t, what)
+        if t.device != dev:
+            raise ValueError(f"{what} is on {t.device}, expected {dev}")
+
+
+def _i32(t: torch.Tensor, shape, what: str) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{what} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _block_size(n: int) -> int:
+    if n not in CACHE_BLOCKS:
+        raise ValueError(f"block_size must be one of {CACHE_BLOCKS}, got {n}")
+    return int(n)
+
+
+def _call_on(dev: torch.device, fn: str, *args) -> None:
+    """``call`` with ``dev`` as the current device and its current stream as the last argument."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            call(fn, *args, raw_stream(dev.index))
+    else:
+        call(fn, *args, raw_stream(dev.index))
+
+
+def _tables(lens, block_table, free_list, free_count):
+    if lens.dim() != 1 or block_table.dim() != 2 or free_list.dim() != 1:
+        raise ValueError("lens and free_list must have one dimension, block_table two")
+    B = lens.shape[0]
+    _i32(lens, (B,), "lens")
+    _i32(block_table, (B, block_table.shape[1]), "block_table")
+    _i32(free_list, (free_list.shape[0],), "free_list")
+    _i32(free_count, (1,), "free_count")
+    return B
+
+
+def cache_reserve(
+    lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    free_list: torch.Tensor,
+    free_count: torch.Tensor,
+    block_size: int,
+    tokens: int,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Room in a block pool for ``new_lens[b]`` more tokens of each request -> ``(slots, cu, missing)``.
+
+    ``lens`` [B], ``block_table`` [B, W] and ``free_count`` [1] (the height of the stack
+    ``free_list``) are updated in place; all are int32 device tensors.  ``slots`` [tokens] int64
+    is the slot of each new token, requests one after the other (-1 past the last), ``cu``
+    [B + 1] where each request's begin.  ``missing`` [1] is 0; or the number of blocks the pool
+    lacks, or -1 for lengths that do not fit (``cobra_cache_reserve``), and then nothing was
+    reserved, every slot is -1 and ``cu`` 0.  Nothing here waits for the GPU.
+    """
+    B = _tables(lens, block_table, free_list, free_count)
+    _i32(new_lens, (B,), "new_lens")
+    dev = lens.device
+    _same_dev(dev, lens=lens, new_lens=new_lens, block_table=block_table, free_list=free_list, free_count=free_count)
+    bs = _block_size(block_size)
+    tokens = int(tokens)
+    if not 0 <= tokens <= 0x7FFFFFFF:
+        raise ValueError(f"tokens must be 0 .. 2^31 - 1, got {tokens}")
+    if B == 0:
+        return (torch.full((tokens,), -1, dtype=torch.int64, device=dev),
+                torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev))
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
+    rest = torch.empty(B + 2, dtype=torch.int32, device=dev)  # missing, workspace
+    at = rest.data_ptr()
+    _call_on(dev, "cobra_cache_reserve", lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+             block_table.shape[1], free_list.data_ptr(), free_list.shape[0], free_count.data_ptr(), slots.data_ptr(),
+             tokens, cu.data_ptr(), at, at + 4, B, bs)
+    return slots, cu, rest[:1]
+
+
+def cache_trim(
+    lens: torch.Tensor,
+    keep_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    free_list: torch.Tensor,
+    free_count: torch.Tensor,
+    block_size: int,
+) -> torch.Tensor:
+    """Requests cut to ``min(lens, max(keep_lens, 0))`` tokens, the blocks past that back on the
+    stack of free ones -> ``refused`` [1] int32.
+
+    For rejected drafts, and with 0 for requests that are over.  Undoes a ``cache_reserve``
+    when ``keep_lens`` are the lengths before it.  ``lens``, ``free_list`` and ``free_count``
+    are updated in place; ``refused`` is 1, and nothing changed, where they do not fit
+    (``cobra_cache_trim``).
+    """
+    B = _tables(lens, block_table, free_list, free_count)
+    _i32(keep_lens, (B,), "keep_lens")
+    dev = lens.device
+    _same_dev(dev, lens=lens, keep_lens=keep_lens, block_table=block_table, free_list=free_list,
+              free_count=free_count)
+    bs = _block_size(block_size)
+    if B == 0:
+        return torch.zeros(1, dtype=torch.int32, device=dev)
+    rest = torch.empty(B + 1, dtype=torch.int32, device=dev)  # refused, workspace
+    at = rest.data_ptr()
+    _call_on(dev, "cobra_cache_trim", lens.data_ptr(), keep_lens.data_ptr(), block_table.data_ptr(),
+             block_table.shape[1], free_list.data_ptr(), free_list.shape[0], free_count.data_ptr(), at, at + 4, B, bs)
+    return rest[:1]
+
+
+def _cache_geometry(k, v, k_scale, v_scale, heads, head_dim):
+    """(cache code, num_blocks, kv_heads, block_size) of a layer's cache tensors."""
+    if k.dtype not in _CACHE or v.dtype != k.dtype:
+        raise TypeError(f"k and v must be both float8_e4m3fn or both int8, got {k.dtype} and {v.dtype}")
+    if k.dim() != 4:
+        raise ValueError("k must be [num_blocks, kv_heads, block_size, width]")
+    nb, kvh, bs, w = k.shape
+    _block_size(bs)
+    if w != cache_width(head_dim):
+        raise ValueError(f"head_dim {head_dim} is cached in rows of {cache_width(head_dim)}, got {w}")
+    if tuple(v.shape) != (nb, kvh, w, bs):
+        raise ValueError(f"v must be [{nb}, {kvh}, {w}, {bs}], got {list(v.shape)}")
+    if heads <= 0 or kvh <= 0 or heads % kvh:
+        raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kvh})")
+    for what, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s.dtype != torch.float32 or tuple(s.shape) != (nb, kvh):
+            raise ValueError(f"{what} must be float32 [{nb}, {kvh}]")
+    return _CACHE[k.dtype], nb, kvh, bs
+
+
+def cache_append(
+    qkv: torch.Tensor,
+    slots: torch.Tensor,
+    heads: int,
+    head_dim: int,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+) -> None:
+    """New keys and values, quantised to 8 bits, into their slots of a layer's cache (in place).
+
+    ``qkv`` [T, (heads + 2 kv_heads) * head_dim] fp16 or bf16, packed q | k | v as for ``attn``
+    (with fewer k and v heads where they are shared); ``slots`` [T] int64 from
+    ``cache_reserve``, negative ones are passed over.  ``k`` [num_blocks, kv_heads, block_size,
+    width], ``v`` [num_blocks, kv_heads, width, block_size] (float8_e4m3fn or int8, width =
+    ``cache_width(head_dim)``), ``k_scale`` and ``v_scale`` [num_blocks, kv_heads] fp32.  Each
+    block and head has one scale, a power of two; a token too large for it makes the scale grow
+    and the block's earlier codes are rounded again.  NaN is stored as 0, an infinity as the
+    largest code.
+    """
+    cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
+    if qkv.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
+    T = slots.shape[0] if slots.dim() == 1 else -1
+    if slots.dtype != torch.int64 or tuple(qkv.shape) != (T, (heads + 2 * kvh) * head_dim):
+        raise ValueError(f"slots must be int64 [T] and qkv [T, {(heads + 2 * kvh) * head_dim}], got {slots.dtype} "
+                         f"{list(slots.shape)} and {list(qkv.shape)}")
+    dev = qkv.device
+    _same_dev(dev, qkv=qkv, slots=slots, k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+    _call_on(dev, "cobra_cache_append", qkv.data_ptr(), _DT[qkv.dtype], qkv.shape[1], slots.data_ptr(), k.data_ptr(),
+             v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cache, T, nb, bs, heads, kvh, head_dim)
+
+
+def cache_attn(
+    q: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    block_table: torch.Tensor,
+    heads: int,
+    head_dim: int,
+    scale: float,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    causal: bool = True,
+    max_new: Optional[int] = None,
+    max_len: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of new tokens over an 8-bit cache that already holds them -> ``ctx [T, heads * head_dim]``.
+
+    ``q`` [T, C] fp16 or bf16 with the queries in its first heads * head_dim columns (the packed
+    ``qkv`` of ``cache_append`` will do; C a multiple of 8); request b's new tokens are rows
+    ``cu[b] .. cu[b + 1]``, it holds ``lens[b]`` tokens, these included, in the blocks that
+    ``block_table[b]`` lists.  Query head j reads kv head ``j // (heads // kv_heads)``.  With
+    ``causal`` a token sees the keys up to itself, else all of its request; a token that sees
+    none gets a zero row.  Rows past ``cu[B]`` are left as they are (unset without ``out``).
+    ``max_new`` and ``max_len``, the most new tokens and keys of a request (defaults: what T and
+    the table allow), shape the launch, not the result.
+    """
+    cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if q.dim() != 2 or q.shape[1] < heads * head_dim or q.shape[1] % 8:
+        raise ValueError(f"q must be [T, >= {heads * head_dim}] with a multiple of 8 columns, got {list(q.shape)}")
+    if lens.dim() != 1 or block_table.dim() != 2:
+        raise ValueError("lens must have one dimension, block_table two")
+    T, B = q.shape[0], lens.shape[0]
+    _i32(lens, (B,), "lens")
+    _i32(cu, (B + 1,), "cu")
+    _i32(block_table, (B, block_table.shape[1]), "block_table")
+    if scale <= 0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    dev = q.device
+    _same_dev(dev, q=q, cu=cu, lens=lens, block_table=block_table, k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+    W = block_table.shape[1]
+    if out is None:
+        out = torch.empty((T, heads * head_dim), device=dev, dtype=q.dtype)
+    else:
+        _same_dev(dev, out=out)
+        if out.dtype != q.dtype or tuple(out.shape) != (T, heads * head_dim):
+            raise ValueError(f"out must be {q.dtype} [{T}, {heads * head_dim}]")
+    if T == 0 or B == 0:
+        return out
+    if W == 0 or nb == 0:
+        raise ValueError("block_table and the cache must hold at least one block")
+    new = max(1, T - B + 1) if max_new is None else max(1, int(max_new))
+    keys = W * bs if max_len is None else max(1, int(max_len))
+    need = _lib.lib().cobra_cache_attn_workspace_bytes(T, B, heads, kvh, head_dim, new, keys)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _call_on(dev, "cobra_cache_attn_fwd", q.data_ptr(), _DT[q.dtype], q.shape[1], cu.data_ptr(), lens.data_ptr(),
+             block_table.data_ptr(), W, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cache,
+             out.data_ptr(), _ptr(ws), max(0, need), T, B, nb, bs, heads, kvh, head_dim, new, keys, float(scale),
+             1 if causal else 0)
+    return out
+
+
 def qkv_attn(
     h: torch.Tensor,
     w_qkv: torch.Tensor,

@@ -1,0 +1,467 @@
+// Block tables, slot maps and the write of new keys and values for a cache held in 8 bits.
+//
+// A layer's cache is a pool of blocks of bs tokens (bs = 16, 32, 64 or 128):
+//   k [num_blocks, kv_heads, bs, hdp],  v [num_blocks, kv_heads, hdp, bs]   codes, 1 byte
+//   k_scale, v_scale [num_blocks, kv_heads]                                 fp32
+// with hdp = cache_width(head_dim) and the columns past head_dim zero.  V is kept with its
+// tokens innermost: the attention's P.V product wants consecutive keys of one dimension in a
+// lane, and reads them from memory as they lie.  A code c stands for c * scale.  Scales are
+// powers of two, so that dividing by one is exact: a code depends on the value and the scale's
+// exponent alone, never on how a quotient was rounded, and a block whose scale grows loses
+// only the bits that no longer fit (e4m3: none above its subnormals).
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace cobra {
+
+namespace {
+
+constexpr int kThreads = 1024;  // the table kernels run one workgroup
+constexpr int kWaves = kThreads / 64;
+
+__device__ __forceinline__ int64_t wave_incl(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Inclusive prefix sum over the workgroup; `total` gets the sum.  red: kWaves words of LDS.
+__device__ __forceinline__ int64_t block_incl(int64_t v, int64_t* red, int64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_incl(v, lane);
+  __syncthreads();  // red may still be read from the call before
+  if (lane == 63) red[wave] = v;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += red[w];
+    all += red[w];
+  }
+  *total = all;
+  return v + before;
+}
+
+__device__ __forceinline__ int64_t blocks_of(int64_t tokens, int shift) {
+  return (tokens + (int64_t(1) << shift) - 1) >> shift;
+}
+
+// The first i in [0, n) with v[i] > x (v does not decrease, v[n - 1] > x).
+__device__ __forceinline__ int first_above(const int32_t* v, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] > x)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+// The slots of tokens t0, t0 + step, .. and the table entries k0, k0 + step, .. of a reserve
+// whose lengths and prefix sums are final: incl[b] = new blocks of requests 0 .. b, count =
+// the free blocks before it.
+__device__ __forceinline__ void reserve_fill(const CacheReserveArgs& a, const int32_t* cu, const int32_t* incl,
+                                             int count, int64_t first, int64_t step) {
+  const int used = cu[a.batch], blocks = incl[a.batch - 1];
+  for (int64_t t = first; t < a.tokens; t += step) {
+    if (t >= used) {
+      a.slots[t] = -1;
+      continue;
+    }
+    const int b = first_above(cu + 1, a.batch, (int)t);
+    const int begin = cu[b];
+    const int64_t held = (int64_t)a.lens[b] - (cu[b + 1] - begin);
+    const int64_t pos = held + (t - begin), had = blocks_of(held, a.shift), page = pos >> a.shift;
+    const int before = b ? incl[b - 1] : 0;
+    const int32_t id = page < had ? a.table[b * a.width + page] : a.free_list[count - 1 - (before + (int)(page - had))];
+    a.slots[t] = ((int64_t)id << a.shift) + (pos & ((1 << a.shift) - 1));
+  }
+  for (int64_t k = first; k < blocks; k += step) {
+    const int b = first_above(incl, a.batch, (int)k);
+    const int64_t held = (int64_t)a.lens[b] - (cu[b + 1] - cu[b]);
+    const int before = b ? incl[b - 1] : 0;
+    a.table[b * a.width + blocks_of(held, a.shift) + (k - before)] = a.free_list[count - 1 - k];
+  }
+}
+
+// need_b = ceil((L + n) / bs) - ceil(L / bs) blocks for request b, handed out from the top of
+// the stack of free blocks in the order of requests; all requests get theirs or none does.
+// One workgroup: the sums are over a few hundred requests, and one barrier is cheaper than a
+// second launch.  It also writes slots and table entries where `fill` says so.
+__global__ __launch_bounds__(kThreads) void cache_reserve_kernel(CacheReserveArgs a, int fill) {
+  __shared__ int64_t red[kWaves];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  const int count = *a.free_count;
+  int64_t toks = 0, need_all = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int64_t n = 0, need = 0;
+    if (b < a.batch) {
+      const int64_t len = a.lens[b];
+      n = a.new_lens[b];
+      if (len < 0 || n < 0 || len + n > 0x7fffffff || blocks_of(len + n, a.shift) > a.width) {
+        bad = 1;
+        n = 0;
+      } else {
+        need = blocks_of(len + n, a.shift) - blocks_of(len, a.shift);
+      }
+    }
+    int64_t ts, ns;
+    const int64_t ti = block_incl(n, red, &ts) + toks, ni = block_incl(need, red, &ns) + need_all;
+    if (b < a.batch) {
+      a.cu[b + 1] = (int32_t)ti;
+      a.incl[b] = (int32_t)ni;
+    }
+    toks += ts;
+    need_all += ns;
+  }
+  if (tid == 0) a.cu[0] = 0;
+  __syncthreads();
+  int missing = 0;
+  if (bad || toks > a.tokens || count < 0 || count > a.num_free)
+    missing = -1;
+  else if (need_all > count)
+    missing = (int)(need_all - count);
+  if (missing) {
+    for (int b = tid; b < a.batch; b += kThreads) {
+      a.cu[b + 1] = 0;
+      a.incl[b] = 0;
+    }
+  } else {
+    for (int b = tid; b < a.batch; b += kThreads) a.lens[b] += a.new_lens[b];
+  }
+  if (tid == 0) {
+    *a.missing = missing;
+    a.incl[a.batch] = count;  // for the fill
+    if (!missing) *a.free_count = count - (int)need_all;
+  }
+  if (fill) {
+    __syncthreads();
+    reserve_fill(a, a.cu, a.incl, count, tid, kThreads);
+  }
+}
+
+__global__ __launch_bounds__(256) void cache_reserve_fill_kernel(CacheReserveArgs a) {
+  reserve_fill(a, a.cu, a.incl, a.incl[a.batch], (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
+// Requests cut to min(L, max(keep, 0)) tokens; the k-th block given back (requests in order,
+// a request's blocks in order) goes k places below the new top of the stack, which undoes a
+// reserve exactly.
+__global__ __launch_bounds__(kThreads) void cache_trim_kernel(CacheTrimArgs a) {
+  __shared__ int64_t red[kWaves];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  const int count = *a.free_count;
+  int64_t all = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int64_t back = 0;
+    if (b < a.batch) {
+      const int64_t len = a.lens[b];
+      const int64_t keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
+      if (len < 0 || blocks_of(len, a.shift) > a.width)
+        bad = 1;
+      else if (keep < len)
+        back = blocks_of(len, a.shift) - blocks_of(keep, a.shift);
+    }
+    int64_t s;
+    const int64_t i = block_incl(back, red, &s) + all;
+    if (b < a.batch) a.incl[b] = (int32_t)(i > 0x7fffffff ? 0x7fffffff : i);
+    all += s;
+  }
+  __syncthreads();
+  const bool refused = bad || count < 0 || all + count > a.num_free;
+  if (tid == 0) *a.refused = refused ? 1 : 0;
+  if (refused) return;
+  for (int64_t k = tid; k < all; k += kThreads) {
+    const int b = first_above(a.incl, a.batch, (int)k);
+    const int64_t keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
+    const int before = b ? a.incl[b - 1] : 0;
+    a.free_list[count + all - 1 - k] = a.table[b * a.width + blocks_of(keep, a.shift) + (k - before)];
+  }
+  __syncthreads();
+  for (int b = tid; b < a.batch; b += kThreads) {
+    const int keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
+    if (keep < a.lens[b]) a.lens[b] = keep;
+  }
+  if (tid == 0) *a.free_count = count + (int)all;
+}
+
+// -- append ---------------------------------------------------------------------------
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxBlock = 128;
+constexpr int kScaleMin = -40, kScaleMax = 40;  // exponents of the scales
+
+// The scale's exponent: the least e in range with amax <= qmax 2^e (the range holds what fp16
+// activations can reach with room to spare; beyond it values saturate or round to zero).
+template <int CACHE>
+__device__ __forceinline__ int scale_exponent(float amax) {
+  if (!(amax > 0.f)) return kScaleMin;
+  // amax = m 2^x with 1 <= m < 2; qmax = 1.75 2^8 (e4m3) or 1.984375 2^6 (int8)
+  int x;
+  const float m = 2.f * frexpf(amax, &x);
+  --x;
+  int e = CACHE == kCacheE4M3 ? x - 8 + (m > 1.75f ? 1 : 0) : x - 6 + (m > 1.984375f ? 1 : 0);
+  e = e < kScaleMin ? kScaleMin : e;
+  return e > kScaleMax ? kScaleMax : e;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Nearest codes (ties to even) of two values, clamped to the code's range; NaN becomes 0 so
+// that the cache holds finite values only.
+template <int CACHE>
+__device__ __forceinline__ uint32_t quant2(float x, float y) {
+  constexpr float qmax = CACHE == kCacheE4M3 ? 448.f : 127.f;
+  x = x == x ? fminf(fmaxf(x, -qmax), qmax) : 0.f;
+  y = y == y ? fminf(fmaxf(y, -qmax), qmax) : 0.f;
+  if constexpr (CACHE == kCacheE4M3) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false) & 0xffffu;
+  } else {
+    const int i = (int)rintf(x), j = (int)rintf(y);
+    return ((uint32_t)i & 0xffu) | (((uint32_t)j & 0xffu) << 8);
+  }
+}
+
+template <int CACHE>
+__device__ __forceinline__ uint32_t quant1(float x) {
+  return quant2<CACHE>(x, 0.f) & 0xffu;
+}
+
+// The value of code i (0 .. 3) of a word.
+template <int CACHE, int I>
+__device__ __forceinline__ float code_value(uint32_t w) {
+  if constexpr (CACHE == kCacheE4M3)
+    return __builtin_amdgcn_cvt_f32_fp8(w, I);
+  else
+    return (float)(int8_t)(w >> (8 * I));
+}
+
+// The codes of a word under a scale grown by 1 / ratio.
+template <int CACHE>
+__device__ __forceinline__ uint32_t regrade(uint32_t w, float ratio) {
+  const uint32_t lo = quant2<CACHE>(code_value<CACHE, 0>(w) * ratio, code_value<CACHE, 1>(w) * ratio);
+  const uint32_t hi = quant2<CACHE>(code_value<CACHE, 2>(w) * ratio, code_value<CACHE, 3>(w) * ratio);
+  return lo | (hi << 16);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float y = fabsf(x);
+  return y < __builtin_huge_valf() ? y : 0.f;  // NaN compares false
+}
+
+__device__ __forceinline__ float block_max(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float m = red[0];
+#pragma unroll
+  for (int w = 1; w < kAppendThreads / 64; ++w) m = fmaxf(m, red[w]);
+  __syncthreads();
+  return m;
+}
+
+// One workgroup writes what a call brings to one (block, head).  It belongs to the block's
+// first token in the call (tokens of a block stand next to each other in the call); the others
+// pass.  A workgroup looks at `window` tokens for first ones.  Where a run writes offset 0 the
+// block starts anew: its scales come from this call's tokens alone.
+template <typename T, int CACHE>
+__global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs a, int window) {
+  __shared__ int src[kMaxBlock];  // token of each offset of the block, -1: none
+  __shared__ float red[kAppendThreads / 64];
+  __shared__ int stop, lowest, highest;
+  const int tid = threadIdx.x, head = blockIdx.y;
+  const int bs = 1 << a.shift, hd = a.head_dim, hdp = a.width;
+  const int64_t slots_end = a.num_blocks << a.shift;
+  const int64_t t_end = min((int64_t)(blockIdx.x + 1) * window, a.tokens);
+  for (int64_t t0 = (int64_t)blockIdx.x * window; t0 < t_end; ++t0) {
+    const int64_t slot = a.slots[t0];
+    if (slot < 0 || slot >= slots_end) continue;
+    const int64_t blk = slot >> a.shift;
+    if (t0 > 0 && (a.slots[t0 - 1] >> a.shift) == blk) continue;
+    // The run of tokens that go to this block; of two for one slot the later one stays.
+    __syncthreads();
+    if (tid < bs) src[tid] = -1;
+    if (tid == 0) {
+      lowest = bs;
+      highest = -1;
+    }
+    for (int64_t c = t0;; c += kAppendThreads) {
+      __syncthreads();
+      if (tid == 0) stop = kAppendThreads;
+      __syncthreads();
+      const int64_t t = c + tid;
+      int64_t s = -1;
+      if (t < a.tokens) s = a.slots[t];
+      const bool mine = s >= 0 && (s >> a.shift) == blk;
+      if (!mine) atomicMin(&stop, tid);
+      __syncthreads();
+      if (tid < stop) {
+        const int off = (int)(s & (bs - 1));
+        atomicMax(&src[off], (int)t);
+        atomicMin(&lowest, off);
+        atomicMax(&highest, off);
+      }
+      if (stop < kAppendThreads) break;
+    }
+    __syncthreads();
+    const int lo = lowest, hi = highest;
+    const T* kq = static_cast<const T*>(a.qkv) + (int64_t)(a.heads + head) * hd;
+    const T* vq = kq + (int64_t)a.kv_heads * hd;
+    const int pieces = hd / 8;
+    float ka = 0.f, va = 0.f;
+    for (int i = lo * pieces + tid; i < (hi + 1) * pieces; i += kAppendThreads) {
+      const int off = i / pieces, p = i - off * pieces, t = src[off];
+      if (t < 0) continue;
+      float x[8], y[8];
+      load8(kq + t * a.ld + 8 * p, x);
+      load8(vq + t * a.ld + 8 * p, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ka = fmaxf(ka, finite_abs(x[e]));
+        va = fmaxf(va, finite_abs(y[e]));
+      }
+    }
+    ka = block_max(ka, red);
+    va = block_max(va, red);
+    const int64_t bh = blk * a.kv_heads + head;
+    float ks = pow2(scale_exponent<CACHE>(ka)), vs = pow2(scale_exponent<CACHE>(va));
+    float kr = 1.f, vr = 1.f;
+    bool kgrow = false, vgrow = false;
+    if (lo > 0) {
+      const float least = pow2(kScaleMin), most = pow2(kScaleMax);
+      const float k0 = fminf(fmaxf(a.k_scale[bh], least), most), v0 = fminf(fmaxf(a.v_scale[bh], least), most);
+      kgrow = ks > k0;
+      vgrow = vs > v0;
+      kr = kgrow ? k0 / ks : 1.f;
+      vr = vgrow ? v0 / vs : 1.f;
+      ks = fmaxf(ks, k0);
+      vs = fmaxf(vs, v0);
+    }
+    __syncthreads();  // every thread has read the old scales
+    if (tid == 0) {
+      a.k_scale[bh] = ks;
+      a.v_scale[bh] = vs;
+    }
+    const float ki = 1.f / ks, vi = 1.f / vs;
+    // K: rows of hdp codes, eight to a store.
+    uint8_t* kc = static_cast<uint8_t*>(a.k) + bh * bs * hdp;
+    const int wide = hdp / 8;
+    for (int i = (kgrow ? 0 : lo) * wide + tid; i < (hi + 1) * wide; i += kAppendThreads) {
+      const int off = i / wide, p = i - off * wide, t = src[off];
+      uint2* to = reinterpret_cast<uint2*>(kc + (int64_t)i * 8);
+      uint2 w = {0u, 0u};
+      if (t >= 0) {
+        if (p < pieces) {
+          float x[8];
+          load8(kq + t * a.ld + 8 * p, x);
+          w.x = quant2<CACHE>(x[0] * ki, x[1] * ki) | (quant2<CACHE>(x[2] * ki, x[3] * ki) << 16);
+          w.y = quant2<CACHE>(x[4] * ki, x[5] * ki) | (quant2<CACHE>(x[6] * ki, x[7] * ki) << 16);
+        }
+      } else if (kgrow && off < lo) {
+        w = *to;
+        w.x = regrade<CACHE>(w.x, kr);
+        w.y = regrade<CACHE>(w.y, kr);
+      } else {
+        continue;
+      }
+      *to = w;
+    }
+    // V: rows of bs codes, one for each dimension, four to a store.
+    uint8_t* vc = static_cast<uint8_t*>(a.v) + bh * bs * hdp;
+    const int q0 = (vgrow ? 0 : lo) >> 2, q1 = (hi >> 2) + 1, quads = q1 - q0;
+    for (int i = tid; i < quads * hdp; i += kAppendThreads) {
+      const int d = i / quads, q = q0 + (i - d * quads);
+      uint32_t* to = reinterpret_cast<uint32_t*>(vc + d * bs + 4 * q);
+      uint32_t put = 0, w = 0;  // bytes to replace, and with what
+      bool old = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int off = 4 * q + j, t = src[off];
+        if (t >= 0) {
+          put |= 0xffu << (8 * j);
+          if (d < hd) w |= quant1<CACHE>((float)vq[t * a.ld + d] * vi) << (8 * j);
+        } else if (vgrow && off < lo) {
+          put |= 0xffu << (8 * j);
+          old = true;
+        }
+      }
+      if (!put) continue;
+      if (put != 0xffffffffu || old) {
+        const uint32_t had = *to;
+        if (old) {
+          const uint32_t g = regrade<CACHE>(had, vr);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (src[4 * q + j] < 0 && 4 * q + j < lo) w |= g & (0xffu << (8 * j));
+        }
+        w = (w & put) | (had & ~put);
+      }
+      *to = w;
+    }
+  }
+}
+
+}  // namespace
+
+int cache_width(int64_t head_dim) {
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 8) return -1;
+  for (int w : {32, 64, 96, 128, 192, 256})
+    if (head_dim <= w) return w;
+  return -1;
+}
+
+int cache_shift(int64_t block) {
+  return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
+}
+
+hipError_t run_cache_reserve(const CacheReserveArgs& a, hipStream_t stream) {
+  if (a.batch <= 0 || a.width < 0 || a.tokens < 0 || a.tokens > 0x7fffffff || a.num_free < 0) return hipErrorInvalidValue;
+  // One workgroup fills 1024 slots at a time; past a few rounds of it a second launch over
+  // the whole chip is faster.
+  const bool one = a.tokens <= 8192;
+  hipLaunchKernelGGL(cache_reserve_kernel, dim3(1), dim3(kThreads), 0, stream, a, one ? 1 : 0);
+  if (!one) {
+    const int64_t g = (a.tokens + 1023) / 1024;
+    hipLaunchKernelGGL(cache_reserve_fill_kernel, dim3((unsigned)(g < 2048 ? g : 2048)), dim3(256), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream) {
+  if (a.batch <= 0 || a.width < 0 || a.num_free < 0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(cache_trim_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t run_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
+  if (a.tokens <= 0 || a.tokens > 0x7fffffff || a.kv_heads > 65535) return hipErrorInvalidValue;
+  // Few tokens: a workgroup for each.  Many: they are prompts, whose blocks begin every bs
+  // tokens, and a workgroup looks through 16 tokens for beginnings.
+  const int window = a.tokens * a.kv_heads <= 8192 ? 1 : 16;
+  const dim3 grid((unsigned)((a.tokens + window - 1) / window), (unsigned)a.kv_heads);
+  const bool f16in = a.dtype == kF16, e4m3 = a.cache == kCacheE4M3;
+  if (f16in && e4m3)
+    hipLaunchKernelGGL((cache_append_kernel<f16, kCacheE4M3>), grid, dim3(kAppendThreads), 0, stream, a, window);
+  else if (f16in)
+    hipLaunchKernelGGL((cache_append_kernel<f16, kCacheI8>), grid, dim3(kAppendThreads), 0, stream, a, window);
+  else if (e4m3)
+    hipLaunchKernelGGL((cache_append_kernel<bf16, kCacheE4M3>), grid, dim3(kAppendThreads), 0, stream, a, window);
+  else
+    hipLaunchKernelGGL((cache_append_kernel<bf16, kCacheI8>), grid, dim3(kAppendThreads), 0, stream, a, window);
+  return hipGetLastError();
+}
+
+}  // namespace cobra

@@ -1,0 +1,629 @@
+// Attention of new tokens over a key/value cache held in 8 bits (layout: cache.hip).
+//
+// For new token i of a request with L keys, n of them new, and a query head of kv head h:
+//   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j),  k_j = sk(j) kc_j,  v_j = sv(j) vc_j
+// over j <= L - n + i (causal) or j < L, with codes kc, vc and one scale for each block and head.
+//
+// In one pass over the keys, with running values for each row (log2 units):
+//   u_j = (q . kc_j) sk(j) scale log2(e) + log2 sv(j),   M = max u,   w_j = 2^(u_j - M + 14)
+//   O = sum w_j vc_j,   l = sum w_j / sv(j),   o = O / l
+// so that V's scales ride in the exponent the softmax computes anyway, and the P.V product
+// runs on plain codes.  w lies in [0, 2^14] and is rounded to fp16 for that product (11 bits,
+// and 2^-28 of the largest before fp16's subnormals) whatever the activations' type: codes
+// are exact in fp16.  Scores, M, l and O are fp32.  Scales lie in [2^-40, 2^40], so no w that
+// counts underflows and neither sum overflows.
+//
+// Tiles are 64 keys and 16 rows (v_mfma_f32_16x16x32): S^T = K Q^T, then O^T = V^T P^T.  Row r
+// of K's subtile s is key 16 (r / 4) + 4 s + r % 4, which leaves the scores of keys
+// 16 g .. 16 g + 15 in lane group g = lane / 16, in order: exactly the keys whose codes that
+// group reads of V^T in one 16-byte load.  P goes from the softmax into the product without
+// leaving its lane, K and V from memory into the matrix cores without passing LDS, and since a
+// block is at least 16 tokens a lane needs one K scale and one V scale for a tile.
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace cobra {
+
+namespace {
+
+constexpr int kTile = 64;
+constexpr float kBias = 14.f;  // log2 of the largest w
+
+__device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Eight codes to the operand type, exactly.
+template <int CACHE, typename T>
+struct Widen;
+template <>
+struct Widen<kCacheE4M3, f16> {
+  static __device__ __forceinline__ f16x8 of(uint32_t x, uint32_t y) {
+    struct {
+      f16x2 p[4];
+    } q;
+    q.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, false);
+    q.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, true);
+    q.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.f, false);
+    q.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.f, true);
+    return __builtin_bit_cast(f16x8, q);
+  }
+};
+template <>
+struct Widen<kCacheE4M3, bf16> {
+  static __device__ __forceinline__ bf16x8 of(uint32_t x, uint32_t y) {
+    struct {
+      bf16x2 p[4];
+    } q;
+    q.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, false);
+    q.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, true);
+    q.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, false);
+    q.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, true);
+    return __builtin_bit_cast(bf16x8, q);
+  }
+};
+// int8 to fp16: the byte with its sign flipped, u = c + 128, as the low byte of 0x6400 is the
+// number 1024 + u, from which 1152 is taken (both exact).  The subtraction is left to the
+// compiler, which keeps the two wait states that a matrix instruction needs after a vector
+// one has written its operand; it does not for inline asm.
+__device__ __forceinline__ f16x2 i8_pair(uint32_t flipped, uint32_t sel) {
+  const uint32_t w = __builtin_amdgcn_perm(0x64646464u, flipped, sel);
+  const f16x2 off = {(f16)1152.f, (f16)1152.f};
+  return __builtin_bit_cast(f16x2, w) - off;
+}
+template <>
+struct Widen<kCacheI8, f16> {
+  static __device__ __forceinline__ f16x8 of(uint32_t x, uint32_t y) {
+    struct {
+      f16x2 p[4];
+    } q;
+    x ^= 0x80808080u;
+    y ^= 0x80808080u;
+    q.p[0] = i8_pair(x, 0x04010400u);
+    q.p[1] = i8_pair(x, 0x04030402u);
+    q.p[2] = i8_pair(y, 0x04010400u);
+    q.p[3] = i8_pair(y, 0x04030402u);
+    return __builtin_bit_cast(f16x8, q);
+  }
+};
+template <>
+struct Widen<kCacheI8, bf16> {
+  static __device__ __forceinline__ bf16x8 of(uint32_t x, uint32_t y) {
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[i] = (bf16)(float)(int8_t)(x >> (8 * i));
+      r[4 + i] = (bf16)(float)(int8_t)(y >> (8 * i));
+    }
+    return r;
+  }
+};
+
+struct Args {
+  const void* q;
+  void* out;
+  const int32_t *cu, *lens, *table;
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  float* part_o;   // [splits][tokens * heads][hdp], O of each split
+  float2* part_m;  // [splits][tokens * heads], (M, l)
+  int64_t ldq, table_width, num_blocks;
+  int tokens, batch, heads, kv_heads, group, head_dim, shift, causal;
+  float c2;        // scale * log2(e)
+  int splits;      // grid splits of a request's keys
+  int chunk;       // keys of a split, at least (a multiple of the workgroup's step)
+  int row_tiles;   // grid tiles of a request's rows
+};
+
+// A request as the kernels see it, whatever its lengths say: bounds that keep every access
+// inside the tensors.
+struct Request {
+  int t0, n, len;
+};
+__device__ __forceinline__ Request request_of(const Args& a, int b) {
+  Request r;
+  r.t0 = a.cu[b];
+  const int t1 = a.cu[b + 1];
+  r.n = t1 - r.t0;
+  if (r.t0 < 0 || t1 > a.tokens || r.n < 0) r.n = 0;
+  const int64_t most = min(a.table_width << a.shift, (int64_t)0x7fffff00);
+  const int len = a.lens[b];
+  r.len = len < 0 ? 0 : len > most ? (int)most : len;
+  return r;
+}
+
+// Keys of one split of a request: a.chunk, or more where the grid's splits would not cover it.
+__device__ __forceinline__ int chunk_of(const Args& a, int len, int step) {
+  const int even = (len + a.splits - 1) / a.splits;
+  const int up = (even + step - 1) / step * step;
+  return up > a.chunk ? up : a.chunk;
+}
+
+// One wave's state for NR sets of 16 rows and its pass over some tiles of keys.
+template <typename T, int CACHE, int HDP, int NR>
+struct Rows {
+  typedef typename Op16<T>::V8 V8;
+  static constexpr int kSteps = HDP / 32, kWide = HDP / 64, kOdd = kSteps & 1, kDims = HDP / 16;
+
+  V8 q[NR][kSteps];
+  f32x4 o[NR][kDims];
+  float m[NR], l[NR];  // l: this lane group's share
+  int lim[NR];         // keys that this lane's row sees
+
+  __device__ __forceinline__ void init(const Args& a, const Request& rq, int h, int64_t row0) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int64_t row = row0 + 16 * r + n;
+      const bool there = row < (int64_t)rq.n * a.group;
+      const int tok = there ? (int)(row / a.group) : 0;
+      const int head = h * a.group + (there ? (int)(row - (int64_t)tok * a.group) : 0);
+      const T* p = static_cast<const T*>(a.q) + (int64_t)(rq.t0 + tok) * a.ldq + (int64_t)head * a.head_dim;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int d = s < 2 * kWide ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 64 * kWide + 8 * g;
+        q[r][s] = zero8_of<T>();
+        if (there && d < a.head_dim) q[r][s] = *reinterpret_cast<const V8*>(p + d);
+      }
+      const int seen = a.causal ? rq.len - rq.n + tok + 1 : rq.len;
+      lim[r] = there ? (seen < 0 ? 0 : seen) : 0;
+      m[r] = kNegInf;
+      l[r] = 0.f;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t) o[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // Tiles t0, t0 + step, .. below t_end; keys from `full` on are checked against each row's limit.
+  __device__ __forceinline__ void pass(const Args& a, const Request& rq, int b, int h, int t0, int t_end, int step,
+                                       int full) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, gk = n >> 2;
+    const int32_t* table = a.table + b * a.table_width;
+    const int bs = 1 << a.shift, last_page = (int)a.table_width - 1;
+    const int64_t plane = (int64_t)bs * HDP;
+    if (t0 >= t_end) return;
+
+    // Block ids of a tile: of the group whose K rows this lane reads, and of its own V keys.
+    auto page = [&](int tile, int grp) {
+      const int p = (tile * kTile + 16 * grp) >> a.shift;
+      return table[p < last_page ? p : last_page];
+    };
+    uint4 kw[4][kWide > 0 ? kWide : 1];
+    uint2 ko[4];
+    uint4 vw[kDims];
+    float sk, sv;
+    int idk = page(t0, gk), idv = page(t0, g);
+    bool bad_next = false;
+    auto clamp_id = [&](int id) { return (unsigned)id < (unsigned)a.num_blocks ? id : 0; };
+    auto load_k = [&](int tile) {
+      const int64_t at = ((int64_t)clamp_id(idk) * a.kv_heads + h) * plane;
+      const int off = (tile * kTile + 16 * gk + (n & 3)) & (bs - 1);
+      const uint8_t* p = a.k + at + (int64_t)off * HDP;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) kw[s][j] = *reinterpret_cast<const uint4*>(p + s * 4 * HDP + 64 * j + 16 * g);
+        if constexpr (kOdd) ko[s] = *reinterpret_cast<const uint2*>(p + s * 4 * HDP + 64 * kWide + 8 * g);
+      }
+    };
+    auto load_v = [&](int tile) {
+      const int64_t bh = (int64_t)clamp_id(idv) * a.kv_heads + h;
+      const int off = (tile * kTile + 16 * g) & (bs - 1);
+      const uint8_t* p = a.v + bh * plane + (int64_t)n * bs + off;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t) vw[t] = *reinterpret_cast<const uint4*>(p + (int64_t)t * 16 * bs);
+    };
+    auto load_scales = [&]() {
+      const int64_t bh = (int64_t)clamp_id(idv) * a.kv_heads + h;
+      sk = a.k_scale[bh];
+      sv = a.v_scale[bh];
+      bad_next = (unsigned)idv >= (unsigned)a.num_blocks;
+    };
+    load_k(t0);
+    load_scales();
+    load_v(t0);
+    int idk2 = 0, idv2 = 0;
+    if (t0 + step < t_end) {
+      idk2 = page(t0 + step, gk);
+      idv2 = page(t0 + step, g);
+    }
+    for (int tile = t0; tile < t_end; tile += step) {
+      const bool more = tile + step < t_end;
+      const int key0 = tile * kTile + 16 * g;  // this lane's first key
+      // S^T = K Q^T on codes.
+      f32x4 s[NR][4];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+          const V8 lo = Widen<CACHE, T>::of(kw[i][j].x, kw[i][j].y), hi = Widen<CACHE, T>::of(kw[i][j].z, kw[i][j].w);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) s[r][i] = mfma16(lo, q[r][2 * j], s[r][i]);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) s[r][i] = mfma16(hi, q[r][2 * j + 1], s[r][i]);
+        }
+        if constexpr (kOdd) {
+          const V8 lo = Widen<CACHE, T>::of(ko[i].x, ko[i].y);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) s[r][i] = mfma16(lo, q[r][kSteps - 1], s[r][i]);
+        }
+      }
+      const bool bad = bad_next;
+      const float skc = sk * a.c2, svc = fminf(fmaxf(sv, 0x1p-40f), 0x1p40f);
+      const float ev = __builtin_amdgcn_logf(svc), inv = 1.f / svc;
+      // The next tile's keys and scales while this one's softmax runs.
+      if (more) {
+        idk = idk2;
+        idv = idv2;
+        load_k(tile + step);
+        load_scales();
+        if (tile + 2 * step < t_end) {
+          idk2 = page(tile + 2 * step, gk);
+          idv2 = page(tile + 2 * step, g);
+        }
+      }
+      const bool slow = tile * kTile + kTile > full || __any(bad);
+      f16x8 p[NR][2];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float u[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[4 * i + e] = fmaf(s[r][i][e], skc, ev);
+        if (slow) {
+          const int seen = bad ? 0 : lim[r] - key0;  // keys of this lane that count
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = e < seen ? u[e] : kNegInf;
+        }
+        float mx = u[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, u[e]);
+        {
+          const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+        }
+        const float mn = fmaxf(m[r], mx);
+        const float base = mn == kNegInf ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
+        m[r] = mn;
+        const float shift = kBias - base;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float w = __builtin_amdgcn_exp2f(u[e] + shift);
+          sum += w;
+          p[r][e >> 3][e & 7] = (f16)w;
+        }
+        l[r] = l[r] * alpha + sum * inv;
+#pragma unroll
+        for (int t = 0; t < kDims; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
+      }
+      if (slow) {
+        // Memory past the request's end, or of a block that is none, may hold NaN codes.
+        const int there = bad ? 0 : rq.len - key0;
+#pragma unroll
+        for (int t = 0; t < kDims; ++t) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(&vw[t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = there - 4 * i;
+            w[i] = c >= 4 ? w[i] : c <= 0 ? 0u : w[i] & (0xffffffffu >> (8 * (4 - c)));
+          }
+        }
+      }
+      // O^T += V^T P^T on codes.
+#pragma unroll
+      for (int t = 0; t < kDims; ++t) {
+        const f16x8 lo = Widen<CACHE, f16>::of(vw[t].x, vw[t].y), hi = Widen<CACHE, f16>::of(vw[t].z, vw[t].w);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) o[r][t] = mfma16(lo, p[r][0], o[r][t]);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) o[r][t] = mfma16(hi, p[r][1], o[r][t]);
+      }
+      if (more) load_v(tile + step);
+    }
+  }
+
+  __device__ __forceinline__ void total_l() {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) l[r] = sum_xor32(sum_xor16(l[r]));
+  }
+
+  // Row set r to its place: the result, or a split's share of it.
+  __device__ __forceinline__ void store(const Args& a, const Request& rq, int h, int64_t row0, int r, int split,
+                                        bool whole) const {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int64_t row = row0 + 16 * r + n;
+    if (row >= (int64_t)rq.n * a.group) return;
+    const int tok = (int)(row / a.group);
+    const int64_t at = (int64_t)(rq.t0 + tok) * a.heads + h * a.group + (row - (int64_t)tok * a.group);
+    if (whole) {
+      const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+      T* p = static_cast<T*>(a.out) + at * a.head_dim;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t) {
+        const int d = 16 * t + 4 * g;
+        if (d < a.head_dim) {
+          typename Op16<T>::V4 x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = (T)(o[r][t][i] * inv);
+          *reinterpret_cast<typename Op16<T>::V4*>(p + d) = x;
+        }
+      }
+    } else {
+      const int64_t i = (int64_t)split * a.tokens * a.heads + at;
+      if (g == 0) a.part_m[i] = make_float2(m[r], l[r]);
+      float* p = a.part_o + i * HDP + 4 * g;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t) *reinterpret_cast<f32x4*>(p + 16 * t) = o[r][t];
+    }
+  }
+};
+
+// Few rows for each kv head: a workgroup has 16 of them and one split of the keys, its waves
+// every kWaves-th tile of it; their shares are joined through LDS, the splits' by
+// cache_join_kernel.
+template <typename T, int CACHE, int HDP>
+__global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
+  constexpr int kWaves = 4;
+  typedef Rows<T, CACHE, HDP, 1> R;
+  __shared__ f32x4 sh_o[2][R::kDims][64];
+  __shared__ float sh_m[2][64], sh_l[2][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int id = blockIdx.x;
+  const int h = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int b = id % a.batch;
+  const Request rq = request_of(a, b);
+  const int64_t rows = (int64_t)rq.n * a.group;
+  const int chunk = chunk_of(a, rq.len, kWaves * kTile);
+  if (split > 0 && (int64_t)split * chunk >= rq.len) return;
+  for (int64_t row0 = (int64_t)(id / a.batch) * 16; row0 < rows; row0 += (int64_t)a.row_tiles * 16) {
+    R w;
+    w.init(a, rq, h, row0);
+    // Keys up to what the tile's last row sees; all of its rows see those below `full`.
+    const int64_t end_row = min(row0 + 16, rows) - 1;
+    int end = rq.len, full = rq.len;
+    if (a.causal) {
+      end = rq.len - rq.n + (int)(end_row / a.group) + 1;
+      full = rq.len - rq.n + (int)(row0 / a.group) + 1;
+      end = end < 0 ? 0 : end;
+    }
+    const int64_t k0 = (int64_t)split * chunk;
+    const int64_t k1 = min((int64_t)end, k0 + chunk);
+    w.pass(a, rq, b, h, (int)(k0 / kTile) + wave, (int)((k1 + kTile - 1) / kTile), kWaves, full);
+    w.total_l();
+    // Waves 2, 3 into 0, 1, then 1 into 0.
+#pragma unroll
+    for (int half = 2; half; half >>= 1) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half) {
+        sh_m[wave - half][lane] = w.m[0];
+        sh_l[wave - half][lane] = w.l[0];
+#pragma unroll
+        for (int t = 0; t < R::kDims; ++t) sh_o[wave - half][t][lane] = w.o[0][t];
+      }
+      __syncthreads();
+      if (wave < half) {
+        const float m2 = sh_m[wave][lane], mn = fmaxf(w.m[0], m2), base = mn == kNegInf ? 0.f : mn;
+        const float f1 = __builtin_amdgcn_exp2f(w.m[0] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        w.m[0] = mn;
+        w.l[0] = w.l[0] * f1 + sh_l[wave][lane] * f2;
+#pragma unroll
+        for (int t = 0; t < R::kDims; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[0][t][i] = w.o[0][t][i] * f1 + sh_o[wave][t][lane][i] * f2;
+      }
+    }
+    if (wave == 0) w.store(a, rq, h, row0, 0, split, chunk >= rq.len);
+  }
+}
+
+// The splits of a row joined: o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s, in order of s.
+template <typename T, int HDP>
+__global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  if (row >= rows) return;
+  const int t = (int)(row / a.heads);
+  int lo = 0, hi = a.batch;  // the last request with cu[b] <= t
+  while (lo + 1 < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const Request rq = request_of(a, lo);
+  if (t < rq.t0 || t >= rq.t0 + rq.n) return;
+  const int chunk = chunk_of(a, rq.len, step);
+  if (chunk >= rq.len) return;  // written by the workgroup that had all of it
+  const int n = (int)(((int64_t)rq.len + chunk - 1) / chunk);
+  float m = kNegInf;
+  for (int s = 0; s < n; ++s) m = fmaxf(m, a.part_m[s * rows + row].x);
+  const float base = m == kNegInf ? 0.f : m;
+  constexpr int kPer = (HDP + 63) / 64;
+  float o[kPer], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+  for (int s = 0; s < n; ++s) {
+    const float2 ml = a.part_m[s * rows + row];
+    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+    l += f * ml.y;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + 64 * i < HDP) o[i] += f * a.part_o[(s * rows + row) * HDP + lane + 64 * i];
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int d = lane + 64 * i;
+    if (d < a.head_dim) static_cast<T*>(a.out)[row * a.head_dim + d] = (T)(o[i] * inv);
+  }
+}
+
+// Many rows for each kv head: a wave has NR sets of 16 and passes over all of their keys.
+template <typename T, int CACHE, int HDP, int NR>
+__global__ __launch_bounds__(256) void cache_chunk_kernel(Args a) {
+  constexpr int kWaves = 4, kRows = kWaves * NR * 16;
+  typedef Rows<T, CACHE, HDP, NR> R;
+  const int wave = threadIdx.x >> 6;
+  int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int tile0 = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int h = id % a.kv_heads, b = id / a.kv_heads;
+  const Request rq = request_of(a, b);
+  const int64_t rows = (int64_t)rq.n * a.group;
+  for (int64_t at = (int64_t)tile0 * kRows; at < rows; at += (int64_t)a.row_tiles * kRows) {
+    const int64_t row0 = at + wave * NR * 16;
+    if (row0 >= rows) continue;
+    R w;
+    w.init(a, rq, h, row0);
+    const int64_t end_row = min(row0 + NR * 16, rows) - 1;
+    int end = rq.len, full = rq.len;
+    if (a.causal) {
+      end = rq.len - rq.n + (int)(end_row / a.group) + 1;
+      full = rq.len - rq.n + (int)(row0 / a.group) + 1;
+      end = end < 0 ? 0 : end;
+    }
+    w.pass(a, rq, b, h, 0, (end + kTile - 1) / kTile, 1, full);
+    w.total_l();
+#pragma unroll
+    for (int r = 0; r < NR; ++r) w.store(a, rq, h, row0, r, 0, true);
+  }
+}
+
+constexpr int kStep = 4 * kTile;  // keys that a decode workgroup takes at a time
+
+struct Plan {
+  bool chunked;
+  int splits, chunk;
+  int64_t row_tiles;
+};
+
+// How a call is cut.  max_new and max_len are expectations; a call that exceeds them is still
+// covered (rows in a loop, longer splits).
+Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_new, int64_t max_len) {
+  Plan p{};
+  max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
+  max_len = max_len < 1 ? 1 : max_len > 0x7fffff00 ? 0x7fffff00 : max_len;
+  const int64_t group = heads / kv_heads, rows = max_new * group;
+  p.chunked = rows > 64;
+  p.splits = 1;
+  if (p.chunked) {
+    p.row_tiles = (rows + 127) / 128;
+    p.chunk = 0x40000000;
+    return p;
+  }
+  p.row_tiles = (rows + 15) / 16;
+  const int64_t base = batch * kv_heads * p.row_tiles;
+  int64_t splits = (2048 + base - 1) / base;
+  const int64_t most = (max_len + kStep - 1) / kStep;
+  splits = splits < most ? splits : most;
+  splits = splits < 1 ? 1 : splits > 1024 ? 1024 : splits;
+  const int64_t even = (max_len + splits - 1) / splits;
+  int64_t chunk = (even + kStep - 1) / kStep * kStep;
+  if (chunk < kStep) chunk = kStep;
+  p.splits = (int)((max_len + chunk - 1) / chunk);
+  if (p.splits < 1) p.splits = 1;
+  p.chunk = (int)chunk;
+  return p;
+}
+
+template <typename T, int CACHE, int HDP>
+hipError_t launch(const Args& a, const Plan& p, hipStream_t stream) {
+  if (p.chunked) {
+    const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles;
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((cache_chunk_kernel<T, CACHE, HDP, HDP <= 128 ? 2 : 1>), dim3((unsigned)grid), dim3(256), 0, stream,
+                       a);
+    return hipGetLastError();
+  }
+  const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles * p.splits;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)a.tokens * a.heads;
+    hipLaunchKernelGGL((cache_join_kernel<T, HDP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, kStep);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int CACHE>
+hipError_t launch_width(const Args& a, const Plan& p, int width, hipStream_t stream) {
+  switch (width) {
+    case 32: return launch<T, CACHE, 32>(a, p, stream);
+    case 64: return launch<T, CACHE, 64>(a, p, stream);
+    case 96: return launch<T, CACHE, 96>(a, p, stream);
+    case 128: return launch<T, CACHE, 128>(a, p, stream);
+    case 192: return launch<T, CACHE, 192>(a, p, stream);
+    case 256: return launch<T, CACHE, 256>(a, p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t max_new, int64_t max_len) {
+  const Plan p = plan_of(tokens, batch, heads, kv_heads, max_new, max_len);
+  if (p.splits <= 1) return 0;
+  return (int64_t)p.splits * tokens * heads * (cache_width(head_dim) * 4 + 8);
+}
+
+hipError_t run_cache_attn(const CacheAttnArgs& c, int64_t workspace_bytes, hipStream_t stream) {
+  const int width = cache_width(c.head_dim);
+  if (width < 0 || c.tokens <= 0 || c.tokens > 0x7fffffff || c.batch <= 0 || c.table_width <= 0) return hipErrorInvalidValue;
+  const Plan p = plan_of(c.tokens, c.batch, c.heads, c.kv_heads, c.max_new, c.max_len);
+  Args a{};
+  a.q = c.q;
+  a.out = c.out;
+  a.cu = c.cu;
+  a.lens = c.lens;
+  a.table = c.table;
+  a.k = static_cast<const uint8_t*>(c.k);
+  a.v = static_cast<const uint8_t*>(c.v);
+  a.k_scale = c.k_scale;
+  a.v_scale = c.v_scale;
+  a.ldq = c.ldq;
+  a.table_width = c.table_width;
+  a.num_blocks = c.num_blocks;
+  a.tokens = (int)c.tokens;
+  a.batch = c.batch;
+  a.heads = c.heads;
+  a.kv_heads = c.kv_heads;
+  a.group = c.heads / c.kv_heads;
+  a.head_dim = c.head_dim;
+  a.shift = c.shift;
+  a.causal = c.causal;
+  a.c2 = c.scale * 1.4426950408889634f;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.row_tiles = (int)p.row_tiles;
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)p.splits * c.tokens * c.heads;
+    if (!c.part || workspace_bytes < rows * (width * 4 + 8)) return hipErrorInvalidValue;
+    a.part_o = c.part;
+    a.part_m = reinterpret_cast<float2*>(c.part + rows * width);
+  }
+  if (c.dtype == kF16)
+    return c.cache == kCacheE4M3 ? launch_width<f16, kCacheE4M3>(a, p, width, stream)
+                                 : launch_width<f16, kCacheI8>(a, p, width, stream);
+  return c.cache == kCacheE4M3 ? launch_width<bf16, kCacheE4M3>(a, p, width, stream)
+                               : launch_width<bf16, kCacheI8>(a, p, width, stream);
+}
+
+}  // namespace cobra

@@ -447,6 +447,134 @@ int cobra_attn_fwd(const void* qkv, void* ctx, int dtype, const uint64_t* key_bi
   return code(cobra::run_attn(a));
 }
 
+// -- key/value cache held in 8 bits ------------------------------------------------------
+
+static_assert(COBRA_CACHE_E4M3 == cobra::kCacheE4M3 && COBRA_CACHE_I8 == cobra::kCacheI8, "cache codes");
+
+int cobra_cache_width(int64_t head_dim) { return cobra::cache_width(head_dim); }
+
+int cobra_cache_reserve(int32_t* lens, const int32_t* new_lens, int32_t* block_table, int64_t table_width,
+                        const int32_t* free_list, int64_t num_free, int32_t* free_count, int64_t* slots,
+                        int64_t tokens, int32_t* cu, int32_t* missing, int32_t* workspace, int64_t batch,
+                        int64_t block_size, void* stream) {
+  const int shift = cobra::cache_shift(block_size);
+  if (shift < 0 || batch < 0 || batch > 0x7ffffffe || tokens < 0 || tokens > 0x7fffffff || table_width < 0 ||
+      table_width > 0x7fffffff || num_free < 0 || num_free > 0x7fffffff)
+    return kBad;
+  if (batch == 0) return 0;
+  if (!lens || !new_lens || !free_count || !cu || !missing || !workspace || (!block_table && table_width) ||
+      (!free_list && num_free) || (!slots && tokens))
+    return kBad;
+  for (const void* p : {(const void*)lens, (const void*)new_lens, (const void*)block_table, (const void*)free_list,
+                        (const void*)free_count, (const void*)cu, (const void*)missing, (const void*)workspace})
+    if (!aligned_to(p, 4)) return kBad;
+  if (!aligned_to(slots, 8)) return kBad;
+  const cobra::CacheReserveArgs a{lens, new_lens, block_table, free_list, free_count, slots, cu, missing, workspace,
+                                  tokens, table_width, num_free, (int)batch, shift};
+  return code(cobra::run_cache_reserve(a, static_cast<hipStream_t>(stream)));
+}
+
+int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* block_table, int64_t table_width,
+                     int32_t* free_list, int64_t num_free, int32_t* free_count, int32_t* refused, int32_t* workspace,
+                     int64_t batch, int64_t block_size, void* stream) {
+  const int shift = cobra::cache_shift(block_size);
+  if (shift < 0 || batch < 0 || batch > 0x7ffffffe || table_width < 0 || table_width > 0x7fffffff || num_free < 0 ||
+      num_free > 0x7fffffff)
+    return kBad;
+  if (batch == 0) return 0;
+  if (!lens || !keep_lens || !free_count || !refused || !workspace || (!block_table && table_width) ||
+      (!free_list && num_free))
+    return kBad;
+  for (const void* p : {(const void*)lens, (const void*)keep_lens, (const void*)block_table, (const void*)free_list,
+                        (const void*)free_count, (const void*)refused, (const void*)workspace})
+    if (!aligned_to(p, 4)) return kBad;
+  const cobra::CacheTrimArgs a{lens, keep_lens, block_table, free_list, free_count, refused, workspace,
+                               table_width, num_free, (int)batch, shift};
+  return code(cobra::run_cache_trim(a, static_cast<hipStream_t>(stream)));
+}
+
+namespace {
+
+// Whether a cache of this geometry is taken (num_blocks block ids fit an int32).
+bool cache_ok(int cache, int64_t num_blocks, int64_t kv_heads, int64_t heads, int64_t head_dim, int64_t block_size) {
+  return (cache == COBRA_CACHE_E4M3 || cache == COBRA_CACHE_I8) && num_blocks >= 0 && num_blocks <= 0x7fffffff &&
+         kv_heads > 0 && kv_heads <= 65535 && heads > 0 && heads <= 0x7fffff && heads % kv_heads == 0 &&
+         cobra::cache_width(head_dim) > 0 && cobra::cache_shift(block_size) > 0;
+}
+
+}  // namespace
+
+int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* slots, void* k, void* v, float* k_scale,
+                       float* v_scale, int cache, int64_t tokens, int64_t num_blocks, int64_t block_size,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream) {
+  if (!is_op_dtype(dtype) || !cache_ok(cache, num_blocks, kv_heads, heads, head_dim, block_size) || tokens < 0 ||
+      tokens > 0x7fffffff || ld < (heads + 2 * kv_heads) * head_dim || ld % 8)
+    return kBad;
+  if (tokens == 0 || num_blocks == 0) return 0;
+  if (!qkv || !slots || !k || !v || !k_scale || !v_scale || !aligned16(qkv) || !aligned16(k) || !aligned16(v) ||
+      !aligned_to(slots, 8) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+    return kBad;
+  const cobra::CacheAppendArgs a{qkv, slots, k, v, k_scale, v_scale, tokens, ld, num_blocks, (int)heads,
+                                 (int)kv_heads, (int)head_dim, cobra::cache_width(head_dim),
+                                 cobra::cache_shift(block_size), dtype, cache};
+  return code(cobra::run_cache_append(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t cobra_cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t max_new, int64_t max_len) {
+  if (tokens < 0 || tokens > 0x7fffffff || batch < 0 || batch > 0x7ffffffe || max_new < 0 || max_len < 0 ||
+      !cache_ok(0, 1, kv_heads, heads, head_dim, 16))
+    return -1;
+  if (tokens == 0 || batch == 0) return 0;
+  return cobra::cache_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+}
+
+int cobra_cache_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* cu, const int32_t* lens,
+                         const int32_t* block_table, int64_t table_width, const void* k, const void* v,
+                         const float* k_scale, const float* v_scale, int cache, void* ctx, void* workspace,
+                         int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_blocks,
+                         int64_t block_size, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
+                         int64_t max_len, float scale, int causal, void* stream) {
+  if (!is_op_dtype(dtype) || !cache_ok(cache, num_blocks, kv_heads, heads, head_dim, block_size) || num_blocks == 0 ||
+      table_width <= 0 || table_width > 0x7fffffff || ldq < heads * head_dim || ldq % 8 || !(scale > 0.f))
+    return kBad;
+  const int64_t need = cobra_cache_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  if (need < 0) return kBad;
+  if (tokens == 0 || batch == 0) return 0;
+  if (!q || !cu || !lens || !block_table || !k || !v || !k_scale || !v_scale || !ctx || !aligned16(q) ||
+      !aligned16(k) || !aligned16(v) || !aligned16(ctx) || !aligned_to(cu, 4) || !aligned_to(lens, 4) ||
+      !aligned_to(block_table, 4) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+    return kBad;
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return kBad;
+  cobra::CacheAttnArgs a{};
+  a.q = q;
+  a.out = ctx;
+  a.cu = cu;
+  a.lens = lens;
+  a.table = block_table;
+  a.k = k;
+  a.v = v;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.part = static_cast<float*>(workspace);
+  a.tokens = tokens;
+  a.ldq = ldq;
+  a.num_blocks = num_blocks;
+  a.table_width = table_width;
+  a.batch = (int)batch;
+  a.heads = (int)heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.shift = cobra::cache_shift(block_size);
+  a.dtype = dtype;
+  a.cache = cache;
+  a.causal = causal ? 1 : 0;
+  a.scale = scale;
+  a.max_new = max_new;
+  a.max_len = max_len;
+  return code(cobra::run_cache_attn(a, workspace_bytes, static_cast<hipStream_t>(stream)));
+}
+
 int64_t cobra_qkv_attn_workspace_bytes(int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim) {
   if (batch < 0 || seq_len < 0 || heads <= 0 || head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) return -1;
   if (cobra::qkv_attn_head_ok(seq_len, heads, head_dim)) return 0;  // one fused launch, no q / k / v buffer

@@ -318,4 +318,67 @@ bool block_split_ok(int64_t seq_len, int64_t d_model, int64_t heads, int64_t ffn
 bool block_split_pays(int64_t batch, int64_t seq_len);
 hipError_t run_block_split(const BlockArgs& a);
 
+// Key/value cache held in 8 bits (cache.hip, cache_attn.hip): a pool of blocks of 1 << shift
+// tokens; k [num_blocks, kv_heads, bs, hdp], v [num_blocks, kv_heads, hdp, bs] codes of one
+// byte, hdp = cache_width(head_dim), scales [num_blocks, kv_heads] fp32.
+enum : int { kCacheE4M3 = 0, kCacheI8 = 1 };
+int cache_width(int64_t head_dim);  // columns of a cached row, or -1
+int cache_shift(int64_t block);     // log2 of a block size that is taken, or -1
+
+struct CacheReserveArgs {
+  int32_t* lens;             // [batch] tokens held, in and out
+  const int32_t* new_lens;   // [batch]
+  int32_t* table;            // [batch, width] block ids, new entries written
+  const int32_t* free_list;  // [num_free] stack of free block ids
+  int32_t* free_count;       // [1] its height, in and out
+  int64_t* slots;            // [tokens] out
+  int32_t* cu;               // [batch + 1] out
+  int32_t* missing;          // [1] out
+  int32_t* incl;             // [batch + 1] scratch
+  int64_t tokens, width, num_free;
+  int batch, shift;
+};
+hipError_t run_cache_reserve(const CacheReserveArgs& a, hipStream_t stream);
+
+struct CacheTrimArgs {
+  int32_t* lens;             // [batch] in and out
+  const int32_t* keep_lens;  // [batch]
+  const int32_t* table;      // [batch, width]
+  int32_t* free_list;        // [num_free] in and out
+  int32_t* free_count;       // [1] in and out
+  int32_t* refused;          // [1] out
+  int32_t* incl;             // [batch] scratch
+  int64_t width, num_free;
+  int batch, shift;
+};
+hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream);
+
+struct CacheAppendArgs {
+  const void* qkv;       // [tokens, ld]: q | k | v columns, dtype
+  const int64_t* slots;  // [tokens]
+  void *k, *v;           // codes
+  float *k_scale, *v_scale;
+  int64_t tokens, ld, num_blocks;
+  int heads, kv_heads, head_dim, width, shift, dtype, cache;
+};
+hipError_t run_cache_append(const CacheAppendArgs& a, hipStream_t stream);
+
+struct CacheAttnArgs {
+  const void* q;            // [tokens, ldq]: the first heads * head_dim columns, dtype
+  void* out;                // [tokens, heads * head_dim] dtype
+  const int32_t* cu;        // [batch + 1]
+  const int32_t* lens;      // [batch] keys of each request
+  const int32_t* table;     // [batch, table_width]
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  float* part;              // partial results of a split call
+  int64_t tokens, ldq, num_blocks, table_width;
+  int batch, heads, kv_heads, head_dim, shift, dtype, cache, causal;
+  float scale;
+  int64_t max_new, max_len; // expected bounds (speed only)
+};
+int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t max_new, int64_t max_len);
+hipError_t run_cache_attn(const CacheAttnArgs& a, int64_t workspace_bytes, hipStream_t stream);
+
 }  // namespace cobra

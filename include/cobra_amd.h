@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define COBRA_ABI_VERSION 12
+#define COBRA_ABI_VERSION 13
 
 enum { COBRA_F16 = 0, COBRA_F32 = 1, COBRA_BF16 = 2 };
 
@@ -157,6 +157,93 @@ int cobra_mask_bits(const uint8_t* mask, uint64_t* key_bits, int64_t batch, int6
  */
 int cobra_attn_fwd(const void* qkv, void* ctx, int dtype, const uint64_t* key_bits, int64_t batch, int64_t seq_len,
                    int64_t heads, int64_t head_dim, float scale, int causal, void* stream);
+
+/*
+ * A key/value cache held in 8 bits, for requests that grow by some tokens a call (it has no
+ * counterpart in the reference, whose attention sees whole sequences).  A layer's cache is a
+ * pool of num_blocks blocks of block_size (16, 32, 64 or 128) tokens:
+ *     k: [num_blocks, kv_heads, block_size, width] codes of one byte,
+ *     v: [num_blocks, kv_heads, width, block_size] codes (tokens innermost),
+ *     k_scale, v_scale: [num_blocks, kv_heads] fp32; a code c stands for c * scale,
+ * codes being COBRA_CACHE_E4M3 (8-bit floats: 4 exponent and 3 mantissa bits, largest value
+ * 448, no infinities) or COBRA_CACHE_I8 (-127 .. 127).  width = cobra_cache_width(head_dim):
+ * head_dim (a multiple of 8, at most 256) rounded up to 32, 64, 96, 128, 192 or 256, else -1;
+ * the columns past head_dim are zero.  A block table row lists a request's blocks in the order
+ * of its tokens; token p of request b is in slot block_table[b][p / block_size] * block_size +
+ * p % block_size.  Tables, lengths and slots serve every layer of a model.
+ */
+enum { COBRA_CACHE_E4M3 = 0, COBRA_CACHE_I8 = 1 };
+int cobra_cache_width(int64_t head_dim);
+
+/*
+ * Room for new_lens[b] more tokens of each request b:
+ *     need_b = ceil((lens[b] + new_lens[b]) / block_size) - ceil(lens[b] / block_size);
+ *     the k-th new block (requests in order, a request's blocks in order) is
+ *     free_list[free_count - 1 - k] and goes to the request's next entry of block_table;
+ *     cu[b] = new_lens[0] + .. + new_lens[b - 1];  slots[cu[b] + i] = slot of token
+ *     lens[b] + i, for tokens past cu[batch] -1;  lens += new_lens;  free_count -= sum need.
+ * missing = 0 then.  All requests get their room or nothing changes but slots (all -1), cu
+ * (all 0) and missing: the number of blocks that are missing, or -1 where a length is negative
+ * or past 2^31 - 1, a row of the table too short, sum new_lens > tokens, or free_count
+ * outside [0, num_free].  lens, new_lens: [batch]; block_table: [batch, table_width];
+ * free_list: [num_free]; free_count, missing: [1]; cu, workspace: [batch + 1] int32; slots:
+ * [tokens] int64.
+ */
+int cobra_cache_reserve(int32_t* lens, const int32_t* new_lens, int32_t* block_table, int64_t table_width,
+                        const int32_t* free_list, int64_t num_free, int32_t* free_count, int64_t* slots,
+                        int64_t tokens, int32_t* cu, int32_t* missing, int32_t* workspace, int64_t batch,
+                        int64_t block_size, void* stream);
+
+/*
+ * Requests cut to min(lens[b], max(keep_lens[b], 0)) tokens (0: the request is over), their
+ * blocks past that given back: the k-th of them (requests in order, a request's blocks in
+ * order) to free_list[free_count' - 1 - k], free_count' the new height, so that a trim to the
+ * old lengths undoes a reserve.  block_table keeps its entries.  refused = 0; or 1, and nothing
+ * else changes, where a length is negative or longer than a row of the table, or the stack
+ * would not hold the blocks.  workspace: [batch] int32.
+ */
+int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* block_table, int64_t table_width,
+                     int32_t* free_list, int64_t num_free, int32_t* free_count, int32_t* refused, int32_t* workspace,
+                     int64_t batch, int64_t block_size, void* stream);
+
+/*
+ * New keys and values into their slots.  qkv: [tokens, ld] in dtype (COBRA_F16 or COBRA_BF16),
+ * columns q | k | v of heads, kv_heads and kv_heads slices of head_dim; ld % 8 == 0.  For each
+ * block and head that gets tokens, with a = max |x| over their finite values:
+ *     e = the least integer in [-40, 40] with a <= qmax * 2^e (qmax 448 or 127);
+ *     scale = 2^e where the call writes offset 0 of the block (which starts it anew), else
+ *     max(old scale, 2^e), and where it grew the codes of the offsets before the first one
+ *     written become those of the same values under it;
+ *     code = x / scale rounded to the nearest (ties to even), within +-qmax; NaN gives 0.
+ * Tokens of one block stand next to each other in the call, as cobra_cache_reserve lays them
+ * out; of two for one slot the later one stays.  A token whose slot is negative or past the
+ * pool is passed over.  Blocks without a token are left as they are.
+ */
+int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* slots, void* k, void* v, float* k_scale,
+                       float* v_scale, int cache, int64_t tokens, int64_t num_blocks, int64_t block_size,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/*
+ * Attention of each request's new tokens over its cached keys (their own among them):
+ *     ctx_i = softmax_j((q_i . k_j) * scale) v_j over keys j <= lens[b] - n_b + i (causal) or
+ *     j < lens[b], for new token i of n_b = cu[b + 1] - cu[b]; no key: a zero row.
+ * q: [tokens, ldq] in dtype, its first heads * head_dim columns (a packed q | k | v buffer will
+ * do); query head j reads kv head j / (heads / kv_heads).  ctx: [tokens, heads * head_dim];
+ * rows outside [cu[0], cu[batch]) are left as they are.  Scores, softmax and sums are fp32,
+ * the probabilities rounded to fp16 for the product with V's codes; scales are taken within
+ * [2^-40, 2^40].  Keys in a block whose id is outside the pool are masked.  max_new and max_len: the most new
+ * tokens and keys that a request is expected to have; they shape the launch and never the
+ * result.  workspace: cobra_cache_attn_workspace_bytes() bytes (16-byte aligned, may be NULL
+ * when that is 0); launches that share it must not overlap.
+ */
+int64_t cobra_cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t max_new, int64_t max_len);
+int cobra_cache_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* cu, const int32_t* lens,
+                         const int32_t* block_table, int64_t table_width, const void* k, const void* v,
+                         const float* k_scale, const float* v_scale, int cache, void* ctx, void* workspace,
+                         int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_blocks,
+                         int64_t block_size, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
+                         int64_t max_len, float scale, int causal, void* stream);
 
 /*
  * Fused QKV projection + multi-head attention on a normalised activation:
