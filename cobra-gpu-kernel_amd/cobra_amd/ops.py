@@ -514,6 +514,9 @@ def cache_reserve(
     lacks, or -1 for lengths that do not fit (``cobra_cache_reserve``), and then nothing was
     reserved, every slot is -1 and ``cu`` 0.  Nothing here waits for the GPU.
     """
+    got = _lib.host().cache_reserve(lens, new_lens, block_table, free_list, free_count, block_size, tokens)
+    if got is not None:
+        return got
     B = _tables(lens, block_table, free_list, free_count)
     _i32(new_lens, (B,), "new_lens")
     dev = lens.device
@@ -551,6 +554,9 @@ def cache_trim(
     are updated in place; ``refused`` is 1, and nothing changed, where they do not fit
     (``cobra_cache_trim``).
     """
+    got = _lib.host().cache_trim(lens, keep_lens, block_table, free_list, free_count, block_size)
+    if got is not None:
+        return got
     B = _tables(lens, block_table, free_list, free_count)
     _i32(keep_lens, (B,), "keep_lens")
     dev = lens.device
@@ -607,6 +613,8 @@ def cache_append(
     and the block's earlier codes are rounded again.  NaN is stored as 0, an infinity as the
     largest code.
     """
+    if _lib.host().cache_append(qkv, slots, heads, head_dim, k, v, k_scale, v_scale):
+        return
     cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
     if qkv.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
@@ -648,6 +656,10 @@ def cache_attn(
     ``max_new`` and ``max_len``, the most new tokens and keys of a request (defaults: what T and
     the table allow), shape the launch, not the result.
     """
+    got = _lib.host().cache_attn(q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, causal,
+                                 max_new, max_len, out)
+    if got is not None:
+        return got
     cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
@@ -661,6 +673,7 @@ def cache_attn(
     _i32(block_table, (B, block_table.shape[1]), "block_table")
     if scale <= 0:
         raise ValueError(f"scale must be positive, got {scale}")
+    scale = float(scale)
     dev = q.device
     _same_dev(dev, q=q, cu=cu, lens=lens, block_table=block_table, k=k, v=v, k_scale=k_scale, v_scale=v_scale)
     W = block_table.shape[1]

@@ -199,7 +199,6 @@ __global__ __launch_bounds__(kThreads) void cache_trim_kernel(CacheTrimArgs a) {
 
 // -- append ---------------------------------------------------------------------------
 
-constexpr int kAppendThreads = 256;
 constexpr int kMaxBlock = 128;
 constexpr int kScaleMin = -40, kScaleMax = 40;  // exponents of the scales
 
@@ -261,68 +260,93 @@ __device__ __forceinline__ float finite_abs(float x) {
   return y < __builtin_huge_valf() ? y : 0.f;  // NaN compares false
 }
 
-__device__ __forceinline__ float block_max(float v, float* red) {
+// Largest value over the workgroup's NT threads.
+template <int NT>
+__device__ __forceinline__ float group_max(float v, float* red) {
+  v = fmaxf(v, dpp_f32<0xB1>(v));
+  v = fmaxf(v, dpp_f32<0x4E>(v));
+  v = fmaxf(v, dpp_f32<0x141>(v));
+  v = fmaxf(v, dpp_f32<0x140>(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  if constexpr (NT > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float m = red[0];
-#pragma unroll
-  for (int w = 1; w < kAppendThreads / 64; ++w) m = fmaxf(m, red[w]);
-  __syncthreads();
-  return m;
+    for (int w = 0; w < NT / 64; ++w) v = fmaxf(v, red[w]);
+    __syncthreads();
+  }
+  return v;
 }
 
 // One workgroup writes what a call brings to one (block, head).  It belongs to the block's
-// first token in the call (tokens of a block stand next to each other in the call); the others
-// pass.  A workgroup looks at `window` tokens for first ones.  Where a run writes offset 0 the
-// block starts anew: its scales come from this call's tokens alone.
-template <typename T, int CACHE>
-__global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs a, int window) {
+// first token in the call (tokens of a block stand next to each other in the call).  A
+// workgroup looks for first ones among `window` (<= 63) tokens, one a lane.  Where a run writes
+// offset 0 the block starts anew: its scales come from this call's tokens alone.
+//
+// The values are read twice, for the largest and for the codes; the second time they come from
+// the caches.  K's rows are written eight codes to a store.  V's rows run along tokens: a thread
+// takes 4 tokens x 8 dimensions and writes eight words of 4 codes, neighbouring lanes
+// neighbouring words of a row.
+template <typename T, int CACHE, int NT>
+__global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window) {
   __shared__ int src[kMaxBlock];  // token of each offset of the block, -1: none
-  __shared__ float red[kAppendThreads / 64];
-  __shared__ int stop, lowest, highest;
-  const int tid = threadIdx.x, head = blockIdx.y;
-  const int bs = 1 << a.shift, hd = a.head_dim, hdp = a.width;
+  __shared__ float red[2][NT / 64];
+  __shared__ int range[2];
+  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
+  const int bs = 1 << a.shift, hd = a.head_dim, hdp = a.width, pieces = hd >> 3, wide = hdp >> 3;
   const int64_t slots_end = a.num_blocks << a.shift;
-  const int64_t t_end = min((int64_t)(blockIdx.x + 1) * window, a.tokens);
-  for (int64_t t0 = (int64_t)blockIdx.x * window; t0 < t_end; ++t0) {
-    const int64_t slot = a.slots[t0];
-    if (slot < 0 || slot >= slots_end) continue;
-    const int64_t blk = slot >> a.shift;
-    if (t0 > 0 && (a.slots[t0 - 1] >> a.shift) == blk) continue;
+  const int64_t w0 = (int64_t)blockIdx.x * window;
+  // Lane i has the slot of token w0 - 1 + i.
+  int64_t slot = -1;
+  {
+    const int64_t t = w0 - 1 + lane;
+    if (lane <= window && t >= 0 && t < a.tokens) slot = a.slots[t];
+  }
+  const int64_t before = __shfl_up(slot, 1);
+  uint64_t firsts = __ballot(lane >= 1 && lane <= window && slot >= 0 && slot < slots_end &&
+                             (before < 0 || (before >> a.shift) != (slot >> a.shift)));
+  while (firsts) {
+    const int f = __builtin_ctzll(firsts);
+    firsts &= firsts - 1;
+    const int64_t t0 = w0 - 1 + f, blk = __shfl(slot, f) >> a.shift;
+    const int64_t bh = blk * a.kv_heads + head;
+    const float least = pow2(kScaleMin), most = pow2(kScaleMax);
+    const float k0 = fminf(fmaxf(a.k_scale[bh], least), most), v0 = fminf(fmaxf(a.v_scale[bh], least), most);
     // The run of tokens that go to this block; of two for one slot the later one stays.
     __syncthreads();
-    if (tid < bs) src[tid] = -1;
-    if (tid == 0) {
-      lowest = bs;
-      highest = -1;
-    }
-    for (int64_t c = t0;; c += kAppendThreads) {
-      __syncthreads();
-      if (tid == 0) stop = kAppendThreads;
-      __syncthreads();
-      const int64_t t = c + tid;
-      int64_t s = -1;
-      if (t < a.tokens) s = a.slots[t];
-      const bool mine = s >= 0 && (s >> a.shift) == blk;
-      if (!mine) atomicMin(&stop, tid);
-      __syncthreads();
-      if (tid < stop) {
-        const int off = (int)(s & (bs - 1));
-        atomicMax(&src[off], (int)t);
-        atomicMin(&lowest, off);
-        atomicMax(&highest, off);
+    for (int o = tid; o < bs; o += NT) src[o] = -1;
+    __syncthreads();
+    if (tid < 64) {
+      int lo = bs, hi = -1;
+      for (int64_t c = t0;; c += 64) {
+        const int64_t t = c + lane;
+        const int64_t s = t < a.tokens ? a.slots[t] : -1;
+        const uint64_t other = __ballot(s < 0 || (s >> a.shift) != blk);
+        if (lane < (other ? __builtin_ctzll(other) : 64)) {
+          const int off = (int)(s & (bs - 1));
+          atomicMax(&src[off], (int)t);
+          lo = min(lo, off);
+          hi = max(hi, off);
+        }
+        if (other) break;
       }
-      if (stop < kAppendThreads) break;
+#pragma unroll
+      for (int x = 32; x; x >>= 1) {
+        lo = min(lo, __shfl_xor(lo, x));
+        hi = max(hi, __shfl_xor(hi, x));
+      }
+      if (lane == 0) {
+        range[0] = lo;
+        range[1] = hi;
+      }
     }
     __syncthreads();
-    const int lo = lowest, hi = highest;
+    const int lo = range[0], hi = range[1];
     const T* kq = static_cast<const T*>(a.qkv) + (int64_t)(a.heads + head) * hd;
     const T* vq = kq + (int64_t)a.kv_heads * hd;
-    const int pieces = hd / 8;
     float ka = 0.f, va = 0.f;
-    for (int i = lo * pieces + tid; i < (hi + 1) * pieces; i += kAppendThreads) {
+    for (int i = lo * pieces + tid; i < (hi + 1) * pieces; i += NT) {
       const int off = i / pieces, p = i - off * pieces, t = src[off];
       if (t < 0) continue;
       float x[8], y[8];
@@ -334,15 +358,12 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
         va = fmaxf(va, finite_abs(y[e]));
       }
     }
-    ka = block_max(ka, red);
-    va = block_max(va, red);
-    const int64_t bh = blk * a.kv_heads + head;
+    ka = group_max<NT>(ka, red[0]);
+    va = group_max<NT>(va, red[1]);
     float ks = pow2(scale_exponent<CACHE>(ka)), vs = pow2(scale_exponent<CACHE>(va));
     float kr = 1.f, vr = 1.f;
     bool kgrow = false, vgrow = false;
     if (lo > 0) {
-      const float least = pow2(kScaleMin), most = pow2(kScaleMax);
-      const float k0 = fminf(fmaxf(a.k_scale[bh], least), most), v0 = fminf(fmaxf(a.v_scale[bh], least), most);
       kgrow = ks > k0;
       vgrow = vs > v0;
       kr = kgrow ? k0 / ks : 1.f;
@@ -350,16 +371,13 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
       ks = fmaxf(ks, k0);
       vs = fmaxf(vs, v0);
     }
-    __syncthreads();  // every thread has read the old scales
-    if (tid == 0) {
+    if (tid == 0) {  // every thread has read the old ones: there was a barrier since
       a.k_scale[bh] = ks;
       a.v_scale[bh] = vs;
     }
     const float ki = 1.f / ks, vi = 1.f / vs;
-    // K: rows of hdp codes, eight to a store.
     uint8_t* kc = static_cast<uint8_t*>(a.k) + bh * bs * hdp;
-    const int wide = hdp / 8;
-    for (int i = (kgrow ? 0 : lo) * wide + tid; i < (hi + 1) * wide; i += kAppendThreads) {
+    for (int i = (kgrow ? 0 : lo) * wide + tid; i < (hi + 1) * wide; i += NT) {
       const int off = i / wide, p = i - off * wide, t = src[off];
       uint2* to = reinterpret_cast<uint2*>(kc + (int64_t)i * 8);
       uint2 w = {0u, 0u};
@@ -379,39 +397,64 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
       }
       *to = w;
     }
-    // V: rows of bs codes, one for each dimension, four to a store.
     uint8_t* vc = static_cast<uint8_t*>(a.v) + bh * bs * hdp;
-    const int q0 = (vgrow ? 0 : lo) >> 2, q1 = (hi >> 2) + 1, quads = q1 - q0;
-    for (int i = tid; i < quads * hdp; i += kAppendThreads) {
-      const int d = i / quads, q = q0 + (i - d * quads);
-      uint32_t* to = reinterpret_cast<uint32_t*>(vc + d * bs + 4 * q);
-      uint32_t put = 0, w = 0;  // bytes to replace, and with what
-      bool old = false;
+    const int q0 = (vgrow ? 0 : lo) >> 2, quads = (hi >> 2) + 1 - q0;
+    for (int i = tid; i < quads * wide; i += NT) {
+      const int p = i / quads, q = q0 + (i - p * quads);
+      uint8_t* to = vc + (int64_t)p * 8 * bs + 4 * q;
+      uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+      uint32_t put = 0, old = 0;  // bytes of new codes, of codes to round again
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int off = 4 * q + j, t = src[off];
+        const int t = src[4 * q + j];
         if (t >= 0) {
           put |= 0xffu << (8 * j);
-          if (d < hd) w |= quant1<CACHE>((float)vq[t * a.ld + d] * vi) << (8 * j);
-        } else if (vgrow && off < lo) {
-          put |= 0xffu << (8 * j);
-          old = true;
-        }
-      }
-      if (!put) continue;
-      if (put != 0xffffffffu || old) {
-        const uint32_t had = *to;
-        if (old) {
-          const uint32_t g = regrade<CACHE>(had, vr);
+          if (p < pieces) {
+            float x[8];
+            load8(vq + t * a.ld + 8 * p, x);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (src[4 * q + j] < 0 && 4 * q + j < lo) w |= g & (0xffu << (8 * j));
+            for (int e = 0; e < 8; e += 2) {
+              const uint32_t c = quant2<CACHE>(x[e] * vi, x[e + 1] * vi);
+              w[e] |= (c & 0xffu) << (8 * j);
+              w[e + 1] |= (c >> 8) << (8 * j);
+            }
+          }
+        } else if (vgrow && 4 * q + j < lo) {
+          old |= 0xffu << (8 * j);
         }
-        w = (w & put) | (had & ~put);
       }
-      *to = w;
+      if (put == 0xffffffffu) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint32_t*>(to + e * bs) = w[e];
+      } else if (old) {
+        uint32_t had[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) had[e] = *reinterpret_cast<const uint32_t*>(to + e * bs);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint32_t*>(to + e * bs) =
+              (w[e] & put) | (regrade<CACHE>(had[e], vr) & old) | (had[e] & ~(put | old));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (put >> (8 * j) & 1u) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e * bs + j] = (uint8_t)(w[e] >> (8 * j));
+          }
+      }
     }
   }
+}
+
+template <typename T, int CACHE>
+void launch_append(const CacheAppendArgs& a, hipStream_t stream) {
+  // Few tokens: a wave for each.  Many: they are prompts, whose blocks begin every bs tokens.
+  const int window = a.tokens * a.kv_heads <= 8192 ? 1 : 16;
+  const dim3 grid((unsigned)((a.tokens + window - 1) / window), (unsigned)a.kv_heads);
+  if (window == 1 || (a.head_dim << a.shift) <= 4096)
+    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 64>), grid, dim3(64), 0, stream, a, window);
+  else
+    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 256>), grid, dim3(256), 0, stream, a, window);
 }
 
 }  // namespace
@@ -448,19 +491,10 @@ hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream) {
 
 hipError_t run_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
   if (a.tokens <= 0 || a.tokens > 0x7fffffff || a.kv_heads > 65535) return hipErrorInvalidValue;
-  // Few tokens: a workgroup for each.  Many: they are prompts, whose blocks begin every bs
-  // tokens, and a workgroup looks through 16 tokens for beginnings.
-  const int window = a.tokens * a.kv_heads <= 8192 ? 1 : 16;
-  const dim3 grid((unsigned)((a.tokens + window - 1) / window), (unsigned)a.kv_heads);
-  const bool f16in = a.dtype == kF16, e4m3 = a.cache == kCacheE4M3;
-  if (f16in && e4m3)
-    hipLaunchKernelGGL((cache_append_kernel<f16, kCacheE4M3>), grid, dim3(kAppendThreads), 0, stream, a, window);
-  else if (f16in)
-    hipLaunchKernelGGL((cache_append_kernel<f16, kCacheI8>), grid, dim3(kAppendThreads), 0, stream, a, window);
-  else if (e4m3)
-    hipLaunchKernelGGL((cache_append_kernel<bf16, kCacheE4M3>), grid, dim3(kAppendThreads), 0, stream, a, window);
+  if (a.dtype == kF16)
+    a.cache == kCacheE4M3 ? launch_append<f16, kCacheE4M3>(a, stream) : launch_append<f16, kCacheI8>(a, stream);
   else
-    hipLaunchKernelGGL((cache_append_kernel<bf16, kCacheI8>), grid, dim3(kAppendThreads), 0, stream, a, window);
+    a.cache == kCacheE4M3 ? launch_append<bf16, kCacheE4M3>(a, stream) : launch_append<bf16, kCacheI8>(a, stream);
   return hipGetLastError();
 }
 

@@ -5,13 +5,15 @@
 // over j <= L - n + i (causal) or j < L, with codes kc, vc and one scale for each block and head.
 //
 // In one pass over the keys, with running values for each row (log2 units):
-//   u_j = (q . kc_j) sk(j) scale log2(e) + log2 sv(j),   M = max u,   w_j = 2^(u_j - M + 14)
+//   u_j = (q . kc_j) sk(j) scale log2(e) + log2 sv(j),   w_j = 2^(u_j - M + 8)
 //   O = sum w_j vc_j,   l = sum w_j / sv(j),   o = O / l
 // so that V's scales ride in the exponent the softmax computes anyway, and the P.V product
-// runs on plain codes.  w lies in [0, 2^14] and is rounded to fp16 for that product (11 bits,
-// and 2^-28 of the largest before fp16's subnormals) whatever the activations' type: codes
-// are exact in fp16.  Scores, M, l and O are fp32.  Scales lie in [2^-40, 2^40], so no w that
-// counts underflows and neither sum overflows.
+// runs on plain codes.  M is a maximum of u that moves only when a tile has a w near fp16's
+// largest number: most tiles need no maximum, no exchange between lanes and no rescaling of O.
+// w is rounded to fp16 for the product (11 bits; 2^-22 of the reference's before subnormals)
+// whatever the activations' type: codes are exact in fp16.
+// Scores, M, l and O are fp32.  Scales are taken within [2^-40, 2^40], so no w that counts
+// underflows and neither sum overflows.
 //
 // Tiles are 64 keys and 16 rows (v_mfma_f32_16x16x32): S^T = K Q^T, then O^T = V^T P^T.  Row r
 // of K's subtile s is key 16 (r / 4) + 4 s + r % 4, which leaves the scores of keys
@@ -27,7 +29,8 @@ namespace cobra {
 namespace {
 
 constexpr int kTile = 64;
-constexpr float kBias = 14.f;  // log2 of the largest w
+constexpr float kBias = 8.f;         // log2 of w where u equals its reference
+constexpr float kAccept = 57344.f;   // a lane's sum of w that is taken without a maximum
 
 __device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -177,6 +180,22 @@ struct Rows {
     }
   }
 
+  // w = 2^(s skc + shift) of a lane's 16 keys, rounded to fp16 in p, and their sum (not rounded: a
+  // key whose V scale is far below the row's largest has a w that fp16 has no bits for, and
+  // counts in l all the same).
+  static __device__ __forceinline__ float weigh(const f32x4 (&s)[4], float skc, float shift, f16x8 (&p)[2]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], skc, shift));
+      const float y = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], skc, shift));
+      p[e >> 3][e & 7] = (f16)x;
+      p[e >> 3][(e & 7) + 1] = (f16)y;
+      sum += x + y;
+    }
+    return sum;
+  }
+
   // Tiles t0, t0 + step, .. below t_end; keys from `full` on are checked against each row's limit.
   __device__ __forceinline__ void pass(const Args& a, const Request& rq, int b, int h, int t0, int t_end, int step,
                                        int full) {
@@ -256,7 +275,7 @@ struct Rows {
         }
       }
       const bool bad = bad_next;
-      const float skc = sk * a.c2, svc = fminf(fmaxf(sv, 0x1p-40f), 0x1p40f);
+      const float skc = fminf(fmaxf(sk, 0x1p-40f), 0x1p40f) * a.c2, svc = fminf(fmaxf(sv, 0x1p-40f), 0x1p40f);
       const float ev = __builtin_amdgcn_logf(svc), inv = 1.f / svc;
       // The next tile's keys and scales while this one's softmax runs.
       if (more) {
@@ -273,40 +292,37 @@ struct Rows {
       f16x8 p[NR][2];
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        float u[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[4 * i + e] = fmaf(s[r][i][e], skc, ev);
-        if (slow) {
-          const int seen = bad ? 0 : lim[r] - key0;  // keys of this lane that count
-#pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = e < seen ? u[e] : kNegInf;
+        // Against the reference that the row has, without a maximum of this tile: right as long
+        // as every w stays inside fp16, which a sum at most kAccept of a lane's 16 w shows.
+        float shift = ev + kBias - m[r], sum;
+        bool ok = false;
+        if (!slow) {
+          sum = weigh(s[r], skc, shift, p[r]);
+          ok = sum <= kAccept;  // false for NaN, and where the row has no reference yet
         }
-        float mx = u[0];
+        if (!__all(ok)) {
+          const int seen = bad ? 0 : slow ? lim[r] - key0 : 16;  // keys of this lane that count
+          float mx = kNegInf;
 #pragma unroll
-        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, u[e]);
-        {
+          for (int e = 0; e < 16; ++e) {
+            const float u = fmaf(s[r][e >> 2][e & 3], skc, ev);
+            s[r][e >> 2][e & 3] = e < seen ? s[r][e >> 2][e & 3] : kNegInf;
+            mx = fmaxf(mx, e < seen ? u : kNegInf);
+          }
           const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
           mx = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+          const float mn = fmaxf(m[r], mx);
+          const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn);
+          m[r] = mn;
+          shift = mn == kNegInf ? kNegInf : ev + kBias - mn;
+          sum = weigh(s[r], skc, shift, p[r]);
+          l[r] *= alpha;
+#pragma unroll
+          for (int t = 0; t < kDims; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
         }
-        const float mn = fmaxf(m[r], mx);
-        const float base = mn == kNegInf ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
-        m[r] = mn;
-        const float shift = kBias - base;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float w = __builtin_amdgcn_exp2f(u[e] + shift);
-          sum += w;
-          p[r][e >> 3][e & 7] = (f16)w;
-        }
-        l[r] = l[r] * alpha + sum * inv;
-#pragma unroll
-        for (int t = 0; t < kDims; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
+        l[r] = fmaf(sum, inv, l[r]);
       }
       if (slow) {
         // Memory past the request's end, or of a block that is none, may hold NaN codes.
@@ -373,12 +389,11 @@ struct Rows {
 // Few rows for each kv head: a workgroup has 16 of them and one split of the keys, its waves
 // every kWaves-th tile of it; their shares are joined through LDS, the splits' by
 // cache_join_kernel.
-template <typename T, int CACHE, int HDP>
-__global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
-  constexpr int kWaves = 4;
+template <typename T, int CACHE, int HDP, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void cache_decode_kernel(Args a) {
   typedef Rows<T, CACHE, HDP, 1> R;
-  __shared__ f32x4 sh_o[2][R::kDims][64];
-  __shared__ float sh_m[2][64], sh_l[2][64];
+  __shared__ f32x4 sh_o[kWaves / 2][R::kDims][64];
+  __shared__ float sh_m[kWaves / 2][64], sh_l[kWaves / 2][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   int id = blockIdx.x;
   const int h = id % a.kv_heads;
@@ -405,9 +420,9 @@ __global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
     const int64_t k1 = min((int64_t)end, k0 + chunk);
     w.pass(a, rq, b, h, (int)(k0 / kTile) + wave, (int)((k1 + kTile - 1) / kTile), kWaves, full);
     w.total_l();
-    // Waves 2, 3 into 0, 1, then 1 into 0.
+    // The upper half of the waves into the lower, until one is left.
 #pragma unroll
-    for (int half = 2; half; half >>= 1) {
+    for (int half = kWaves / 2; half; half >>= 1) {
       __syncthreads();
       if (wave >= half && wave < 2 * half) {
         sh_m[wave - half][lane] = w.m[0];
@@ -431,11 +446,14 @@ __global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
   }
 }
 
-// The splits of a row joined: o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s, in order of s.
-template <typename T, int HDP>
+// The splits of a row joined: o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s, always in the same
+// order.  W waves have a row; a wave takes as many splits at a time as it has lanes for.
+template <typename T, int HDP, int W>
 __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kLanes = HDP / 4, kAt = 64 / kLanes;  // lanes of a split, splits of a wave
+  __shared__ f32x4 sh[W > 1 ? W : 1][kLanes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = W > 1 ? wave : 0;
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t rows = (int64_t)a.tokens * a.heads;
   if (row >= rows) return;
   const int t = (int)(row / a.heads);
@@ -453,25 +471,48 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
   if (chunk >= rq.len) return;  // written by the workgroup that had all of it
   const int n = (int)(((int64_t)rq.len + chunk - 1) / chunk);
   float m = kNegInf;
-  for (int s = 0; s < n; ++s) m = fmaxf(m, a.part_m[s * rows + row].x);
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, a.part_m[s * rows + row].x);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
   const float base = m == kNegInf ? 0.f : m;
-  constexpr int kPer = (HDP + 63) / 64;
-  float o[kPer], l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int s = 0; s < n; ++s) {
+  float l = 0.f;
+  for (int s = lane; s < n; s += 64) {
     const float2 ml = a.part_m[s * rows + row];
-    const float f = __builtin_amdgcn_exp2f(ml.x - base);
-    l += f * ml.y;
+    l += __builtin_amdgcn_exp2f(ml.x - base) * ml.y;
+  }
+  l = group_sum<64>(l);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4;
+  if (sub < kAt) {
+#pragma unroll 4
+    for (int s = part * kAt + sub; s < n; s += W * kAt) {
+      const float f = __builtin_amdgcn_exp2f(a.part_m[s * rows + row].x - base);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + 64 * i < HDP) o[i] += f * a.part_o[(s * rows + row) * HDP + lane + 64 * i];
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) v += __shfl(o[i], lane % kLanes + k * kLanes);
+    o[i] = v;
+  }
+  if constexpr (W > 1) {
+    if (lane < kLanes) sh[part][lane] = o;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w)
+      if (lane < kLanes) o += sh[w][lane];
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (lane < kLanes && d < a.head_dim) {
+    typename Op16<T>::V4 y;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int d = lane + 64 * i;
-    if (d < a.head_dim) static_cast<T*>(a.out)[row * a.head_dim + d] = (T)(o[i] * inv);
+    for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+    *reinterpret_cast<typename Op16<T>::V4*>(static_cast<T*>(a.out) + row * a.head_dim + d) = y;
   }
 }
 
@@ -506,23 +547,25 @@ __global__ __launch_bounds__(256) void cache_chunk_kernel(Args a) {
   }
 }
 
-constexpr int kStep = 4 * kTile;  // keys that a decode workgroup takes at a time
-
 struct Plan {
   bool chunked;
-  int splits, chunk;
+  int waves, splits, chunk;
   int64_t row_tiles;
 };
 
+#include <stdlib.h>
+static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
 // How a call is cut.  max_new and max_len are expectations; a call that exceeds them is still
 // covered (rows in a loop, longer splits).
-Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_new, int64_t max_len) {
+Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
+             int64_t max_len) {
   Plan p{};
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
   max_len = max_len < 1 ? 1 : max_len > 0x7fffff00 ? 0x7fffff00 : max_len;
   const int64_t group = heads / kv_heads, rows = max_new * group;
   p.chunked = rows > 64;
   p.splits = 1;
+  p.waves = 4;
   if (p.chunked) {
     p.row_tiles = (rows + 127) / 128;
     p.chunk = 0x40000000;
@@ -530,13 +573,17 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   }
   p.row_tiles = (rows + 15) / 16;
   const int64_t base = batch * kv_heads * p.row_tiles;
-  int64_t splits = (2048 + base - 1) / base;
-  const int64_t most = (max_len + kStep - 1) / kStep;
+  static const int target = tune("CT", 2048), wv = tune("CW", 4), one = tune("CO", 0);
+  p.waves = head_dim <= 128 ? wv : 4;
+  const int64_t step = p.waves * kTile;
+  int64_t splits = (target + base - 1) / base;
+  const int64_t most = (max_len + step - 1) / step;
   splits = splits < most ? splits : most;
   splits = splits < 1 ? 1 : splits > 1024 ? 1024 : splits;
+  if (max_len <= one) splits = 1;
   const int64_t even = (max_len + splits - 1) / splits;
-  int64_t chunk = (even + kStep - 1) / kStep * kStep;
-  if (chunk < kStep) chunk = kStep;
+  int64_t chunk = (even + step - 1) / step * step;
+  if (chunk < step) chunk = step;
   p.splits = (int)((max_len + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
   p.chunk = (int)chunk;
@@ -554,10 +601,18 @@ hipError_t launch(const Args& a, const Plan& p, hipStream_t stream) {
   }
   const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles * p.splits;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  if (p.waves == 8 && HDP <= 128)
+    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP <= 128 ? HDP : 128, 8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP, 4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)a.tokens * a.heads;
-    hipLaunchKernelGGL((cache_join_kernel<T, HDP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, kStep);
+    static const int jw = tune("CJ", 16);
+    if (p.splits > jw)
+      hipLaunchKernelGGL((cache_join_kernel<T, HDP, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, p.waves * kTile);
+    else
+      hipLaunchKernelGGL((cache_join_kernel<T, HDP, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a,
+                         p.waves * kTile);
   }
   return hipGetLastError();
 }
@@ -579,7 +634,7 @@ hipError_t launch_width(const Args& a, const Plan& p, int width, hipStream_t str
 
 int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t max_new, int64_t max_len) {
-  const Plan p = plan_of(tokens, batch, heads, kv_heads, max_new, max_len);
+  const Plan p = plan_of(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
   if (p.splits <= 1) return 0;
   return (int64_t)p.splits * tokens * heads * (cache_width(head_dim) * 4 + 8);
 }
@@ -587,7 +642,7 @@ int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads,
 hipError_t run_cache_attn(const CacheAttnArgs& c, int64_t workspace_bytes, hipStream_t stream) {
   const int width = cache_width(c.head_dim);
   if (width < 0 || c.tokens <= 0 || c.tokens > 0x7fffffff || c.batch <= 0 || c.table_width <= 0) return hipErrorInvalidValue;
-  const Plan p = plan_of(c.tokens, c.batch, c.heads, c.kv_heads, c.max_new, c.max_len);
+  const Plan p = plan_of(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.max_new, c.max_len);
   Args a{};
   a.q = c.q;
   a.out = c.out;

@@ -1,5 +1,6 @@
-// Native steady-state calls of CobraAttentionSublayer.forward (cobra_amd/layer.py) and
-// of CobraTransformer.forward in its one-kernel-per-block mode (cobra_amd/model.py).
+// Native steady-state calls of CobraAttentionSublayer.forward (cobra_amd/layer.py),
+// of CobraTransformer.forward in its one-kernel-per-block mode (cobra_amd/model.py) and
+// of the key/value cache's operators (cobra_amd/ops.py).
 //
 // At the small shapes one sublayer forward is a single ~7 us kernel, and the Python
 // around its launch (signature and parameter-version checks, the output allocation,
@@ -10,6 +11,7 @@
 // caching allocator, launches on the device's current stream and returns y; for any
 // other call it returns None and the module takes its general path.  It never
 // computes anything itself: the launch is the library's (libcobra_amd.so).
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/EmptyTensor.h>
@@ -189,9 +191,241 @@ class BoundStack {
   py::object on_error_;
 };
 
+// -- key/value cache ------------------------------------------------------------------
+//
+// The calls of cobra_amd/ops.py's cache_* functions in C++: a decode step's kernels take a few
+// microseconds each, about what the checks and allocations of one call take in Python.  Same
+// contract as above: a call whose tensors are all as they should be, on the current device, is
+// made here; for any other these return None, and Python's own checks name what is wrong (or
+// make the call on another device).  Arguments come by position (the vector-call protocol);
+// what is not of the expected Python type makes a call "any other" too.
+
+bool py_int(PyObject* o, int64_t* v) {
+  if (!PyLong_Check(o)) return false;
+  *v = PyLong_AsLongLong(o);
+  if (*v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+// A dense tensor on device `dev` of type `dt`, or null.
+const at::Tensor* dev_tensor(PyObject* o, int dev, at::ScalarType dt) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.device().index() != dev || t.scalar_type() != dt || !t.is_contiguous()) return nullptr;
+  return &t;
+}
+
+bool shape_is(const at::Tensor* t, std::initializer_list<int64_t> want) {
+  return t && t->sizes() == at::IntArrayRef(want);
+}
+
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, dt, dev, c10::nullopt);
+}
+
+// The current device, if it is a tensor's.
+int device_of(PyObject* o) {
+  if (!THPVariable_Check(o)) return -1;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda()) return -1;
+  const int dev = t.device().index();
+  return dev == c10::hip::current_device() ? dev : -1;
+}
+
+// A failed call: None, so that the general path makes it again and raises the library's error.
+PyObject* none() { Py_RETURN_NONE; }
+
+template <typename F>
+PyObject* guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+struct Tables {
+  const at::Tensor *lens, *change, *table, *free_list, *count;
+  int64_t batch, block;
+  int dev;
+  bool read(PyObject* const* a) {
+    dev = device_of(a[0]);
+    if (dev < 0) return false;
+    lens = dev_tensor(a[0], dev, at::kInt);
+    change = dev_tensor(a[1], dev, at::kInt);
+    table = dev_tensor(a[2], dev, at::kInt);
+    free_list = dev_tensor(a[3], dev, at::kInt);
+    count = dev_tensor(a[4], dev, at::kInt);
+    if (!lens || lens->dim() != 1 || !table || table->dim() != 2 || !free_list || free_list->dim() != 1) return false;
+    batch = lens->size(0);
+    return batch > 0 && shape_is(change, {batch}) && table->size(0) == batch && shape_is(count, {1}) &&
+           py_int(a[5], &block);
+  }
+};
+
+// (lens, new_lens, block_table, free_list, free_count, block_size, tokens) -> (slots, cu, missing) | None
+PyObject* cache_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Tables t;
+    int64_t tokens;
+    if (n != 7 || !t.read(a) || !py_int(a[6], &tokens) || tokens < 0) return none();
+    const at::Device dev = t.lens->device();
+    at::Tensor slots = new_tensor({tokens}, at::kLong, dev), cu = new_tensor({t.batch + 1}, at::kInt, dev);
+    at::Tensor missing = new_tensor({1}, at::kInt, dev), ws = new_tensor({t.batch + 1}, at::kInt, dev);
+    const int code = cobra_cache_reserve(
+        t.lens->data_ptr<int>(), t.change->data_ptr<int>(), t.table->data_ptr<int>(), t.table->size(1),
+        t.free_list->data_ptr<int>(), t.free_list->size(0), t.count->data_ptr<int>(), slots.data_ptr<int64_t>(), tokens,
+        cu.data_ptr<int>(), missing.data_ptr<int>(), ws.data_ptr<int>(), t.batch, t.block,
+        c10::hip::getCurrentHIPStream(t.dev).stream());
+    if (code != 0) return none();
+    PyObject* got = PyTuple_New(3);
+    if (!got) return nullptr;
+    PyTuple_SET_ITEM(got, 0, THPVariable_Wrap(std::move(slots)));
+    PyTuple_SET_ITEM(got, 1, THPVariable_Wrap(std::move(cu)));
+    PyTuple_SET_ITEM(got, 2, THPVariable_Wrap(std::move(missing)));
+    return got;
+  });
+}
+
+// (lens, keep_lens, block_table, free_list, free_count, block_size) -> refused | None
+PyObject* cache_trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Tables t;
+    if (n != 6 || !t.read(a)) return none();
+    const at::Device dev = t.lens->device();
+    at::Tensor refused = new_tensor({1}, at::kInt, dev), ws = new_tensor({t.batch}, at::kInt, dev);
+    const int code = cobra_cache_trim(t.lens->data_ptr<int>(), t.change->data_ptr<int>(), t.table->data_ptr<int>(),
+                                      t.table->size(1), t.free_list->data_ptr<int>(), t.free_list->size(0),
+                                      t.count->data_ptr<int>(), refused.data_ptr<int>(), ws.data_ptr<int>(), t.batch,
+                                      t.block, c10::hip::getCurrentHIPStream(t.dev).stream());
+    if (code != 0) return none();
+    return THPVariable_Wrap(std::move(refused));
+  });
+}
+
+struct Pool {
+  const at::Tensor *k, *v, *k_scale, *v_scale;
+  int64_t blocks, kv_heads, block;
+  int cache;
+  bool read(PyObject* const* a, int dev, int64_t heads, int64_t head_dim) {
+    if (!THPVariable_Check(a[0])) return false;
+    const at::ScalarType dt = THPVariable_Unpack(a[0]).scalar_type();
+    if (dt != at::kFloat8_e4m3fn && dt != at::kChar) return false;
+    cache = dt == at::kChar ? COBRA_CACHE_I8 : COBRA_CACHE_E4M3;
+    k = dev_tensor(a[0], dev, dt);
+    v = dev_tensor(a[1], dev, dt);
+    k_scale = dev_tensor(a[2], dev, at::kFloat);
+    v_scale = dev_tensor(a[3], dev, at::kFloat);
+    if (!k || k->dim() != 4) return false;
+    blocks = k->size(0);
+    kv_heads = k->size(1);
+    block = k->size(2);
+    const int64_t width = k->size(3);
+    return width == cobra_cache_width(head_dim) && shape_is(v, {blocks, kv_heads, width, block}) &&
+           shape_is(k_scale, {blocks, kv_heads}) && shape_is(v_scale, {blocks, kv_heads}) && kv_heads > 0 &&
+           heads > 0 && heads % kv_heads == 0;
+  }
+};
+
+// 16-bit activations on the current device, or null; dt: the C ABI's code.
+const at::Tensor* rows16(PyObject* o, int* dt) {
+  const int dev = device_of(o);
+  if (dev < 0) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.dim() != 2 || !t.is_contiguous()) return nullptr;
+  if (t.scalar_type() == at::kHalf)
+    *dt = COBRA_F16;
+  else if (t.scalar_type() == at::kBFloat16)
+    *dt = COBRA_BF16;
+  else
+    return nullptr;
+  return &t;
+}
+
+// (qkv, slots, heads, head_dim, k, v, k_scale, v_scale) -> True | None
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int dt;
+    int64_t heads, hd;
+    const at::Tensor* x = n == 8 ? rows16(a[0], &dt) : nullptr;
+    if (!x || !py_int(a[2], &heads) || !py_int(a[3], &hd)) return none();
+    const int dev = x->device().index();
+    const at::Tensor* slots = dev_tensor(a[1], dev, at::kLong);
+    Pool p;
+    if (!slots || !p.read(a + 4, dev, heads, hd) || !shape_is(slots, {x->size(0)}) ||
+        x->size(1) != (heads + 2 * p.kv_heads) * hd)
+      return none();
+    const int code = cobra_cache_append(x->data_ptr(), dt, x->size(1), slots->data_ptr<int64_t>(), p.k->data_ptr(),
+                                        p.v->data_ptr(), p.k_scale->data_ptr<float>(), p.v_scale->data_ptr<float>(),
+                                        p.cache, x->size(0), p.blocks, p.block, heads, p.kv_heads, hd,
+                                        c10::hip::getCurrentHIPStream(dev).stream());
+    if (code != 0) return none();
+    Py_RETURN_TRUE;
+  });
+}
+
+// (q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, causal, max_new | None,
+// max_len | None, out | None) -> ctx | None
+PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int dt;
+    int64_t heads, hd;
+    const at::Tensor* q = n == 15 ? rows16(a[0], &dt) : nullptr;
+    if (!q || !py_int(a[4], &heads) || !py_int(a[5], &hd) || !PyFloat_Check(a[6])) return none();
+    const int dev = q->device().index();
+    const at::Tensor *cu = dev_tensor(a[1], dev, at::kInt), *lens = dev_tensor(a[2], dev, at::kInt),
+                     *table = dev_tensor(a[3], dev, at::kInt);
+    Pool p;
+    if (!cu || !lens || !table || !p.read(a + 7, dev, heads, hd) || lens->dim() != 1 || table->dim() != 2) return none();
+    const int64_t T = q->size(0), B = lens->size(0), W = table->size(1);
+    if (T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) || table->size(0) != B) return none();
+    int64_t new_most = T - B + 1, len_most = W * p.block;
+    if (a[12] != Py_None && !py_int(a[12], &new_most)) return none();
+    if (a[13] != Py_None && !py_int(a[13], &len_most)) return none();
+    if (new_most < 1) new_most = 1;
+    if (len_most < 1) len_most = 1;
+    at::Tensor out;
+    if (a[14] == Py_None) {
+      out = new_tensor({T, heads * hd}, q->scalar_type(), q->device());
+    } else {
+      const at::Tensor* o = dev_tensor(a[14], dev, q->scalar_type());
+      if (!shape_is(o, {T, heads * hd})) return none();
+      out = *o;
+    }
+    const int64_t need = cobra_cache_attn_workspace_bytes(T, B, heads, p.kv_heads, hd, new_most, len_most);
+    if (need < 0) return none();
+    at::Tensor ws;
+    if (need > 0) ws = new_tensor({need}, at::kByte, q->device());
+    const int code = cobra_cache_attn_fwd(
+        q->data_ptr(), dt, q->size(1), cu->data_ptr<int>(), lens->data_ptr<int>(), table->data_ptr<int>(), W,
+        p.k->data_ptr(), p.v->data_ptr(), p.k_scale->data_ptr<float>(), p.v_scale->data_ptr<float>(), p.cache,
+        out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, T, B, p.blocks, p.block, heads, p.kv_heads, hd,
+        new_most, len_most, static_cast<float>(PyFloat_AS_DOUBLE(a[6])), PyObject_IsTrue(a[11]) == 1 ? 1 : 0,
+        c10::hip::getCurrentHIPStream(dev).stream());
+    if (code != 0) return none();
+    if (a[14] != Py_None) {
+      Py_INCREF(a[14]);
+      return a[14];
+    }
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+PyMethodDef kCacheCalls[] = {
+    {"cache_reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_reserve)), METH_FASTCALL, nullptr},
+    {"cache_trim", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_trim)), METH_FASTCALL, nullptr},
+    {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_append)), METH_FASTCALL, nullptr},
+    {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_attn)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  PyModule_AddFunctions(m.ptr(), kCacheCalls);
   m.doc() = "Native steady-state forward of the cobra_amd attention sublayer";
   py::class_<BoundForward>(m, "BoundForward")
       .def(py::init<int64_t, const at::Tensor&, std::vector<at::Tensor>, std::vector<int64_t>, py::object, double,

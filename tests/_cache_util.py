@@ -48,17 +48,17 @@ def poison(k, v, blk, first):
 def attn_tolerance(want, mag, top, reach, keys, head_dim, dtype, v_scale_max):
     """Largest |got - want| by element.
 
-    p_j = w_j / l: w_j rounded to fp16 (half a step: 2^-11 of it; under 2^-14 of the kernel's
-    units, whose largest w is 2^14, at most 2^-25), from a score in fp32.  A score is a sum of
+    p_j = w_j / l: w_j rounded to fp16 (half a step: 2^-11 of it; under 2^-14, where the row's
+    reference has 2^8, at most 2^-25), from a score in fp32.  A score is a sum of
     head_dim products: at most head_dim + 4 roundings of 2^-24 of sum |q k|; in log2 units it is
-    multiplied, has the scale's logarithm (at most 40) and the maximum taken away: 6 roundings
+    multiplied, has the scale's logarithm (at most 40) and the reference taken away: 6 roundings
     of 2^-24 of at most |score| log2(e) + 40, each; exp2 adds 2^-22.  Sums over the keys in
     fp32: keys roundings of 2^-24 each in O and l.  The result rounds once more to its type."""
     u = 2.0 ** -24
     score = (head_dim + 4) * u * reach + 6 * u * (top * math.log2(math.e) + 40 + 14) * math.log(2.0)
     rel = 2.0 ** -11 + 2 * score + 2.0 ** -21 + 2 * (keys + 8) * u
     eps = torch.finfo(dtype).eps / 2
-    return (eps * (1 + rel)) * want.abs() + rel * mag * 1.01 + keys * 2.0 ** -39 * 448 * v_scale_max + \
+    return (eps * (1 + rel)) * want.abs() + rel * mag * 1.01 + keys * 2.0 ** -33 * 448 * v_scale_max + \
         (2.0 ** -25 if dtype == torch.float16 else 0.0)
 
 
