@@ -16,8 +16,7 @@ namespace cobra {
 
 namespace {
 
-constexpr int kThreads = 1024;  // the table kernels run one workgroup
-constexpr int kWaves = kThreads / 64;
+constexpr int kInLds = 1024;  // requests whose prefix sums the table kernels keep in LDS
 
 __device__ __forceinline__ int64_t wave_incl(int64_t v, int lane) {
 #pragma unroll
@@ -28,20 +27,32 @@ __device__ __forceinline__ int64_t wave_incl(int64_t v, int lane) {
   return v;
 }
 
-// Inclusive prefix sum over the workgroup; `total` gets the sum.  red: kWaves words of LDS.
-__device__ __forceinline__ int64_t block_incl(int64_t v, int64_t* red, int64_t* total) {
+// Inclusive prefix sums of two values over the workgroup's NT threads; their totals in sx, sy.
+template <int NT>
+__device__ __forceinline__ void block_incl(int64_t& x, int64_t& y, int64_t (*red)[2], int64_t* sx, int64_t* sy) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = wave_incl(v, lane);
+  x = wave_incl(x, lane);
+  y = wave_incl(y, lane);
   __syncthreads();  // red may still be read from the call before
-  if (lane == 63) red[wave] = v;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += red[w];
-    all += red[w];
+  if (lane == 63) {
+    red[wave][0] = x;
+    red[wave][1] = y;
   }
-  *total = all;
-  return v + before;
+  __syncthreads();
+  int64_t bx = 0, by = 0, ax = 0, ay = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < wave) {
+      bx += red[w][0];
+      by += red[w][1];
+    }
+    ax += red[w][0];
+    ay += red[w][1];
+  }
+  x += bx;
+  y += by;
+  *sx = ax;
+  *sy = ay;
 }
 
 __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int shift) {
@@ -61,50 +72,52 @@ __device__ __forceinline__ int first_above(const int32_t* v, int n, int x) {
   return lo;
 }
 
-// The slots of tokens t0, t0 + step, .. and the table entries k0, k0 + step, .. of a reserve
-// whose lengths and prefix sums are final: incl[b] = new blocks of requests 0 .. b, count =
-// the free blocks before it.
-__device__ __forceinline__ void reserve_fill(const CacheReserveArgs& a, const int32_t* cu, const int32_t* incl,
-                                             int count, int64_t first, int64_t step) {
-  const int used = cu[a.batch], blocks = incl[a.batch - 1];
+// The slots of tokens first, first + step, .. and the table entries of new blocks first,
+// first + step, .. of a reserve whose sums are final: ends[b] = new tokens, incl[b] = new blocks
+// of requests 0 .. b, had[b] = tokens of request b before it, count = the free blocks before it.
+__device__ __forceinline__ void reserve_fill(const CacheReserveArgs& a, const int32_t* ends, const int32_t* incl,
+                                             const int32_t* lens, int count, int64_t first, int64_t step) {
+  const int used = ends[a.batch - 1], blocks = incl[a.batch - 1];
+#pragma unroll 4
   for (int64_t t = first; t < a.tokens; t += step) {
-    if (t >= used) {
-      a.slots[t] = -1;
-      continue;
+    int64_t slot = -1;
+    if (t < used) {
+      const int b = first_above(ends, a.batch, (int)t);
+      const int begin = b ? ends[b - 1] : 0, before = b ? incl[b - 1] : 0;
+      const int64_t held = (int64_t)lens[b] - (ends[b] - begin);
+      const int64_t pos = held + (t - begin), had = blocks_of(held, a.shift), page = pos >> a.shift;
+      const int32_t id = page < had ? a.table[b * a.width + page] : a.free_list[count - 1 - (before + (int)(page - had))];
+      slot = ((int64_t)id << a.shift) + (pos & ((1 << a.shift) - 1));
     }
-    const int b = first_above(cu + 1, a.batch, (int)t);
-    const int begin = cu[b];
-    const int64_t held = (int64_t)a.lens[b] - (cu[b + 1] - begin);
-    const int64_t pos = held + (t - begin), had = blocks_of(held, a.shift), page = pos >> a.shift;
-    const int before = b ? incl[b - 1] : 0;
-    const int32_t id = page < had ? a.table[b * a.width + page] : a.free_list[count - 1 - (before + (int)(page - had))];
-    a.slots[t] = ((int64_t)id << a.shift) + (pos & ((1 << a.shift) - 1));
+    a.slots[t] = slot;
   }
   for (int64_t k = first; k < blocks; k += step) {
     const int b = first_above(incl, a.batch, (int)k);
-    const int64_t held = (int64_t)a.lens[b] - (cu[b + 1] - cu[b]);
-    const int before = b ? incl[b - 1] : 0;
-    a.table[b * a.width + blocks_of(held, a.shift) + (k - before)] = a.free_list[count - 1 - k];
+    const int64_t held = (int64_t)lens[b] - (ends[b] - (b ? ends[b - 1] : 0));
+    a.table[b * a.width + blocks_of(held, a.shift) + (k - (b ? incl[b - 1] : 0))] = a.free_list[count - 1 - k];
   }
 }
 
 // need_b = ceil((L + n) / bs) - ceil(L / bs) blocks for request b, handed out from the top of
 // the stack of free blocks in the order of requests; all requests get theirs or none does.
-// One workgroup: the sums are over a few hundred requests, and one barrier is cheaper than a
+// One workgroup: the sums are over a few hundred requests, and a barrier is cheaper than a
 // second launch.  It also writes slots and table entries where `fill` says so.
-__global__ __launch_bounds__(kThreads) void cache_reserve_kernel(CacheReserveArgs a, int fill) {
-  __shared__ int64_t red[kWaves];
+template <int NT>
+__global__ __launch_bounds__(NT) void cache_reserve_kernel(CacheReserveArgs a, int fill) {
+  __shared__ int64_t red[NT / 64][2];
+  __shared__ int32_t s_ends[kInLds], s_incl[kInLds], s_lens[kInLds];
   __shared__ int bad;
   const int tid = threadIdx.x;
+  const bool near = a.batch <= kInLds;
   if (tid == 0) bad = 0;
   __syncthreads();
   const int count = *a.free_count;
   int64_t toks = 0, need_all = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += NT) {
     const int b = b0 + tid;
-    int64_t n = 0, need = 0;
+    int64_t n = 0, need = 0, len = 0;
     if (b < a.batch) {
-      const int64_t len = a.lens[b];
+      len = a.lens[b];
       n = a.new_lens[b];
       if (len < 0 || n < 0 || len + n > 0x7fffffff || blocks_of(len + n, a.shift) > a.width) {
         bad = 1;
@@ -113,59 +126,99 @@ __global__ __launch_bounds__(kThreads) void cache_reserve_kernel(CacheReserveArg
         need = blocks_of(len + n, a.shift) - blocks_of(len, a.shift);
       }
     }
-    int64_t ts, ns;
-    const int64_t ti = block_incl(n, red, &ts) + toks, ni = block_incl(need, red, &ns) + need_all;
+    int64_t ts, ns, ti = n, ni = need;
+    block_incl<NT>(ti, ni, red, &ts, &ns);
     if (b < a.batch) {
-      a.cu[b + 1] = (int32_t)ti;
-      a.incl[b] = (int32_t)ni;
+      a.cu[b + 1] = (int32_t)(ti + toks);
+      a.incl[b] = (int32_t)(ni + need_all);
+      if (near) {
+        s_ends[b] = (int32_t)(ti + toks);
+        s_incl[b] = (int32_t)(ni + need_all);
+        s_lens[b] = (int32_t)(len + n);
+      }
     }
     toks += ts;
     need_all += ns;
   }
-  if (tid == 0) a.cu[0] = 0;
   __syncthreads();
   int missing = 0;
   if (bad || toks > a.tokens || count < 0 || count > a.num_free)
     missing = -1;
   else if (need_all > count)
     missing = (int)(need_all - count);
-  if (missing) {
-    for (int b = tid; b < a.batch; b += kThreads) {
+  for (int b = tid; b < a.batch; b += NT) {
+    if (missing) {
       a.cu[b + 1] = 0;
       a.incl[b] = 0;
+      if (near) s_ends[b] = s_incl[b] = 0;
+    } else if (near) {
+      a.lens[b] = s_lens[b];
+    } else {
+      a.lens[b] += a.new_lens[b];
     }
-  } else {
-    for (int b = tid; b < a.batch; b += kThreads) a.lens[b] += a.new_lens[b];
   }
   if (tid == 0) {
+    a.cu[0] = 0;
     *a.missing = missing;
     a.incl[a.batch] = count;  // for the fill
     if (!missing) *a.free_count = count - (int)need_all;
   }
   if (fill) {
     __syncthreads();
-    reserve_fill(a, a.cu, a.incl, count, tid, kThreads);
+    if (near)
+      reserve_fill(a, s_ends, s_incl, s_lens, count, tid, NT);
+    else
+      reserve_fill(a, a.cu + 1, a.incl, a.lens, count, tid, NT);
   }
 }
 
+// The fill over the whole chip, where there are many tokens.
 __global__ __launch_bounds__(256) void cache_reserve_fill_kernel(CacheReserveArgs a) {
-  reserve_fill(a, a.cu, a.incl, a.incl[a.batch], (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+  __shared__ int32_t s_ends[kInLds], s_incl[kInLds], s_lens[kInLds];
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  const int count = a.incl[a.batch];
+  if (a.batch <= kInLds) {
+    for (int b = threadIdx.x; b < a.batch; b += 256) {
+      s_ends[b] = a.cu[b + 1];
+      s_incl[b] = a.incl[b];
+      s_lens[b] = a.lens[b];
+    }
+    __syncthreads();
+    reserve_fill(a, s_ends, s_incl, s_lens, count, first, step);
+  } else {
+    reserve_fill(a, a.cu + 1, a.incl, a.lens, count, first, step);
+  }
+}
+
+// The blocks first, first + step, .. that a trim gives back, to their places below `top`.
+__device__ __forceinline__ void trim_fill(const CacheTrimArgs& a, const int32_t* incl, int64_t top, int64_t first,
+                                          int64_t step) {
+  const int all = incl[a.batch - 1];
+#pragma unroll 4
+  for (int64_t k = first; k < all; k += step) {
+    const int b = first_above(incl, a.batch, (int)k);
+    const int64_t keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
+    a.free_list[top - 1 - k] = a.table[b * a.width + blocks_of(keep, a.shift) + (k - (b ? incl[b - 1] : 0))];
+  }
 }
 
 // Requests cut to min(L, max(keep, 0)) tokens; the k-th block given back (requests in order,
 // a request's blocks in order) goes k places below the new top of the stack, which undoes a
 // reserve exactly.
-__global__ __launch_bounds__(kThreads) void cache_trim_kernel(CacheTrimArgs a) {
-  __shared__ int64_t red[kWaves];
+template <int NT>
+__global__ __launch_bounds__(NT) void cache_trim_kernel(CacheTrimArgs a, int fill) {
+  __shared__ int64_t red[NT / 64][2];
+  __shared__ int32_t s_incl[kInLds];
   __shared__ int bad;
   const int tid = threadIdx.x;
+  const bool near = a.batch <= kInLds;
   if (tid == 0) bad = 0;
   __syncthreads();
   const int count = *a.free_count;
   int64_t all = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += NT) {
     const int b = b0 + tid;
-    int64_t back = 0;
+    int64_t back = 0, none = 0;
     if (b < a.batch) {
       const int64_t len = a.lens[b];
       const int64_t keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
@@ -174,27 +227,41 @@ __global__ __launch_bounds__(kThreads) void cache_trim_kernel(CacheTrimArgs a) {
       else if (keep < len)
         back = blocks_of(len, a.shift) - blocks_of(keep, a.shift);
     }
-    int64_t s;
-    const int64_t i = block_incl(back, red, &s) + all;
-    if (b < a.batch) a.incl[b] = (int32_t)(i > 0x7fffffff ? 0x7fffffff : i);
+    int64_t s, z;
+    block_incl<NT>(back, none, red, &s, &z);
+    const int64_t i = back + all;
+    if (b < a.batch) {
+      a.incl[b] = (int32_t)(i > 0x7fffffff ? 0x7fffffff : i);
+      if (near) s_incl[b] = (int32_t)(i > 0x7fffffff ? 0x7fffffff : i);
+    }
     all += s;
   }
   __syncthreads();
   const bool refused = bad || count < 0 || all + count > a.num_free;
   if (tid == 0) *a.refused = refused ? 1 : 0;
-  if (refused) return;
-  for (int64_t k = tid; k < all; k += kThreads) {
-    const int b = first_above(a.incl, a.batch, (int)k);
-    const int64_t keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
-    const int before = b ? a.incl[b - 1] : 0;
-    a.free_list[count + all - 1 - k] = a.table[b * a.width + blocks_of(keep, a.shift) + (k - before)];
+  if (refused) {
+    for (int b = tid; b < a.batch; b += NT) a.incl[b] = 0;  // for the fill
+    return;
   }
-  __syncthreads();
-  for (int b = tid; b < a.batch; b += kThreads) {
+  if (fill) trim_fill(a, near ? s_incl : a.incl, count + all, tid, NT);
+  for (int b = tid; b < a.batch; b += NT) {
     const int keep = a.keep_lens[b] < 0 ? 0 : a.keep_lens[b];
     if (keep < a.lens[b]) a.lens[b] = keep;
   }
   if (tid == 0) *a.free_count = count + (int)all;
+}
+
+__global__ __launch_bounds__(256) void cache_trim_fill_kernel(CacheTrimArgs a) {
+  __shared__ int32_t s_incl[kInLds];
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  const int64_t top = *a.free_count;
+  if (a.batch <= kInLds) {
+    for (int b = threadIdx.x; b < a.batch; b += 256) s_incl[b] = a.incl[b];
+    __syncthreads();
+    trim_fill(a, s_incl, top, first, step);
+  } else {
+    trim_fill(a, a.incl, top, first, step);
+  }
 }
 
 // -- append ---------------------------------------------------------------------------
@@ -475,7 +542,10 @@ hipError_t run_cache_reserve(const CacheReserveArgs& a, hipStream_t stream) {
   // One workgroup fills 1024 slots at a time; past a few rounds of it a second launch over
   // the whole chip is faster.
   const bool one = a.tokens <= 8192;
-  hipLaunchKernelGGL(cache_reserve_kernel, dim3(1), dim3(kThreads), 0, stream, a, one ? 1 : 0);
+  if (a.batch <= 256 && a.tokens <= 1024)
+    hipLaunchKernelGGL((cache_reserve_kernel<256>), dim3(1), dim3(256), 0, stream, a, 1);
+  else
+    hipLaunchKernelGGL((cache_reserve_kernel<1024>), dim3(1), dim3(1024), 0, stream, a, one ? 1 : 0);
   if (!one) {
     const int64_t g = (a.tokens + 1023) / 1024;
     hipLaunchKernelGGL(cache_reserve_fill_kernel, dim3((unsigned)(g < 2048 ? g : 2048)), dim3(256), 0, stream, a);
@@ -485,7 +555,13 @@ hipError_t run_cache_reserve(const CacheReserveArgs& a, hipStream_t stream) {
 
 hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream) {
   if (a.batch <= 0 || a.width < 0 || a.num_free < 0) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(cache_trim_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  // How many blocks come back is not known here, only that it is at most the table's size.
+  const bool one = a.batch * a.width <= 16384;
+  if (a.batch <= 256 && one)
+    hipLaunchKernelGGL((cache_trim_kernel<256>), dim3(1), dim3(256), 0, stream, a, 1);
+  else
+    hipLaunchKernelGGL((cache_trim_kernel<1024>), dim3(1), dim3(1024), 0, stream, a, one ? 1 : 0);
+  if (!one) hipLaunchKernelGGL(cache_trim_fill_kernel, dim3(64), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

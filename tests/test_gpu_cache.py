@@ -46,7 +46,8 @@ def run_tables(held, new, block, num_blocks, width, tokens, seed, steps=1):
 
 @pytest.mark.parametrize("batch,block,hi_len,hi_new", [
     (1, 16, 0, 1), (1, 128, 40, 300), (3, 16, 100, 40), (64, 64, 700, 6), (37, 32, 60, 500), (1025, 16, 33, 5),
-    (2050, 128, 10, 3), (5, 16, 200, 2500)])
+    (2050, 128, 10, 3), (5, 16, 200, 2500),
+    (400, 16, 9, 700), (1100, 16, 33, 100)])
 def test_tables_follow_the_plain_form(batch, block, hi_len, hi_new):
     rng = random.Random(batch * 1000 + block)
     held = [rng.choice([0, 1, block, block - 1, rng.randint(0, hi_len)]) for _ in range(batch)]
