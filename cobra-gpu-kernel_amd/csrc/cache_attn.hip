@@ -21,6 +21,8 @@
 // group reads of V^T in one 16-byte load.  P goes from the softmax into the product without
 // leaving its lane, K and V from memory into the matrix cores without passing LDS, and since a
 // block is at least 16 tokens a lane needs one K scale and one V scale for a tile.
+#include <type_traits>
+
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lds_dma.hpp"
@@ -107,6 +109,17 @@ struct Widen<kCacheI8, bf16> {
   }
 };
 
+// The first n codes of v, zeros after them: memory past a request's end, or of a block that is
+// none, may hold NaN codes.
+template <typename V>
+__device__ __forceinline__ void keep_first(V& v, int n) {
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) {
+    const int c = n - 4 * i;
+    v[i] = c >= 4 ? v[i] : c <= 0 ? 0u : v[i] & (0xffffffffu >> (8 * (4 - c)));
+  }
+}
+
 struct Args {
   const void* q;
   void* out;
@@ -147,6 +160,53 @@ __device__ __forceinline__ int chunk_of(const Args& a, int len, int step) {
   return up > a.chunk ? up : a.chunk;
 }
 
+// Entries of a request's row of the table, 64 from `first` on a lane each, and the next 64.
+// Loads of single entries would be waited for one by one: scalar ones share a counter with
+// LDS, vector ones theirs with the tiles in flight.  A tile's blocks never straddle two 64s,
+// which begin a whole number of tiles apart.
+struct Pages {
+  int first, held, ahead, last;
+  const int32_t* row;
+  __device__ __forceinline__ Pages(const Args& a, int b, int p)
+      : first(p), last((int)a.table_width - 1), row(a.table + b * a.table_width) {
+    held = entry(p);
+    ahead = entry(p + 64);
+  }
+  __device__ __forceinline__ int entry(int p) const {
+    p += threadIdx.x & 63;
+    return row[(uint32_t)(p < last ? p : last)];
+  }
+  __device__ __forceinline__ void reach(const Args& a, int p) {
+    if (p - first >= 64) {
+      first += 64;
+      held = ahead;
+      ahead = entry(first + 64);
+    }
+  }
+  __device__ __forceinline__ int any(int p) const {  // p may differ from lane to lane
+    return __builtin_amdgcn_ds_bpermute((p - first) * 4, held);
+  }
+  __device__ __forceinline__ int one(int p) const { return __builtin_amdgcn_readlane(held, p - first); }
+};
+
+// Where block id of one kv head lies.  A block's bytes over all heads are under 2^31.
+struct Strides {
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  uint32_t stride, heads, blocks;
+  __device__ __forceinline__ Strides(const Args& a, int h, int plane)
+      : k(a.k + (int64_t)h * plane),
+        v(a.v + (int64_t)h * plane),
+        k_scale(a.k_scale + h),
+        v_scale(a.v_scale + h),
+        stride((uint32_t)a.kv_heads * (uint32_t)plane),
+        heads((uint32_t)a.kv_heads),
+        blocks((uint32_t)a.num_blocks) {}
+  __device__ __forceinline__ bool there(int id) const { return (uint32_t)id < blocks; }
+  __device__ __forceinline__ uint64_t block(int id) const { return (uint64_t)(there(id) ? (uint32_t)id : 0u) * stride; }
+  __device__ __forceinline__ uint64_t scale(int id) const { return (uint64_t)(there(id) ? (uint32_t)id : 0u) * heads; }
+};
+
 // One wave's state for NR sets of 16 rows and its pass over some tiles of keys.
 template <typename T, int CACHE, int HDP, int NR, int KT>
 struct Rows {
@@ -160,14 +220,14 @@ struct Rows {
   float m[NR], l[NR];  // l: this lane group's share
   int lim[NR];         // keys that this lane's row sees
 
-  __device__ __forceinline__ void init(const Args& a, const Request& rq, int h, int64_t row0) {
+  __device__ __forceinline__ void init(const Args& a, const Request& rq, int h, int row0) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      const int64_t row = row0 + 16 * r + n;
-      const bool there = row < (int64_t)rq.n * a.group;
-      const int tok = there ? (int)(row / a.group) : 0;
-      const int head = h * a.group + (there ? (int)(row - (int64_t)tok * a.group) : 0);
+      const int row = row0 + 16 * r + n;
+      const bool there = row < rq.n * a.group;
+      const int tok = there ? row / a.group : 0;
+      const int head = h * a.group + (there ? row - tok * a.group : 0);
       const T* p = static_cast<const T*>(a.q) + (int64_t)(rq.t0 + tok) * a.ldq + (int64_t)head * a.head_dim;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
@@ -200,103 +260,100 @@ struct Rows {
     return sum;
   }
 
-  // S^T = K Q^T on codes; wide(i, j) and odd(i): this lane's K codes of subtile i.
-  template <typename W, typename O>
-  __device__ __forceinline__ void scores(f32x4 (&s)[NR][kSub], W&& wide, O&& odd) {
+  // The queries are waited for here, behind the first tile's loads: waited for in the loop, they
+  // would take every later tile's along.
+  __device__ __forceinline__ void wait_queries() {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[r][i]));
+  }
+
+  // S^T = K Q^T on codes; k(i, j): this lane's K operand of subtile i, step j.
+  template <typename K>
+  __device__ __forceinline__ void scores(f32x4 (&s)[NR][kSub], K&& k) {
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int i = 0; i < kSub; ++i) s[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Steps outside, so that neighbouring instructions add to different registers.
 #pragma unroll
-    for (int i = 0; i < kSub; ++i) {
+    for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-      for (int j = 0; j < kWide; ++j) {
-        const u32x4 k = wide(i, j);
-        const V8 lo = Widen<CACHE, T>::of(k.x, k.y), hi = Widen<CACHE, T>::of(k.z, k.w);
+      for (int i = 0; i < kSub; ++i) {
+        const V8 x = k(i, j);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][i] = mfma16(lo, q[r][2 * j], s[r][i]);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][i] = mfma16(hi, q[r][2 * j + 1], s[r][i]);
+        for (int r = 0; r < NR; ++r) s[r][i] = mfma16(x, q[r][j], s[r][i]);
       }
-      if constexpr (kOdd) {
-        const u32x2 k = odd(i);
-        const V8 lo = Widen<CACHE, T>::of(k.x, k.y);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][i] = mfma16(lo, q[r][kSteps - 1], s[r][i]);
-      }
-    }
   }
 
   // Scores to weights: this lane's keys begin at key0, its block's scales are sk and sv (of a
-  // block outside the pool: bad); slow: not every row sees every key of the tile.
-  __device__ __forceinline__ void softmax(const Args& a, f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], float sk,
-                                          float sv, int key0, bool bad, bool slow) {
-    const float skc = fminf(fmaxf(sk, 0x1p-40f), 0x1p40f) * a.c2, svc = fminf(fmaxf(sv, 0x1p-40f), 0x1p40f);
-    const float ev = __builtin_amdgcn_logf(svc), inv = 1.f / svc;
+  // block outside the pool: bad); slow: not every row sees every key of the tile.  First against
+  // the reference that the row has, without a maximum of this tile: right as long as every w
+  // stays inside fp16, which a sum at most kAccept of a lane's w shows.
+  struct Block {
+    float skc, ev, inv;
+    __device__ __forceinline__ Block(const Args& a, float sk, float sv) {
+      const float svc = fminf(fmaxf(sv, 0x1p-40f), 0x1p40f);
+      skc = fminf(fmaxf(sk, 0x1p-40f), 0x1p40f) * a.c2;
+      ev = __builtin_amdgcn_logf(svc);
+      inv = __builtin_amdgcn_rcpf(svc);  // both exact for powers of two
+    }
+  };
+  __device__ __forceinline__ bool weights(const f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b,
+                                          float (&sum)[NR]) const {
+    bool ok = true;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      // Against the reference that the row has, without a maximum of this tile: right as long
-      // as every w stays inside fp16, which a sum at most kAccept of a lane's w shows.
-      float shift = ev + kBias - m[r], sum;
-      bool ok = false;
-      if (!slow) {
-        sum = weigh(s[r], skc, shift, p[r]);
-        ok = sum <= kAccept;  // false for NaN, and where the row has no reference yet
-      }
-      if (!__all(ok)) {
-        const int seen = bad ? 0 : slow ? lim[r] - key0 : kKeys;  // keys of this lane that count
-        float mx = kNegInf;
-#pragma unroll
-        for (int e = 0; e < kKeys; ++e) {
-          const float u = fmaf(s[r][e >> 2][e & 3], skc, ev);
-          s[r][e >> 2][e & 3] = e < seen ? s[r][e >> 2][e & 3] : kNegInf;
-          mx = fmaxf(mx, e < seen ? u : kNegInf);
-        }
-        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-        const float mn = fmaxf(m[r], mx);
-        const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn);
-        m[r] = mn;
-        shift = mn == kNegInf ? kNegInf : ev + kBias - mn;
-        sum = weigh(s[r], skc, shift, p[r]);
-        l[r] *= alpha;
-#pragma unroll
-        for (int t = 0; t < kDims; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
-      }
-      l[r] = fmaf(sum, inv, l[r]);
+      sum[r] = weigh(s[r], b.skc, b.ev + kBias - m[r], p[r]);
+      ok &= sum[r] <= kAccept;  // false for NaN, and where the row has no reference yet
     }
+    return ok;
+  }
+  __device__ __forceinline__ void weights_by_max(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b,
+                                                 float (&sum)[NR], int key0, bool bad, bool slow) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int seen = bad ? 0 : slow ? lim[r] - key0 : kKeys;  // keys of this lane that count
+      float mx = kNegInf;
+#pragma unroll
+      for (int e = 0; e < kKeys; ++e) {
+        const float u = fmaf(s[r][e >> 2][e & 3], b.skc, b.ev);
+        s[r][e >> 2][e & 3] = e < seen ? s[r][e >> 2][e & 3] : kNegInf;
+        mx = fmaxf(mx, e < seen ? u : kNegInf);
+      }
+      const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+      const float mn = fmaxf(m[r], mx);
+      const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn);
+      m[r] = mn;
+      sum[r] = weigh(s[r], b.skc, mn == kNegInf ? kNegInf : b.ev + kBias - mn, p[r]);
+      l[r] *= alpha;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
+    }
+  }
+  __device__ __forceinline__ void softmax(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b, int key0,
+                                          bool bad, bool slow) {
+    float sum[NR];
+    if (slow || !__all(weights(s, p, b, sum))) weights_by_max(s, p, b, sum, key0, bad, slow);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) l[r] = fmaf(sum[r], b.inv, l[r]);
   }
 
-  // O^T += V^T P^T on codes; codes(t): this lane's keys of dimension 16 t + n, of which the
-  // first `there` count where cut (memory past a request's end, or of a block that is none,
-  // may hold NaN codes).
+  // O^T += V^T P^T on codes; v(t, i): this lane's V operand of dimensions 16 t .., part i of its keys.
   template <typename V>
-  __device__ __forceinline__ void gather(const f16x8 (&p)[NR][kParts], V&& codes, bool cut, int there) {
-    if (cut) {
+  __device__ __forceinline__ void gather(const f16x8 (&p)[NR][kParts], V&& v) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
 #pragma unroll
       for (int t = 0; t < kDims; ++t) {
-        VWords v = codes(t);
+        const f16x8 x = v(t, i);
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          const int c = there - 4 * i;
-          v[i] = c >= 4 ? v[i] : c <= 0 ? 0u : v[i] & (0xffffffffu >> (8 * (4 - c)));
-        }
-        add(t, v, p);
+        for (int r = 0; r < NR; ++r) o[r][t] = mfma16(x, p[r][i], o[r][t]);
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < kDims; ++t) add(t, codes(t), p);
-    }
-  }
-  __device__ __forceinline__ void add(int t, const VWords& v, const f16x8 (&p)[NR][kParts]) {
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const f16x8 w = Widen<CACHE, f16>::of(v[2 * i], v[2 * i + 1]);
-#pragma unroll
-      for (int r = 0; r < NR; ++r) o[r][t] = mfma16(w, p[r][i], o[r][t]);
-    }
   }
 
   // Tiles t0, t0 + step, .. below t_end, K and V straight from memory to registers; keys from
@@ -304,79 +361,74 @@ struct Rows {
   __device__ __forceinline__ void pass(const Args& a, const Request& rq, int b, int h, int t0, int t_end, int step,
                                        int full) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, gk = n >> 2;
-    const int32_t* table = a.table + b * a.table_width;
-    const int bs = 1 << a.shift, last_page = (int)a.table_width - 1;
-    const int64_t plane = (int64_t)bs * HDP;
+    const int bs = 1 << a.shift;
     if (t0 >= t_end) return;
 
-    // Block ids of a tile: of the group whose K rows this lane reads, and of its own V keys.
-    auto page = [&](int tile, int grp) {
-      const int p = (tile * KT + kKeys * grp) >> a.shift;
-      return table[p < last_page ? p : last_page];
-    };
+    Pages pages(a, b, (t0 * KT) >> a.shift);
+    const Strides st(a, h, bs * HDP);
     u32x4 kw[kSub][kWide > 0 ? kWide : 1];
     u32x2 ko[kSub];
     VWords vw[kDims];
     float sk, sv;
-    int idk = page(t0, gk), idv = page(t0, g);
-    bool bad_next = false;
-    auto clamp_id = [&](int id) { return (unsigned)id < (unsigned)a.num_blocks ? id : 0; };
+    bool bad = false;
+    int idk, idv;  // blocks of the group whose K rows this lane reads, and of its own keys
+    auto find = [&](int tile) {
+      pages.reach(a, (tile * KT) >> a.shift);
+      idk = pages.any((tile * KT + kKeys * gk) >> a.shift);
+      idv = pages.any((tile * KT + kKeys * g) >> a.shift);
+    };
     auto load_k = [&](int tile) {
-      const int64_t at = ((int64_t)clamp_id(idk) * a.kv_heads + h) * plane;
       const int off = (tile * KT + kKeys * gk + (n & 3)) & (bs - 1);
-      const uint8_t* p = a.k + at + (int64_t)off * HDP;
+      const uint8_t* p = st.k + st.block(idk) + (uint32_t)(off * HDP + 16 * g);
 #pragma unroll
       for (int s = 0; s < kSub; ++s) {
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) kw[s][j] = *reinterpret_cast<const u32x4*>(p + s * 4 * HDP + 64 * j + 16 * g);
-        if constexpr (kOdd) ko[s] = *reinterpret_cast<const u32x2*>(p + s * 4 * HDP + 64 * kWide + 8 * g);
+        for (int j = 0; j < kWide; ++j) kw[s][j] = *reinterpret_cast<const u32x4*>(p + s * 4 * HDP + 64 * j);
+        if constexpr (kOdd) ko[s] = *reinterpret_cast<const u32x2*>(p + s * 4 * HDP + 64 * kWide - 8 * g);
       }
     };
     auto load_v = [&](int tile) {
-      const int64_t bh = (int64_t)clamp_id(idv) * a.kv_heads + h;
       const int off = (tile * KT + kKeys * g) & (bs - 1);
-      const uint8_t* p = a.v + bh * plane + (int64_t)n * bs + off;
+      const uint8_t* p = st.v + st.block(idv) + (uint32_t)(n * bs + off);
+      sk = st.k_scale[st.scale(idv)];
+      sv = st.v_scale[st.scale(idv)];
+      bad = !st.there(idv);
 #pragma unroll
-      for (int t = 0; t < kDims; ++t) vw[t] = *reinterpret_cast<const VWords*>(p + (int64_t)t * 16 * bs);
+      for (int t = 0; t < kDims; ++t) vw[t] = *reinterpret_cast<const VWords*>(p + (uint32_t)(t * 16 * bs));
     };
-    auto load_scales = [&]() {
-      const int64_t bh = (int64_t)clamp_id(idv) * a.kv_heads + h;
-      sk = a.k_scale[bh];
-      sv = a.v_scale[bh];
-      bad_next = (unsigned)idv >= (unsigned)a.num_blocks;
-    };
+    find(t0);
     load_k(t0);
-    load_scales();
     load_v(t0);
-    int idk2 = 0, idv2 = 0;
-    if (t0 + step < t_end) {
-      idk2 = page(t0 + step, gk);
-      idv2 = page(t0 + step, g);
-    }
-    for (int tile = t0; tile < t_end; tile += step) {
-      const bool more = tile + step < t_end;
+    wait_queries();
+    // One tile; `more`: with the loads of the wave's next, the keys' while the softmax runs.  Not
+    // a test inside: where the paths met, a wait for one tile's loads would be one for the next's.
+    auto one = [&](int tile, auto more) {
       const int key0 = tile * KT + kKeys * g;  // this lane's first key
       f32x4 s[NR][kSub];
-      scores(s, [&](int i, int j) { return kw[i][j]; }, [&](int i) { return ko[i]; });
-      const bool bad = bad_next;
-      const float sk0 = sk, sv0 = sv;
-      // The next tile's keys and scales while this one's softmax runs.
-      if (more) {
-        idk = idk2;
-        idv = idv2;
-        load_k(tile + step);
-        load_scales();
-        if (tile + 2 * step < t_end) {
-          idk2 = page(tile + 2 * step, gk);
-          idv2 = page(tile + 2 * step, g);
-        }
-      }
+      scores(s, [&](int i, int j) {
+        if (kOdd && j == kSteps - 1) return Widen<CACHE, T>::of(ko[i][0], ko[i][1]);
+        return Widen<CACHE, T>::of(kw[i][j >> 1][2 * (j & 1)], kw[i][j >> 1][2 * (j & 1) + 1]);
+      });
       const bool slow = tile * KT + KT > full || __any(bad);
+      const int there = bad ? 0 : rq.len - key0;
+      const bool bad0 = bad;
+      const Block blk(a, sk, sv);
+      if constexpr (decltype(more)::value) {
+        find(tile + step);
+        load_k(tile + step);
+      }
       f16x8 p[NR][kParts];
-      softmax(a, s, p, sk0, sv0, key0, bad, slow);
-      gather(p, [&](int t) { return vw[t]; }, slow, bad ? 0 : rq.len - key0);
-      if (more) load_v(tile + step);
-    }
+      softmax(s, p, blk, key0, bad0, slow);
+      if (slow) {
+#pragma unroll
+        for (int t = 0; t < kDims; ++t) keep_first(vw[t], there);
+      }
+      gather(p, [&](int t, int i) { return Widen<CACHE, f16>::of(vw[t][2 * i], vw[t][2 * i + 1]); });
+      if constexpr (decltype(more)::value) load_v(tile + step);
+    };
+    int tile = t0;
+    for (; tile + step < t_end; tile += step) one(tile, std::true_type());
+    one(tile, std::false_type());
   }
 
   __device__ __forceinline__ void total_l() {
@@ -385,13 +437,13 @@ struct Rows {
   }
 
   // Row set r to its place: the result, or a split's share of it.
-  __device__ __forceinline__ void store(const Args& a, const Request& rq, int h, int64_t row0, int r, int split,
+  __device__ __forceinline__ void store(const Args& a, const Request& rq, int h, int row0, int r, int split,
                                         bool whole) const {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int64_t row = row0 + 16 * r + n;
-    if (row >= (int64_t)rq.n * a.group) return;
-    const int tok = (int)(row / a.group);
-    const int64_t at = (int64_t)(rq.t0 + tok) * a.heads + h * a.group + (row - (int64_t)tok * a.group);
+    const int row = row0 + 16 * r + n;
+    if (row >= rq.n * a.group) return;
+    const int tok = row / a.group;
+    const int64_t at = (int64_t)(rq.t0 + tok) * a.heads + h * a.group + (row - tok * a.group);
     if (whole) {
       const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
       T* p = static_cast<T*>(a.out) + at * a.head_dim;
@@ -418,10 +470,10 @@ struct Rows {
 // Few rows for each kv head: a workgroup has 16 of them and one split of the keys, its waves
 // every kWaves-th tile of it; their shares are joined through LDS, the splits' by
 // cache_join_kernel.
-template <typename T, int CACHE, int HDP, int NR, int KT, int kWaves>
-__global__ __launch_bounds__(kWaves * 64) void cache_decode_kernel(Args a) {
-  typedef Rows<T, CACHE, HDP, NR, KT> R;
-  constexpr int kRows = 16 * NR;
+template <typename T, int CACHE, int HDP, int KT>
+__global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
+  typedef Rows<T, CACHE, HDP, 1, KT> R;
+  constexpr int kWaves = 4, kRows = 16;
   __shared__ f32x4 sh_o[kWaves / 2][R::kDims][64];
   __shared__ float sh_m[kWaves / 2][64], sh_l[kWaves / 2][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -437,7 +489,7 @@ __global__ __launch_bounds__(kWaves * 64) void cache_decode_kernel(Args a) {
   if (split > 0 && (int64_t)split * chunk >= rq.len) return;
   for (int64_t row0 = (int64_t)(id / a.batch) * kRows; row0 < rows; row0 += (int64_t)a.row_tiles * kRows) {
     R w;
-    w.init(a, rq, h, row0);
+    w.init(a, rq, h, (int)row0);
     // Keys up to what the tile's last row sees; all of its rows see those below `full`.
     const int64_t end_row = min(row0 + kRows, rows) - 1;
     int end = rq.len, full = rq.len;
@@ -452,30 +504,27 @@ __global__ __launch_bounds__(kWaves * 64) void cache_decode_kernel(Args a) {
     w.total_l();
     // The upper half of the waves into the lower, until one is left.
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
+    for (int half = kWaves / 2; half; half >>= 1) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half) {
+        sh_m[wave - half][lane] = w.m[0];
+        sh_l[wave - half][lane] = w.l[0];
 #pragma unroll
-      for (int half = kWaves / 2; half; half >>= 1) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-          sh_m[wave - half][lane] = w.m[r];
-          sh_l[wave - half][lane] = w.l[r];
-#pragma unroll
-          for (int t = 0; t < R::kDims; ++t) sh_o[wave - half][t][lane] = w.o[r][t];
-        }
-        __syncthreads();
-        if (wave < half) {
-          const float m2 = sh_m[wave][lane], mn = fmaxf(w.m[r], m2), base = mn == kNegInf ? 0.f : mn;
-          const float f1 = __builtin_amdgcn_exp2f(w.m[r] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-          w.m[r] = mn;
-          w.l[r] = w.l[r] * f1 + sh_l[wave][lane] * f2;
-#pragma unroll
-          for (int t = 0; t < R::kDims; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w.o[r][t][i] = w.o[r][t][i] * f1 + sh_o[wave][t][lane][i] * f2;
-        }
+        for (int t = 0; t < R::kDims; ++t) sh_o[wave - half][t][lane] = w.o[0][t];
       }
-      if (wave == 0) w.store(a, rq, h, row0, r, split, chunk >= rq.len);
+      __syncthreads();
+      if (wave < half) {
+        const float m2 = sh_m[wave][lane], mn = fmaxf(w.m[0], m2), base = mn == kNegInf ? 0.f : mn;
+        const float f1 = __builtin_amdgcn_exp2f(w.m[0] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        w.m[0] = mn;
+        w.l[0] = w.l[0] * f1 + sh_l[wave][lane] * f2;
+#pragma unroll
+        for (int t = 0; t < R::kDims; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[0][t][i] = w.o[0][t][i] * f1 + sh_o[wave][t][lane][i] * f2;
+      }
     }
+    if (wave == 0) w.store(a, rq, h, (int)row0, 0, split, chunk >= rq.len);
   }
 }
 
@@ -550,163 +599,223 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
 }
 
 // Many rows for each kv head: a wave has NR sets of 16 and passes over all of their keys.  Tiles
-// of 64 keys go through LDS, whence all four waves read their codes (each taking them from the
-// caches by itself asked 7 TB/s of L2 and waited for half of its time): 16-byte chunks in the
-// order in which a wave reads them, XOR-swizzled by row so that eight lanes in a row meet eight
-// different ones of 128 bytes' places.  Two stages: a tile is in registers while the one before
-// it is in LDS and the one before that in use.
+// of 64 keys go through LDS, widened to 16 bits on the way, once for the four waves (each wave
+// taking its codes from the caches by itself asked 7 TB/s of L2 and waited for half of its
+// time; each widening all of them took a quarter of its vector instructions).  LDS holds
+// 16-byte chunks in the order in which lanes read them, XOR-swizzled by row so that the 16
+// lanes of a column meet 16 different places of 256 bytes.  Two stages: a tile is in
+// registers while the one before it is in LDS and the one before that in use.
 template <typename T, int CACHE, int HDP, int NR>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a) {
   constexpr int kWaves = 4, kRows = kWaves * NR * 16, KT = 64;
   typedef Rows<T, CACHE, HDP, NR, KT> R;
-  constexpr int kC = HDP / 16, kPer = (HDP + 63) / 64;  // chunks of a K row; a thread's of K, of V
+  typedef typename R::V8 V8;
+  constexpr int kC = HDP / 16, kPer = (HDP + 63) / 64;  // 16 codes each: of a K row; a thread's of K, of V
+  constexpr bool kAll = HDP % 64 == 0;
+  // At head_dim 128 int8's widening leaves no registers for a product's codes at once.
+  constexpr bool kBatch = CACHE == kCacheE4M3 || HDP != 128;
   __shared__ u32x4 sh_k[2][KT * kC], sh_v[2][HDP * 4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, n = lane & 15;
-  auto swz = [](int row) {
-    return kC == 8 || kC == 16 ? row & 7 : kC == 4 || kC == 12 ? (row >> 1) & 3 : (row >> 2) & 1;
-  };
-  // Workgroups go to XCDs round-robin: every eighth (request, kv head) pair to the same one,
-  // whose L2 then serves the pair's keys to all of its row tiles.
-  const int pairs = a.batch * a.kv_heads;
-  const int l = blockIdx.x / 8, pair = l / a.row_tiles * 8 + blockIdx.x % 8, tile0 = l % a.row_tiles;
-  if (pair >= pairs) return;
-  const int h = pair % a.kv_heads, b = pair / a.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto swz = [](int row) { return kC == 8 || kC == 16 ? row & 7 : kC == 4 || kC == 12 ? (row >> 1) & 3 : (row >> 2) & 1; };
+  auto swz_v = [](int d) { return (d >> 1) & 3; };
+  // The longest request first (where a wave can rank them), of a request the row tiles with the
+  // most keys first: workgroups start in order of their ids, and what starts last should be
+  // short.  Neighbours, which go to XCDs round-robin, take different kv heads.
+  int id = blockIdx.x;
+  const int h = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int tile0 = a.row_tiles - 1 - id % a.row_tiles;
+  id /= a.row_tiles;
+  const int split = id % a.splits;
+  int b = id / a.splits;
+  if (a.batch <= 64) {
+    const int len = lane < a.batch ? a.lens[lane] : -1;
+    int rank = 0;
+    for (int k = 0; k < a.batch; ++k) {
+      const int other = __builtin_amdgcn_readlane(len, k);
+      rank += other > len || (other == len && k < lane);
+    }
+    b = __builtin_ctzll(__ballot(lane < a.batch && rank == b));
+  }
   const Request rq = request_of(a, b);
   const int64_t rows = (int64_t)rq.n * a.group;
-  const int bs = 1 << a.shift, last_page = (int)a.table_width - 1;
-  const int64_t plane = (int64_t)bs * HDP;
-  typedef const __attribute__((address_space(4))) int32_t* cptr;
-  const cptr table = (cptr)(a.table + b * a.table_width);
+  const int chunk = chunk_of(a, rq.len, KT);
+  if (split > 0 && (int64_t)split * chunk >= rq.len) return;
+  const int first = split * (chunk / KT);
+  const int bs = 1 << a.shift;
+  const Strides st(a, h, bs * HDP);
+  Pages pages(a, b, (first * KT) >> a.shift);
 
-  // What this thread brings of a tile: K chunks lane, lane + 64, .. of the 16 keys of group
-  // `wave`, V chunks tid, tid + 256, .. (four to a dimension).
+  // What this thread brings of a tile: of K 16-code pieces lane, lane + 64, .. of the keys of
+  // group `wave`, of V pieces tid, tid + 256, .. (four to a dimension).
   u32x4 rk[kPer], rv[kPer];
-  int id0, id1, id2, id3;  // block ids of a tile's four groups of 16 keys
-  float sk, sv, sk1, sv1;
-  bool bad = false, bad1 = false;
+  // Blocks of a tile's four groups of 16 keys.  With blocks of 64 tokens and more they are one,
+  // and everything that depends on it is the same for all lanes.
+  const bool one = a.shift >= 6;
+  struct Ids {
+    int i0, i1, i2, i3;
+    __device__ __forceinline__ int of(int i) const {
+      const int even = i & 2 ? +i2 : +i0, odd = i & 2 ? +i3 : +i1;
+      return i & 1 ? odd : even;
+    }
+  };
   auto load_ids = [&](int tile) {
-    auto id = [&](int i) {
-      const int p = (tile * KT + 16 * i) >> a.shift;
-      return (int)table[p < last_page ? p : last_page];
-    };
-    id0 = id(0);
-    id1 = id(1);
-    id2 = id(2);
-    id3 = id(3);
+    pages.reach(a, (tile * KT) >> a.shift);
+    Ids x;
+    x.i0 = pages.one((tile * KT) >> a.shift);
+    if (!one) {
+      x.i1 = pages.one((tile * KT + 16) >> a.shift);
+      x.i2 = pages.one((tile * KT + 32) >> a.shift);
+      x.i3 = pages.one((tile * KT + 48) >> a.shift);
+    }
+    return x;
   };
-  auto pick = [&](int i) {
-    const int even = i & 2 ? +id2 : +id0, odd = i & 2 ? +id3 : +id1;
-    return i & 1 ? odd : even;
-  };
-  auto block = [&](int id) { return (int64_t)((unsigned)id < (unsigned)a.num_blocks ? id : 0) * a.kv_heads + h; };
-  auto load = [&](int tile) {
-    const uint8_t* pk = a.k + block(pick(wave)) * plane + (int64_t)((tile * KT + 16 * wave) & (bs - 1)) * HDP;
+  const uint32_t k_off = lane * 16, v_off = (tid >> 2) * bs;
+  auto load_k = [&](int tile, const Ids& ids) {
+    const int id = one ? ids.i0 : ids.of(wave);
+    const uint8_t* pk = st.k + st.block(id) + (uint32_t)(((tile * KT + 16 * wave) & (bs - 1)) * HDP);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (HDP % 64 == 0 || lane + 64 * i < HDP) rk[i] = *reinterpret_cast<const u32x4*>(pk + (lane + 64 * i) * 16);
-    const int part = tid & 3;
-    const uint8_t* pv = a.v + block(pick(part)) * plane + ((tile * KT + 16 * part) & (bs - 1)) + (int64_t)(tid >> 2) * bs;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (HDP % 64 == 0 || (tid >> 2) + 64 * i < HDP) rv[i] = *reinterpret_cast<const u32x4*>(pv + (int64_t)i * 64 * bs);
-    const int id = pick(g);
-    sk1 = a.k_scale[block(id)];
-    sv1 = a.v_scale[block(id)];
-    bad1 = (unsigned)id >= (unsigned)a.num_blocks;
+      if (kAll || lane + 64 * i < HDP) rk[i] = *reinterpret_cast<const u32x4*>(pk + (k_off + 1024u * i));
   };
-  auto put = [&](int stage) {
+  int there = 64;  // tokens of the V piece that are the request's
+  float sk = 1.f, sv = 1.f;
+  bool bad = false;
+  auto load_v = [&](int tile, const Ids& ids) {
+    there = rq.len - tile * KT - 16 * (tid & 3);
+    if (one) {
+      const uint8_t* pv = st.v + st.block(ids.i0) + (uint32_t)((tile * KT) & (bs - 1));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (kAll || (tid >> 2) + 64 * i < HDP) rv[i] = *reinterpret_cast<const u32x4*>(pv + (v_off + (tid & 3) * 16 + 64u * i * bs));
+      if (!st.there(ids.i0)) there = 0;
+    } else {
+      const int id = ids.of(tid & 3);
+      const uint8_t* pv = st.v + st.block(id) + (uint32_t)((tile * KT + 16 * (tid & 3)) & (bs - 1));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (kAll || (tid >> 2) + 64 * i < HDP) rv[i] = *reinterpret_cast<const u32x4*>(pv + (v_off + 64u * i * bs));
+      if (!st.there(id)) there = 0;
+    }
+  };
+  auto load_scales = [&](const Ids& ids) {
+    const int id = one ? ids.i0 : ids.of(g);
+    sk = st.k_scale[st.scale(id)];
+    sv = st.v_scale[st.scale(id)];
+    bad = !st.there(id);
+  };
+  auto put_k = [&](int stage) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int c = lane + 64 * i, key = c / kC, row = 16 * (key >> 2) + 4 * wave + (key & 3);
-      if (HDP % 64 == 0 || c < HDP) sh_k[stage][row * kC + ((c % kC) ^ swz(row))] = rk[i];
+      if (kAll || c < HDP) sh_k[stage][row * kC + ((c % kC) ^ swz(row))] = rk[i];
+    }
+  };
+  auto put_v = [&](int stage) {
+    if (__any(there < 16)) {
+      asm volatile("");  // a branch, not 20 instructions for every tile
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) keep_first(rv[i], there);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int d = (tid >> 2) + 64 * i;
-      if (HDP % 64 == 0 || d < HDP) sh_v[stage][d * 4 + ((tid & 3) ^ ((d >> 1) & 3))] = rv[i];
+      if (kAll || d < HDP) sh_v[stage][d * 4 + ((tid & 3) ^ swz_v(d))] = rv[i];
     }
-    sk = sk1;
-    sv = sv1;
-    bad = bad1;
   };
 
   for (int64_t at = (int64_t)tile0 * kRows; at < rows; at += (int64_t)a.row_tiles * kRows) {
+    if (at != (int64_t)tile0 * kRows) pages = Pages(a, b, (first * KT) >> a.shift);
     const int64_t row0 = at + wave * NR * 16;
     R w;
-    w.init(a, rq, h, row0);
-    // Tiles that this wave's rows see, and that any of the workgroup's do.
-    const int64_t end_row = min(row0 + NR * 16, rows) - 1;
-    int end = rq.len, full = rq.len, most = rq.len;
+    w.init(a, rq, h, (int)row0);
+    wait_vmcnt<0>();  // the queries: waited for in the loop, they would take every tile's loads along
+    // Tiles that any of the workgroup's rows see; keys that all of this wave's do.
+    int full = rq.len, most = rq.len;
     if (a.causal) {
-      end = rq.len - rq.n + (int)(end_row / a.group) + 1;
       full = rq.len - rq.n + (int)(row0 / a.group) + 1;
       most = rq.len - rq.n + (int)((min(at + kRows, rows) - 1) / a.group) + 1;
     }
-    end = row0 < rows && end > 0 ? (end + KT - 1) / KT : 0;
     most = most > 0 ? (most + KT - 1) / KT : 0;
+    if (most > first + chunk / KT) most = first + chunk / KT;
     __syncthreads();
-    if (most > 0) {
-      load_ids(0);
-      load(0);
-      put(0);
-      if (most > 1) {
-        load_ids(1);
-        load(1);
-        load_ids(2);
-      }
+    Ids ids, next;  // of the tiles two ahead and one ahead
+    int begin = first;
+    asm volatile("" : "+s"(begin));  // nothing of a first tile's addresses is kept for the next round of rows
+    if (begin < most) {
+      ids = load_ids(begin);
+      load_k(begin, ids);
+      load_v(begin, ids);
+      load_scales(ids);
+      put_k(begin & 1);
+      put_v(begin & 1);
+      next = load_ids(begin + 1);
+      load_k(begin + 1, next);
+      load_v(begin + 1, next);
+      ids = load_ids(begin + 2);
     }
-    for (int tile = 0; tile < most; ++tile) {
+    for (int tile = first; tile < most; ++tile) {
       lds_barrier();  // this tile's stage is written, the other one read
       const int key0 = tile * KT + 16 * g;
-      const float sk0 = sk, sv0 = sv;
-      const bool bad0 = bad;
-      if (tile < end) {
-        const u32x4 *pk = sh_k[tile & 1] + n * kC, *pv = sh_v[tile & 1];
-        f32x4 s[NR][4];
-        w.scores(
-            s, [&](int i, int j) { return pk[i * 16 * kC + ((4 * j + g) ^ swz(n))]; },
-            [&](int i) {
-              return reinterpret_cast<const u32x2*>(pk + i * 16 * kC + ((4 * R::kWide + (g >> 1)) ^ swz(n)))[g & 1];
-            });
-        const bool slow = tile * KT + KT > full || __any(bad0);
-        f16x8 p[NR][2];
-        w.softmax(a, s, p, sk0, sv0, key0, bad0, slow);
-        w.gather(
-            p,
-            [&](int t) {
-              const int d = 16 * t + n;
-              return __builtin_bit_cast(typename R::VWords, pv[d * 4 + (g ^ ((d >> 1) & 3))]);
-            },
-            slow, bad0 ? 0 : rq.len - key0);
+      const bool bad0 = bad, slow = tile * KT + KT > full || __any(bad);
+      const u32x4 *pk = sh_k[tile & 1] + n * kC, *pv = sh_v[tile & 1] + n * 4 + (g ^ swz_v(n));
+      // All of a product's codes are asked for before its first instruction, V's before the
+      // softmax where there are registers: one wait for LDS, or none, in place of one for each.
+      u32x4 kw[4][R::kWide > 0 ? R::kWide : 1];
+      u32x2 ko[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < R::kWide; ++j) kw[i][j] = pk[i * 16 * kC + ((4 * j + g) ^ swz(n))];
+        if constexpr (R::kOdd)
+          ko[i] = reinterpret_cast<const u32x2*>(pk + i * 16 * kC + ((4 * R::kWide + (g >> 1)) ^ swz(n)))[g & 1];
       }
+      if constexpr (kBatch) __builtin_amdgcn_sched_barrier(0);
+      f32x4 s[NR][4];
+      w.scores(s, [&](int i, int j) {
+        if (R::kOdd && j == R::kSteps - 1) return Widen<CACHE, T>::of(ko[i][0], ko[i][1]);
+        return Widen<CACHE, T>::of(kw[i][j >> 1][2 * (j & 1)], kw[i][j >> 1][2 * (j & 1) + 1]);
+      });
+      u32x4 vw[R::kDims];
+      auto ask_v = [&]() {
+#pragma unroll
+        for (int t = 0; t < R::kDims; ++t) vw[t] = pv[t * 64];
+        if constexpr (kBatch) __builtin_amdgcn_sched_barrier(0);
+      };
+      if constexpr (HDP < 96) ask_v();
+      f16x8 p[NR][2];
+      w.softmax(s, p, typename R::Block(a, sk, sv), key0, bad0, slow);
+      if constexpr (HDP >= 96) ask_v();
+      w.gather(p, [&](int t, int i) { return Widen<CACHE, f16>::of(vw[t][2 * i], vw[t][2 * i + 1]); });
       if (tile + 1 < most) {
-        put((tile + 1) & 1);
-        if (tile + 2 < most) {
-          load(tile + 2);
-          load_ids(tile + 3);
-        }
+        put_k((tile + 1) & 1);
+        put_v((tile + 1) & 1);
+        load_scales(next);
+        load_k(tile + 2, ids);
+        load_v(tile + 2, ids);
+        next = ids;
+        ids = load_ids(tile + 3);
       }
     }
     if (row0 < rows) {
       w.total_l();
 #pragma unroll
-      for (int r = 0; r < NR; ++r) w.store(a, rq, h, row0, r, 0, true);
+      for (int r = 0; r < NR; ++r) w.store(a, rq, h, (int)row0, r, split, chunk >= rq.len);
     }
   }
 }
 
 struct Plan {
   bool chunked;
-  int sets;    // of 16 rows, a workgroup's (decode)
-  int step;    // keys that a decode workgroup takes at a time
+  int step;  // keys that a workgroup takes at a time
   int splits, chunk;
   int64_t row_tiles;
 };
 
+// Keys of a tile: at head_dim over 128 two waves of a SIMD have no registers for 64.
 constexpr int decode_keys(int width) { return width <= 128 ? 64 : 32; }
 
-#include <stdlib.h>
-static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
 // How a call is cut.  max_new and max_len are expectations; a call that exceeds them is still
 // covered (rows in a loop, longer splits).
 Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
@@ -715,50 +824,39 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
   max_len = max_len < 1 ? 1 : max_len > 0x7fffff00 ? 0x7fffff00 : max_len;
   const int64_t group = heads / kv_heads, rows = max_new * group;
-  static const int cr = tune("CR", 64), c2 = tune("C2", 16);
-  p.chunked = rows > cr;
-  p.splits = 1;
-  if (p.chunked) {
-    const int per = cache_width(head_dim) <= 128 ? 128 : 64;
-    p.row_tiles = (rows + per - 1) / per;
-    p.chunk = 0x40000000;
-    return p;
-  }
-  p.sets = rows > c2 ? 2 : 1;
-  p.row_tiles = (rows + 16 * p.sets - 1) / (16 * p.sets);
-  p.step = 4 * decode_keys(cache_width(head_dim));
-  const int64_t base = batch * kv_heads * p.row_tiles;
-  static const int target = tune("CT", 512), one = tune("CO", 0);
-  int64_t splits = (target + base - 1) / base;
-  const int64_t most = (max_len + p.step - 1) / p.step;
+  // Past 64 rows a workgroup's keys are worth sharing among four waves' rows (18 rows of 23
+  // requests at 3000 keys of 256: 71 us so, 26 us in tiles of 16).
+  p.chunked = rows > 64;
+  p.row_tiles = p.chunked ? (rows + 127) / 128 : (rows + 15) / 16;
+  p.step = p.chunked ? 64 : 4 * decode_keys(cache_width(head_dim));
+  // Units of work before the keys are split, and splits up to 512 of them, two for each CU:
+  // 64 requests of up to 2048 keys and 8 heads took 16.9 us so and 24.7 in 1024.  A row tile
+  // of the chunk kernel is long enough to split its keys only where the chip would be empty.
+  const int64_t units = p.chunked ? (tokens * group + 127) / 128 * kv_heads : batch * kv_heads * p.row_tiles;
+  const int64_t least = p.chunked ? 1024 : p.step;
+  int64_t splits = (512 + units - 1) / units;
+  if (p.chunked && units >= 256) splits = 1;
+  // Up to 1024 keys one workgroup takes less time than the second launch that joins splits
+  // (999 keys of 4 x 32: 6.6 against 8.0 us).
+  if (!p.chunked && max_len <= 1024 && cache_width(head_dim) <= 128) splits = 1;
+  const int64_t most = (max_len + least - 1) / least;
   splits = splits < most ? splits : most;
   splits = splits < 1 ? 1 : splits > 1024 ? 1024 : splits;
-  if (max_len <= one) splits = 1;
   const int64_t even = (max_len + splits - 1) / splits;
-  int64_t chunk = (even + p.step - 1) / p.step * p.step;
-  if (chunk < p.step) chunk = p.step;
-  p.splits = (int)((max_len + chunk - 1) / chunk);
-  if (p.splits < 1) p.splits = 1;
-  p.chunk = (int)chunk;
+  p.chunk = (int)((even + p.step - 1) / p.step * p.step);
+  p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
   return p;
 }
 
 template <typename T, int CACHE, int HDP>
 hipError_t launch(const Args& a, const Plan& p, hipStream_t stream) {
-  constexpr int kKeys = decode_keys(HDP);
-  if (p.chunked) {
-    const int64_t grid = ((int64_t)a.batch * a.kv_heads + 7) / 8 * 8 * p.row_tiles;
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((cache_chunk_kernel<T, CACHE, HDP, HDP <= 128 ? 2 : 1>), dim3((unsigned)grid),
-                       dim3(256), 0, stream, a);
-    return hipGetLastError();
-  }
   const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles * p.splits;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (p.sets == 1)
-    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP, 1, kKeys, 4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  if (p.chunked)
+    hipLaunchKernelGGL((cache_chunk_kernel<T, CACHE, HDP, 2>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP, 2, kKeys, 4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP, decode_keys(HDP)>), dim3((unsigned)grid), dim3(256), 0,
+                       stream, a);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)a.tokens * a.heads;
     if (p.splits > 16)
@@ -794,7 +892,9 @@ int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads,
 
 hipError_t run_cache_attn(const CacheAttnArgs& c, int64_t workspace_bytes, hipStream_t stream) {
   const int width = cache_width(c.head_dim);
-  if (width < 0 || c.tokens <= 0 || c.tokens > 0x7fffffff || c.batch <= 0 || c.table_width <= 0) return hipErrorInvalidValue;
+  if (width < 0 || c.tokens <= 0 || c.tokens > 0x7fffffff || c.batch <= 0 || c.table_width <= 0 ||
+      c.tokens * c.heads > 0x7fffff00)  // rows of a kv head are counted in 32 bits
+    return hipErrorInvalidValue;
   const Plan p = plan_of(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.max_new, c.max_len);
   Args a{};
   a.q = c.q;

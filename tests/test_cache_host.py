@@ -96,7 +96,7 @@ def test_workspace_query():
     assert q(0, 4, 8, 8, 64, 1, 1000) == 0 and q(4, 0, 8, 8, 64, 1, 1000) == 0
     assert q(4, 4, 8, 3, 64, 1, 1000) == -1 and q(4, 4, 8, 8, 60, 1, 1000) == -1
     assert q(-1, 4, 8, 8, 64, 1, 1000) == -1 and q(4, 4, 8, 8, 64, -1, 1000) == -1
-    assert q(2048, 1, 8, 8, 64, 2048, 4096) == 0  # many rows: no split
+    assert q(8192, 4, 32, 8, 64, 2048, 4096) == 0  # many rows of many heads: no split
     for length in (1, 1000, 100000, 2 ** 31 - 1, 2 ** 40):
         n = q(64, 64, 8, 8, 64, 1, length)
         assert 0 <= n <= 1025 * 64 * 8 * (64 * 4 + 8)
