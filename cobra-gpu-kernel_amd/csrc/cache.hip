@@ -346,40 +346,48 @@ __device__ __forceinline__ float group_max(float v, float* red) {
   return v;
 }
 
-// One workgroup writes what a call brings to one (block, head).  It belongs to the block's
-// first token in the call (tokens of a block stand next to each other in the call).  A
-// workgroup looks for first ones among `window` (<= 63) tokens, one a lane.  Where a run writes
-// offset 0 the block starts anew: its scales come from this call's tokens alone.
+// One workgroup writes what a call brings to the keys (blockIdx.z 0) or values (1) of one
+// (block, head).  It belongs to the block's first token in the call (tokens of a block stand
+// next to each other in the call).  A workgroup looks for first ones among `window` (<= 63)
+// tokens, one a lane.  Where a run writes offset 0 the block starts anew: its scale comes from
+// this call's tokens alone.
 //
 // The values are read twice, for the largest and for the codes; the second time they come from
-// the caches.  K's rows are written eight codes to a store.  V's rows run along tokens: a thread
-// takes 4 tokens x 8 dimensions and writes eight words of 4 codes, neighbouring lanes
-// neighbouring words of a row.
+// the caches (kept in registers in between they cost the occupancy that hides the first: 14000
+// tokens of 8 x 128 took 66 us so, 30 us as it is).  K's rows are written eight codes to a
+// store.  V's rows run along tokens: a thread takes 4 tokens x 8 dimensions and writes eight
+// words of 4 codes, neighbouring lanes neighbouring words of a row.
 template <typename T, int CACHE, int NT>
-__global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window) {
+__global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window, int share) {
+  typedef typename Op16<T>::V8 V8;
   __shared__ int src[kMaxBlock];  // token of each offset of the block, -1: none
-  __shared__ float red[2][NT / 64];
+  __shared__ float red[NT / 64];
   __shared__ int range[2];
   const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
+  const bool values = blockIdx.z != 0;
   const int bs = 1 << a.shift, hd = a.head_dim, hdp = a.width, pieces = hd >> 3, wide = hdp >> 3;
   const int64_t slots_end = a.num_blocks << a.shift;
-  const int64_t w0 = (int64_t)blockIdx.x * window;
+  const int windows = gridDim.x / share;  // ids apart by it share one: neighbours, on different XCDs, all have work
+  const int64_t w0 = (int64_t)(blockIdx.x % windows) * window;
+  const T* x0 = static_cast<const T*>(a.qkv) + (int64_t)(a.heads + (values ? a.kv_heads : 0) + head) * hd;
+  uint8_t* codes = static_cast<uint8_t*>(values ? a.v : a.k);
+  float* scales = values ? a.v_scale : a.k_scale;
   // Lane i has the slot of token w0 - 1 + i.
   int64_t slot = -1;
   {
     const int64_t t = w0 - 1 + lane;
-    if (lane <= window && t >= 0 && t < a.tokens) slot = a.slots[t];
+    if (t >= 0 && t < a.tokens) slot = a.slots[t];
   }
   const int64_t before = __shfl_up(slot, 1);
   uint64_t firsts = __ballot(lane >= 1 && lane <= window && slot >= 0 && slot < slots_end &&
                              (before < 0 || (before >> a.shift) != (slot >> a.shift)));
-  while (firsts) {
+  for (int turn = blockIdx.x / windows; firsts; firsts &= firsts - 1) {
+    if (turn-- > 0) continue;
+    turn = share - 1;
     const int f = __builtin_ctzll(firsts);
-    firsts &= firsts - 1;
     const int64_t t0 = w0 - 1 + f, blk = __shfl(slot, f) >> a.shift;
     const int64_t bh = blk * a.kv_heads + head;
-    const float least = pow2(kScaleMin), most = pow2(kScaleMax);
-    const float k0 = fminf(fmaxf(a.k_scale[bh], least), most), v0 = fminf(fmaxf(a.v_scale[bh], least), most);
+    const float had = fminf(fmaxf(scales[bh], pow2(kScaleMin)), pow2(kScaleMax));
     // The run of tokens that go to this block; of two for one slot the later one stays.
     __syncthreads();
     for (int o = tid; o < bs; o += NT) src[o] = -1;
@@ -410,118 +418,149 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
     }
     __syncthreads();
     const int lo = range[0], hi = range[1];
-    const T* kq = static_cast<const T*>(a.qkv) + (int64_t)(a.heads + head) * hd;
-    const T* vq = kq + (int64_t)a.kv_heads * hd;
-    float ka = 0.f, va = 0.f;
-    for (int i = lo * pieces + tid; i < (hi + 1) * pieces; i += NT) {
-      const int off = i / pieces, p = i - off * pieces, t = src[off];
-      if (t < 0) continue;
-      float x[8], y[8];
-      load8(kq + t * a.ld + 8 * p, x);
-      load8(vq + t * a.ld + 8 * p, y);
+    // Item i: piece p of offset `off` (keys), or piece p of quad q's four offsets (values).
+    const int q0 = lo >> 2, quads = (hi >> 2) + 1 - q0;
+    const int items = values ? quads * pieces : (hi + 1 - lo) * pieces;
+    float amax = 0.f;
+    // Where there is no token the run's first one is read: loads without a branch between them
+    // are in flight together.
+    auto read = [&](int token, int p) {
+      return *reinterpret_cast<const V8*>(x0 + (token < 0 ? (int)t0 : token) * a.ld + 8 * p);
+    };
+    auto largest = [&](const V8& x) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ka = fmaxf(ka, finite_abs(x[e]));
-        va = fmaxf(va, finite_abs(y[e]));
-      }
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs((float)x[e]));
+    };
+    // For the largest the order does not matter: keys and values alike in rows.
+    const int all = (hi + 1 - lo) * pieces;
+#pragma unroll 4
+    for (int i = tid; i < all; i += NT) {
+      const int r = i / pieces;
+      largest(read(src[lo + r], i - r * pieces));
     }
-    ka = group_max<NT>(ka, red[0]);
-    va = group_max<NT>(va, red[1]);
-    float ks = pow2(scale_exponent<CACHE>(ka)), vs = pow2(scale_exponent<CACHE>(va));
-    float kr = 1.f, vr = 1.f;
-    bool kgrow = false, vgrow = false;
+    amax = group_max<NT>(amax, red);
+    float scale = pow2(scale_exponent<CACHE>(amax)), ratio = 1.f;
+    bool grow = false;
     if (lo > 0) {
-      kgrow = ks > k0;
-      vgrow = vs > v0;
-      kr = kgrow ? k0 / ks : 1.f;
-      vr = vgrow ? v0 / vs : 1.f;
-      ks = fmaxf(ks, k0);
-      vs = fmaxf(vs, v0);
+      grow = scale > had;
+      ratio = grow ? had / scale : 1.f;
+      scale = fmaxf(scale, had);
     }
-    if (tid == 0) {  // every thread has read the old ones: there was a barrier since
-      a.k_scale[bh] = ks;
-      a.v_scale[bh] = vs;
-    }
-    const float ki = 1.f / ks, vi = 1.f / vs;
-    uint8_t* kc = static_cast<uint8_t*>(a.k) + bh * bs * hdp;
-    for (int i = (kgrow ? 0 : lo) * wide + tid; i < (hi + 1) * wide; i += NT) {
-      const int off = i / wide, p = i - off * wide, t = src[off];
-      uint2* to = reinterpret_cast<uint2*>(kc + (int64_t)i * 8);
-      uint2 w = {0u, 0u};
-      if (t >= 0) {
-        if (p < pieces) {
-          float x[8];
-          load8(kq + t * a.ld + 8 * p, x);
-          w.x = quant2<CACHE>(x[0] * ki, x[1] * ki) | (quant2<CACHE>(x[2] * ki, x[3] * ki) << 16);
-          w.y = quant2<CACHE>(x[4] * ki, x[5] * ki) | (quant2<CACHE>(x[6] * ki, x[7] * ki) << 16);
-        }
-      } else if (kgrow && off < lo) {
-        w = *to;
-        w.x = regrade<CACHE>(w.x, kr);
-        w.y = regrade<CACHE>(w.y, kr);
-      } else {
-        continue;
+    if (tid == 0) scales[bh] = scale;  // every thread has read the old one: there was a barrier since
+    const float inv = 1.f / scale;
+    uint8_t* to = codes + bh * bs * hdp;
+    if (!values) {
+      auto put = [&](int off, int p, const V8& x) {
+        uint2 w;
+        w.x = quant2<CACHE>((float)x[0] * inv, (float)x[1] * inv) |
+              (quant2<CACHE>((float)x[2] * inv, (float)x[3] * inv) << 16);
+        w.y = quant2<CACHE>((float)x[4] * inv, (float)x[5] * inv) |
+              (quant2<CACHE>((float)x[6] * inv, (float)x[7] * inv) << 16);
+        *reinterpret_cast<uint2*>(to + off * hdp + 8 * p) = w;
+      };
+#pragma unroll 4
+      for (int i = tid; i < items; i += NT) {
+        const int r = i / pieces, p = i - r * pieces;
+        const V8 x = read(src[lo + r], p);
+        if (src[lo + r] >= 0) put(lo + r, p, x);
       }
-      *to = w;
-    }
-    uint8_t* vc = static_cast<uint8_t*>(a.v) + bh * bs * hdp;
-    const int q0 = (vgrow ? 0 : lo) >> 2, quads = (hi >> 2) + 1 - q0;
-    for (int i = tid; i < quads * wide; i += NT) {
-      const int p = i / quads, q = q0 + (i - p * quads);
-      uint8_t* to = vc + (int64_t)p * 8 * bs + 4 * q;
-      uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-      uint32_t put = 0, old = 0;  // bytes of new codes, of codes to round again
+      const int tail = wide - pieces;  // zeros up to the row's width
+      if (tail > 0)
+        for (int i = tid; i < (hi + 1 - lo) * tail; i += NT) {
+          const int r = i / tail, p = pieces + (i - r * tail);
+          if (src[lo + r] >= 0) *reinterpret_cast<uint2*>(to + (lo + r) * hdp + 8 * p) = uint2{0u, 0u};
+        }
+      if (grow)  // tokens of a run may leave offsets out: they are not the call's
+        for (int i = tid; i < lo * wide; i += NT) {
+          uint2* w = reinterpret_cast<uint2*>(to + (int64_t)i * 8);
+          uint2 c = *w;
+          c.x = regrade<CACHE>(c.x, ratio);
+          c.y = regrade<CACHE>(c.y, ratio);
+          *w = c;
+        }
+    } else {
+      // Eight rows' words of quad q: new codes where there are tokens, old ones rounded again
+      // below lo, others left.
+      auto put = [&](int q, int p, const V8 (&x)[4]) {
+        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}, mask = 0, old = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = src[4 * q + j];
-        if (t >= 0) {
-          put |= 0xffu << (8 * j);
-          if (p < pieces) {
-            float x[8];
-            load8(vq + t * a.ld + 8 * p, x);
+        for (int j = 0; j < 4; ++j) {
+          if (src[4 * q + j] >= 0) {
+            mask |= 0xffu << (8 * j);
+            if (p < pieces) {
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const uint32_t c = quant2<CACHE>(x[e] * vi, x[e + 1] * vi);
-              w[e] |= (c & 0xffu) << (8 * j);
-              w[e + 1] |= (c >> 8) << (8 * j);
+              for (int e = 0; e < 8; e += 2) {
+                const uint32_t c = quant2<CACHE>((float)x[j][e] * inv, (float)x[j][e + 1] * inv);
+                w[e] |= (c & 0xffu) << (8 * j);
+                w[e + 1] |= (c >> 8) << (8 * j);
+              }
             }
+          } else if (grow && 4 * q + j < lo) {
+            old |= 0xffu << (8 * j);
           }
-        } else if (vgrow && 4 * q + j < lo) {
-          old |= 0xffu << (8 * j);
         }
+        uint8_t* at = to + (int64_t)p * 8 * bs + 4 * q;
+        if (mask == 0xffffffffu) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) *reinterpret_cast<uint32_t*>(at + e * bs) = w[e];
+        } else if (old) {
+          uint32_t was[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) was[e] = *reinterpret_cast<const uint32_t*>(at + e * bs);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint32_t*>(at + e * bs) =
+                (w[e] & mask) | (regrade<CACHE>(was[e], ratio) & old) | (was[e] & ~(mask | old));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (mask >> (8 * j) & 1u) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) at[e * bs + j] = (uint8_t)(w[e] >> (8 * j));
+            }
+        }
+      };
+      V8 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = zero8_of<T>();
+#pragma unroll 2
+      for (int i = tid; i < items; i += NT) {
+        const int p = i / quads, q = q0 + (i - p * quads);
+        V8 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] = read(src[4 * q + j], p);
+        }
+        put(q, p, y);
       }
-      if (put == 0xffffffffu) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint32_t*>(to + e * bs) = w[e];
-      } else if (old) {
-        uint32_t had[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) had[e] = *reinterpret_cast<const uint32_t*>(to + e * bs);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<uint32_t*>(to + e * bs) =
-              (w[e] & put) | (regrade<CACHE>(had[e], vr) & old) | (had[e] & ~(put | old));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (put >> (8 * j) & 1u) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) to[e * bs + j] = (uint8_t)(w[e] >> (8 * j));
-          }
+      const int tail = wide - pieces;
+      for (int i = tid; i < quads * tail; i += NT) {
+        const int p = i / quads;
+        put(q0 + (i - p * quads), pieces + p, x);
       }
+      if (grow)  // the quads below the first one written
+        for (int i = tid; i < q0 * wide; i += NT) {
+          const int p = i / q0;
+          put(i - p * q0, p, x);
+        }
     }
   }
 }
 
 template <typename T, int CACHE>
 void launch_append(const CacheAppendArgs& a, hipStream_t stream) {
-  // Few tokens: a wave for each.  Many: they are prompts, whose blocks begin every bs tokens.
-  const int window = a.tokens * a.kv_heads <= 8192 ? 1 : 16;
-  const dim3 grid((unsigned)((a.tokens + window - 1) / window), (unsigned)a.kv_heads);
-  if (window == 1 || (a.head_dim << a.shift) <= 4096)
-    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 64>), grid, dim3(64), 0, stream, a, window);
+  // Few tokens: a workgroup for each.  Many: they are prompts, whose blocks begin every bs
+  // tokens; one and a half times as many workgroups for 63 of them as they have blocks, as some
+  // end inside one (2400 tokens of 6 x 40 in blocks of 16: 7.9 us with 6, 10.2 with 4, 22 with
+  // one; 14000 of 8 x 128 in blocks of 64: 30.4 us with 2, 36.5 with one).
+  const bool few = a.tokens * a.kv_heads <= 8192;
+  const int window = few ? 1 : 63, share = few ? 1 : (96 + (1 << a.shift) - 1) >> a.shift;
+  const dim3 grid((unsigned)((a.tokens + window - 1) / window * share), (unsigned)a.kv_heads, 2);
+  // A wave for up to 8192 values (64 x 128: 30.4 us, 33.0 with four waves).
+  if (few || (a.head_dim << a.shift) <= 8192)
+    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 64>), grid, dim3(64), 0, stream, a, window, share);
   else
-    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 256>), grid, dim3(256), 0, stream, a, window);
+    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 256>), grid, dim3(256), 0, stream, a, window, share);
 }
 
 }  // namespace
