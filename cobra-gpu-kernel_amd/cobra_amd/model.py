@@ -41,12 +41,13 @@ from __future__ import annotations
 
 import gc
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
 
 from . import ops, streaming
+from .cache import CobraCache
 from .layer import CobraSelfAttention
 from .padding import PadGeometry, pad_block_weights
 
@@ -361,6 +362,61 @@ class CobraTransformer(nn.Module):
             if not last:
                 h, h_next = out, h
         return out
+
+    # -- new tokens over a cache ------------------------------------------------------
+
+    def make_cache(self, requests: int, num_blocks: int, block_size: int = 64,
+                   dtype: torch.dtype = torch.float8_e4m3fn, max_len: Optional[int] = None) -> CobraCache:
+        """A ``CobraCache`` of this model's layers and heads, on its device."""
+        return CobraCache(self.config.num_layers, self.config.num_heads, self._geom.hdp, requests, num_blocks,
+                          block_size, dtype, max_len, self.final_norm.weight.device)
+
+    def extend(self, x: torch.Tensor, cache: CobraCache, new_lens: torch.Tensor, max_new: Optional[int] = None,
+               max_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The causal stack over new tokens of the requests in ``cache`` -> ``(y, missing)``.
+
+        x: [T, d_model], request b's ``new_lens[b]`` (int32 device tensor) tokens after those of
+        b - 1; y: [T, d_model] in x.dtype, what ``forward`` gives for these tokens at the ends of
+        their sequences, up to the cache's 8 bits for keys and values.  The cache then holds them
+        too (``cache.trim`` takes them back).  ``missing``: as ``ops.cache_reserve``; where it is
+        not 0 nothing was reserved and y holds no results.  Rows past the last request's have none
+        either.  ``max_new`` / ``max_len``: expected bounds on a request's new tokens and length
+        (speed only).  Every launch is the library's own, with the ops of the composed forward.
+        """
+        cfg, g = self.config, self._geom
+        if not cfg.causal:
+            raise ValueError("extend needs a causal model: a cached token has not seen the ones after it")
+        if x.dim() != 2 or x.shape[1] != cfg.d_model:
+            raise ValueError(f"x must be [T, {cfg.d_model}], got {tuple(x.shape)}")
+        if x.dtype not in (torch.float16, torch.float32, torch.bfloat16):
+            raise TypeError(f"x dtype {x.dtype} not supported (float16, bfloat16 or float32)")
+        if (cache.layers, cache.kv_heads, cache.head_dim) != (cfg.num_layers, cfg.num_heads, g.hdp):
+            raise ValueError(f"the cache is for {cache.layers} layers of {cache.kv_heads} heads of {cache.head_dim}, "
+                             f"the model has {cfg.num_layers} of {cfg.num_heads} of {g.hdp}")
+        packs = self._packed(x.dtype)
+        op = self._op
+        x = x.contiguous()
+        T, D = x.shape
+        H, eps, scale = cfg.num_heads, self.final_norm.eps, g.hd ** -0.5
+        slots, cu, missing = cache.reserve(new_lens, T)
+        if T == 0:
+            return torch.empty_like(x), missing
+        r = torch.zeros((T, g.dp), device=x.device, dtype=torch.float32)
+        ctx = torch.zeros((T, g.e), device=x.device, dtype=op)  # rows of no request stay zero
+        h = ops.ln_strided(x, D, packs[0].ln1_w, packs[0].ln1_b, out_cols=g.dp, out_dtype=op, resid_out=r, eps=eps)
+        n = len(packs)
+        for i, p in enumerate(packs):
+            last = i == n - 1
+            nw, nb = self._final if last else (packs[i + 1].ln1_w, packs[i + 1].ln1_b)
+            qkv = ops.linear(h, p.w_qkv, p.b_qkv)
+            cache.append(i, qkv, slots, H)
+            cache.attn(i, qkv, cu, H, scale, max_new=max_new, max_len=max_len, out=ctx)
+            r = ops.linear(ctx, p.w_o, p.b_o, out_fp32=True, resid=r)
+            h2 = ops.ln_strided(r, D, p.ln2_w, p.ln2_b, out_cols=g.dp, out_dtype=op, eps=eps)
+            hid = ops.linear(h2, p.w1, p.b1, gelu=True)
+            r = ops.linear(hid, p.w2, p.b2, out_fp32=True, resid=r)
+            h = ops.ln_strided(r, D, nw, nb, out_cols=D if last else g.dp, out_dtype=x.dtype if last else op, eps=eps)
+        return h, missing
 
     def _run_graphed(self, x, m, packs):
         if self._graph is None:

@@ -178,3 +178,16 @@ def test_plain_form_tables_round_trip():
     assert slots == [7 * 16 + i for i in range(5, 16)] + [4 * 16, 5 * 16, -1]
     assert oc.trim(lens, before[0], table, free, 16, count, 6) == (0, 5)
     assert [lens, free] == before
+
+
+def test_cache_refuses_before_it_allocates():
+    from cobra_amd import CobraCache
+
+    ok = dict(layers=1, kv_heads=2, head_dim=64, requests=2, num_blocks=4, device="cpu")
+    for kw, match in ((dict(layers=0), "layers"), (dict(kv_heads=0), "kv_heads"), (dict(requests=-1), "requests"),
+                      (dict(num_blocks=0), "num_blocks"), (dict(block_size=48), "block_size"),
+                      (dict(head_dim=60), "multiples of 8"), (dict(), "GPU")):
+        with pytest.raises(ValueError, match=match):
+            CobraCache(**dict(ok, **kw))
+    with pytest.raises(TypeError, match="float8_e4m3fn or int8"):
+        CobraCache(**dict(ok, dtype=torch.float16))
