@@ -390,6 +390,9 @@ class CobraTransformer(nn.Module):
             raise ValueError(f"x must be [T, {cfg.d_model}], got {tuple(x.shape)}")
         if x.dtype not in (torch.float16, torch.float32, torch.bfloat16):
             raise TypeError(f"x dtype {x.dtype} not supported (float16, bfloat16 or float32)")
+        if x.device != cache.lens.device or x.device != self.final_norm.weight.device:
+            raise ValueError(f"x is on {x.device}, the cache on {cache.lens.device}, the model on "
+                             f"{self.final_norm.weight.device}")
         if (cache.layers, cache.kv_heads, cache.head_dim) != (cfg.num_layers, cfg.num_heads, g.hdp):
             raise ValueError(f"the cache is for {cache.layers} layers of {cache.kv_heads} heads of {cache.head_dim}, "
                              f"the model has {cfg.num_layers} of {cfg.num_heads} of {g.hdp}")

@@ -548,19 +548,23 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
 }
 
 template <typename T, int CACHE>
-void launch_append(const CacheAppendArgs& a, hipStream_t stream) {
+hipError_t launch_append(const CacheAppendArgs& a, hipStream_t stream) {
   // Few tokens: a workgroup for each.  Many: they are prompts, whose blocks begin every bs
   // tokens; one and a half times as many workgroups for 63 of them as they have blocks, as some
   // end inside one (2400 tokens of 6 x 40 in blocks of 16: 7.9 us with 6, 10.2 with 4, 22 with
   // one; 14000 of 8 x 128 in blocks of 64: 30.4 us with 2, 36.5 with one).
   const bool few = a.tokens * a.kv_heads <= 8192;
   const int window = few ? 1 : 63, share = few ? 1 : (96 + (1 << a.shift) - 1) >> a.shift;
-  const dim3 grid((unsigned)((a.tokens + window - 1) / window * share), (unsigned)a.kv_heads, 2);
   // A wave for up to 8192 values (64 x 128: 30.4 us, 33.0 with four waves).
-  if (few || (a.head_dim << a.shift) <= 8192)
+  const bool wave = few || (a.head_dim << a.shift) <= 8192;
+  const int64_t groups = (a.tokens + window - 1) / window * share;
+  if (groups * (wave ? 64 : 256) > 0xffffffff) return hipErrorInvalidValue;  // threads are counted in 32 bits
+  const dim3 grid((unsigned)groups, (unsigned)a.kv_heads, 2);
+  if (wave)
     hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 64>), grid, dim3(64), 0, stream, a, window, share);
   else
     hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 256>), grid, dim3(256), 0, stream, a, window, share);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -607,10 +611,8 @@ hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream) {
 hipError_t run_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
   if (a.tokens <= 0 || a.tokens > 0x7fffffff || a.kv_heads > 65535) return hipErrorInvalidValue;
   if (a.dtype == kF16)
-    a.cache == kCacheE4M3 ? launch_append<f16, kCacheE4M3>(a, stream) : launch_append<f16, kCacheI8>(a, stream);
-  else
-    a.cache == kCacheE4M3 ? launch_append<bf16, kCacheE4M3>(a, stream) : launch_append<bf16, kCacheI8>(a, stream);
-  return hipGetLastError();
+    return a.cache == kCacheE4M3 ? launch_append<f16, kCacheE4M3>(a, stream) : launch_append<f16, kCacheI8>(a, stream);
+  return a.cache == kCacheE4M3 ? launch_append<bf16, kCacheE4M3>(a, stream) : launch_append<bf16, kCacheI8>(a, stream);
 }
 
 }  // namespace cobra

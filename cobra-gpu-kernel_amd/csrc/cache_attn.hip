@@ -35,6 +35,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kBias = 8.f;         // log2 of w where u equals its reference
 constexpr float kAccept = 57344.f;   // a lane's sum of w that is taken without a maximum
+// Keys of a request that are attended to: what is left to 2^31 covers the rounding up of splits
+// and the tiles that loads are ahead.
+constexpr int64_t kMaxKeys = 0x7ffff000;
+// Workgroups of a launch: of 256 threads, which are counted in 32 bits.
+constexpr int64_t kMaxGrid = 0xffffff;
 
 __device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -147,7 +152,7 @@ __device__ __forceinline__ Request request_of(const Args& a, int b) {
   const int t1 = a.cu[b + 1];
   r.n = t1 - r.t0;
   if (r.t0 < 0 || t1 > a.tokens || r.n < 0) r.n = 0;
-  const int64_t most = min(a.table_width << a.shift, (int64_t)0x7fffff00);
+  const int64_t most = min(a.table_width << a.shift, kMaxKeys);
   const int len = a.lens[b];
   r.len = len < 0 ? 0 : len > most ? (int)most : len;
   return r;
@@ -599,17 +604,23 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
 }
 
 // Many rows for each kv head: a wave has NR sets of 16 and passes over all of their keys.  Tiles
-// of 64 keys go through LDS, widened to 16 bits on the way, once for the four waves (each wave
-// taking its codes from the caches by itself asked 7 TB/s of L2 and waited for half of its
-// time; each widening all of them took a quarter of its vector instructions).  LDS holds
-// 16-byte chunks in the order in which lanes read them, XOR-swizzled by row so that the 16
-// lanes of a column meet 16 different places of 256 bytes.  Two stages: a tile is in
-// registers while the one before it is in LDS and the one before that in use.
+// of 64 keys go through LDS as codes, once for the four waves: each wave taking them from the
+// caches by itself asked 7 TB/s of L2 and waited for half of its time.  Each wave widens what
+// it reads: held in 16 bits, widened once, a tile takes twice the LDS reads, which cost more
+// (1187 us against 1132).  Codes lie in 16-byte pieces, XOR-swizzled by row so that the eight
+// lanes which LDS serves at a time meet eight different places of 128 bytes.  Two stages: a
+// tile is in registers while the one before it is in LDS and the one before that in use.
+// Sets of 32 rows a wave, so that each widened code feeds two matrix instructions; two
+// workgroups to a CU up to head_dim 128.
+//
+// Bound by the vector ALU: for each of a lane's scores an fma, an exponential, a conversion and
+// an addition beside the matrix instructions, of which only the exponential and the codes'
+// conversion overlap them.  8 requests of 2048 new tokens over up to 8192 keys, 32 heads of 128
+// on 8 (bf16): 960 to 997 us, 0.92 to 0.95 PFLOP/s.
 template <typename T, int CACHE, int HDP, int NR>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a) {
   constexpr int kWaves = 4, kRows = kWaves * NR * 16, KT = 64;
   typedef Rows<T, CACHE, HDP, NR, KT> R;
-  typedef typename R::V8 V8;
   constexpr int kC = HDP / 16, kPer = (HDP + 63) / 64;  // 16 codes each: of a K row; a thread's of K, of V
   constexpr bool kAll = HDP % 64 == 0;
   // At head_dim 128 int8's widening leaves no registers for a product's codes at once.
@@ -822,7 +833,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
              int64_t max_len) {
   Plan p{};
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
-  max_len = max_len < 1 ? 1 : max_len > 0x7fffff00 ? 0x7fffff00 : max_len;
+  max_len = max_len < 1 ? 1 : max_len > kMaxKeys ? kMaxKeys : max_len;
   const int64_t group = heads / kv_heads, rows = max_new * group;
   // Past 64 rows a workgroup's keys are worth sharing among four waves' rows (18 rows of 23
   // requests at 3000 keys of 256: 71 us so, 26 us in tiles of 16).
@@ -836,6 +847,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   const int64_t least = p.chunked ? 1024 : p.step;
   int64_t splits = (512 + units - 1) / units;
   if (p.chunked && units >= 256) splits = 1;
+  if (tokens * heads > kMaxGrid) splits = 1;  // max_new is far off
   // Up to 1024 keys one workgroup takes less time than the second launch that joins splits
   // (999 keys of 4 x 32: 6.6 against 8.0 us).
   if (!p.chunked && max_len <= 1024 && cache_width(head_dim) <= 128) splits = 1;
@@ -845,13 +857,16 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   const int64_t even = (max_len + splits - 1) / splits;
   p.chunk = (int)((even + p.step - 1) / p.step * p.step);
   p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
+  // Workgroups go round the row tiles of their request where these are fewer than it has.
+  const int64_t tiles = kMaxGrid / (batch * kv_heads * p.splits);
+  if (p.row_tiles > tiles) p.row_tiles = tiles > 1 ? tiles : 1;
   return p;
 }
 
 template <typename T, int CACHE, int HDP>
 hipError_t launch(const Args& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles * p.splits;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (grid > kMaxGrid) return hipErrorInvalidValue;
   if (p.chunked)
     hipLaunchKernelGGL((cache_chunk_kernel<T, CACHE, HDP, 2>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   else

@@ -546,6 +546,9 @@ int cobra_cache_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* c
       !aligned_to(block_table, 4) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
     return kBad;
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return kBad;
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), c0 = reinterpret_cast<uintptr_t>(ctx);
+  const uintptr_t row = static_cast<uintptr_t>(heads * head_dim);  // ctx would be read as queries
+  if (q0 < c0 + 2 * tokens * row && c0 < q0 + 2 * ((tokens - 1) * ldq + row)) return kBad;
   cobra::CacheAttnArgs a{};
   a.q = q;
   a.out = ctx;

@@ -382,7 +382,7 @@ PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Pool p;
     if (!cu || !lens || !table || !p.read(a + 7, dev, heads, hd) || lens->dim() != 1 || table->dim() != 2) return none();
     const int64_t T = q->size(0), B = lens->size(0), W = table->size(1);
-    if (T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) || table->size(0) != B) return none();
+    if (!PyBool_Check(a[11]) || T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) || table->size(0) != B) return none();
     int64_t new_most = T - B + 1, len_most = W * p.block;
     if (a[12] != Py_None && !py_int(a[12], &new_most)) return none();
     if (a[13] != Py_None && !py_int(a[13], &len_most)) return none();
@@ -404,7 +404,7 @@ PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         q->data_ptr(), dt, q->size(1), cu->data_ptr<int>(), lens->data_ptr<int>(), table->data_ptr<int>(), W,
         p.k->data_ptr(), p.v->data_ptr(), p.k_scale->data_ptr<float>(), p.v_scale->data_ptr<float>(), p.cache,
         out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, T, B, p.blocks, p.block, heads, p.kv_heads, hd,
-        new_most, len_most, static_cast<float>(PyFloat_AS_DOUBLE(a[6])), PyObject_IsTrue(a[11]) == 1 ? 1 : 0,
+        new_most, len_most, static_cast<float>(PyFloat_AS_DOUBLE(a[6])), a[11] == Py_True ? 1 : 0,
         c10::hip::getCurrentHIPStream(dev).stream());
     if (code != 0) return none();
     if (a[14] != Py_None) {

@@ -198,7 +198,8 @@ int cobra_cache_reserve(int32_t* lens, const int32_t* new_lens, int32_t* block_t
  * Requests cut to min(lens[b], max(keep_lens[b], 0)) tokens (0: the request is over), their
  * blocks past that given back: the k-th of them (requests in order, a request's blocks in
  * order) to free_list[free_count' - 1 - k], free_count' the new height, so that a trim to the
- * old lengths undoes a reserve.  block_table keeps its entries.  refused = 0; or 1, and nothing
+ * old lengths undoes a reserve.  A block belongs to one request: one that two rows list is
+ * given back twice.  block_table keeps its entries.  refused = 0; or 1, and nothing
  * else changes, where a length is negative or longer than a row of the table, or the stack
  * would not hold the blocks.  workspace: [batch] int32.
  */
@@ -216,7 +217,8 @@ int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* blo
  *     written become those of the same values under it;
  *     code = x / scale rounded to the nearest (ties to even), within +-qmax; NaN gives 0.
  * Tokens of one block stand next to each other in the call, as cobra_cache_reserve lays them
- * out; of two for one slot the later one stays.  A token whose slot is negative or past the
+ * out (where they do not, that block's contents are unspecified); of two for one slot the
+ * later one stays.  A token whose slot is negative or past the
  * pool is passed over.  Blocks without a token are left as they are.
  */
 int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* slots, void* k, void* v, float* k_scale,
@@ -228,8 +230,10 @@ int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* sl
  *     ctx_i = softmax_j((q_i . k_j) * scale) v_j over keys j <= lens[b] - n_b + i (causal) or
  *     j < lens[b], for new token i of n_b = cu[b + 1] - cu[b]; no key: a zero row.
  * q: [tokens, ldq] in dtype, its first heads * head_dim columns (a packed q | k | v buffer will
- * do); query head j reads kv head j / (heads / kv_heads).  ctx: [tokens, heads * head_dim];
- * rows outside [cu[0], cu[batch]) are left as they are.  Scores, softmax and sums are fp32,
+ * do); query head j reads kv head j / (heads / kv_heads).  ctx: [tokens, heads * head_dim],
+ * tokens * heads < 2^31 - 256, batch * kv_heads < 2^24, not overlapping q (refused); of a
+ * request's keys the first 2^31 - 4096 count; rows outside [cu[0], cu[batch]) are left as
+ * they are.  Scores, softmax and sums are fp32,
  * the probabilities rounded to fp16 for the product with V's codes; scales are taken within
  * [2^-40, 2^40].  Keys in a block whose id is outside the pool are masked.  max_new and max_len: the most new
  * tokens and keys that a request is expected to have; they shape the launch and never the

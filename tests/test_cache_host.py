@@ -53,7 +53,7 @@ def test_abi_rejects_bad_tables():
 def test_abi_rejects_bad_append_and_attention():
     lib, m = _lib()
     ok = dict(q=256, dt=m.F16, ld=12 * 64, slots=256, k=256, v=256, ks=256, vs=256, cache=m.CACHE_E4M3, t=4, nb=8,
-              bs=16, h=8, kv=2, hd=64, cu=256, lens=256, table=256, w=4, ctx=256, ws=None, wsb=0, b=2, new=1, len=64,
+              bs=16, h=8, kv=2, hd=64, cu=256, lens=256, table=256, w=4, ctx=1 << 20, ws=None, wsb=0, b=2, new=1, len=64,
               scale=0.125)
 
     def append(**kw):
@@ -81,6 +81,10 @@ def test_abi_rejects_bad_append_and_attention():
                dict(ctx=264), dict(nb=0), dict(b=-1), dict(new=-1), dict(len=-1), dict(scale=0.0), dict(scale=-1.0),
                dict(scale=float("nan")), dict(cu=258)):
         assert attn(**kw) != 0, kw
+    assert attn(t=1 << 30, b=1 << 30, ctx=1 << 50) != 0  # tokens x heads past 2^31
+    assert attn(t=1 << 24, b=1 << 24, ctx=1 << 50) != 0  # more workgroups than a launch has
+    for ctx in (256, 256 + 3 * 12 * 128 + 8 * 128 - 16, 16):  # over the queries
+        assert attn(ctx=ctx) != 0, ctx
     assert attn(t=0, q=None, ctx=None) == 0 and attn(b=0, cu=None) == 0
     # a call that splits its keys needs the workspace it asks for
     need = lib.cobra_cache_attn_workspace_bytes(1, 1, 8, 2, 64, 1, 100000)
@@ -97,6 +101,7 @@ def test_workspace_query():
     assert q(4, 4, 8, 3, 64, 1, 1000) == -1 and q(4, 4, 8, 8, 60, 1, 1000) == -1
     assert q(-1, 4, 8, 8, 64, 1, 1000) == -1 and q(4, 4, 8, 8, 64, -1, 1000) == -1
     assert q(8192, 4, 32, 8, 64, 2048, 4096) == 0  # many rows of many heads: no split
+    assert q(1 << 22, 1, 8, 8, 64, 1, 100000) == 0  # no workspace for every row of so many
     for length in (1, 1000, 100000, 2 ** 31 - 1, 2 ** 40):
         n = q(64, 64, 8, 8, 64, 1, length)
         assert 0 <= n <= 1025 * 64 * 8 * (64 * 4 + 8)

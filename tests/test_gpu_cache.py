@@ -265,7 +265,7 @@ def attn_case(heads, kv, head_dim, block, held, new, dtype, cache, seed, extra_r
     return {"q": q.to(dtype), "cu": cu, "lens": total, "table": table, "cache": state}
 
 
-def check_attn(c, heads, head_dim, causal=True, scale=None, log_as="", **kw):
+def check_attn(c, heads, head_dim, causal=True, scale=None, log_as="", extra_tol=0.0, **kw):
     from cobra_amd import ops
 
     scale = head_dim ** -0.5 if scale is None else scale
@@ -285,7 +285,7 @@ def check_attn(c, heads, head_dim, causal=True, scale=None, log_as="", **kw):
     lo, hi = c["cu"][0], c["cu"][-1]
     assert (got[:lo] == 7).all() and (got[hi:] == 7).all()  # rows of no request are left as they were
     tol = attn_tolerance(want, mag, top, reach, max(c["lens"] + [1]), head_dim, dtype,
-                         float(torch.nan_to_num(vs, nan=0.0, posinf=0.0).max()))
+                         float(torch.nan_to_num(vs, nan=0.0, posinf=0.0).max())) + extra_tol
     # Past the largest number of the type and half a step the nearest value is an infinity.
     border = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4)
     over = want.abs() - tol > border
@@ -414,6 +414,66 @@ def test_attn_scales_far_apart(cache, dtype):
         ks.copy_(torch.ldexp(torch.ones(n, 2), -(torch.arange(n) % 3)[:, None] * 10 - 5 + torch.tensor([[0, 1]])))
         poison(k, v, c["table"][0][oc.blocks(c["lens"][0], 16) - 1], c["lens"][0] % 16)
         check_attn(c, 2, 64)
+
+
+def test_attn_scales_of_any_value():
+    """Scales that are no powers of two, and some outside [2^-40, 2^40], which are taken as its ends."""
+    for new in ([1, 1], [90, 4]):
+        c = attn_case(4, 2, 64, 16, [300, 70], new, torch.bfloat16, E4M3, seed=12)
+        k, v, ks, vs = c["cache"]
+        g = torch.Generator().manual_seed(13)
+        used = torch.isfinite(vs)
+        ks.copy_(torch.where(used, torch.exp(torch.randn(ks.shape, generator=g)) * 0.01, ks))
+        vs.copy_(torch.where(used, torch.exp(3 * torch.randn(vs.shape, generator=g)), vs))
+        check_attn(c, 4, 64)
+        first = c["table"][0][0]
+        vs[first] = 1e-20
+        vs[c["table"][1][0]] = 0.0
+        want = [t.clone() for t in c["cache"]]
+        want[3][first] = want[3][c["table"][1][0]] = 2.0 ** -40
+        got = check_attn(dict(c, cache=want), 4, 64)
+        assert torch.equal(got, check_attn(c, 4, 64, extra_tol=64 * 448 * 2.0 ** -40))
+
+
+def test_attn_one_long_request_of_thousands():
+    """Without max_new the launch is shaped for any request's having all the tokens: more row tiles
+    than a grid takes, which workgroups go round.  The result is that of the fitting hint."""
+    from cobra_amd import ops
+
+    B, long, H, hd, keys = 6000, 60000, 8, 8, 30
+    k, v, ks, vs = (t.to(DEV) for t in random_cache(2, H, 32, hd, E4M3, seed=3))
+    T = B - 1 + long
+    q = (torch.randn(T, H * hd, generator=torch.Generator().manual_seed(5)) / 8).to(DEV, torch.bfloat16)
+    cu = torch.arange(B + 1, dtype=torch.int32)
+    cu[4001:] += long - 1
+    lens = torch.full((B,), keys, dtype=torch.int32, device=DEV)
+    table = torch.ones(B, 1, dtype=torch.int32, device=DEV)
+
+    def run(**kw):
+        return ops.cache_attn(q, cu.to(DEV), lens, table, H, hd, 0.3, k, v, ks, vs, causal=False, **kw)
+
+    got = run()
+    assert torch.equal(got, run(max_new=long))
+    kd = codes_of(k)[1, :, :keys, :hd] * ks[1].cpu().double()[:, None, None]
+    vd = (codes_of(v)[1, :, :hd, :keys] * vs[1].cpu().double()[:, None, None]).transpose(1, 2)
+    rows = torch.cat([torch.arange(3995, 4100), torch.arange(4000 + long - 90, 4000 + long + 90)])
+    s = 0.3 * q.cpu().double()[rows].view(-1, H, hd).transpose(0, 1) @ kd.transpose(1, 2).contiguous()
+    want = (torch.softmax(s, -1) @ vd).transpose(0, 1).reshape(len(rows), -1)
+    # bf16's half step; every weight 2^-11 of itself for fp16, at most the largest |v| of a head
+    err = (got.cpu().double()[rows] - want).abs()
+    assert (err <= want.abs() * 2.0 ** -8 + vd.abs().max() * 2.0 ** -9).all()
+
+
+def test_attn_refuses_an_output_over_its_queries():
+    from cobra_amd import ops
+
+    c = attn_case(4, 2, 64, 16, [30], [6], torch.float16, E4M3, seed=2)
+    k, v, ks, vs = (t.to(DEV) for t in c["cache"])
+    q = c["q"].to(DEV)
+    a = (i32(c["cu"]), i32(c["lens"]), i32(c["table"]), 4, 64, 0.125, k, v, ks, vs)
+    for x, out in ((q, q.view(-1)[:6 * 256].view(6, 256)), (q[:, :256].contiguous(), None)):
+        with pytest.raises(RuntimeError):
+            ops.cache_attn(x, *a, out=x if out is None else out)
 
 
 def test_attn_long_split():

@@ -118,6 +118,9 @@ def test_extend_refuses():
             mod.extend(x.double(), cache, new)
         with pytest.raises(ValueError, match="new_lens"):
             mod.extend(x, cache, new[:1])
+        with pytest.raises(ValueError, match="x is on cpu"):
+            mod.extend(x.cpu(), cache, new)
+        assert cache.lens.tolist() == [0, 0]
         # more than the pool has: nothing is reserved, no length changes
         big = torch.zeros(90, 128, dtype=torch.float16, device=DEV)
         y, missing = mod.extend(big, cache, torch.tensor([40, 50], dtype=torch.int32, device=DEV))
@@ -126,3 +129,30 @@ def test_extend_refuses():
         assert missing.tolist() == [0] and cache.lens.tolist() == [3, 2] and torch.isfinite(y).all()
         y, missing = mod.extend(x[:0], cache, torch.zeros_like(new))
         assert y.shape == (0, 128) and missing.tolist() == [0] and cache.lens.tolist() == [3, 2]
+
+
+def test_captured_extend_replays():
+    """A step of two tokens each captured once: every replay is the eager call on the same state."""
+    from cobra_amd import CobraTransformer, TransformerConfig
+
+    mod = CobraTransformer(TransformerConfig(3, 256, 128, 4, 128, 2, True)).to(DEV, torch.float16).eval()
+    caches = [mod.make_cache(3, 40, 16) for _ in range(2)]
+    new = torch.tensor([2, 2, 2], dtype=torch.int32, device=DEV)
+    x = torch.zeros(6, 128, dtype=torch.float16, device=DEV)
+    g = torch.Generator().manual_seed(6)
+    with torch.inference_mode():
+        prompt = torch.randn(70, 128, generator=g).to(DEV, torch.float16)
+        for c in caches:
+            mod.extend(prompt, c, torch.tensor([40, 0, 30], dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, missing = mod.extend(x, caches[0], new, max_new=2)
+        for _ in range(5):
+            x.copy_(torch.randn(6, 128, generator=g).to(torch.float16))
+            graph.replay()
+            want, none = mod.extend(x, caches[1], new, max_new=2)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(missing, none) and missing.item() == 0
+            assert torch.equal(caches[0].lens, caches[1].lens)
+    assert caches[0].lens.tolist() == [50, 10, 40]
