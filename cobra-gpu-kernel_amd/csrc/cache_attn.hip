@@ -475,6 +475,14 @@ struct Rows {
 // Few rows for each kv head: a workgroup has 16 of them and one split of the keys, its waves
 // every kWaves-th tile of it; their shares are joined through LDS, the splits' by
 // cache_join_kernel.
+//
+// Bound by memory where the cache is large: 16 requests of 16000 to 32700 keys, 8 heads of 128
+// read by 32 (bf16 queries), 804 MB in 135 to 142 us, 5.7 TB/s against a large copy's 5.1 (reads alone are
+// faster).  Below that by latency: a wave has one tile's loads in flight and two workgroups
+// have a CU (64 requests of up to 2048 keys, 72 MB: 16.3 us; 999 keys of one request: 6.4).
+// Eight waves to a workgroup took 24 us for the 64 requests, registers for four waves of a SIMD
+// (with scratch) 23, 32 rows a wave 33.6 us for 18 rows where 16 a wave take 26 twice over the
+// keys.
 template <typename T, int CACHE, int HDP, int KT>
 __global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
   typedef Rows<T, CACHE, HDP, 1, KT> R;
@@ -535,22 +543,37 @@ __global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
 
 // The splits of a row joined: o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s, always in the same
 // order.  W waves have a row; a wave takes as many splits at a time as it has lanes for.
+// Bound by latency: 4.2 to 4.8 us for a few splits of 134 rows of 256, 5.4 to 6.1 us for 196
+// splits of 16 rows of 64.  With one wave the first kEarly rounds are asked for before it is
+// known how many splits the row's request has (5.1 us otherwise for the first); four waves
+// gained nothing from it (6.3 us for the second), sixteen waves lost (7.6).
 template <typename T, int HDP, int W>
 __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
   constexpr int kLanes = HDP / 4, kAt = 64 / kLanes;  // lanes of a split, splits of a wave
+  constexpr int kEarly = W > 1 ? 0 : 4;
   __shared__ f32x4 sh[W > 1 ? W : 1][kLanes];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = W > 1 ? wave : 0;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = W > 1 ? wave : 0;
   const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t rows = (int64_t)a.tokens * a.heads;
   if (row >= rows) return;
+  const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4, s0 = part * kAt + sub;
+  float em[kEarly + 1];
+  f32x4 early[kEarly + 1];
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i) {
+    const int s = s0 + i * W * kAt;
+    if (sub < kAt && s < a.splits) {
+      em[i] = a.part_m[s * rows + row].x;
+      early[i] = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
+    }
+  }
   const int t = (int)(row / a.heads);
-  int lo = 0, hi = a.batch;  // the last request with cu[b] <= t
-  while (lo + 1 < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
+  int lo = 0;  // the last request with cu[b] <= t
+  for (int b0 = 0; b0 < a.batch && a.batch > 1; b0 += 64) {
+    const int below = __popcll(__ballot(b0 + lane < a.batch && a.cu[min(b0 + lane, a.batch)] <= t));
+    if (below) lo = b0 + below - 1;
+    if (below < 64) break;
   }
   const Request rq = request_of(a, lo);
   if (t < rq.t0 || t >= rq.t0 + rq.n) return;
@@ -569,15 +592,18 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
   }
   l = group_sum<64>(l);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4;
-  if (sub < kAt) {
-#pragma unroll 4
-    for (int s = part * kAt + sub; s < n; s += W * kAt) {
-      const float f = __builtin_amdgcn_exp2f(a.part_m[s * rows + row].x - base);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
+  auto take = [&](float ms, const f32x4& x) {
+    const float f = __builtin_amdgcn_exp2f(ms - base);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
-    }
+    for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+  };
+  if (sub < kAt) {
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i)
+      if (s0 + i * W * kAt < n) take(em[i], early[i]);
+#pragma unroll 4
+    for (int s = s0 + kEarly * W * kAt; s < n; s += W * kAt)
+      take(a.part_m[s * rows + row].x, *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d));
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -615,8 +641,8 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
 //
 // Bound by the vector ALU: for each of a lane's scores an fma, an exponential, a conversion and
 // an addition beside the matrix instructions, of which only the exponential and the codes'
-// conversion overlap them.  8 requests of 2048 new tokens over up to 8192 keys, 32 heads of 128
-// on 8 (bf16): 960 to 997 us, 0.92 to 0.95 PFLOP/s.
+// conversion overlap them.  2 requests of 2000 new tokens behind 8000 to 14000, 32 heads of 128
+// on 8 (bf16): 940 to 997 us, 0.92 to 0.97 PFLOP/s.
 template <typename T, int CACHE, int HDP, int NR>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a) {
   constexpr int kWaves = 4, kRows = kWaves * NR * 16, KT = 64;
