@@ -380,7 +380,8 @@ class CobraTransformer(nn.Module):
         their sequences, up to the cache's 8 bits for keys and values.  The cache then holds them
         too (``cache.trim`` takes them back).  ``missing``: as ``ops.cache_reserve``; where it is
         not 0 nothing was reserved and y holds no results.  Rows past the last request's have none
-        either.  ``max_new`` / ``max_len``: expected bounds on a request's new tokens and length
+        either.  An error raised on the way (out of memory) leaves the room reserved; ``cache.trim``
+        to the lengths before gives it back.  ``max_new`` / ``max_len``: expected bounds on a request's new tokens and length
         (speed only).  Every launch is the library's own, with the ops of the composed forward.
         """
         cfg, g = self.config, self._geom

@@ -11,6 +11,7 @@
 // caching allocator, launches on the device's current stream and returns y; for any
 // other call it returns None and the module takes its general path.  It never
 // computes anything itself: the launch is the library's (libcobra_amd.so).
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -238,14 +239,12 @@ int device_of(PyObject* o) {
 // A failed call: None, so that the general path makes it again and raises the library's error.
 PyObject* none() { Py_RETURN_NONE; }
 
+// Exceptions as torch raises them (out of memory is its own type).
 template <typename F>
 PyObject* guarded(F&& f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
 }
 
 struct Tables {

@@ -476,6 +476,66 @@ def test_attn_refuses_an_output_over_its_queries():
             ops.cache_attn(x, *a, out=x if out is None else out)
 
 
+def test_tensors_that_are_not_rows_are_refused():
+    """Strided views, wrong types and shapes: an error before anything is launched or changed."""
+    from cobra_amd import ops
+
+    c = attn_case(4, 2, 64, 16, [30, 5], [6, 1], torch.float16, E4M3, seed=2)
+    k, v, ks, vs = (t.to(DEV) for t in c["cache"])
+    q, cu, lens, table = c["q"].to(DEV), i32(c["cu"]), i32(c["lens"]), i32(c["table"])
+    wide = torch.cat([q, q], 1)
+    good = dict(q=q, cu=cu, lens=lens, table=table, k=k, v=v, ks=ks, vs=vs)
+
+    def attn(**kw):
+        a = dict(good, **kw)
+        return ops.cache_attn(a["q"], a["cu"], a["lens"], a["table"], 4, 64, 0.125, a["k"], a["v"], a["ks"], a["vs"])
+
+    def append(**kw):
+        a = dict(good, slots=torch.arange(7, device=DEV), **kw)
+        ops.cache_append(a["q"], a["slots"], 4, 64, a["k"], a["v"], a["ks"], a["vs"])
+
+    state = (k.view(torch.uint8), v.view(torch.uint8), ks.view(torch.int32))  # bits: unused scales are NaN
+    before = [t.clone() for t in state]
+    flat = q.view(-1)
+    bad = [dict(q=wide[:, :512]), dict(q=wide[:, ::2]), dict(q=q.float()), dict(q=q.cpu()), dict(q=q[None]),
+           dict(q=flat[4:4 + 6 * 512].view(6, 512)), dict(k=k.transpose(0, 1)), dict(k=k.view(torch.uint8)),
+           dict(v=v.transpose(2, 3)), dict(v=v[:-1]), dict(ks=ks.t()), dict(vs=vs.double()), dict(vs=vs[:, :1])]
+    for kw in bad:
+        for fn in (attn, append):
+            with pytest.raises((ValueError, TypeError, RuntimeError)):
+                fn(**kw)
+    for kw in (dict(cu=cu.long()), dict(cu=cu[:-1]), dict(lens=i32(c["lens"] * 2)[::2]), dict(table=table.t()),
+               dict(table=table[:, ::2]), dict(lens=lens.cpu())):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            attn(**kw)
+    lens4 = i32([3, 3, 3, 3])
+    for kw in (dict(lens=lens4[::2]), dict(new=lens4), dict(table=table.t()), dict(count=i32([1, 1])), dict(bs=24)):
+        a = dict(dict(lens=lens, new=i32([1, 1]), table=table, count=i32([0]), bs=16), **kw)
+        for call in (lambda: ops.cache_reserve(a["lens"], a["new"], a["table"], i32([0]), a["count"], a["bs"], 4),
+                     lambda: ops.cache_trim(a["lens"], a["new"], a["table"], i32([0]), a["count"], a["bs"])):
+            with pytest.raises((ValueError, TypeError, RuntimeError)):
+                call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(before, state))
+    assert lens.tolist() == c["lens"]
+
+
+def test_reserve_without_memory_changes_nothing():
+    from cobra_amd import ops
+
+    lens, count = i32([3]), i32([1])
+    table, free = i32([[0, 0]]), i32([1])
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.02)
+    try:
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            ops.cache_reserve(lens, i32([1]), table, free, count, 16, 2 ** 31 - 1)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert lens.tolist() == [3] and count.tolist() == [1]
+
+
 def test_attn_long_split():
     """One request of tens of thousands of keys over many splits, and a short one beside it."""
     for cache, dtype in ((E4M3, torch.float16), (I8, torch.bfloat16)):
