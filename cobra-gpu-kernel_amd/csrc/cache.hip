@@ -302,10 +302,40 @@ __device__ __forceinline__ uint32_t quant2(float x, float y) {
   }
 }
 
+// quant2 of four values that are finite and inside the code's range.
 template <int CACHE>
-__device__ __forceinline__ uint32_t quant1(float x) {
-  return quant2<CACHE>(x, 0.f) & 0xffu;
+__device__ __forceinline__ uint32_t quant4(float x, float y, float z, float w) {
+  if constexpr (CACHE == kCacheE4M3) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z, w, __builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false), true);
+  } else {
+    // Next to 1.5 x 2^23 a step is 1 and a sum's low byte the rounded integer's.
+    constexpr float at = 12582912.f;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y + at), __float_as_uint(x + at), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(w + at), __float_as_uint(z + at), 0x04000c0cu);
+    return lo | hi;
+  }
 }
+
+// What quant2 does with a value before it rounds.
+template <int CACHE>
+__device__ __forceinline__ float inside(float x) {
+  constexpr float qmax = CACHE == kCacheE4M3 ? 448.f : 127.f;
+  return x == x ? fminf(fmaxf(x, -qmax), qmax) : 0.f;
+}
+
+// Magnitudes of 16-bit floating point numbers are ordered as their bits are; from kNoNumber on
+// they are infinities and NaN.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+struct Magnitude;
+template <>
+struct Magnitude<f16> {
+  static constexpr int kNoNumber = 0x7c00;
+};
+template <>
+struct Magnitude<bf16> {
+  static constexpr int kNoNumber = 0x7f80;
+};
 
 // The value of code i (0 .. 3) of a word.
 template <int CACHE, int I>
@@ -356,13 +386,15 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 //
 // The values are read twice, for the largest and for the codes; the second time they come from
 // the caches (kept in registers in between they cost the occupancy that hides the first: 14000
-// tokens of 8 x 128 took 66 us so, 30 us as it is).  K's rows are written eight codes to a
+// tokens of 8 x 128 took 66 us so, 30 us from the caches).  K's rows are written eight codes to a
 // store.  V's rows run along tokens: a thread takes 4 tokens x 8 dimensions and writes eight
 // words of 4 codes, neighbouring lanes neighbouring words of a row.
 //
-// Bound by latency at one token a request (64 of 8 x 64: 5.0 us), by memory with whole prompts:
-// 14000 tokens of 8 x 128 read 58 MB and write 29 in 30 us, 2.9 TB/s where a large copy makes
-// 5.1: a block's codes wait for its largest value, and are read again for it.
+// Bound by latency at one token a request (64 of 8 x 64: 4.9 us).  With whole prompts by the
+// vector ALU, active in 78 % of cycles at 22 instructions a value; magnitudes two at a time as
+// integers, nothing clamped where nothing can need it, and codes of four tokens joined by the
+// conversion itself took 14000 tokens of 8 x 128 from 30.7 to 27.0 us (58 MB read, 29 written:
+// 3.2 TB/s where a large copy makes 5.1).
 template <typename T, int CACHE, int NT>
 __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window, int share) {
   typedef typename Op16<T>::V8 V8;
@@ -427,24 +459,37 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
     // Item i: piece p of offset `off` (keys), or piece p of quad q's four offsets (values).
     const int q0 = lo >> 2, quads = (hi >> 2) + 1 - q0;
     const int items = values ? quads * pieces : (hi + 1 - lo) * pieces;
-    float amax = 0.f;
     // Where there is no token the run's first one is read: loads without a branch between them
     // are in flight together.
     auto read = [&](int token, int p) {
       return *reinterpret_cast<const V8*>(x0 + (token < 0 ? (int)t0 : token) * a.ld + 8 * p);
     };
-    auto largest = [&](const V8& x) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs((float)x[e]));
-    };
-    // For the largest the order does not matter: keys and values alike in rows.
+    // For the largest the order does not matter: keys and values alike in rows, and magnitudes two
+    // at a time as integers.  Where one is no number the finite ones' largest is looked for anew.
     const int all = (hi + 1 - lo) * pieces;
+    u16x2 top = {0, 0};
 #pragma unroll 4
     for (int i = tid; i < all; i += NT) {
       const int r = i / pieces;
-      largest(read(src[lo + r], i - r * pieces));
+      struct {
+        u16x2 w[4];
+      } x = __builtin_bit_cast(decltype(x), read(src[lo + r], i - r * pieces));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, x.w[e] & (uint16_t)0x7fff);
     }
-    amax = group_max<NT>(amax, red);
+    const int bits = (int)group_max<NT>((float)(top[0] > top[1] ? top[0] : top[1]), red);
+    const bool numbers = bits < Magnitude<T>::kNoNumber;
+    float amax = (float)__builtin_bit_cast(T, (uint16_t)bits);
+    if (!numbers) {
+      amax = 0.f;
+      for (int i = tid; i < all; i += NT) {
+        const int r = i / pieces;
+        const V8 x = read(src[lo + r], i - r * pieces);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs((float)x[e]));
+      }
+      amax = group_max<NT>(amax, red);
+    }
     float scale = pow2(scale_exponent<CACHE>(amax)), ratio = 1.f;
     bool grow = false;
     if (lo > 0) {
@@ -454,14 +499,24 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
     }
     if (tid == 0) scales[bh] = scale;  // every thread has read the old one: there was a barrier since
     const float inv = 1.f / scale;
+    // Nothing to clamp: every value is a number, and within the scale's range (all but bf16's largest).
+    const bool plain = numbers && amax <= (CACHE == kCacheE4M3 ? 448.f : 127.f) * scale;
+    auto scaled = [&](float (&f)[8], const V8& x) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (float)x[e] * inv;
+      if (!plain) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = inside<CACHE>(f[e]);
+      }
+    };
     uint8_t* to = codes + bh * bs * hdp;
     if (!values) {
       auto put = [&](int off, int p, const V8& x) {
+        float f[8];
+        scaled(f, x);
         uint2 w;
-        w.x = quant2<CACHE>((float)x[0] * inv, (float)x[1] * inv) |
-              (quant2<CACHE>((float)x[2] * inv, (float)x[3] * inv) << 16);
-        w.y = quant2<CACHE>((float)x[4] * inv, (float)x[5] * inv) |
-              (quant2<CACHE>((float)x[6] * inv, (float)x[7] * inv) << 16);
+        w.x = quant4<CACHE>(f[0], f[1], f[2], f[3]);
+        w.y = quant4<CACHE>(f[4], f[5], f[6], f[7]);
         *reinterpret_cast<uint2*>(to + off * hdp + 8 * p) = w;
       };
 #pragma unroll 4
@@ -488,23 +543,18 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
       // Eight rows' words of quad q: new codes where there are tokens, old ones rounded again
       // below lo, others left.
       auto put = [&](int q, int p, const V8 (&x)[4]) {
-        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}, mask = 0, old = 0;
+        uint32_t w[8], mask = 0, old = 0;
+        float f[4][8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (src[4 * q + j] >= 0) {
+          scaled(f[j], x[j]);
+          if (src[4 * q + j] >= 0)
             mask |= 0xffu << (8 * j);
-            if (p < pieces) {
-#pragma unroll
-              for (int e = 0; e < 8; e += 2) {
-                const uint32_t c = quant2<CACHE>((float)x[j][e] * inv, (float)x[j][e + 1] * inv);
-                w[e] |= (c & 0xffu) << (8 * j);
-                w[e + 1] |= (c >> 8) << (8 * j);
-              }
-            }
-          } else if (grow && 4 * q + j < lo) {
+          else if (grow && 4 * q + j < lo)
             old |= 0xffu << (8 * j);
-          }
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = quant4<CACHE>(f[0][e], f[1][e], f[2][e], f[3][e]);
         uint8_t* at = to + (int64_t)p * 8 * bs + 4 * q;
         if (mask == 0xffffffffu) {
 #pragma unroll
