@@ -459,10 +459,11 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
     // Item i: piece p of offset `off` (keys), or piece p of quad q's four offsets (values).
     const int q0 = lo >> 2, quads = (hi >> 2) + 1 - q0;
     const int items = values ? quads * pieces : (hi + 1 - lo) * pieces;
-    // Where there is no token the run's first one is read: loads without a branch between them
-    // are in flight together.
+    // Where there is no token the lowest offset's is read (not the run's first, which a later one
+    // for its slot may have replaced): loads without a branch between them are in flight together.
+    const int some = src[lo];
     auto read = [&](int token, int p) {
-      return *reinterpret_cast<const V8*>(x0 + (token < 0 ? (int)t0 : token) * a.ld + 8 * p);
+      return *reinterpret_cast<const V8*>(x0 + (token < 0 ? some : token) * a.ld + 8 * p);
     };
     // For the largest the order does not matter: keys and values alike in rows, and magnitudes two
     // at a time as integers.  Where one is no number the finite ones' largest is looked for anew.

@@ -218,8 +218,8 @@ int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* blo
  *     code = x / scale rounded to the nearest (ties to even), within +-qmax; NaN gives 0.
  * Tokens of one block stand next to each other in the call, as cobra_cache_reserve lays them
  * out (where they do not, that block's contents are unspecified); of two for one slot the
- * later one stays.  A token whose slot is negative or past the
- * pool is passed over.  Blocks without a token are left as they are.
+ * later one stays (and counts for a).  A token whose slot is negative or past the pool is
+ * passed over.  Blocks without a token are left as they are.
  */
 int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* slots, void* k, void* v, float* k_scale,
                        float* v_scale, int cache, int64_t tokens, int64_t num_blocks, int64_t block_size,

@@ -183,6 +183,18 @@ def test_append_skips_and_repeats(cache):
 
 
 @pytest.mark.parametrize("cache", [E4M3, I8])
+def test_append_replaced_token_beside_a_gap(cache):
+    """A run whose first token a later one replaces, with offsets that it leaves out: the replaced
+    token's values, a hundred times the others', leave no trace in the scale."""
+    heads, kv, hd, block = 2, 2, 64, 16
+    state = random_cache(3, kv, block, hd, cache, seed=1)
+    x = append_inputs(6, heads, kv, hd, torch.float16, seed=5)
+    x[0] *= 100
+    x[3] *= 100
+    check_append(x, [16 + 5, 16 + 8, 16 + 5, 32, 32 + 9, 32], heads, hd, state)
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_append_of_extreme_values(cache, dtype):
     """NaN, infinities, zeros, subnormals, the type's largest values, and magnitudes past the
