@@ -391,10 +391,10 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 // words of 4 codes, neighbouring lanes neighbouring words of a row.
 //
 // Bound by latency at one token a request (64 of 8 x 64: 4.9 us).  With whole prompts by the
-// vector ALU, active in 78 % of cycles at 22 instructions a value; magnitudes two at a time as
-// integers, nothing clamped where nothing can need it, and codes of four tokens joined by the
-// conversion itself took 14000 tokens of 8 x 128 from 30.7 to 27.0 us (58 MB read, 29 written:
-// 3.2 TB/s where a large copy makes 5.1).
+// vector ALU, active in 62 % of cycles (78 % before magnitudes went two at a time as integers,
+// values unclamped where nothing can need it, and codes of four tokens were joined by the
+// conversion itself: 14000 tokens of 8 x 128 from 30.7 to 27.0 us, 58 MB read, 29 written, 3.2
+// TB/s where a large copy makes 5.1).
 template <typename T, int CACHE, int NT>
 __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window, int share) {
   typedef typename Op16<T>::V8 V8;

@@ -11,7 +11,8 @@
 // runs on plain codes.  M is a maximum of u that moves only when a tile has a w near fp16's
 // largest number: most tiles need no maximum, no exchange between lanes and no rescaling of O.
 // w is rounded to fp16 for the product (11 bits; 2^-22 of the reference's before subnormals)
-// whatever the activations' type: codes are exact in fp16.
+// whatever the activations' type: codes are exact in fp16.  With fp16 activations and few rows
+// the product takes what was rounded off as a second term.
 // Scores, M, l and O are fp32.  Scales are taken within [2^-40, 2^40], so no w that counts
 // underflows and neither sum overflows.
 //
@@ -219,6 +220,12 @@ struct Rows {
   static constexpr int kSteps = HDP / 32, kWide = HDP / 64, kOdd = kSteps & 1, kDims = HDP / 16;
   static constexpr int kSub = KT / 16, kKeys = KT / 4, kWords = KT / 16, kParts = KT / 32;
   typedef uint32_t VWords __attribute__((ext_vector_type(kWords)));
+  // A weight's rounding to fp16 is as large as an fp16 result's own (with bf16 an eighth of it).
+  // Few rows are not bound by their arithmetic, so there the product takes what was rounded off
+  // as a second term: one key's weight often makes up most of a row, and the error of 128 such
+  // results came to 1.7 times their own rounding's.  It costs 64 requests of 8 x 64 0.9 us of 17.7.
+  static constexpr bool kTwo = NR == 1 && std::is_same<T, f16>::value;
+  static constexpr int kTerms = kTwo ? 2 * kParts : kParts;
 
   V8 q[NR][kSteps];
   f32x4 o[NR][kDims];
@@ -252,7 +259,7 @@ struct Rows {
   // w = 2^(s skc + shift) of a lane's keys, rounded to fp16 in p, and their sum (not rounded: a
   // key whose V scale is far below the row's largest has a w that fp16 has no bits for, and
   // counts in l all the same).
-  static __device__ __forceinline__ float weigh(const f32x4 (&s)[kSub], float skc, float shift, f16x8 (&p)[kParts]) {
+  static __device__ __forceinline__ float weigh(const f32x4 (&s)[kSub], float skc, float shift, f16x8 (&p)[kTerms]) {
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < kKeys; e += 2) {
@@ -260,6 +267,10 @@ struct Rows {
       const float y = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], skc, shift));
       p[e >> 3][e & 7] = (f16)x;
       p[e >> 3][(e & 7) + 1] = (f16)y;
+      if constexpr (kTwo) {
+        p[kParts + (e >> 3)][e & 7] = (f16)(x - (float)(f16)x);
+        p[kParts + (e >> 3)][(e & 7) + 1] = (f16)(y - (float)(f16)y);
+      }
       sum += x + y;
     }
     return sum;
@@ -305,7 +316,7 @@ struct Rows {
       inv = __builtin_amdgcn_rcpf(svc);  // both exact for powers of two
     }
   };
-  __device__ __forceinline__ bool weights(const f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b,
+  __device__ __forceinline__ bool weights(const f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kTerms], const Block& b,
                                           float (&sum)[NR]) const {
     bool ok = true;
 #pragma unroll
@@ -315,7 +326,7 @@ struct Rows {
     }
     return ok;
   }
-  __device__ __forceinline__ void weights_by_max(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b,
+  __device__ __forceinline__ void weights_by_max(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kTerms], const Block& b,
                                                  float (&sum)[NR], int key0, bool bad, bool slow) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -340,7 +351,7 @@ struct Rows {
         for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha;
     }
   }
-  __device__ __forceinline__ void softmax(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kParts], const Block& b, int key0,
+  __device__ __forceinline__ void softmax(f32x4 (&s)[NR][kSub], f16x8 (&p)[NR][kTerms], const Block& b, int key0,
                                           bool bad, bool slow) {
     float sum[NR];
     if (slow || !__all(weights(s, p, b, sum))) weights_by_max(s, p, b, sum, key0, bad, slow);
@@ -350,7 +361,7 @@ struct Rows {
 
   // O^T += V^T P^T on codes; v(t, i): this lane's V operand of dimensions 16 t .., part i of its keys.
   template <typename V>
-  __device__ __forceinline__ void gather(const f16x8 (&p)[NR][kParts], V&& v) {
+  __device__ __forceinline__ void gather(const f16x8 (&p)[NR][kTerms], V&& v) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
 #pragma unroll
@@ -358,6 +369,7 @@ struct Rows {
         const f16x8 x = v(t, i);
 #pragma unroll
         for (int r = 0; r < NR; ++r) o[r][t] = mfma16(x, p[r][i], o[r][t]);
+        if constexpr (kTwo) o[0][t] = mfma16(x, p[0][kParts + i], o[0][t]);
       }
   }
 
@@ -422,7 +434,7 @@ struct Rows {
         find(tile + step);
         load_k(tile + step);
       }
-      f16x8 p[NR][kParts];
+      f16x8 p[NR][kTerms];
       softmax(s, p, blk, key0, bad0, slow);
       if (slow) {
 #pragma unroll
@@ -479,7 +491,7 @@ struct Rows {
 // Bound by memory where the cache is large: 16 requests of 16000 to 32700 keys, 8 heads of 128
 // read by 32 (bf16 queries), 804 MB in 135 to 142 us, 5.7 TB/s against a large copy's 5.1 (reads alone are
 // faster).  Below that by latency: a wave has one tile's loads in flight and two workgroups
-// have a CU (64 requests of up to 2048 keys, 72 MB: 16.3 us; 999 keys of one request: 6.4).
+// have a CU (64 requests of up to 2048 keys, 72 MB: 17.3 us; 999 keys of one request: 6.7).
 // Eight waves to a workgroup took 24 us for the 64 requests, registers for four waves of a SIMD
 // (with scratch) 23, 32 rows a wave 33.6 us for 18 rows where 16 a wave take 26 twice over the
 // keys.
@@ -821,7 +833,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Ar
         if constexpr (kBatch) __builtin_amdgcn_sched_barrier(0);
       };
       if constexpr (HDP < 96) ask_v();
-      f16x8 p[NR][2];
+      f16x8 p[NR][R::kTerms];
       w.softmax(s, p, typename R::Block(a, sk, sv), key0, bad0, slow);
       if constexpr (HDP >= 96) ask_v();
       w.gather(p, [&](int t, int i) { return Widen<CACHE, f16>::of(vw[t][2 * i], vw[t][2 * i + 1]); });
