@@ -271,7 +271,7 @@ PyObject* cache_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Tables t;
     int64_t tokens;
-    if (n != 7 || !t.read(a) || !py_int(a[6], &tokens) || tokens < 0) return none();
+    if (n != 7 || !t.read(a) || !py_int(a[6], &tokens) || tokens < 0 || tokens > 0x7fffffff) return none();
     const at::Device dev = t.lens->device();
     at::Tensor slots = new_tensor({tokens}, at::kLong, dev), cu = new_tensor({t.batch + 1}, at::kInt, dev);
     at::Tensor missing = new_tensor({1}, at::kInt, dev), ws = new_tensor({t.batch + 1}, at::kInt, dev);
