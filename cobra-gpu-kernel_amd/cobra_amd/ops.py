@@ -512,7 +512,8 @@ def cache_reserve(
     is the slot of each new token, requests one after the other (-1 past the last), ``cu``
     [B + 1] where each request's begin.  ``missing`` [1] is 0; or the number of blocks the pool
     lacks, or -1 for lengths that do not fit (``cobra_cache_reserve``), and then nothing was
-    reserved, every slot is -1 and ``cu`` 0.  Nothing here waits for the GPU.
+    reserved, every slot is -1 and ``cu`` 0.  Nothing here waits for the GPU.  A launch that fails
+    raises ``CobraError``; the call may be two launches, so lengths may have changed then.
     """
     got = _lib.host().cache_reserve(lens, new_lens, block_table, free_list, free_count, block_size, tokens)
     if got is not None:

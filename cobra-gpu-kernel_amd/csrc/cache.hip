@@ -617,11 +617,8 @@ hipError_t launch_append(const CacheAppendArgs& a, hipStream_t stream) {
   const int64_t groups = (a.tokens + window - 1) / window * share;
   if (groups * (wave ? 64 : 256) > 0xffffffff) return hipErrorInvalidValue;  // threads are counted in 32 bits
   const dim3 grid((unsigned)groups, (unsigned)a.kv_heads, 2);
-  if (wave)
-    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 64>), grid, dim3(64), 0, stream, a, window, share);
-  else
-    hipLaunchKernelGGL((cache_append_kernel<T, CACHE, 256>), grid, dim3(256), 0, stream, a, window, share);
-  return hipGetLastError();
+  return wave ? launch_status(cache_append_kernel<T, CACHE, 64>, grid, dim3(64), stream, a, window, share)
+              : launch_status(cache_append_kernel<T, CACHE, 256>, grid, dim3(256), stream, a, window, share);
 }
 
 }  // namespace
@@ -642,27 +639,24 @@ hipError_t run_cache_reserve(const CacheReserveArgs& a, hipStream_t stream) {
   // One workgroup fills 1024 slots at a time; past a few rounds of it a second launch over
   // the whole chip is faster.
   const bool one = a.tokens <= 8192;
-  if (a.batch <= 256 && a.tokens <= 1024)
-    hipLaunchKernelGGL((cache_reserve_kernel<256>), dim3(1), dim3(256), 0, stream, a, 1);
-  else
-    hipLaunchKernelGGL((cache_reserve_kernel<1024>), dim3(1), dim3(1024), 0, stream, a, one ? 1 : 0);
-  if (!one) {
-    const int64_t g = (a.tokens + 255) / 256;  // up to 2048, a full chip of them
-    hipLaunchKernelGGL(cache_reserve_fill_kernel, dim3((unsigned)(g < 2048 ? g : 2048)), dim3(256), 0, stream, a);
-  }
-  return hipGetLastError();
+  const hipError_t e =
+      a.batch <= 256 && a.tokens <= 1024
+          ? launch_status(cache_reserve_kernel<256>, dim3(1), dim3(256), stream, a, 1)
+          : launch_status(cache_reserve_kernel<1024>, dim3(1), dim3(1024), stream, a, one ? 1 : 0);
+  if (one || e != hipSuccess) return e;
+  const int64_t g = (a.tokens + 255) / 256;  // up to 2048, a full chip of them
+  return launch_status(cache_reserve_fill_kernel, dim3((unsigned)(g < 2048 ? g : 2048)), dim3(256), stream, a);
 }
 
 hipError_t run_cache_trim(const CacheTrimArgs& a, hipStream_t stream) {
   if (a.batch <= 0 || a.width < 0 || a.num_free < 0) return hipErrorInvalidValue;
   // How many blocks come back is not known here, only that it is at most the table's size.
   const bool one = a.batch * a.width <= 16384;
-  if (a.batch <= 256 && one)
-    hipLaunchKernelGGL((cache_trim_kernel<256>), dim3(1), dim3(256), 0, stream, a, 1);
-  else
-    hipLaunchKernelGGL((cache_trim_kernel<1024>), dim3(1), dim3(1024), 0, stream, a, one ? 1 : 0);
-  if (!one) hipLaunchKernelGGL(cache_trim_fill_kernel, dim3(64), dim3(256), 0, stream, a);
-  return hipGetLastError();
+  const hipError_t e = a.batch <= 256 && one
+                           ? launch_status(cache_trim_kernel<256>, dim3(1), dim3(256), stream, a, 1)
+                           : launch_status(cache_trim_kernel<1024>, dim3(1), dim3(1024), stream, a, one ? 1 : 0);
+  if (one || e != hipSuccess) return e;
+  return launch_status(cache_trim_fill_kernel, dim3(64), dim3(256), stream, a);
 }
 
 hipError_t run_cache_append(const CacheAppendArgs& a, hipStream_t stream) {

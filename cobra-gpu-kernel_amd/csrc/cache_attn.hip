@@ -905,20 +905,15 @@ template <typename T, int CACHE, int HDP>
 hipError_t launch(const Args& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.batch * a.kv_heads * p.row_tiles * p.splits;
   if (grid > kMaxGrid) return hipErrorInvalidValue;
-  if (p.chunked)
-    hipLaunchKernelGGL((cache_chunk_kernel<T, CACHE, HDP, 2>), dim3((unsigned)grid), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((cache_decode_kernel<T, CACHE, HDP, decode_keys(HDP)>), dim3((unsigned)grid), dim3(256), 0,
-                       stream, a);
-  if (p.splits > 1) {
-    const int64_t rows = (int64_t)a.tokens * a.heads;
-    if (p.splits > 16)
-      hipLaunchKernelGGL((cache_join_kernel<T, HDP, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, p.step);
-    else
-      hipLaunchKernelGGL((cache_join_kernel<T, HDP, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a,
-                         p.step);
-  }
-  return hipGetLastError();
+  const dim3 groups((unsigned)grid), block(256);
+  const hipError_t e =
+      p.chunked ? launch_status(cache_chunk_kernel<T, CACHE, HDP, 2>, groups, block, stream, a)
+                : launch_status(cache_decode_kernel<T, CACHE, HDP, decode_keys(HDP)>, groups, block, stream, a);
+  if (p.splits <= 1 || e != hipSuccess) return e;
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  return p.splits > 16 ? launch_status(cache_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, a, p.step)
+                       : launch_status(cache_join_kernel<T, HDP, 1>, dim3((unsigned)((rows + 3) / 4)), block, stream, a,
+                                       p.step);
 }
 
 template <typename T, int CACHE>

@@ -197,8 +197,9 @@ class BoundStack {
 // The calls of cobra_amd/ops.py's cache_* functions in C++: a decode step's kernels take a few
 // microseconds each, about what the checks and allocations of one call take in Python.  Same
 // contract as above: a call whose tensors are all as they should be, on the current device, is
-// made here; for any other these return None, and Python's own checks name what is wrong (or
-// make the call on another device).  Arguments come by position (the vector-call protocol);
+// made here, once, and raises the library's error; for any other these return None before the
+// library is asked, and Python's own checks name what is wrong (or make the call on another
+// device).  Arguments come by position (the vector-call protocol);
 // what is not of the expected Python type makes a call "any other" too.
 
 bool py_int(PyObject* o, int64_t* v) {
@@ -236,8 +237,18 @@ int device_of(PyObject* o) {
   return dev == c10::hip::current_device() ? dev : -1;
 }
 
-// A failed call: None, so that the general path makes it again and raises the library's error.
+// A call that is not made here.
 PyObject* none() { Py_RETURN_NONE; }
+
+// A call that failed: it may have changed something (a reserve is two launches), so it is not
+// left to the general path to be made again.
+void check(const char* fn, int code) {
+  if (code == 0) return;
+  py::module_::import("cobra_amd._lib").attr("check")(fn, code);  // raises
+  throw std::runtime_error(std::string(fn) + " failed");
+}
+
+bool block_ok(int64_t n) { return n == 16 || n == 32 || n == 64 || n == 128; }
 
 // Exceptions as torch raises them (out of memory is its own type).
 template <typename F>
@@ -262,7 +273,7 @@ struct Tables {
     if (!lens || lens->dim() != 1 || !table || table->dim() != 2 || !free_list || free_list->dim() != 1) return false;
     batch = lens->size(0);
     return batch > 0 && shape_is(change, {batch}) && table->size(0) == batch && shape_is(count, {1}) &&
-           py_int(a[5], &block);
+           py_int(a[5], &block) && block_ok(block);
   }
 };
 
@@ -280,7 +291,7 @@ PyObject* cache_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         t.free_list->data_ptr<int>(), t.free_list->size(0), t.count->data_ptr<int>(), slots.data_ptr<int64_t>(), tokens,
         cu.data_ptr<int>(), missing.data_ptr<int>(), ws.data_ptr<int>(), t.batch, t.block,
         c10::hip::getCurrentHIPStream(t.dev).stream());
-    if (code != 0) return none();
+    check("cobra_cache_reserve", code);
     PyObject* got = PyTuple_New(3);
     if (!got) return nullptr;
     PyTuple_SET_ITEM(got, 0, THPVariable_Wrap(std::move(slots)));
@@ -301,7 +312,7 @@ PyObject* cache_trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       t.table->size(1), t.free_list->data_ptr<int>(), t.free_list->size(0),
                                       t.count->data_ptr<int>(), refused.data_ptr<int>(), ws.data_ptr<int>(), t.batch,
                                       t.block, c10::hip::getCurrentHIPStream(t.dev).stream());
-    if (code != 0) return none();
+    check("cobra_cache_trim", code);
     return THPVariable_Wrap(std::move(refused));
   });
 }
@@ -324,9 +335,9 @@ struct Pool {
     kv_heads = k->size(1);
     block = k->size(2);
     const int64_t width = k->size(3);
-    return width == cobra_cache_width(head_dim) && shape_is(v, {blocks, kv_heads, width, block}) &&
-           shape_is(k_scale, {blocks, kv_heads}) && shape_is(v_scale, {blocks, kv_heads}) && kv_heads > 0 &&
-           heads > 0 && heads % kv_heads == 0;
+    return block_ok(block) && width == cobra_cache_width(head_dim) &&
+           shape_is(v, {blocks, kv_heads, width, block}) && shape_is(k_scale, {blocks, kv_heads}) &&
+           shape_is(v_scale, {blocks, kv_heads}) && kv_heads > 0 && heads > 0 && heads % kv_heads == 0;
   }
 };
 
@@ -362,7 +373,7 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                         p.v->data_ptr(), p.k_scale->data_ptr<float>(), p.v_scale->data_ptr<float>(),
                                         p.cache, x->size(0), p.blocks, p.block, heads, p.kv_heads, hd,
                                         c10::hip::getCurrentHIPStream(dev).stream());
-    if (code != 0) return none();
+    check("cobra_cache_append", code);
     Py_RETURN_TRUE;
   });
 }
@@ -381,7 +392,9 @@ PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Pool p;
     if (!cu || !lens || !table || !p.read(a + 7, dev, heads, hd) || lens->dim() != 1 || table->dim() != 2) return none();
     const int64_t T = q->size(0), B = lens->size(0), W = table->size(1);
-    if (!PyBool_Check(a[11]) || T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) || table->size(0) != B) return none();
+    if (!PyBool_Check(a[11]) || T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) ||
+        table->size(0) != B || q->size(1) < heads * hd || q->size(1) % 8 || !(PyFloat_AS_DOUBLE(a[6]) > 0.0))
+      return none();
     int64_t new_most = T - B + 1, len_most = W * p.block;
     if (a[12] != Py_None && !py_int(a[12], &new_most)) return none();
     if (a[13] != Py_None && !py_int(a[13], &len_most)) return none();
@@ -405,7 +418,7 @@ PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, T, B, p.blocks, p.block, heads, p.kv_heads, hd,
         new_most, len_most, static_cast<float>(PyFloat_AS_DOUBLE(a[6])), a[11] == Py_True ? 1 : 0,
         c10::hip::getCurrentHIPStream(dev).stream());
-    if (code != 0) return none();
+    check("cobra_cache_attn_fwd", code);
     if (a[14] != Py_None) {
       Py_INCREF(a[14]);
       return a[14];

@@ -7,6 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 namespace cobra {
 
 constexpr int kLnMaxD = 4096;  // widest row the LayerNorm kernels hold in registers
@@ -317,6 +319,22 @@ struct BlockArgs {
 bool block_split_ok(int64_t seq_len, int64_t d_model, int64_t heads, int64_t ffn_dim);
 bool block_split_pays(int64_t batch, int64_t seq_len);
 hipError_t run_block_split(const BlockArgs& a);
+
+// A kernel's launch -> this launch's own status.  hipGetLastError() after it would give any
+// earlier error that the thread still has, for a launch that went well; such an error is left
+// where it is, and this launch's is taken away with its return.
+template <typename... P, typename... A>
+hipError_t launch_status(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, const A&... args) {
+  std::tuple<P...> held(static_cast<P>(args)...);
+  return std::apply(
+      [&](P&... at) {
+        void* list[] = {static_cast<void*>(&at)...};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, 0, stream);
+        if (e != hipSuccess) (void)hipGetLastError();
+        return e;
+      },
+      held);
+}
 
 // Key/value cache held in 8 bits (cache.hip, cache_attn.hip): a pool of blocks of 1 << shift
 // tokens; k [num_blocks, kv_heads, bs, hdp], v [num_blocks, kv_heads, hdp, bs] codes of one

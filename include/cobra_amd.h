@@ -187,7 +187,8 @@ int cobra_cache_width(int64_t head_dim);
  * or past 2^31 - 1, a row of the table too short, sum new_lens > tokens, or free_count
  * outside [0, num_free].  lens, new_lens: [batch]; block_table: [batch, table_width];
  * free_list: [num_free]; free_count, missing: [1]; cu, workspace: [batch + 1] int32; slots:
- * [tokens] int64.
+ * [tokens] int64.  A call takes one launch or two: where it returns the error of a launch, do
+ * not make it again, lens and free_count may have changed.
  */
 int cobra_cache_reserve(int32_t* lens, const int32_t* new_lens, int32_t* block_table, int64_t table_width,
                         const int32_t* free_list, int64_t num_free, int32_t* free_count, int64_t* slots,
@@ -201,7 +202,7 @@ int cobra_cache_reserve(int32_t* lens, const int32_t* new_lens, int32_t* block_t
  * old lengths undoes a reserve.  A block belongs to one request: one that two rows list is
  * given back twice.  block_table keeps its entries.  refused = 0; or 1, and nothing
  * else changes, where a length is negative or longer than a row of the table, or the stack
- * would not hold the blocks.  workspace: [batch] int32.
+ * would not hold the blocks.  workspace: [batch] int32.  An error of a launch: as above.
  */
 int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* block_table, int64_t table_width,
                      int32_t* free_list, int64_t num_free, int32_t* free_count, int32_t* refused, int32_t* workspace,
