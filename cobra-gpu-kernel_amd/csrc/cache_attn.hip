@@ -41,6 +41,8 @@ constexpr float kAccept = 57344.f;   // a lane's sum of w that is taken without 
 constexpr int64_t kMaxKeys = 0x7ffff000;
 // Workgroups of a launch: of 256 threads, which are counted in 32 bits.
 constexpr int64_t kMaxGrid = 0xffffff;
+// Rows of a head that all splits of a call leave partial results of (541 MB at head_dim 256).
+constexpr int64_t kMaxParts = 1 << 19;
 
 __device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -885,13 +887,16 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   const int64_t least = p.chunked ? 1024 : p.step;
   int64_t splits = (512 + units - 1) / units;
   if (p.chunked && units >= 256) splits = 1;
-  if (tokens * heads > kMaxGrid) splits = 1;  // max_new is far off
+  // Hints that fit leave under 2^17 partial rows (twice 512 units of 16, or 256 of 128 three times).
+  // Where max_new is too low for the tokens it is the workspace that has to be bounded.
+  const int64_t room = kMaxParts / (tokens * heads);
+  splits = splits < room ? splits : room;
   // Up to 1024 keys one workgroup takes less time than the second launch that joins splits
   // (999 keys of 4 x 32: 6.6 against 8.0 us).
   if (!p.chunked && max_len <= 1024 && cache_width(head_dim) <= 128) splits = 1;
   const int64_t most = (max_len + least - 1) / least;
   splits = splits < most ? splits : most;
-  splits = splits < 1 ? 1 : splits > 1024 ? 1024 : splits;
+  splits = splits < 1 ? 1 : splits;
   const int64_t even = (max_len + splits - 1) / splits;
   p.chunk = (int)((even + p.step - 1) / p.step * p.step);
   p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
