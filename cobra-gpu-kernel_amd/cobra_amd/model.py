@@ -152,10 +152,15 @@ class CobraTransformer(nn.Module):
         self._fast = None
         return out
 
-    def _packed(self, x_dtype: torch.dtype = torch.float16) -> List[_BlockPack]:
+    def _pack_state(self, x_dtype: torch.dtype):
+        """(operand type, parameter versions, whether the packs are laid out for them)."""
         op = torch.bfloat16 if x_dtype == torch.bfloat16 else torch.float16
         versions = tuple([p._version if v else p.data_ptr() for p, v in zip(self._params, self._versioned)])
-        if self._packs is None or self._versions != versions or self._op != op:
+        return op, versions, self._packs is not None and self._versions == versions and self._op == op
+
+    def _packed(self, x_dtype: torch.dtype = torch.float16) -> List[_BlockPack]:
+        op, versions, ready = self._pack_state(x_dtype)
+        if not ready:
             if not self.final_norm.weight.is_cuda:
                 raise RuntimeError("CobraTransformer runs on the GPU only: move it with .to('cuda')")
             self._packs = [_BlockPack(blk, self._geom, op) for blk in self.layers]
@@ -381,8 +386,13 @@ class CobraTransformer(nn.Module):
         too (``cache.trim`` takes them back).  ``missing``: as ``ops.cache_reserve``; where it is
         not 0 nothing was reserved and y holds no results.  Rows past the last request's have none
         either.  An error raised on the way (out of memory) leaves the room reserved; ``cache.trim``
-        to the lengths before gives it back.  ``max_new`` / ``max_len``: expected bounds on a request's new tokens and length
-        (speed only).  Every launch is the library's own, with the ops of the composed forward.
+        to the lengths before gives it back.  ``max_new`` / ``max_len``: expected bounds on a request's
+        new tokens and length (speed only).  Every launch is the library's own, with the ops of the
+        composed forward.
+
+        A step can be captured in a graph once the model has run with activations of x's type and
+        its present parameters (it lays its weights out then, which must not become part of the
+        graph).
         """
         cfg, g = self.config, self._geom
         if not cfg.causal:
@@ -397,6 +407,10 @@ class CobraTransformer(nn.Module):
         if (cache.layers, cache.kv_heads, cache.head_dim) != (cfg.num_layers, cfg.num_heads, g.hdp):
             raise ValueError(f"the cache is for {cache.layers} layers of {cache.kv_heads} heads of {cache.head_dim}, "
                              f"the model has {cfg.num_layers} of {cfg.num_heads} of {g.hdp}")
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not self._pack_state(x.dtype)[2]:
+            raise RuntimeError("run extend (or forward) once with activations of this type before it is captured: the "
+                               "weights are laid out for the kernels then")
         packs = self._packed(x.dtype)
         op = self._op
         x = x.contiguous()
