@@ -52,6 +52,11 @@ class CobraCache:
         self.block_table = torch.zeros((requests, max(1, rows)), dtype=torch.int32, device=dev)
         self.free_list = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), num_blocks, dtype=torch.int32, device=dev)
+        self._held: List[object] = []
+
+    def hold(self, *things: object) -> None:
+        """Keeps what a captured step over this cache reads alive for as long as the cache lives."""
+        self._held += [t for t in things if not any(t is h for h in self._held)]
 
     def reserve(self, new_lens: torch.Tensor, tokens: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Room for ``new_lens`` more tokens of each request -> ``(slots, cu, missing)`` (``ops.cache_reserve``)."""

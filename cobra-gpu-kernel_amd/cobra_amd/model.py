@@ -392,7 +392,8 @@ class CobraTransformer(nn.Module):
 
         A step can be captured in a graph once the model has run with activations of x's type and
         its present parameters (it lays its weights out then, which must not become part of the
-        graph).
+        graph).  The cache keeps the laid out weights alive for the replays; a parameter that
+        changes needs a new capture, as some of them are copies and some the parameters' own memory.
         """
         cfg, g = self.config, self._geom
         if not cfg.causal:
@@ -412,6 +413,8 @@ class CobraTransformer(nn.Module):
             raise RuntimeError("run extend (or forward) once with activations of this type before it is captured: the "
                                "weights are laid out for the kernels then")
         packs = self._packed(x.dtype)
+        if capturing:
+            cache.hold(packs, self._final)
         op = self._op
         x = x.contiguous()
         T, D = x.shape
