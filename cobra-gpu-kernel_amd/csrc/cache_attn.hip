@@ -11,8 +11,8 @@
 // runs on plain codes.  M is a maximum of u that moves only when a tile has a w near fp16's
 // largest number: most tiles need no maximum, no exchange between lanes and no rescaling of O.
 // w is rounded to fp16 for the product (11 bits; 2^-22 of the reference's before subnormals)
-// whatever the activations' type: codes are exact in fp16.  With fp16 activations and few rows
-// the product takes what was rounded off as a second term.
+// whatever the activations' type: codes are exact in fp16.  With fp16 activations the product
+// takes what was rounded off as a second term.
 // Scores, M, l and O are fp32.  Scales are taken within [2^-40, 2^40], so no w that counts
 // underflows and neither sum overflows.
 //
@@ -222,11 +222,14 @@ struct Rows {
   static constexpr int kSteps = HDP / 32, kWide = HDP / 64, kOdd = kSteps & 1, kDims = HDP / 16;
   static constexpr int kSub = KT / 16, kKeys = KT / 4, kWords = KT / 16, kParts = KT / 32;
   typedef uint32_t VWords __attribute__((ext_vector_type(kWords)));
-  // A weight's rounding to fp16 is as large as an fp16 result's own (with bf16 an eighth of it).
-  // Few rows are not bound by their arithmetic, so there the product takes what was rounded off
-  // as a second term: one key's weight often makes up most of a row, and the error of 128 such
-  // results came to 1.7 times their own rounding's.  It costs 64 requests of 8 x 64 0.9 us of 17.7.
-  static constexpr bool kTwo = NR == 1 && std::is_same<T, f16>::value;
+  // A weight's rounding to fp16 is as large as an fp16 result's own: with one term the results were
+  // up to 1.7 times their own rounding off (one key's weight often makes up most of a row), in
+  // chunks of prompts 1.08 times.  So with fp16 activations the product takes what was rounded off
+  // as a second term: half as many matrix instructions again, and for a pair of weights a multiply-
+  // add each and a conversion.  64 requests of 8 x 64 take 0.6 us of 16.9 for it, chunks of 16 x 64
+  // 159 us in place of 138, of 32 x 128 1200 in place of 944.  Not with bf16, whose results' own
+  // rounding is eight times a weight's (0.00156 from 64 bits with one term, as the plain form's).
+  static constexpr bool kTwo = std::is_same<T, f16>::value;
   static constexpr int kTerms = kTwo ? 2 * kParts : kParts;
 
   V8 q[NR][kSteps];
@@ -260,19 +263,24 @@ struct Rows {
 
   // w = 2^(s skc + shift) of a lane's keys, rounded to fp16 in p, and their sum (not rounded: a
   // key whose V scale is far below the row's largest has a w that fp16 has no bits for, and
-  // counts in l all the same).
+  // counts in l all the same).  Of two terms the first is rounded towards zero, by an instruction
+  // that takes a pair, so that the rest keeps its sign; the rest, under 2^-10 of w, is rounded to
+  // the nearest: 2^-21 of w in all.
   static __device__ __forceinline__ float weigh(const f32x4 (&s)[kSub], float skc, float shift, f16x8 (&p)[kTerms]) {
-    float sum = 0.f;
+    float sum = 0.f, minus = -1.f;
+    asm("" : "+s"(minus));  // kept a factor: x - w as a multiply-add of an fp16 w is one instruction
 #pragma unroll
     for (int e = 0; e < kKeys; e += 2) {
       const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], skc, shift));
       const float y = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], skc, shift));
-      p[e >> 3][e & 7] = (f16)x;
-      p[e >> 3][(e & 7) + 1] = (f16)y;
+      f16x2 w = {(f16)x, (f16)y};
       if constexpr (kTwo) {
-        p[kParts + (e >> 3)][e & 7] = (f16)(x - (float)(f16)x);
-        p[kParts + (e >> 3)][(e & 7) + 1] = (f16)(y - (float)(f16)y);
+        w = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+        p[kParts + (e >> 3)][e & 7] = (f16)fmaf((float)w[0], minus, x);
+        p[kParts + (e >> 3)][(e & 7) + 1] = (f16)fmaf((float)w[1], minus, y);
       }
+      p[e >> 3][e & 7] = w[0];
+      p[e >> 3][(e & 7) + 1] = w[1];
       sum += x + y;
     }
     return sum;
@@ -371,7 +379,10 @@ struct Rows {
         const f16x8 x = v(t, i);
 #pragma unroll
         for (int r = 0; r < NR; ++r) o[r][t] = mfma16(x, p[r][i], o[r][t]);
-        if constexpr (kTwo) o[0][t] = mfma16(x, p[0][kParts + i], o[0][t]);
+        if constexpr (kTwo) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) o[r][t] = mfma16(x, p[r][kParts + i], o[r][t]);
+        }
       }
   }
 
@@ -493,7 +504,7 @@ struct Rows {
 // Bound by memory where the cache is large: 16 requests of 16000 to 32700 keys, 8 heads of 128
 // read by 32 (bf16 queries), 804 MB in 135 to 142 us, 5.7 TB/s against a large copy's 5.1 (reads alone are
 // faster).  Below that by latency: a wave has one tile's loads in flight and two workgroups
-// have a CU (64 requests of up to 2048 keys, 72 MB: 17.3 us; 999 keys of one request: 6.7).
+// have a CU (64 requests of up to 2048 keys, 72 MB: 16.9 us; 999 keys of one request: 6.5).
 // Eight waves to a workgroup took 24 us for the 64 requests, registers for four waves of a SIMD
 // (with scratch) 23, 32 rows a wave 33.6 us for 18 rows where 16 a wave take 26 twice over the
 // keys.

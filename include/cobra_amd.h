@@ -234,9 +234,8 @@ int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* sl
  * do); query head j reads kv head j / (heads / kv_heads).  ctx: [tokens, heads * head_dim],
  * tokens * heads < 2^31 - 256, batch * kv_heads < 2^24, not overlapping q (refused); of a
  * request's keys the first 2^31 - 4096 count; rows outside [cu[0], cu[batch]) are left as
- * they are.  Scores, softmax and sums are fp32,
- * the probabilities rounded to fp16 for the product with V's codes (with fp16 q and at most
- * 64 query rows to a kv head to twice its bits); scales are taken within
+ * they are.  Scores, softmax and sums are fp32, the probabilities rounded for the product with
+ * V's codes, with fp16 q to twice fp16's bits, with bf16 q to fp16; scales are taken within
  * [2^-40, 2^40].  Keys in a block whose id is outside the pool are masked.  max_new and max_len: the most new
  * tokens and keys that a request is expected to have; they shape the launch and never the
  * result.  workspace: cobra_cache_attn_workspace_bytes() bytes (16-byte aligned, may be NULL
