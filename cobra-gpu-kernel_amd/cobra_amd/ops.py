@@ -654,8 +654,10 @@ def cache_attn(
     ``block_table[b]`` lists.  Query head j reads kv head ``j // (heads // kv_heads)``.  With
     ``causal`` a token sees the keys up to itself, else all of its request; a token that sees
     none gets a zero row.  Rows past ``cu[B]`` are left as they are (unset without ``out``).
-    ``max_new`` and ``max_len``, the most new tokens and keys of a request (defaults: what T and
-    the table allow), shape the launch, not the result.
+    ``max_new`` and ``max_len`` are the most new tokens and keys that a request is expected to have
+    (defaults: what T and the table allow).  They choose the kernel, the splits of the keys and
+    with them the order of the sums: a result is right whatever they say, but not the same to the
+    bit, and the call is fast where they fit.
     """
     got = _lib.host().cache_attn(q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, causal,
                                  max_new, max_len, out)

@@ -236,10 +236,12 @@ int cobra_cache_append(const void* qkv, int dtype, int64_t ld, const int64_t* sl
  * request's keys the first 2^31 - 4096 count; rows outside [cu[0], cu[batch]) are left as
  * they are.  Scores, softmax and sums are fp32, the probabilities rounded for the product with
  * V's codes, with fp16 q to twice fp16's bits, with bf16 q to fp16; scales are taken within
- * [2^-40, 2^40].  Keys in a block whose id is outside the pool are masked.  max_new and max_len: the most new
- * tokens and keys that a request is expected to have; they shape the launch and never the
- * result.  workspace: cobra_cache_attn_workspace_bytes() bytes (16-byte aligned, may be NULL
- * when that is 0); launches that share it must not overlap.
+ * [2^-40, 2^40].  Keys in a block whose id is outside the pool are masked.
+ * max_new and max_len: the most new tokens and keys that a request is expected to have.  They
+ * choose the kernel, the splits of the keys and with them the order of the sums: a result is
+ * right whatever they say, but not the same to the bit.  workspace:
+ * cobra_cache_attn_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0);
+ * launches that share it must not overlap.
  */
 int64_t cobra_cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
                                          int64_t head_dim, int64_t max_new, int64_t max_len);

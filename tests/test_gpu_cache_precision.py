@@ -1,5 +1,6 @@
 """GPU tests of the cache attention's precision: with fp16 activations the weights are held in two
-fp16 terms in both kernels, so that a result is off by little more than its own rounding."""
+fp16 terms in both kernels, so that a result is off by little more than its own rounding, and a
+call's hints move it by no more."""
 
 import pytest
 import torch
@@ -83,3 +84,28 @@ def test_scales_far_apart_head_by_head(cache, dtype):
         assert ((got - want).abs() <= tol)[sure].all()
         over = want.abs() - tol > border * 1.001
         assert torch.equal(got[over], torch.copysign(torch.full_like(want, float("inf")), want)[over])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("held,new", [([700, 0, 90], [1, 1, 1]), ([700, 64, 90], [40, 3, 9]), ([300, 0, 90], [150, 70, 3])])
+def test_hints_move_a_result_within_its_rounding(held, new, dtype):
+    """Hints choose the kernel and the splits, which changes the order of sums and no more.
+
+    Two results that are off by e before they are rounded differ by a step where a border lies
+    between them, with a probability of 2 e by the step, else not at all.  fp16: e is a three
+    hundredth of a step (two terms), 0.007 of the results a step apart, root mean square 0.08 of a step,
+    against 0.29 for the rounding itself; twice that is taken.  bf16: a weight's 2^-12 and a result's
+    2^-9 (root mean squares of half a step each) leave e at an eighth of the rounding."""
+    c = attn_case(8, 2, 64, 32, held, new, dtype, E4M3, seed=3)
+    want, mag, top, reach = attend(c, 8, 64)
+    hints = [(max(new), max(c["lens"])), (None, None), (1, 1), (1, 64), (3, 700), (100000, 5), (1, 10 ** 12), (200, 1)]
+    got = [run(c, 8, 64, max_new=n, max_len=m) for n, m in hints]
+    own = rms((want.to(dtype).double() - want) / mag.clamp(min=1e-30))
+    step = torch.finfo(dtype).eps * want.abs()
+    weight = 2.0 ** -21 if dtype == torch.float16 else 2.0 ** -11
+    room = step + 2 * (weight + 2.0 ** -18) * mag + 2.0 ** -24
+    for hint, g in zip(hints[1:], got[1:]):
+        apart = rms((g - got[0]) / mag.clamp(min=1e-30)) / own
+        log(f"[hints] {dtype} new {new} {hint}: {apart:.4f} of the rounding")
+        assert ((g - got[0]).abs() <= room).all(), hint
+        assert apart <= (0.6 if dtype == torch.float16 else 1.0), hint
