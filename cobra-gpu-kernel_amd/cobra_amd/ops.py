@@ -607,12 +607,13 @@ def cache_append(
 
     ``qkv`` [T, (heads + 2 kv_heads) * head_dim] fp16 or bf16, packed q | k | v as for ``attn``
     (with fewer k and v heads where they are shared); ``slots`` [T] int64 from
-    ``cache_reserve``, negative ones are passed over.  ``k`` [num_blocks, kv_heads, block_size,
-    width], ``v`` [num_blocks, kv_heads, width, block_size] (float8_e4m3fn or int8, width =
-    ``cache_width(head_dim)``), ``k_scale`` and ``v_scale`` [num_blocks, kv_heads] fp32.  Each
-    block and head has one scale, a power of two; a token too large for it makes the scale grow
-    and the block's earlier codes are rounded again.  NaN is stored as 0, an infinity as the
-    largest code.
+    ``cache_reserve``, negative ones are passed over (tokens of one block have to stand next to each
+    other, with no such one between them, and come after those that the block keeps).  ``k``
+    [num_blocks, kv_heads, block_size, width], ``v`` [num_blocks, kv_heads, width, block_size]
+    (float8_e4m3fn or int8, width = ``cache_width(head_dim)``), ``k_scale`` and ``v_scale``
+    [num_blocks, kv_heads] fp32.  Each block and head has one scale, a power of two; a token too
+    large for it makes the scale grow and the block's earlier codes are rounded again.  NaN is
+    stored as 0, an infinity as the largest code.
     """
     if _lib.host().cache_append(qkv, slots, heads, head_dim, k, v, k_scale, v_scale):
         return

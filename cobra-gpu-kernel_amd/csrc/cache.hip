@@ -386,15 +386,15 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 //
 // The values are read twice, for the largest and for the codes; the second time they come from
 // the caches (kept in registers in between they cost the occupancy that hides the first: 14000
-// tokens of 8 x 128 took 66 us so, 30 us from the caches).  K's rows are written eight codes to a
-// store.  V's rows run along tokens: a thread takes 4 tokens x 8 dimensions and writes eight
-// words of 4 codes, neighbouring lanes neighbouring words of a row.
+// tokens of 8 x 128 took twice as long).  K's rows are written eight codes to a store.  V's rows
+// run along tokens: a thread takes 4 tokens x 8 dimensions and writes eight words of 4 codes,
+// neighbouring lanes neighbouring words of a row.
 //
-// Bound by latency at one token a request (64 of 8 x 64: 4.9 us).  With whole prompts by the
-// vector ALU, active in 62 % of cycles (78 % before magnitudes went two at a time as integers,
-// values unclamped where nothing can need it, and codes of four tokens were joined by the
-// conversion itself: 14000 tokens of 8 x 128 from 30.7 to 27.0 us, 58 MB read, 29 written, 3.2
-// TB/s where a large copy makes 5.1).
+// Bound by latency at one token a request (64 of 8 x 64: 4.8 us).  With whole prompts by the vector
+// ALU, active in 62 % of cycles, and by each block's wait for its largest value: 14000 tokens of
+// 8 x 128 take 27.3 us, 58 MB read, 29 written, 3.2 TB/s where a large copy makes 5.1 (30.7 us and
+// 78 % before magnitudes went two at a time as integers, values unclamped where nothing can need
+// it, and codes of four tokens were joined by the conversion itself).
 template <typename T, int CACHE, int NT>
 __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int window, int share) {
   typedef typename Op16<T>::V8 V8;
@@ -606,13 +606,19 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(CacheAppendArgs a, int
 
 template <typename T, int CACHE>
 hipError_t launch_append(const CacheAppendArgs& a, hipStream_t stream) {
-  // Few tokens: a workgroup for each.  Many: they are prompts, whose blocks begin every bs
-  // tokens; one and a half times as many workgroups for 63 of them as they have blocks, as some
-  // end inside one (2400 tokens of 6 x 40 in blocks of 16: 7.9 us with 6, 10.2 with 4, 22 with
-  // one; 14000 of 8 x 128 in blocks of 64: 30.4 us with 2, 36.5 with one).
+  // Few tokens: a workgroup for each (64 requests of one token, 8 x 64: 6 to 8 us, in windows of 63
+  // 75; 1024 of them 22 and 84).  Many: they are taken for prompts, whose blocks begin every bs
+  // tokens (8 prompts of 1500 to 2048 tokens, 8 x 64: 18 us in windows, 74 with a workgroup for each
+  // token).  So many requests of one token each are not: 2048 of 8 x 64 take 89 us, a workgroup for each
+  // token would take 39; of 5 tokens each 53 and 63.
+  // One and a half times as many workgroups for a window as it has blocks, as some end inside one:
+  // 7 prompts of up to 700 tokens, 8 x 64, take 7.7, 7.9 and 9.8 us in blocks of 16, 32 and 64, with one
+  // workgroup for a window 17.6, 13.0 and 12.7; the 8 prompts of 8 x 128 28.5, 25.7 and 28.5 for 27.9,
+  // 29.0 and 33.1.  (A block of 128 has one both ways.)
   const bool few = a.tokens * a.kv_heads <= 8192;
   const int window = few ? 1 : 63, share = few ? 1 : (96 + (1 << a.shift) - 1) >> a.shift;
-  // A wave for up to 8192 values (64 x 128: 30.4 us, 33.0 with four waves).
+  // A wave for up to 8192 values, the 8 prompts' blocks of 64 x 128: 28.5 us, 31.8 with four waves (7
+  // prompts of up to 700 tokens 13.7 and 10.1); of 16 x 128 28.5 and 63, of 128 x 64 21.1 and 21.3.
   const bool wave = few || (a.head_dim << a.shift) <= 8192;
   const int64_t groups = (a.tokens + window - 1) / window * share;
   if (groups * (wave ? 64 : 256) > 0xffffffff) return hipErrorInvalidValue;  // threads are counted in 32 bits

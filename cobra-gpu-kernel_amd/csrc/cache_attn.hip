@@ -664,10 +664,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
 // Sets of 32 rows a wave, so that each widened code feeds two matrix instructions; two
 // workgroups to a CU up to head_dim 128.
 //
-// Bound by the vector ALU: for each of a lane's scores an fma, an exponential, a conversion and
-// an addition beside the matrix instructions, of which only the exponential and the codes'
-// conversion overlap them.  2 requests of 2000 new tokens behind 8000 to 14000, 32 heads of 128
-// on 8 (bf16): 940 to 997 us, 0.92 to 0.97 PFLOP/s.
+// Bound by the alternation of products and softmax, which hardly overlap: for each of a lane's scores
+// an fma, an exponential, a conversion and an addition beside the matrix instructions.  2 requests of
+// 2000 new tokens behind 8000 to 14000, 32 heads of 128 on 8 (bf16): 942 us, 0.97 PFLOP/s, the vector
+// ALU active in 64 % of cycles, the matrix cores in 40 %.  With few requests by the longest one's tiles:
+// 5 of 301 to 1024 new tokens, 16 heads of 64 on 4 (fp16), 159 us, CUs busy for two thirds of it (the
+// vector ALU for 67 %, the matrix cores for 32 % of that) while one request's 105 tiles follow each other.
 template <typename T, int CACHE, int HDP, int NR>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a) {
   constexpr int kWaves = 4, kRows = kWaves * NR * 16, KT = 64;
@@ -886,8 +888,10 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
   max_len = max_len < 1 ? 1 : max_len > kMaxKeys ? kMaxKeys : max_len;
   const int64_t group = heads / kv_heads, rows = max_new * group;
-  // Past 64 rows a workgroup's keys are worth sharing among four waves' rows (18 rows of 23
-  // requests at 3000 keys of 256: 71 us so, 26 us in tiles of 16).
+  // Past 64 rows a workgroup's keys are worth sharing among four waves' rows: 64 requests of 1000 keys,
+  // 32 heads of 128 on 8, take 46 us in tiles of 16 and 64 so at 32 rows, 84 and 68 at 64, 163 and 77
+  // at 128; 16 requests of 4000 keys, 6 of 256 on 2, 73 and 57 at 96.  (Requests that leave the chip
+  // empty would do with tiles of 16 for longer: one of 4000 keys, 32 of 128 on 8, 18 and 42 us at 128.)
   p.chunked = rows > 64;
   p.row_tiles = p.chunked ? (rows + 127) / 128 : (rows + 15) / 16;
   p.step = p.chunked ? 64 : 4 * decode_keys(cache_width(head_dim));
@@ -902,8 +906,9 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int
   // Where max_new is too low for the tokens it is the workspace that has to be bounded.
   const int64_t room = kMaxParts / (tokens * heads);
   splits = splits < room ? splits : room;
-  // Up to 1024 keys one workgroup takes less time than the second launch that joins splits
-  // (999 keys of 4 x 32: 6.6 against 8.0 us).
+  // Up to 1024 keys one workgroup takes less time than the second launch that joins splits: at 1000
+  // 6.6 us against 8.0 for one request of 4 x 32, 10.6 against 14.5 for 64 of 16 x 64 on 4, 12.3 against
+  // 15.3 for 16 of 8 x 128 (one of these 10.7 against 10.0), at 300 5.3 to 8.4 against 7.7 to 11.1.
   if (!p.chunked && max_len <= 1024 && cache_width(head_dim) <= 128) splits = 1;
   const int64_t most = (max_len + least - 1) / least;
   splits = splits < most ? splits : most;

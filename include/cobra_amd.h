@@ -218,7 +218,8 @@ int cobra_cache_trim(int32_t* lens, const int32_t* keep_lens, const int32_t* blo
  *     written become those of the same values under it;
  *     code = x / scale rounded to the nearest (ties to even), within +-qmax; NaN gives 0.
  * Tokens of one block stand next to each other in the call, as cobra_cache_reserve lays them
- * out (where they do not, that block's contents are unspecified); of two for one slot the
+ * out (where they do not, or one that is passed over stands between them, that block's contents
+ * are unspecified), and come after those that the block keeps; of two for one slot the
  * later one stays (and counts for a).  A token whose slot is negative or past the pool is
  * passed over.  Blocks without a token are left as they are.
  */
