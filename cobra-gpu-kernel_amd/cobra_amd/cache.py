@@ -31,6 +31,8 @@ class CobraCache:
                         ("num_blocks", num_blocks)):
             if v <= 0:
                 raise ValueError(f"{name} must be positive")
+        if max_len is not None and max_len <= 0:
+            raise ValueError(f"max_len must be positive, got {max_len}")
         if block_size not in ops.CACHE_BLOCKS:
             raise ValueError(f"block_size must be one of {ops.CACHE_BLOCKS}, got {block_size}")
         if dtype not in (torch.float8_e4m3fn, torch.int8):

@@ -1,6 +1,9 @@
-"""CPU tests of how the cache attention's calls are cut, as far as the workspace shows it."""
+"""CPU tests of how the cache attention's calls are cut, as far as the workspace shows it, and of the
+longest request that a cache is made for."""
 
 import random
+
+import pytest
 
 
 def _workspace():
@@ -34,3 +37,12 @@ def test_fitting_hints_keep_their_splits():
                          ((512, 1, 32, 8, 128, 1, 100000), 31)):
         tokens, _, heads, _, hd = args[:5]
         assert q(*args) == splits * tokens * heads * (4 * hd + 8), args
+
+
+@pytest.mark.parametrize("max_len", [0, -1, -5000])
+def test_a_cache_for_requests_of_no_length_is_refused(max_len):
+    """It would have had tables of one block."""
+    from cobra_amd import CobraCache
+
+    with pytest.raises(ValueError, match="max_len must be positive"):
+        CobraCache(1, 2, 64, 2, 4, max_len=max_len, device="cpu")
