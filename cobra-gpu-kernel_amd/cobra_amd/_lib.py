@@ -15,11 +15,12 @@ from typing import Optional
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcobra_amd.so")
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 F16 = 0
 F32 = 1
 BF16 = 2
+E4M3 = 3  # codes of a matrix held in 8 bits
 # Codes of the key/value cache (COBRA_CACHE_* in include/cobra_amd.h).
 CACHE_E4M3 = 0
 CACHE_I8 = 1
@@ -76,6 +77,26 @@ SIGNATURES = {
         _c_int,
         [_vp, _c_int, _c_i64, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _vp],
+    ),
+    "cobra_cache_prefix_attn_workspace_bytes": (
+        _c_i64, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64],
+    ),
+    "cobra_cache_prefix_attn_fwd": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _vp],
+    ),
+    "cobra_cache_positions": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp]),
+    "cobra_qk_norm_rope": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _vp, _vp, _c_i64, _c_int, _vp, _vp, _c_f32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp],
+    ),
+    "cobra_quantize8": (_c_int, [_vp, _c_int, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "cobra_linear8_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "cobra_linear8_fwd": (
+        _c_int,
+        [_vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+         _vp],
     ),
     "cobra_qkv_attn_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "cobra_qkv_attn_fwd": (

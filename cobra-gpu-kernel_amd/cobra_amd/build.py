@@ -55,6 +55,7 @@ FILE_FLAGS = {
                         "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "cache_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "cache_prefix.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

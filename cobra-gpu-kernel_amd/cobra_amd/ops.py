@@ -630,6 +630,32 @@ def cache_append(
              v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cache, T, nb, bs, heads, kvh, head_dim)
 
 
+def _cache_attn_args(q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, out):
+    """Checks of attention over the cache -> (tokens, requests, table width, scale, out)."""
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if q.dim() != 2 or q.shape[1] < heads * head_dim or q.shape[1] % 8:
+        raise ValueError(f"q must be [T, >= {heads * head_dim}] with a multiple of 8 columns, got {list(q.shape)}")
+    if lens.dim() != 1 or block_table.dim() != 2:
+        raise ValueError("lens must have one dimension, block_table two")
+    T, B = q.shape[0], lens.shape[0]
+    _i32(lens, (B,), "lens")
+    _i32(cu, (B + 1,), "cu")
+    _i32(block_table, (B, block_table.shape[1]), "block_table")
+    if scale <= 0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    scale = float(scale)
+    dev = q.device
+    _same_dev(dev, q=q, cu=cu, lens=lens, block_table=block_table, k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+    if out is None:
+        out = torch.empty((T, heads * head_dim), device=dev, dtype=q.dtype)
+    else:
+        _same_dev(dev, out=out)
+        if out.dtype != q.dtype or tuple(out.shape) != (T, heads * head_dim):
+            raise ValueError(f"out must be {q.dtype} [{T}, {heads * head_dim}]")
+    return T, B, block_table.shape[1], scale, out
+
+
 def cache_attn(
     q: torch.Tensor,
     cu: torch.Tensor,
@@ -665,28 +691,7 @@ def cache_attn(
     if got is not None:
         return got
     cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    if q.dim() != 2 or q.shape[1] < heads * head_dim or q.shape[1] % 8:
-        raise ValueError(f"q must be [T, >= {heads * head_dim}] with a multiple of 8 columns, got {list(q.shape)}")
-    if lens.dim() != 1 or block_table.dim() != 2:
-        raise ValueError("lens must have one dimension, block_table two")
-    T, B = q.shape[0], lens.shape[0]
-    _i32(lens, (B,), "lens")
-    _i32(cu, (B + 1,), "cu")
-    _i32(block_table, (B, block_table.shape[1]), "block_table")
-    if scale <= 0:
-        raise ValueError(f"scale must be positive, got {scale}")
-    scale = float(scale)
-    dev = q.device
-    _same_dev(dev, q=q, cu=cu, lens=lens, block_table=block_table, k=k, v=v, k_scale=k_scale, v_scale=v_scale)
-    W = block_table.shape[1]
-    if out is None:
-        out = torch.empty((T, heads * head_dim), device=dev, dtype=q.dtype)
-    else:
-        _same_dev(dev, out=out)
-        if out.dtype != q.dtype or tuple(out.shape) != (T, heads * head_dim):
-            raise ValueError(f"out must be {q.dtype} [{T}, {heads * head_dim}]")
+    T, B, W, scale, out = _cache_attn_args(q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, out)
     if T == 0 or B == 0:
         return out
     if W == 0 or nb == 0:
@@ -694,11 +699,266 @@ def cache_attn(
     new = max(1, T - B + 1) if max_new is None else max(1, int(max_new))
     keys = W * bs if max_len is None else max(1, int(max_len))
     need = _lib.lib().cobra_cache_attn_workspace_bytes(T, B, heads, kvh, head_dim, new, keys)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call_on(dev, "cobra_cache_attn_fwd", q.data_ptr(), _DT[q.dtype], q.shape[1], cu.data_ptr(), lens.data_ptr(),
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _call_on(q.device, "cobra_cache_attn_fwd", q.data_ptr(), _DT[q.dtype], q.shape[1], cu.data_ptr(), lens.data_ptr(),
              block_table.data_ptr(), W, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cache,
              out.data_ptr(), _ptr(ws), max(0, need), T, B, nb, bs, heads, kvh, head_dim, new, keys, float(scale),
              1 if causal else 0)
+    return out
+
+
+def cache_prefix_attn(
+    q: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    block_table: torch.Tensor,
+    prefix: int,
+    heads: int,
+    head_dim: int,
+    scale: float,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    causal: bool = True,
+    max_new: Optional[int] = None,
+    max_len: Optional[int] = None,
+    max_prefix: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``cache_attn`` for requests that share a prefix, computed once for all of them.
+
+    ``prefix`` is the row of ``block_table`` and ``lens`` that holds it, a request like any other:
+    each new token of the other requests sees all of its keys in front of its own request's, in one
+    softmax; new tokens of that row itself see only its own.  (Keys that are rotated by position
+    have to be rotated for standing behind the prefix: ``cache_positions(prefix=...)``.)
+    Groups of neighbouring rows with a prefix each are a call each, on views of ``cu``, ``lens``
+    and ``block_table``, with one ``out``.  ``max_prefix`` is the most keys that the prefix is
+    expected to have (default: what the table allows), ``max_new`` and ``max_len`` are about the
+    other rows; they matter as in ``cache_attn``.
+    """
+    got = _lib.host().cache_prefix_attn(q, cu, lens, block_table, prefix, heads, head_dim, scale, k, v, k_scale,
+                                        v_scale, causal, max_new, max_len, max_prefix, out)
+    if got is not None:
+        return got
+    cache, nb, kvh, bs = _cache_geometry(k, v, k_scale, v_scale, heads, head_dim)
+    T, B, W, scale, out = _cache_attn_args(q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, out)
+    prefix = int(prefix)
+    if not 0 <= prefix < B:
+        raise ValueError(f"prefix must be a row of the tables, 0 .. {B - 1}, got {prefix}")
+    if T == 0:
+        return out
+    if W == 0 or nb == 0:
+        raise ValueError("block_table and the cache must hold at least one block")
+    new = max(1, T - B + 2) if max_new is None else max(1, int(max_new))
+    keys = W * bs if max_len is None else max(1, int(max_len))
+    shared = W * bs if max_prefix is None else max(1, int(max_prefix))
+    need = _lib.lib().cobra_cache_prefix_attn_workspace_bytes(T, B, heads, kvh, head_dim, new, keys, shared)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _call_on(q.device, "cobra_cache_prefix_attn_fwd", q.data_ptr(), _DT[q.dtype], q.shape[1], cu.data_ptr(),
+             lens.data_ptr(), block_table.data_ptr(), W, prefix, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+             v_scale.data_ptr(), cache, out.data_ptr(), _ptr(ws), max(0, need), T, B, nb, bs, heads, kvh, head_dim, new,
+             keys, shared, float(scale), 1 if causal else 0)
+    return out
+
+
+def cache_positions(cu: torch.Tensor, lens: torch.Tensor, tokens: int, prefix: Optional[int] = None) -> torch.Tensor:
+    """Where each new token stands in its request -> ``positions [tokens]`` int32.
+
+    ``cu`` [B + 1] and ``lens`` [B] as for ``cache_attn`` (after ``cache_reserve``).  With ``prefix``,
+    a row of ``lens``, the tokens of every other row stand behind that row's.  -1 for rows of no
+    request.
+    """
+    if lens.dim() != 1:
+        raise ValueError("lens must have one dimension")
+    B = lens.shape[0]
+    _i32(lens, (B,), "lens")
+    _i32(cu, (B + 1,), "cu")
+    _same_dev(lens.device, lens=lens, cu=cu)
+    tokens = int(tokens)
+    if not 0 <= tokens <= 0x7FFFFFFF:
+        raise ValueError(f"tokens must be 0 .. 2^31 - 1, got {tokens}")
+    row = -1 if prefix is None else int(prefix)
+    if prefix is not None and not 0 <= row < B:
+        raise ValueError(f"prefix must be a row of lens, 0 .. {B - 1}, got {prefix}")
+    if B == 0:
+        return torch.full((tokens,), -1, dtype=torch.int32, device=lens.device)
+    out = torch.empty(tokens, dtype=torch.int32, device=lens.device)
+    _call_on(lens.device, "cobra_cache_positions", cu.data_ptr(), lens.data_ptr(), out.data_ptr(), tokens, B, row)
+    return out
+
+
+def qk_norm_rope(
+    qkv: torch.Tensor,
+    heads: int,
+    kv_heads: int,
+    head_dim: int,
+    positions: Optional[torch.Tensor] = None,
+    inv_freq: Optional[torch.Tensor] = None,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    eps: float = 1e-6,
+    pitch: Optional[int] = None,
+) -> None:
+    """Root-mean-square norms of queries and keys for each head and their rotation by position, in
+    place and in one pass.
+
+    ``qkv`` [T, C] fp16 or bf16, packed q | k | v as for ``attn`` and ``cache_append`` (heads of
+    ``head_dim`` <= 256 columns, ``pitch`` columns apart where they are padded; what stands behind the
+    keys is left as it is).  ``q_weight`` and ``k_weight`` [head_dim]: ``x / sqrt(mean(x^2) + eps) *
+    weight`` for each head; both or neither.  ``inv_freq`` [r]: the first 2 r columns turn by
+    ``positions[t] * inv_freq[i]``, pairs (i, i + r) or, ``interleaved``, (2 i, 2 i + 1); ``positions``
+    [T] int32, tokens at negative ones are left as they are.  fp32 arithmetic (angles in 64 bits), one
+    rounding.
+    """
+    if _lib.host().qk_norm_rope(qkv, heads, kv_heads, head_dim, positions, inv_freq, q_weight, k_weight, interleaved,
+                                eps, pitch):
+        return
+    if qkv.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
+    pitch = head_dim if pitch is None else int(pitch)
+    if heads <= 0 or kv_heads <= 0 or not 0 < head_dim <= 256 or pitch < head_dim:
+        raise ValueError(f"heads and kv_heads must be positive and 0 < head_dim <= 256 within pitch, got {heads}, "
+                         f"{kv_heads}, {head_dim}, {pitch}")
+    if qkv.dim() != 2 or qkv.shape[1] < (heads + kv_heads) * pitch:
+        raise ValueError(f"qkv must be [T, >= {(heads + kv_heads) * pitch}], got {list(qkv.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    dev, T = qkv.device, qkv.shape[0]
+    given = {"qkv": qkv}
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or 2 * inv_freq.shape[0] > head_dim:
+            raise ValueError(f"inv_freq must be float32 [<= {head_dim // 2}], got {inv_freq.dtype} {list(inv_freq.shape)}")
+        if positions is None:
+            raise ValueError("inv_freq needs positions")
+        rot = 2 * inv_freq.shape[0]
+        given["inv_freq"] = inv_freq
+    if positions is not None:
+        _i32(positions, (T,), "positions")
+        given["positions"] = positions
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight must both be given or both be None")
+    _same_dev(dev, **given)
+    qw = kw = None
+    if q_weight is not None:
+        qw, kw = _f32_param(q_weight, head_dim, "q_weight"), _f32_param(k_weight, head_dim, "k_weight")
+        _same_dev(dev, q_weight=qw, k_weight=kw)
+    _call_on(dev, "cobra_qk_norm_rope", qkv.data_ptr(), _DT[qkv.dtype], qkv.shape[1], _ptr(positions), _ptr(inv_freq),
+             rot, 1 if interleaved else 0, _ptr(qw), _ptr(kw), float(eps), T, heads, kv_heads, head_dim, pitch)
+
+
+def width8(k: int) -> Tuple[int, int]:
+    """Columns of codes and of scales that ``quantize8`` gives K columns."""
+    return -(-k // 128) * 128, -(-k // 512) * 4
+
+
+def quantize8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A matrix in 8 bits, in blocks of 128 columns -> ``(codes, scale)``.
+
+    ``x`` [M, K] fp16, bf16 or fp32.  ``codes`` [M, Kp] float8_e4m3fn, Kp = K rounded up to 128 (zeros
+    past K); ``scale`` [M, S] float8_e8m0fnu, S = 4 ceil(K / 512), a power of two for each row and 128
+    columns (1 past Kp / 128): the least one >= 2^-126 with the block's largest finite magnitude
+    within 448 of it.  Codes are rounded to the nearest, ties to even; what is not finite becomes NaN.
+    """
+    got = _lib.host().quantize8(x)
+    if got is not None:
+        return got
+    _dev(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must be [M, K] with K > 0, got {list(x.shape)}")
+    dt = _dtype_code(x, "x")
+    M, K = x.shape
+    kp, s = width8(K)
+    codes = torch.empty((M, kp), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((M, s), dtype=torch.float8_e8m0fnu, device=x.device)
+    _call_on(x.device, "cobra_quantize8", x.data_ptr(), dt, codes.data_ptr(), scale.data_ptr(), M, K)
+    return codes, scale
+
+
+def _codes8(codes: torch.Tensor, scale: torch.Tensor, what: str) -> None:
+    if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2 or codes.shape[1] == 0 or codes.shape[1] % 128:
+        raise ValueError(f"{what} must be float8_e4m3fn codes [rows, a multiple of 128], got {codes.dtype} "
+                         f"{list(codes.shape)}")
+    want = (codes.shape[0], width8(codes.shape[1])[1])
+    if scale.dtype != torch.float8_e8m0fnu or tuple(scale.shape) != want:
+        raise ValueError(f"{what}_scale must be float8_e8m0fnu {list(want)}, got {scale.dtype} {list(scale.shape)}")
+
+
+def linear8(
+    a: torch.Tensor,
+    w: torch.Tensor,
+    w_scale: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    gelu: bool = False,
+    out_dtype: Optional[torch.dtype] = None,
+    resid: Optional[torch.Tensor] = None,
+    rmask: Optional[torch.Tensor] = None,
+    mask_branch: bool = False,
+    a_scale: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``linear`` with both operands in 8 bits: ``a @ w.T + bias`` (GELU) ``(+ resid)``, fp32 sums.
+
+    ``w`` [N, Kp] and ``w_scale`` [N, S] are ``quantize8`` of an nn.Linear weight [N, K].  ``a`` [M, K]
+    fp16 or bf16 is quantised in the call by the same rule; or ``a`` [M, Kp] and ``a_scale`` [M, S] are
+    its result already (activations that several products share).  ``out_dtype`` is fp16, bf16 or
+    fp32 (default: a's own type, which codes do not have).  ``resid`` [M, N] in any of these types;
+    ``gelu``, ``rmask`` and ``mask_branch`` as in ``linear``.
+    """
+    got = _lib.host().linear8(a, w, w_scale, bias, gelu, out_dtype, resid, rmask, mask_branch, a_scale)
+    if got is not None:
+        return got
+    _codes8(w, w_scale, "w")
+    N, kp = w.shape
+    dev = w.device
+    if a.dim() != 2:
+        raise ValueError(f"a must have two dimensions, got {list(a.shape)}")
+    if a_scale is not None:
+        _codes8(a, a_scale, "a")
+        code, K = _lib.E4M3, kp
+        if a.shape[1] != kp:
+            raise ValueError(f"inner dimensions differ: a {list(a.shape)}, w {list(w.shape)}")
+        if out_dtype is None:
+            raise ValueError("codes have no type of their own for the result: out_dtype is needed")
+    else:
+        if a.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"a must be float16 or bfloat16, or codes with a_scale, got {a.dtype}")
+        code, K = _DT[a.dtype], a.shape[1]
+        if K == 0 or width8(K)[0] != kp:
+            raise ValueError(f"inner dimensions differ: a {list(a.shape)}, w {list(w.shape)} (a multiple of 128)")
+        out_dtype = a.dtype if out_dtype is None else out_dtype
+    M = a.shape[0]
+    given = {"w": w, "w_scale": w_scale, "a": a}
+    if a_scale is not None:
+        given["a_scale"] = a_scale
+    b32 = None
+    if bias is not None:
+        b32 = given["bias"] = _f32_param(bias, N, "bias")
+    if resid is not None:
+        if tuple(resid.shape) != (M, N):
+            raise ValueError(f"resid must be [{M}, {N}], got {list(resid.shape)}")
+        given["resid"] = resid
+    mrow = _row_mask(rmask, M, "rmask")
+    if mrow is not None:
+        given["rmask"] = mrow
+    _same_dev(dev, **given)
+    epi = _lib.EPI_GELU if gelu else 0
+    if mrow is not None:
+        if mask_branch:
+            epi |= _lib.EPI_MASK_BRANCH
+        elif resid is not None:
+            epi |= _lib.EPI_MASK_RESID
+        else:
+            mrow = None
+    out = torch.empty((M, N), device=dev, dtype=out_dtype)
+    out_code, resid_code = _dtype_code(out, "out_dtype"), _dtype_code(resid, "resid") if resid is not None else 0
+    if N == 0 or M == 0:
+        return out
+    need = _lib.lib().cobra_linear8_workspace_bytes(M, N, K, code)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _call_on(dev, "cobra_linear8_fwd", a.data_ptr(), code, _ptr(a_scale), w.data_ptr(), w_scale.data_ptr(), _ptr(b32),
+             _ptr(resid), resid_code, _ptr(mrow), epi, out.data_ptr(), out_code, _ptr(ws), max(0, need), M, N, K)
     return out
 
 

@@ -529,53 +529,208 @@ int64_t cobra_cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t 
   return cobra::cache_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
 }
 
+namespace {
+
+// The kernels' arguments of a call of attention over the cache that needs `need` bytes of workspace:
+// false where the call is refused.
+bool cache_attn_call(cobra::CacheAttnArgs* a, int64_t need, const void* q, int dtype, int64_t ldq, const int32_t* cu,
+                     const int32_t* lens, const int32_t* block_table, int64_t table_width, const void* k, const void* v,
+                     const float* k_scale, const float* v_scale, int cache, void* ctx, void* workspace,
+                     int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_blocks, int64_t block_size,
+                     int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len, float scale,
+                     int causal) {
+  if (!q || !cu || !lens || !block_table || !k || !v || !k_scale || !v_scale || !ctx || !aligned16(q) ||
+      !aligned16(k) || !aligned16(v) || !aligned16(ctx) || !aligned_to(cu, 4) || !aligned_to(lens, 4) ||
+      !aligned_to(block_table, 4) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+    return false;
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return false;
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), c0 = reinterpret_cast<uintptr_t>(ctx);
+  const uintptr_t row = static_cast<uintptr_t>(heads * head_dim);  // ctx would be read as queries
+  if (q0 < c0 + 2 * tokens * row && c0 < q0 + 2 * ((tokens - 1) * ldq + row)) return false;
+  a->q = q;
+  a->out = ctx;
+  a->cu = cu;
+  a->lens = lens;
+  a->table = block_table;
+  a->k = k;
+  a->v = v;
+  a->k_scale = k_scale;
+  a->v_scale = v_scale;
+  a->part = static_cast<float*>(workspace);
+  a->tokens = tokens;
+  a->ldq = ldq;
+  a->num_blocks = num_blocks;
+  a->table_width = table_width;
+  a->batch = (int)batch;
+  a->heads = (int)heads;
+  a->kv_heads = (int)kv_heads;
+  a->head_dim = (int)head_dim;
+  a->shift = cobra::cache_shift(block_size);
+  a->dtype = dtype;
+  a->cache = cache;
+  a->causal = causal ? 1 : 0;
+  a->scale = scale;
+  a->max_new = max_new;
+  a->max_len = max_len;
+  return true;
+}
+
+// Whether the sizes and types of such a call are taken.
+bool cache_attn_shape_ok(int dtype, int64_t ldq, int64_t table_width, int cache, int64_t num_blocks,
+                         int64_t block_size, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale) {
+  return is_op_dtype(dtype) && cache_ok(cache, num_blocks, kv_heads, heads, head_dim, block_size) && num_blocks != 0 &&
+         table_width > 0 && table_width <= 0x7fffffff && ldq >= heads * head_dim && ldq % 8 == 0 && scale > 0.f;
+}
+
+// Whether two ranges of bytes meet.
+bool ranges_meet(const void* x, int64_t nx, const void* y, int64_t ny) {
+  const char *px = static_cast<const char*>(x), *py = static_cast<const char*>(y);
+  return px < py + ny && py < px + nx;
+}
+
+}  // namespace
+
 int cobra_cache_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* cu, const int32_t* lens,
                          const int32_t* block_table, int64_t table_width, const void* k, const void* v,
                          const float* k_scale, const float* v_scale, int cache, void* ctx, void* workspace,
                          int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_blocks,
                          int64_t block_size, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                          int64_t max_len, float scale, int causal, void* stream) {
-  if (!is_op_dtype(dtype) || !cache_ok(cache, num_blocks, kv_heads, heads, head_dim, block_size) || num_blocks == 0 ||
-      table_width <= 0 || table_width > 0x7fffffff || ldq < heads * head_dim || ldq % 8 || !(scale > 0.f))
+  if (!cache_attn_shape_ok(dtype, ldq, table_width, cache, num_blocks, block_size, heads, kv_heads, head_dim, scale))
     return kBad;
   const int64_t need = cobra_cache_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
   if (need < 0) return kBad;
   if (tokens == 0 || batch == 0) return 0;
-  if (!q || !cu || !lens || !block_table || !k || !v || !k_scale || !v_scale || !ctx || !aligned16(q) ||
-      !aligned16(k) || !aligned16(v) || !aligned16(ctx) || !aligned_to(cu, 4) || !aligned_to(lens, 4) ||
-      !aligned_to(block_table, 4) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
-    return kBad;
-  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return kBad;
-  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), c0 = reinterpret_cast<uintptr_t>(ctx);
-  const uintptr_t row = static_cast<uintptr_t>(heads * head_dim);  // ctx would be read as queries
-  if (q0 < c0 + 2 * tokens * row && c0 < q0 + 2 * ((tokens - 1) * ldq + row)) return kBad;
   cobra::CacheAttnArgs a{};
-  a.q = q;
-  a.out = ctx;
-  a.cu = cu;
-  a.lens = lens;
-  a.table = block_table;
-  a.k = k;
-  a.v = v;
-  a.k_scale = k_scale;
-  a.v_scale = v_scale;
-  a.part = static_cast<float*>(workspace);
-  a.tokens = tokens;
-  a.ldq = ldq;
-  a.num_blocks = num_blocks;
-  a.table_width = table_width;
-  a.batch = (int)batch;
-  a.heads = (int)heads;
-  a.kv_heads = (int)kv_heads;
-  a.head_dim = (int)head_dim;
-  a.shift = cobra::cache_shift(block_size);
-  a.dtype = dtype;
-  a.cache = cache;
-  a.causal = causal ? 1 : 0;
-  a.scale = scale;
-  a.max_new = max_new;
-  a.max_len = max_len;
+  if (!cache_attn_call(&a, need, q, dtype, ldq, cu, lens, block_table, table_width, k, v, k_scale, v_scale, cache, ctx,
+                       workspace, workspace_bytes, tokens, batch, num_blocks, block_size, heads, kv_heads, head_dim,
+                       max_new, max_len, scale, causal))
+    return kBad;
   return code(cobra::run_cache_attn(a, workspace_bytes, static_cast<hipStream_t>(stream)));
+}
+
+int64_t cobra_cache_prefix_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t max_new, int64_t max_len,
+                                                int64_t max_prefix) {
+  if (max_prefix < 0) return -1;
+  const int64_t own = cobra_cache_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  if (own < 0 || tokens == 0 || batch == 0) return own;
+  return cobra::cache_prefix_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new, max_len, max_prefix);
+}
+
+int cobra_cache_prefix_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* cu, const int32_t* lens,
+                                const int32_t* block_table, int64_t table_width, int64_t prefix, const void* k,
+                                const void* v, const float* k_scale, const float* v_scale, int cache, void* ctx,
+                                void* workspace, int64_t workspace_bytes, int64_t tokens, int64_t batch,
+                                int64_t num_blocks, int64_t block_size, int64_t heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t max_new, int64_t max_len, int64_t max_prefix, float scale,
+                                int causal, void* stream) {
+  if (!cache_attn_shape_ok(dtype, ldq, table_width, cache, num_blocks, block_size, heads, kv_heads, head_dim, scale) ||
+      prefix < 0 || prefix >= batch)
+    return kBad;
+  const int64_t need = cobra_cache_prefix_attn_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, max_new,
+                                                               max_len, max_prefix);
+  if (need < 0) return kBad;
+  if (tokens == 0) return 0;
+  cobra::CachePrefixArgs a{};
+  if (!cache_attn_call(&a.attn, need, q, dtype, ldq, cu, lens, block_table, table_width, k, v, k_scale, v_scale, cache,
+                       ctx, workspace, workspace_bytes, tokens, batch, num_blocks, block_size, heads, kv_heads,
+                       head_dim, max_new, max_len, scale, causal))
+    return kBad;
+  a.prefix = (int)prefix;
+  a.max_prefix = max_prefix;
+  return code(cobra::run_cache_prefix(a, workspace_bytes, static_cast<hipStream_t>(stream)));
+}
+
+int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* positions, int64_t tokens, int64_t batch,
+                          int64_t prefix, void* stream) {
+  if (tokens < 0 || tokens > 0x7fffffff || batch <= 0 || batch > 0x7ffffffe || prefix < -1 || prefix >= batch) return kBad;
+  if (tokens == 0) return 0;
+  for (const void* p : {(const void*)cu, (const void*)lens, (const void*)positions})
+    if (!p || !aligned_to(p, 4)) return kBad;
+  return code(cobra::run_cache_positions(cu, lens, positions, tokens, (int)batch, (int)prefix,
+                                         static_cast<hipStream_t>(stream)));
+}
+
+// -- norms and rotation of queries and keys --------------------------------------------------
+
+int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, const float* inv_freq, int64_t rot,
+                       int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream) {
+  if (!is_op_dtype(dtype) || tokens < 0 || tokens > 0x7fffffff || heads <= 0 || heads > 0x7fffff || kv_heads <= 0 ||
+      kv_heads > 0x7fffff || head_dim <= 0 || head_dim > 256 || pitch < head_dim || pitch > 0x7fffff || rot < 0 ||
+      rot % 2 || rot > head_dim || ld < (heads + kv_heads) * pitch || !(eps >= 0.f) ||
+      (q_weight == nullptr) != (k_weight == nullptr))
+    return kBad;
+  if (tokens == 0 || (rot == 0 && !q_weight)) return 0;
+  if (!qkv || !aligned_to(qkv, 2) || (rot && (!positions || !inv_freq)) || !aligned_to(positions, 4) ||
+      !aligned_to(inv_freq, 4) || !aligned_to(q_weight, 4) || !aligned_to(k_weight, 4))
+    return kBad;
+  const cobra::QkNormRopeArgs a{qkv, positions, inv_freq, q_weight, k_weight, tokens, ld, (int)heads, (int)kv_heads,
+                                (int)head_dim, (int)pitch, (int)rot, interleaved ? 1 : 0, dtype, eps};
+  return code(cobra::run_qk_norm_rope(a, static_cast<hipStream_t>(stream)));
+}
+
+// -- products in 8 bits ---------------------------------------------------------------------
+
+static_assert(COBRA_E4M3 == cobra::kE4M3, "ABI dtype values are the kernels' own");
+
+namespace {
+
+// Columns of codes and bytes of a row of scales for K columns.
+int64_t codes_of(int64_t K) { return (K + 127) & ~int64_t(127); }
+int64_t scales_of(int64_t K) { return (K + 511) / 512 * 4; }
+constexpr int64_t kMaxK = 0x7fff00;
+
+}  // namespace
+
+int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_t M, int64_t K, void* stream) {
+  if (!is_act_dtype(x_dtype) || M < 0 || M > 0x7fffffff || K <= 0 || K > kMaxK || M * scales_of(K) / 4 > 0x7fffffff)
+    return kBad;
+  if (M == 0) return 0;
+  if (!x || !codes || !scale || !aligned_to(x, dtype_bytes(x_dtype)) || !aligned16(codes) || !aligned_to(scale, 4))
+    return kBad;
+  const int64_t xb = M * K * dtype_bytes(x_dtype), cb = M * codes_of(K), sb = M * scales_of(K);
+  if (ranges_meet(x, xb, codes, cb) || ranges_meet(x, xb, scale, sb) || ranges_meet(codes, cb, scale, sb)) return kBad;
+  const cobra::Quantize8Args a{x, codes, scale, M, K, x_dtype};
+  return code(cobra::run_quantize8(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t cobra_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_dtype) {
+  if (!(is_op_dtype(a_dtype) || a_dtype == COBRA_E4M3) || M < 0 || M > 0x7fffffff || N <= 0 || N > 0x7ffffff || K <= 0 ||
+      K > kMaxK || M * scales_of(K) / 4 > 0x7fffffff)
+    return -1;
+  return M == 0 ? 0 : cobra::linear8_workspace_bytes(M, K, a_dtype);
+}
+
+int cobra_linear8_fwd(const void* a, int a_dtype, const void* a_scale, const void* w, const void* w_scale,
+                      const float* bias, const void* resid, int resid_dtype, const uint8_t* row_mask, int epi, void* c,
+                      int c_dtype, void* workspace, int64_t workspace_bytes, int64_t M, int64_t N, int64_t K,
+                      void* stream) {
+  const int64_t need = cobra_linear8_workspace_bytes(M, N, K, a_dtype);
+  constexpr int kMasks = COBRA_EPI_MASK_BRANCH | COBRA_EPI_MASK_RESID;
+  if (need < 0 || !is_act_dtype(c_dtype) || (resid && !is_act_dtype(resid_dtype)) ||
+      (epi & ~(COBRA_EPI_GELU | kMasks)))
+    return kBad;
+  if (M == 0) return 0;
+  if (!a || !w || !w_scale || !c || !aligned16(a) || !aligned16(w) || !aligned_to(w_scale, 4) || !opt_aligned16(bias) ||
+      !opt_aligned16(resid) || !aligned16(c) || ((epi & kMasks) && !row_mask))
+    return kBad;
+  const bool codes = a_dtype == COBRA_E4M3;
+  if (codes && (!a_scale || !aligned_to(a_scale, 4))) return kBad;
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return kBad;
+  // What is written must not be read by another workgroup: resid may be c itself.
+  const int64_t cb = M * N * dtype_bytes(c_dtype), ab = codes ? M * codes_of(K) : M * K * 2;
+  if (ranges_meet(c, cb, a, ab) || ranges_meet(c, cb, w, N * codes_of(K)) ||
+      ranges_meet(c, cb, w_scale, N * scales_of(K)) || (codes && ranges_meet(c, cb, a_scale, M * scales_of(K))))
+    return kBad;
+  if (need > 0 && (ranges_meet(workspace, need, a, ab) || ranges_meet(workspace, need, c, cb))) return kBad;
+  if (resid && !(resid == c && resid_dtype == c_dtype) && ranges_meet(c, cb, resid, M * N * dtype_bytes(resid_dtype)))
+    return kBad;
+  const cobra::Linear8Args l{a, static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(w),
+                             static_cast<const uint8_t*>(w_scale), bias, resid, row_mask, c, workspace, M, N, K, a_dtype,
+                             resid_dtype, c_dtype, epi};
+  return code(cobra::run_linear8(l, workspace_bytes, static_cast<hipStream_t>(stream)));
 }
 
 int64_t cobra_qkv_attn_workspace_bytes(int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim) {

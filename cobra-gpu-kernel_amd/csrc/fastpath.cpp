@@ -378,51 +378,241 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// What both forms of attention over the cache take; their arguments stand in the same order, with
+// the prefix's row behind the tables and its expected length behind max_len.
+struct AttnCall {
+  const at::Tensor *q, *cu, *lens, *table;
+  at::Tensor out, ws;
+  Pool p;
+  int dt, dev, causal;
+  int64_t heads, hd, T, B, W, new_most, len_most, pre, pre_most;
+  float scale;
+  PyObject* given;  // the caller's out, or None
+  bool read(PyObject* const* a, bool prefix) {
+    q = rows16(a[0], &dt);
+    if (!q) return false;
+    dev = q->device().index();
+    cu = dev_tensor(a[1], dev, at::kInt);
+    lens = dev_tensor(a[2], dev, at::kInt);
+    table = dev_tensor(a[3], dev, at::kInt);
+    PyObject* const* b = prefix ? a + 5 : a + 4;
+    if (prefix && !py_int(a[4], &pre)) return false;
+    if (!py_int(b[0], &heads) || !py_int(b[1], &hd) || !PyFloat_Check(b[2])) return false;
+    if (!cu || !lens || !table || !p.read(b + 3, dev, heads, hd) || lens->dim() != 1 || table->dim() != 2) return false;
+    T = q->size(0), B = lens->size(0), W = table->size(1);
+    if (!PyBool_Check(b[7]) || T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) ||
+        table->size(0) != B || q->size(1) < heads * hd || q->size(1) % 8 || !(PyFloat_AS_DOUBLE(b[2]) > 0.0) ||
+        (prefix && (pre < 0 || pre >= B)))
+      return false;
+    scale = static_cast<float>(PyFloat_AS_DOUBLE(b[2]));
+    causal = b[7] == Py_True ? 1 : 0;
+    new_most = T - B + (prefix ? 2 : 1), len_most = W * p.block, pre_most = len_most;
+    if (b[8] != Py_None && !py_int(b[8], &new_most)) return false;
+    if (b[9] != Py_None && !py_int(b[9], &len_most)) return false;
+    if (prefix && b[10] != Py_None && !py_int(b[10], &pre_most)) return false;
+    if (new_most < 1) new_most = 1;
+    if (len_most < 1) len_most = 1;
+    if (pre_most < 1) pre_most = 1;
+    given = prefix ? b[11] : b[10];
+    if (given == Py_None) {
+      out = new_tensor({T, heads * hd}, q->scalar_type(), q->device());
+    } else {
+      const at::Tensor* o = dev_tensor(given, dev, q->scalar_type());
+      if (!shape_is(o, {T, heads * hd})) return false;
+      out = *o;
+    }
+    return true;
+  }
+  void* workspace(int64_t need) {
+    if (need <= 0) return nullptr;
+    ws = new_tensor({need}, at::kByte, q->device());
+    return ws.data_ptr();
+  }
+  PyObject* result() {
+    if (given != Py_None) {
+      Py_INCREF(given);
+      return given;
+    }
+    return THPVariable_Wrap(std::move(out));
+  }
+};
+
 // (q, cu, lens, block_table, heads, head_dim, scale, k, v, k_scale, v_scale, causal, max_new | None,
 // max_len | None, out | None) -> ctx | None
 PyObject* cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    int dt;
-    int64_t heads, hd;
-    const at::Tensor* q = n == 15 ? rows16(a[0], &dt) : nullptr;
-    if (!q || !py_int(a[4], &heads) || !py_int(a[5], &hd) || !PyFloat_Check(a[6])) return none();
-    const int dev = q->device().index();
-    const at::Tensor *cu = dev_tensor(a[1], dev, at::kInt), *lens = dev_tensor(a[2], dev, at::kInt),
-                     *table = dev_tensor(a[3], dev, at::kInt);
-    Pool p;
-    if (!cu || !lens || !table || !p.read(a + 7, dev, heads, hd) || lens->dim() != 1 || table->dim() != 2) return none();
-    const int64_t T = q->size(0), B = lens->size(0), W = table->size(1);
-    if (!PyBool_Check(a[11]) || T == 0 || B == 0 || W == 0 || p.blocks == 0 || !shape_is(cu, {B + 1}) ||
-        table->size(0) != B || q->size(1) < heads * hd || q->size(1) % 8 || !(PyFloat_AS_DOUBLE(a[6]) > 0.0))
-      return none();
-    int64_t new_most = T - B + 1, len_most = W * p.block;
-    if (a[12] != Py_None && !py_int(a[12], &new_most)) return none();
-    if (a[13] != Py_None && !py_int(a[13], &len_most)) return none();
-    if (new_most < 1) new_most = 1;
-    if (len_most < 1) len_most = 1;
-    at::Tensor out;
-    if (a[14] == Py_None) {
-      out = new_tensor({T, heads * hd}, q->scalar_type(), q->device());
-    } else {
-      const at::Tensor* o = dev_tensor(a[14], dev, q->scalar_type());
-      if (!shape_is(o, {T, heads * hd})) return none();
-      out = *o;
-    }
-    const int64_t need = cobra_cache_attn_workspace_bytes(T, B, heads, p.kv_heads, hd, new_most, len_most);
+    AttnCall c;
+    if (n != 15 || !c.read(a, false)) return none();
+    const int64_t need =
+        cobra_cache_attn_workspace_bytes(c.T, c.B, c.heads, c.p.kv_heads, c.hd, c.new_most, c.len_most);
     if (need < 0) return none();
-    at::Tensor ws;
-    if (need > 0) ws = new_tensor({need}, at::kByte, q->device());
+    void* ws = c.workspace(need);
     const int code = cobra_cache_attn_fwd(
-        q->data_ptr(), dt, q->size(1), cu->data_ptr<int>(), lens->data_ptr<int>(), table->data_ptr<int>(), W,
-        p.k->data_ptr(), p.v->data_ptr(), p.k_scale->data_ptr<float>(), p.v_scale->data_ptr<float>(), p.cache,
-        out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, T, B, p.blocks, p.block, heads, p.kv_heads, hd,
-        new_most, len_most, static_cast<float>(PyFloat_AS_DOUBLE(a[6])), a[11] == Py_True ? 1 : 0,
-        c10::hip::getCurrentHIPStream(dev).stream());
+        c.q->data_ptr(), c.dt, c.q->size(1), c.cu->data_ptr<int>(), c.lens->data_ptr<int>(), c.table->data_ptr<int>(),
+        c.W, c.p.k->data_ptr(), c.p.v->data_ptr(), c.p.k_scale->data_ptr<float>(), c.p.v_scale->data_ptr<float>(),
+        c.p.cache, c.out.data_ptr(), ws, need, c.T, c.B, c.p.blocks, c.p.block, c.heads, c.p.kv_heads, c.hd, c.new_most,
+        c.len_most, c.scale, c.causal, c10::hip::getCurrentHIPStream(c.dev).stream());
     check("cobra_cache_attn_fwd", code);
-    if (a[14] != Py_None) {
-      Py_INCREF(a[14]);
-      return a[14];
+    return c.result();
+  });
+}
+
+// (q, cu, lens, block_table, prefix, heads, head_dim, scale, k, v, k_scale, v_scale, causal, max_new | None,
+// max_len | None, max_prefix | None, out | None) -> ctx | None
+PyObject* cache_prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    AttnCall c;
+    if (n != 17 || !c.read(a, true)) return none();
+    const int64_t need = cobra_cache_prefix_attn_workspace_bytes(c.T, c.B, c.heads, c.p.kv_heads, c.hd, c.new_most,
+                                                                 c.len_most, c.pre_most);
+    if (need < 0) return none();
+    void* ws = c.workspace(need);
+    const int code = cobra_cache_prefix_attn_fwd(
+        c.q->data_ptr(), c.dt, c.q->size(1), c.cu->data_ptr<int>(), c.lens->data_ptr<int>(), c.table->data_ptr<int>(),
+        c.W, c.pre, c.p.k->data_ptr(), c.p.v->data_ptr(), c.p.k_scale->data_ptr<float>(),
+        c.p.v_scale->data_ptr<float>(), c.p.cache, c.out.data_ptr(), ws, need, c.T, c.B, c.p.blocks, c.p.block, c.heads,
+        c.p.kv_heads, c.hd, c.new_most, c.len_most, c.pre_most, c.scale, c.causal,
+        c10::hip::getCurrentHIPStream(c.dev).stream());
+    check("cobra_cache_prefix_attn_fwd", code);
+    return c.result();
+  });
+}
+
+// An optional fp32 parameter of n values on a device: false where it is none of that.
+bool opt_f32(PyObject* o, int dev, int64_t n, const at::Tensor** t) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  *t = dev_tensor(o, dev, at::kFloat);
+  return *t && shape_is(*t, {n});
+}
+const float* f32_or_null(const at::Tensor* t) { return t ? t->data_ptr<float>() : nullptr; }
+
+// The C ABI's code of an activation type, or -1.
+int act_code(at::ScalarType t) {
+  return t == at::kHalf ? COBRA_F16 : t == at::kBFloat16 ? COBRA_BF16 : t == at::kFloat ? COBRA_F32 : -1;
+}
+
+// (qkv, heads, kv_heads, head_dim, positions | None, inv_freq | None, q_weight | None, k_weight | None,
+// interleaved, eps, pitch | None) -> True | None
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int dt;
+    int64_t heads, kv, hd, pitch;
+    const at::Tensor* x = n == 11 ? rows16(a[0], &dt) : nullptr;
+    if (!x || !py_int(a[1], &heads) || !py_int(a[2], &kv) || !py_int(a[3], &hd) || !PyBool_Check(a[8]) ||
+        !PyFloat_Check(a[9]))
+      return none();
+    pitch = hd;
+    if (a[10] != Py_None && !py_int(a[10], &pitch)) return none();
+    const int dev = x->device().index();
+    const int64_t T = x->size(0);
+    const at::Tensor *qw, *kw, *freq = nullptr, *pos = nullptr;
+    if (hd <= 0 || hd > 256 || !opt_f32(a[6], dev, hd, &qw) || !opt_f32(a[7], dev, hd, &kw) || !qw != !kw) return none();
+    int64_t rot = 0;
+    if (a[4] != Py_None) {
+      pos = dev_tensor(a[4], dev, at::kInt);
+      if (!pos || !shape_is(pos, {T})) return none();
     }
+    if (a[5] != Py_None) {
+      freq = dev_tensor(a[5], dev, at::kFloat);
+      if (!freq || freq->dim() != 1 || !pos) return none();
+      rot = 2 * freq->size(0);
+    }
+    if (heads <= 0 || kv <= 0 || heads > 0x7fffff || kv > 0x7fffff || pitch < hd || pitch > 0x7fffff || rot > hd ||
+        x->size(1) < (heads + kv) * pitch || !(PyFloat_AS_DOUBLE(a[9]) >= 0.0))
+      return none();
+    const int code = cobra_qk_norm_rope(x->data_ptr(), dt, x->size(1), pos ? pos->data_ptr<int>() : nullptr,
+                                        f32_or_null(freq), rot, a[8] == Py_True ? 1 : 0, f32_or_null(qw),
+                                        f32_or_null(kw), static_cast<float>(PyFloat_AS_DOUBLE(a[9])), T, heads, kv, hd,
+                                        pitch, c10::hip::getCurrentHIPStream(dev).stream());
+    check("cobra_qk_norm_rope", code);
+    Py_RETURN_TRUE;
+  });
+}
+
+int64_t codes_of(int64_t k) { return (k + 127) / 128 * 128; }
+int64_t scales_of(int64_t k) { return (k + 511) / 512 * 4; }
+
+// x -> (codes, scale) | None
+PyObject* quantize8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const int dev = n == 1 ? device_of(a[0]) : -1;
+    if (dev < 0) return none();
+    const at::Tensor& x = THPVariable_Unpack(a[0]);
+    const int dt = act_code(x.scalar_type());
+    if (dt < 0 || x.dim() != 2 || !x.is_contiguous() || x.size(1) == 0) return none();
+    const int64_t M = x.size(0), K = x.size(1);
+    at::Tensor codes = new_tensor({M, codes_of(K)}, at::kFloat8_e4m3fn, x.device());
+    at::Tensor scale = new_tensor({M, scales_of(K)}, at::kFloat8_e8m0fnu, x.device());
+    const int code = cobra_quantize8(x.data_ptr(), dt, codes.data_ptr(), scale.data_ptr(), M, K,
+                                     c10::hip::getCurrentHIPStream(dev).stream());
+    check("cobra_quantize8", code);
+    PyObject* got = PyTuple_New(2);
+    if (!got) return nullptr;
+    PyTuple_SET_ITEM(got, 0, THPVariable_Wrap(std::move(codes)));
+    PyTuple_SET_ITEM(got, 1, THPVariable_Wrap(std::move(scale)));
+    return got;
+  });
+}
+
+// (a, w, w_scale, bias | None, gelu, out_dtype | None, resid | None, rmask | None, mask_branch,
+// a_scale | None) -> out | None
+PyObject* linear8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const int dev = n == 10 ? device_of(a[0]) : -1;
+    if (dev < 0 || !PyBool_Check(a[4]) || !PyBool_Check(a[8])) return none();
+    const at::Tensor& x = THPVariable_Unpack(a[0]);
+    const at::Tensor *w = dev_tensor(a[1], dev, at::kFloat8_e4m3fn), *ws = dev_tensor(a[2], dev, at::kFloat8_e8m0fnu);
+    if (!w || !ws || w->dim() != 2 || x.dim() != 2 || !x.is_contiguous()) return none();
+    const int64_t M = x.size(0), N = w->size(0), kp = w->size(1), K = x.size(1);
+    if (M == 0 || N == 0 || K == 0 || codes_of(K) != kp || !shape_is(ws, {N, scales_of(kp)})) return none();
+    int dt;
+    const at::Tensor* as = nullptr;
+    at::ScalarType out_type = x.scalar_type();
+    if (a[9] != Py_None) {
+      as = dev_tensor(a[9], dev, at::kFloat8_e8m0fnu);
+      if (out_type != at::kFloat8_e4m3fn || K != kp || !as || !shape_is(as, {M, scales_of(kp)}) || a[5] == Py_None)
+        return none();
+      dt = COBRA_E4M3;
+    } else {
+      dt = act_code(out_type);
+      if (dt != COBRA_F16 && dt != COBRA_BF16) return none();
+    }
+    if (a[5] != Py_None) {
+      if (!THPDtype_Check(a[5])) return none();
+      out_type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+    }
+    const int out_dt = act_code(out_type);
+    const at::Tensor *bias, *resid = nullptr;
+    if (out_dt < 0 || !opt_f32(a[3], dev, N, &bias)) return none();
+    int resid_dt = 0;
+    if (a[6] != Py_None) {
+      if (!THPVariable_Check(a[6])) return none();
+      resid = &THPVariable_Unpack(a[6]);
+      resid_dt = act_code(resid->scalar_type());
+      if (resid_dt < 0 || !dev_tensor(a[6], dev, resid->scalar_type()) || !shape_is(resid, {M, N})) return none();
+    }
+    int epi = a[4] == Py_True ? COBRA_EPI_GELU : 0;
+    const uint8_t* mask = nullptr;
+    if (a[7] != Py_None) {
+      if (!THPVariable_Check(a[7])) return none();
+      const at::ScalarType mt = THPVariable_Unpack(a[7]).scalar_type();
+      const at::Tensor* m = mt == at::kBool || mt == at::kByte ? dev_tensor(a[7], dev, mt) : nullptr;
+      if (!m || m->numel() != M) return none();
+      if (a[8] == Py_True || resid) {
+        epi |= a[8] == Py_True ? COBRA_EPI_MASK_BRANCH : COBRA_EPI_MASK_RESID;
+        mask = static_cast<const uint8_t*>(m->data_ptr());
+      }
+    }
+    const int64_t need = cobra_linear8_workspace_bytes(M, N, K, dt);
+    if (need < 0) return none();
+    at::Tensor out = new_tensor({M, N}, out_type, x.device()), space;
+    if (need > 0) space = new_tensor({need}, at::kByte, x.device());
+    const int code = cobra_linear8_fwd(x.data_ptr(), dt, as ? as->data_ptr() : nullptr, w->data_ptr(), ws->data_ptr(),
+                                       f32_or_null(bias), resid ? resid->data_ptr() : nullptr, resid_dt, mask, epi,
+                                       out.data_ptr(), out_dt, need > 0 ? space.data_ptr() : nullptr, need, M, N, K,
+                                       c10::hip::getCurrentHIPStream(dev).stream());
+    check("cobra_linear8_fwd", code);
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -432,6 +622,10 @@ PyMethodDef kCacheCalls[] = {
     {"cache_trim", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_trim)), METH_FASTCALL, nullptr},
     {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_append)), METH_FASTCALL, nullptr},
     {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_attn)), METH_FASTCALL, nullptr},
+    {"cache_prefix_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_prefix_attn)), METH_FASTCALL, nullptr},
+    {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rope)), METH_FASTCALL, nullptr},
+    {"quantize8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize8)), METH_FASTCALL, nullptr},
+    {"linear8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear8)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

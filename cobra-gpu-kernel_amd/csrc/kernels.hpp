@@ -399,4 +399,55 @@ int64_t cache_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads,
                                    int64_t max_new, int64_t max_len);
 hipError_t run_cache_attn(const CacheAttnArgs& a, int64_t workspace_bytes, hipStream_t stream);
 
+// Attention over a cache behind a prefix that all requests share (cache_prefix.hip): as CacheAttnArgs,
+// with row `prefix` of the tables holding the prefix.
+struct CachePrefixArgs {
+  CacheAttnArgs attn;
+  int prefix;
+  int64_t max_prefix;  // expected bound (speed only)
+};
+int64_t cache_prefix_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                     int64_t max_new, int64_t max_len, int64_t max_prefix);
+hipError_t run_cache_prefix(const CachePrefixArgs& a, int64_t workspace_bytes, hipStream_t stream);
+
+// Matrices held in 8 bits (quant8.hpp, quant8.hip, linear8.hip).
+enum : int { kE4M3 = 3 };  // dtype code of such a matrix beside kF16, kF32 and kBF16
+struct Quantize8Args {
+  const void* x;  // [M, K] dtype
+  void* codes;    // [M, Kp]
+  void* scale;    // [M, S] bytes
+  int64_t M, K;
+  int dtype;
+};
+hipError_t run_quantize8(const Quantize8Args& a, hipStream_t stream);
+
+struct Linear8Args {
+  const void* a;           // [M, K] fp16 or bf16, or codes [M, Kp]
+  const uint8_t* a_scale;  // of codes
+  const uint8_t *w, *w_scale;
+  const float* bias;       // [N] or null
+  const void* resid;       // [M, N] or null
+  const uint8_t* row_mask;
+  void* c;                 // [M, N]
+  void* workspace;
+  int64_t M, N, K;
+  int a_dtype, resid_dtype, c_dtype, epi;
+};
+int64_t linear8_workspace_bytes(int64_t M, int64_t K, int a_dtype);
+hipError_t run_linear8(const Linear8Args& a, int64_t workspace_bytes, hipStream_t stream);
+
+// Norms and rotation of packed queries and keys in place (rope.hip).
+struct QkNormRopeArgs {
+  void* qkv;                 // [tokens, ld], heads `pitch` columns apart
+  const int32_t* positions;  // [tokens], or null without rotation
+  const float* inv_freq;     // [rot / 2]
+  const float *q_weight, *k_weight;  // [head_dim], or null without norms
+  int64_t tokens, ld;
+  int heads, kv_heads, head_dim, pitch, rot, interleaved, dtype;
+  float eps;
+};
+hipError_t run_qk_norm_rope(const QkNormRopeArgs& a, hipStream_t stream);
+hipError_t run_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* out, int64_t tokens, int batch,
+                               int prefix, hipStream_t stream);
+
 }  // namespace cobra

@@ -1,0 +1,613 @@
+// C[M,N] = A[M,K] . W[N,K]^T (+ bias, GELU, row masks, + resid) with both matrices in 8 bits and a
+// power-of-two scale for each row and block of 128 columns (quant8.hpp):
+//   c = sum_j 2^(ea[m,j] + ew[n,j]) sum_{k in block j} a[m,k] w[n,k]
+// Two kinds of matrix instructions.
+// * Exact: codes become bf16 in registers, with their scale inside the conversion (4 significant bits
+//   and a power of two: nothing is rounded), and v_mfma_*_bf16 adds their products in fp32.
+// * Scaled: v_mfma_scale_f32_32x32x64_f8f6f4 takes the codes as they are and one scale byte for each
+//   row and 32 columns of an operand, at twice the rate.  All lanes that hold parts of a row's
+//   block give the block's byte, so it does not matter which columns the instruction counts to which
+//   lane.  But it adds eight products at a time and cuts each where it falls under 2^-13 of
+//   the largest one's exponent (measured, as for the instructions without scales; the sums of eight
+//   meet in fp32): 4e-5 of a result in the root mean square.  An fp16 result's own rounding is 2e-4, a
+//   bf16's 1.6e-3, an fp32's 3e-8: fp32 results take the exact kind.
+//
+// Two kernels.  Up to 64 rows of A the weights' bytes are all that counts: linear8_few_kernel
+// (exact) has 16 or more rows of W a workgroup, split along K over its waves, and takes 16-bit
+// activations as they are, quantising them in the registers that the product reads.  More rows go
+// through tiles in LDS.
+#include "kernels.hpp"
+#include "lds_dma.hpp"
+#include "quant8.hpp"
+
+namespace cobra {
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ i32x8 join8(const i32x4& a, const i32x4& b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Eight codes times a scale, exactly.
+__device__ __forceinline__ bf16x8 widen(uint32_t x, uint32_t y, float scale) {
+  struct {
+    bf16x2 p[4];
+  } q;
+  q.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false);
+  q.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true);
+  q.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, scale, false);
+  q.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, scale, true);
+  return __builtin_bit_cast(bf16x8, q);
+}
+__device__ __forceinline__ f32x16 mfma8(const i32x8& a, const i32x8& b, const f32x16& c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
+struct Args {
+  const void* a;
+  const uint8_t *a_scale, *w, *w_scale;
+  const float* bias;
+  const void* resid;
+  const uint8_t* row_mask;
+  void* c;
+  int64_t M;
+  int N, K;      // K: columns of 16-bit activations
+  int kp, s;     // columns of codes, bytes of a row of scales
+  int resid_dtype, c_dtype, epi;
+};
+
+// Element i of a matrix of one of the three types.
+__device__ __forceinline__ float get(const void* p, int dtype, int64_t i) {
+  if (dtype == kF32) return static_cast<const float*>(p)[i];
+  if (dtype == kF16) return (float)static_cast<const f16*>(p)[i];
+  return (float)static_cast<const bf16*>(p)[i];
+}
+__device__ __forceinline__ void put(void* p, int dtype, int64_t i, float v) {
+  if (dtype == kF32) static_cast<float*>(p)[i] = v;
+  else if (dtype == kF16) static_cast<f16*>(p)[i] = (f16)v;
+  else static_cast<bf16*>(p)[i] = (bf16)v;
+}
+// Four consecutive elements from i on (i % 4 == 0).
+__device__ __forceinline__ f32x4 get4(const void* p, int dtype, int64_t i) {
+  if (dtype == kF32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+  f32x4 r;
+  if (dtype == kF16) {
+    const f16x4 h = *reinterpret_cast<const f16x4*>(static_cast<const f16*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (float)h[e];
+  } else {
+    const bf16x4 h = *reinterpret_cast<const bf16x4*>(static_cast<const bf16*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (float)h[e];
+  }
+  return r;
+}
+__device__ __forceinline__ void put4(void* p, int dtype, int64_t i, const f32x4& v) {
+  if (dtype == kF32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+  } else if (dtype == kF16) {
+    f16x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (f16)v[e];
+    *reinterpret_cast<f16x4*>(static_cast<f16*>(p) + i) = h;
+  } else {
+    bf16x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (bf16)v[e];
+    *reinterpret_cast<bf16x4*>(static_cast<bf16*>(p) + i) = h;
+  }
+}
+
+// -- few rows --------------------------------------------------------------------------
+
+// A lane's 32 columns of a block of one row of activations: codes and the block's scale.  16-bit values are quantised here: a row's block lies in the four
+// lanes l, l + 16, l + 32, l + 48.
+template <typename TA>
+struct RowBlock {
+  uint32_t w[16];
+  __device__ __forceinline__ void load(const Args& a, int64_t m, bool there, int j, int g) {
+    const TA* p = static_cast<const TA*>(a.a) + m * a.K;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 128 * j + 64 * h + 16 * g;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (there && c + 8 * q < a.K) v = *reinterpret_cast<const uint4*>(p + c + 8 * q);
+        w[8 * h + 4 * q] = v.x;
+        w[8 * h + 4 * q + 1] = v.y;
+        w[8 * h + 4 * q + 2] = v.z;
+        w[8 * h + 4 * q + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ i32x8 codes(float& scale) {
+    uint32_t m = largest16(w);
+    if (__any(m >= Quant<TA>::kInf)) m = finite16<TA>(w);
+    float v = Quant<TA>::wide(m);
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+    scale = scale_of(scale_byte(__float_as_uint(v)));
+    i32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (int)Quant<TA>::four(w[2 * i], w[2 * i + 1], scale);
+    return r;
+  }
+};
+template <>
+struct RowBlock<uint8_t> {
+  i32x4 lo, hi;
+  uint32_t b;
+  __device__ __forceinline__ void load(const Args& a, int64_t m, bool there, int j, int g) {
+    lo = i32x4{0, 0, 0, 0};
+    hi = lo;
+    b = 127;
+    if (there) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.a) + m * a.kp + 128 * j + 16 * g;
+      lo = *reinterpret_cast<const i32x4*>(p);
+      hi = *reinterpret_cast<const i32x4*>(p + 64);
+      b = a.a_scale[m * a.s + j];
+    }
+  }
+  __device__ __forceinline__ i32x8 codes(float& scale) {
+    scale = scale_of(b);
+    return join8(lo, hi);
+  }
+};
+
+// MT sets of 16 rows of A, NT of W for a workgroup of eight waves, each with every eighth block of K;
+// UB blocks' loads are asked for together.
+template <typename TA, int MT, int NT, int UB>
+__global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
+  constexpr int kWaves = 8;
+  __shared__ f32x4 part[kWaves][NT * MT][64];
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16 * NT;
+  const int blocks = a.kp >> 7;
+  const uint8_t *w[NT], *ws[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {  // rows past N give columns that are never stored
+    const int64_t n = min(n0 + 16 * t + r, a.N - 1);
+    w[t] = a.w + n * a.kp + 16 * g;
+    ws[t] = a.w_scale + n * a.s;
+  }
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j0 = wave; j0 < blocks; j0 += kWaves * UB) {
+    i32x4 lo[UB][NT], hi[UB][NT];
+    uint32_t wb[UB][NT];
+    RowBlock<TA> x[UB][MT];
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int j = j0 + u * kWaves;
+      if (j < blocks) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          lo[u][t] = *reinterpret_cast<const i32x4*>(w[t] + 128 * j);
+          hi[u][t] = *reinterpret_cast<const i32x4*>(w[t] + 128 * j + 64);
+          wb[u][t] = ws[t][j];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[u][i].load(a, 16 * i + r, 16 * i + r < a.M, j, g);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      if (j0 + u * kWaves < blocks) {
+        bf16x8 y[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          float scale;
+          const i32x8 c = x[u][i].codes(scale);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[i][k] = widen(c[2 * k], c[2 * k + 1], scale);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float scale = scale_of(wb[u][t]);
+          const i32x8 c = join8(lo[u][t], hi[u][t]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bf16x8 z = widen(c[2 * k], c[2 * k + 1], scale);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[t][i] = mfma16(z, y[i][k], acc[t][i]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][t * MT + i][lane] = acc[t][i];
+  __syncthreads();
+  // A thread has four columns of a row: the waves' shares in their order.
+  for (int q = threadIdx.x; q < NT * MT * 64; q += kWaves * 64) {
+    const int tile = q >> 6, l = q & 63;
+    const int m = 16 * (tile % MT) + (l & 15);
+    const int n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
+    if (m >= a.M || n >= a.N) continue;
+    f32x4 v = part[0][tile][l];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) v += part[k][tile][l];
+    const bool padded = (a.epi & (kEpiMaskBranch | kEpiMaskResid)) && a.row_mask[m] == 0;
+    const bool four = a.N % 4 == 0;
+    const int64_t at = (int64_t)m * a.N + n;
+    f32x4 b = {0.f, 0.f, 0.f, 0.f}, e = b;
+    if (four) {
+      if (a.bias) b = *reinterpret_cast<const f32x4*>(a.bias + n);
+      if (a.resid) e = get4(a.resid, a.resid_dtype, at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) {
+          if (a.bias) b[i] = a.bias[n + i];
+          if (a.resid) e[i] = get(a.resid, a.resid_dtype, at + i);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] += b[i];
+      if (a.epi & kEpiGelu) v[i] = gelu_erf(v[i]);
+      if (padded && (a.epi & kEpiMaskBranch)) v[i] = 0.f;
+      v[i] += e[i];
+      if (padded && (a.epi & kEpiMaskResid)) v[i] *= 0.f;
+    }
+    if (four) {
+      put4(a.c, a.c_dtype, at, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) put(a.c, a.c_dtype, at + i, v[i]);
+    }
+  }
+}
+
+// -- many rows -------------------------------------------------------------------------
+
+// 4 bytes per lane from a per-lane address to lds + 4 * lane (lds_dma.hpp: dma16_untracked).
+__device__ __forceinline__ void dma4_untracked(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory");
+}
+
+// A tile of BM x BN by WM x WN waves; a k-tile is one block of 128 columns.  A stage of LDS holds
+// the rows' codes (A's, then W's), 128 bytes each with 16-byte chunks swizzled by row as in the
+// 16-bit kernel, and behind them the rows' words of four scale bytes.
+template <int BM, int BN, int WM, int WN, int ST>
+struct Tile {
+  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
+  static constexpr int ROWS = BM + BN;
+  static constexpr int STAGE = ROWS * 132;
+  static constexpr int LPT = ROWS / 8 / NW;     // transfers of 8 rows' codes a wave and k-tile; one more of scales
+  static constexpr int EPW = WN * 32, LDC = EPW + 4;
+  static constexpr int EPI_LDS = BM * LDC * 4;
+  static constexpr int LDS = ST * STAGE > EPI_LDS ? ST * STAGE : EPI_LDS;
+  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && BM % 64 == 0 && BN % 64 == 0, "wave tile");
+  static_assert(ROWS / 8 % NW == 0, "every wave issues the same number of transfers");
+  static_assert(LDS <= 163840, "LDS budget");
+};
+
+__device__ __forceinline__ int chunk_swz(int row) { return (row >> 1) & 7; }
+
+template <int BM, int BN, int WM, int WN, int ST, bool EXACT>
+__device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char* smem,
+                                         f32x16 (&acc)[BN / WN / 32][BM / WM / 32]) {
+  using T = Tile<BM, BN, WM, WN, ST>;
+  constexpr int NW = T::NW, LPT = T::LPT;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int li = lane & 31, g = lane >> 5;
+  const uint8_t* A = static_cast<const uint8_t*>(a.a) + m0 * a.kp;
+  const uint8_t* W = a.w + (int64_t)n0 * a.kp;
+  // Rows past M or N are the last one: their products are never stored.
+  unsigned src_off[LPT];
+#pragma unroll
+  for (int i = 0; i < LPT; ++i) {
+    const int row = 8 * (wave + i * NW) + (lane >> 3);
+    const int chunk = (lane & 7) ^ chunk_swz(row);
+    const int64_t at = row < BM ? min(m0 + row, a.M - 1) - m0 : (int64_t)min(n0 + row - BM, a.N - 1) - n0;
+    src_off[i] = (unsigned)(at * a.kp + chunk * 16);
+  }
+  const int srow = 64 * (wave % (T::ROWS / 64)) + lane;
+  const uint8_t* scales = srow < BM ? a.a_scale + min(m0 + srow, a.M - 1) * a.s
+                                    : a.w_scale + (int64_t)min(n0 + srow - BM, a.N - 1) * a.s;
+  const uint32_t lds0 = lds_addr(smem);
+  auto issue = [&](int stage, int kt) {
+    const uint32_t dst = lds0 + stage * T::STAGE;
+#pragma unroll
+    for (int i = 0; i < LPT; ++i)
+      dma16_untracked((8 * (wave + i * NW) < BM ? A : W) + 128 * kt, src_off[i], dst + (wave + i * NW) * 1024);
+    dma4_untracked(scales + (kt & ~3), dst + T::ROWS * 128 + (wave % (T::ROWS / 64)) * 256);
+  };
+
+#pragma unroll
+  for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) acc[j][i] = zero16();
+
+  const int sw = chunk_swz(li);
+  const int arow = wm * T::WTM + li, wrow = BM + wn * T::WTN + li;
+  const int KT = a.kp >> 7;
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
+    if (s < KT) issue(s, s);
+
+  i32x8 af[2][T::TM], wf[2][T::TN];
+  int as[T::TM], ws[T::TN];
+  auto frags = [&](const char* st, int kk, int b) {
+    const int c0 = ((4 * kk + g) ^ sw) * 16, c1 = ((4 * kk + 2 + g) ^ sw) * 16;
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) {
+      const char* p = st + (wrow + j * 32) * 128;
+      wf[b][j] = join8(*reinterpret_cast<const i32x4*>(p + c0), *reinterpret_cast<const i32x4*>(p + c1));
+    }
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+      const char* p = st + (arow + i * 32) * 128;
+      af[b][i] = join8(*reinterpret_cast<const i32x4*>(p + c0), *reinterpret_cast<const i32x4*>(p + c1));
+    }
+  };
+  int an[T::TM], wnx[T::TN];
+  auto scale_words = [&](const char* st) {
+    const int* p = reinterpret_cast<const int*>(st + T::ROWS * 128);
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) wnx[j] = p[wrow + j * 32];
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) an[i] = p[arow + i * 32];
+  };
+  auto wait_oldest = [&](int n) {
+    constexpr int L = LPT + 1;
+    if (ST >= 4 && n >= 4) wait_vmcnt<(ST >= 4 ? 3 : 0) * L>();
+    else if (ST >= 3 && n >= 3) wait_vmcnt<(ST >= 3 ? 2 : 0) * L>();
+    else if (n >= 2) wait_vmcnt<L>();
+    else wait_vmcnt<0>();
+  };
+  wait_oldest(min(ST, KT));
+  stage_barrier();
+  frags(smem, 0, 0);
+  scale_words(smem);
+  for (int kt = 0; kt < KT; ++kt) {
+    const char* st = smem + (kt % ST) * T::STAGE;
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) ws[j] = wnx[j] >> (8 * (kt & 3));
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) as[i] = an[i] >> (8 * (kt & 3));
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      if (kk == 0) {
+        frags(st, 1, 1);
+      } else if (kt + 1 < KT) {
+        wait_oldest(min(ST - 1, KT - 1 - kt));
+        lds_barrier();
+        if (kt + ST < KT) issue(kt % ST, kt + ST);
+        const char* next = smem + ((kt + 1) % ST) * T::STAGE;
+        frags(next, 0, 0);
+        scale_words(next);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (EXACT) {
+        bf16x8 y[T::TM][4];
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[i][k] = widen(af[kk][i][2 * k], af[kk][i][2 * k + 1], scale_of(as[i] & 255));
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bf16x8 z = widen(wf[kk][j][2 * k], wf[kk][j][2 * k + 1], scale_of(ws[j] & 255));
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma32x32x16(z, y[i][k], acc[j][i]);
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+          for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma8(wf[kk][j], af[kk][i], acc[j][i], ws[j], as[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
+__global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
+  using T = Tile<BM, BN, WM, WN, ST>;
+  constexpr int NT = T::NT;
+  __shared__ __attribute__((aligned(1024))) char smem[T::LDS];
+  // Tile order as in the 16-bit kernel: an XCD runs a contiguous range of ids, which walk GM row
+  // blocks x all column blocks.
+  const int nbn = (a.N + BN - 1) / BN;
+  const int nbm = (int)((a.M + BM - 1) / BM);
+  const int tile = xcd_remap(blockIdx.x, gridDim.x);
+  const int group = tile / (GM * nbn);
+  const int first_m = group * GM;
+  const int gm = min(nbm - first_m, GM);
+  const int in_group = tile - group * GM * nbn;
+  const int64_t m0 = (int64_t)(first_m + in_group % gm) * BM;
+  const int n0 = (in_group / gm) * BN;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int li = lane & 31, g = lane >> 5;
+
+  f32x16 acc[T::TN][T::TM];
+  mainloop<BM, BN, WM, WN, ST, sizeof(TC) == 4>(a, m0, n0, smem, acc);
+  __syncthreads();  // every wave is done with the operand stages
+
+  // In TN slices of 32 columns for each wave column, through LDS as fp32 rows, then written 16
+  // bytes a lane with the epilogue's options; N not in groups of 8 element by element.
+  float* Cs = reinterpret_cast<float*>(smem);
+  constexpr int CPL = 16 / (int)sizeof(TC), LPR = T::EPW / CPL, RPP = NT / LPR, NP = BM / RPP;
+  static_assert(NT % LPR == 0 && BM % RPP == 0 && 32 % CPL == 0, "epilogue geometry");
+  const int cl = (tid % LPR) * CPL;
+  const int ccol = (cl / 32) * T::WTN + (cl % 32);
+  const bool whole = a.N % 8 == 0;
+  constexpr int cdt = sizeof(TC) == 4 ? (int)kF32 : std::is_same<TC, f16>::value ? (int)kF16 : (int)kBF16;
+#pragma unroll
+  for (int j = 0; j < T::TN; ++j) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e];
+        *reinterpret_cast<f32x4*>(Cs + (wm * T::WTM + i * 32 + li) * T::LDC + wn * 32 + 8 * q + 4 * g) = v;
+      }
+    const int n = n0 + ccol + j * 32;
+    f32x4 rv[NP][CPL / 4], bv[CPL / 4];
+#pragma unroll
+    for (int h = 0; h < CPL / 4; ++h) {
+      bv[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < NP; ++p) rv[p][h] = bv[h];
+    }
+    if (whole && n < a.N) {
+#pragma unroll
+      for (int h = 0; h < CPL / 4; ++h) {
+        if (a.bias) bv[h] = *reinterpret_cast<const f32x4*>(a.bias + n + 4 * h);
+        if (a.resid) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            rv[p][h] = get4(a.resid, a.resid_dtype, min(m0 + tid / LPR + p * RPP, a.M - 1) * a.N + n + 4 * h);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < CPL; ++e)
+        if (a.bias && n + e < a.N) bv[e / 4][e % 4] = a.bias[n + e];
+    }
+    __syncthreads();
+    if (n < a.N) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int64_t m = m0 + tid / LPR + p * RPP;
+        if (m >= a.M) break;
+        const bool padded = (a.epi & (kEpiMaskBranch | kEpiMaskResid)) && a.row_mask[m] == 0;
+        const int64_t at = m * a.N + n;
+        float v[CPL];
+#pragma unroll
+        for (int h = 0; h < CPL / 4; ++h) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = t[e] + bv[h][e];
+            if (a.epi & kEpiGelu) x = gelu_erf(x);
+            if (padded && (a.epi & kEpiMaskBranch)) x = 0.f;
+            v[4 * h + e] = x + rv[p][h][e];
+          }
+        }
+        if (whole) {
+          if (padded && (a.epi & kEpiMaskResid)) {
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) v[e] *= 0.f;
+          }
+#pragma unroll
+          for (int h = 0; h < 1; ++h) {
+            if constexpr (sizeof(TC) == 4) {
+              *reinterpret_cast<f32x4*>(static_cast<float*>(a.c) + at) = f32x4{v[0], v[1], v[2], v[3]};
+            } else {
+              typename Op16<TC>::V8 hv;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) hv[e] = (TC)v[e];
+              *reinterpret_cast<typename Op16<TC>::V8*>(static_cast<TC*>(a.c) + at) = hv;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < CPL; ++e)
+            if (n + e < a.N) {
+              float x = v[e];
+              if (a.resid) x += get(a.resid, a.resid_dtype, at + e);
+              if (padded && (a.epi & kEpiMaskResid)) x *= 0.f;
+              put(a.c, cdt, at + e, x);
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
+hipError_t launch_tile(const Args& a, hipStream_t stream) {
+  const int64_t tiles = ((a.M + BM - 1) / BM) * (int64_t)((a.N + BN - 1) / BN);
+  if (tiles > 0x7fffff) return hipErrorInvalidValue;
+  return launch_status(linear8_tile_kernel<BM, BN, WM, WN, ST, GM, TC>, dim3((unsigned)tiles), dim3(WM * WN * 64),
+                       stream, a);
+}
+
+template <typename TC>
+hipError_t dispatch_tile(const Args& a, hipStream_t stream) {
+  auto tiles = [&](int bm, int bn) { return ((a.M + bm - 1) / bm) * (int64_t)((a.N + bn - 1) / bn); };
+  const int64_t cus = compute_units();
+  if (tiles(128, 128) >= cus) return launch_tile<128, 128, 2, 2, 2, 8, TC>(a, stream);
+  return launch_tile<64, 64, 2, 2, 4, 8, TC>(a, stream);
+}
+
+template <typename TA>
+hipError_t launch_few(const Args& a, hipStream_t stream) {
+  const dim3 block(512);
+  auto groups = [&](int nt) { return dim3((unsigned)((a.N + 16 * nt - 1) / (16 * nt))); };
+  if (a.M <= 16)
+    return a.M <= 4 || a.N <= 16 * 2 * compute_units()
+               ? launch_status(linear8_few_kernel<TA, 1, 1, 4>, groups(1), block, stream, a)
+               : launch_status(linear8_few_kernel<TA, 1, 2, 2>, groups(2), block, stream, a);
+  if (a.M <= 32) return launch_status(linear8_few_kernel<TA, 2, 2, 2>, groups(2), block, stream, a);
+  return launch_status(linear8_few_kernel<TA, 4, 2, 1>, groups(2), block, stream, a);
+}
+
+constexpr int64_t kFewRows = 64;
+
+bool whole_rows(const Linear8Args& c) {
+  return c.K % 8 == 0 && (reinterpret_cast<uintptr_t>(c.a) & 15) == 0;
+}
+
+}  // namespace
+
+int64_t linear8_workspace_bytes(int64_t M, int64_t K, int a_dtype) {
+  if (a_dtype == kE4M3 || (M <= kFewRows && K % 8 == 0)) return 0;
+  const int64_t kp = (K + 127) & ~int64_t(127), s = (K + 511) / 512 * 4;
+  return M * (kp + s);
+}
+
+hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_t stream) {
+  const int64_t kp = (c.K + 127) & ~int64_t(127), s = (c.K + 511) / 512 * 4;
+  // Offsets inside a tile's rows are 32 bits wide.
+  if (c.M <= 0 || c.N <= 0 || c.N > 0x7ffffff || kp > 0x7fffff || c.M > 0x7fffffff) return hipErrorInvalidValue;
+  Args a{c.a, c.a_scale, c.w, c.w_scale, c.bias, c.resid, c.row_mask, c.c, c.M, (int)c.N, (int)c.K, (int)kp, (int)s,
+         c.resid_dtype, c.c_dtype, c.epi};
+  const bool codes = c.a_dtype == kE4M3;
+  if (c.M <= kFewRows && !codes && whole_rows(c))
+    return c.a_dtype == kF16 ? launch_few<f16>(a, stream) : launch_few<bf16>(a, stream);
+  if (!codes) {
+    if (!c.workspace || workspace_bytes < c.M * (kp + s)) return hipErrorInvalidValue;
+    uint8_t* scale = static_cast<uint8_t*>(c.workspace) + c.M * kp;
+    const Quantize8Args q{c.a, c.workspace, scale, c.M, c.K, c.a_dtype};
+    const hipError_t e = run_quantize8(q, stream);
+    if (e != hipSuccess) return e;
+    a.a = c.workspace;
+    a.a_scale = scale;
+  }
+  if (c.M <= kFewRows) return launch_few<uint8_t>(a, stream);
+  switch (c.c_dtype) {
+    case kF16: return dispatch_tile<f16>(a, stream);
+    case kBF16: return dispatch_tile<bf16>(a, stream);
+    case kF32: return dispatch_tile<float>(a, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace cobra

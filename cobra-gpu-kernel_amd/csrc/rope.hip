@@ -1,0 +1,244 @@
+// Norms of queries and keys for each head and their rotation by position, in one pass over packed
+// q | k | v rows, in place; and the positions of new tokens of cached requests.
+//
+// A head's vector x of D: y = x / sqrt(sum x^2 / D + eps) * w (fp32; without weights y = x), then of its
+// first R columns each pair turns by the token's position times the pair's frequency f_i:
+//   (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t),  t = p f_i,
+// pairs (i, i + R / 2) or (2 i, 2 i + 1), i < R / 2.  The angle is formed in turns and in 64 bits and
+// brought to half a turn before it is rounded to 32: in 32 bits a position of 100000 would be off by
+// 0.006 already.  One rounding, of the result.
+//
+// Bound by memory for many tokens (every query and key read and written once), by the launch for few.
+// A token's R / 2 sines and cosines are formed once, in LDS, for all of its heads.  A lane has two
+// pieces of V columns, chosen so that a pair's partners are both its own: V columns from i and V from
+// i + R / 2, or two neighbouring pieces.  Heads that 4 columns do not divide (the whole, its pitch or
+// half of what turns) have a wave each and their partners from memory.
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace cobra {
+
+namespace {
+
+constexpr int kMaxDim = 256;
+
+struct Args {
+  void* qkv;
+  const int32_t* positions;
+  const float *inv_freq, *q_weight, *k_weight;
+  int64_t tokens, ld;
+  int heads, all;       // query heads; query and key heads
+  int dim, pitch, half; // columns of a head, from a head to the next, and half of those that turn
+  int lanes;            // of a head
+  float eps;
+};
+
+// V consecutive values as loaded.
+template <typename T, int V>
+struct __attribute__((aligned(V * 2))) Piece {
+  T e[V];
+};
+
+// Sum over a head's lanes: aligned groups of `lanes`, a power of two up to 64, all of them active.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  if (lanes >= 2) v += dpp_f32<0xB1>(v);
+  if (lanes >= 4) v += dpp_f32<0x4E>(v);
+  if (lanes >= 8) v += dpp_f32<0x141>(v);
+  if (lanes >= 16) v += dpp_f32<0x140>(v);
+  if (lanes >= 32) v = sum_xor16(v);
+  if (lanes >= 64) v = sum_xor32(v);
+  return v;
+}
+
+// A token's turns: (cos, sin) of its position times each frequency.
+__device__ __forceinline__ void turns(const Args& a, int pos, float2* turn) {
+  for (int i = threadIdx.x; i < a.half; i += 256) {
+    const double x = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189535);  // 1 / 2 pi
+    float s, c;
+    sincospif(2.f * (float)(x - __builtin_rint(x)), &s, &c);
+    turn[i] = make_float2(c, s);
+  }
+}
+__device__ __forceinline__ void rotate(float& u, float& v, const float2& r) {
+  const float x = u;
+  u = x * r.x - v * r.y;
+  v = v * r.x + x * r.y;
+}
+__device__ __forceinline__ float norm_of(const Args& a, float sum) { return 1.0f / sqrtf(sum / (float)a.dim + a.eps); }
+
+template <typename T, int V, bool INTER>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a) {
+  __shared__ float2 turn[kMaxDim / 2];
+  const int tid = threadIdx.x;
+  const int p = tid & (a.lanes - 1), per = 256 / a.lanes;
+  const bool pair = !INTER && p * V < a.half;  // this lane's pieces are partners
+  const int c0 = pair ? p * V : 2 * p * V, c1 = pair ? a.half + p * V : c0 + V;
+  const bool on0 = c0 < a.dim, on1 = c1 < a.dim;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int pos = a.positions ? a.positions[t] : 0;
+    if (pos < 0) continue;
+    __syncthreads();  // the last token's turns are used up
+    turns(a, pos, turn);
+    __syncthreads();
+    T* row = static_cast<T*>(a.qkv) + t * a.ld;
+    for (int h = tid / a.lanes; h < a.all; h += per) {
+      T* x = row + (int64_t)h * a.pitch;
+      Piece<T, V> p0{}, p1{};
+      if (on0) p0 = *reinterpret_cast<const Piece<T, V>*>(x + c0);
+      if (on1) p1 = *reinterpret_cast<const Piece<T, V>*>(x + c1);
+      float y0[V], y1[V], ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        y0[e] = (float)p0.e[e];
+        y1[e] = (float)p1.e[e];
+        ss = fmaf(y0[e], y0[e], fmaf(y1[e], y1[e], ss));
+      }
+      const float* w = h < a.heads ? a.q_weight : a.k_weight;
+      if (w) {
+        const float inv = norm_of(a, lanes_sum(ss, a.lanes));
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (on0) y0[e] *= inv * w[c0 + e];
+          if (on1) y1[e] *= inv * w[c1 + e];
+        }
+      }
+      if constexpr (INTER) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          if (c0 + e < 2 * a.half) rotate(y0[e], y0[e + 1], turn[(c0 + e) >> 1]);
+          if (c1 + e < 2 * a.half) rotate(y1[e], y1[e + 1], turn[(c1 + e) >> 1]);
+        }
+      } else if (pair) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) rotate(y0[e], y1[e], turn[c0 + e]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        p0.e[e] = (T)y0[e];
+        p1.e[e] = (T)y1[e];
+      }
+      if (on0) *reinterpret_cast<Piece<T, V>*>(x + c0) = p0;
+      if (on1) *reinterpret_cast<Piece<T, V>*>(x + c1) = p1;
+    }
+  }
+}
+
+// Any geometry: a wave has a head, a lane its columns lane, lane + 64, ..; all of a head's loads come
+// before its stores.
+template <typename T>
+__global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(Args a, int inter) {
+  constexpr int kPer = kMaxDim / 64;
+  __shared__ float2 turn[kMaxDim / 2];
+  const int lane = threadIdx.x & 63;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int pos = a.positions ? a.positions[t] : 0;
+    if (pos < 0) continue;
+    __syncthreads();
+    turns(a, pos, turn);
+    __syncthreads();
+    T* row = static_cast<T*>(a.qkv) + t * a.ld;
+    for (int h = threadIdx.x >> 6; h < a.all; h += 4) {
+      T* x = row + (int64_t)h * a.pitch;
+      float y[kPer], z[kPer], ss = 0.f;  // a column and its partner
+      int at[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int i = lane + 64 * e;
+        at[e] = i >= 2 * a.half ? i : inter ? i ^ 1 : i < a.half ? i + a.half : i - a.half;
+        y[e] = i < a.dim ? (float)x[i] : 0.f;
+        z[e] = i < a.dim ? (float)x[at[e]] : 0.f;
+        ss = fmaf(y[e], y[e], ss);
+      }
+      const float* w = h < a.heads ? a.q_weight : a.k_weight;
+      if (w) {
+        const float inv = norm_of(a, group_sum<64>(ss));
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (lane + 64 * e < a.dim) {
+            y[e] *= inv * w[lane + 64 * e];
+            z[e] *= inv * w[at[e]];
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int i = lane + 64 * e;
+        if (i < 2 * a.half) {
+          const float2 r = turn[inter ? i >> 1 : i < a.half ? i : i - a.half];
+          y[e] = y[e] * r.x + (at[e] > i ? -z[e] : z[e]) * r.y;
+        }
+        if (i < a.dim) x[i] = (T)y[e];
+      }
+    }
+  }
+}
+
+dim3 groups_of(const Args& a) { return dim3((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20)); }
+
+template <typename T, int V, bool INTER>
+hipError_t launch(Args a, hipStream_t stream) {
+  a.lanes = 1;
+  while (a.lanes * 2 * V < a.dim) a.lanes *= 2;
+  return launch_status(qk_norm_rope_kernel<T, V, INTER>, groups_of(a), dim3(256), stream, a);
+}
+
+template <typename T>
+hipError_t launch_type(const Args& a, int inter, hipStream_t stream) {
+  const auto fits = [&](int v) {
+    return a.dim % v == 0 && a.pitch % v == 0 && a.ld % v == 0 && (inter || a.half % v == 0) &&
+           (reinterpret_cast<uintptr_t>(a.qkv) & (2 * v - 1)) == 0;
+  };
+  if (fits(8)) return inter ? launch<T, 8, true>(a, stream) : launch<T, 8, false>(a, stream);
+  if (fits(4)) return inter ? launch<T, 4, true>(a, stream) : launch<T, 4, false>(a, stream);
+  return launch_status(qk_norm_rope_any_kernel<T>, groups_of(a), dim3(256), stream, a, inter);
+}
+
+// Position of each new token: its request's tokens before it, behind those of the prefix; -1 where
+// no request has it.  The requests' bounds are searched in LDS where they fit: a search in memory is
+// a chain of dependent reads.
+constexpr int kBounds = 4096;
+template <bool SHARED>
+__global__ __launch_bounds__(256) void cache_positions_kernel(const int32_t* __restrict__ cu,
+                                                              const int32_t* __restrict__ lens, int32_t* __restrict__ out,
+                                                              int64_t tokens, int batch, int prefix) {
+  __shared__ int32_t held[SHARED ? kBounds : 1];
+  if constexpr (SHARED) {
+    for (int i = threadIdx.x; i <= batch; i += 256) held[i] = cu[i];
+    __syncthreads();
+  }
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= tokens) return;
+  auto bound = [&](int i) { return SHARED ? held[i] : cu[i]; };
+  int lo = 0, hi = batch;  // the last request with cu[b] <= t is in [lo, hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (bound(mid) <= t) lo = mid;
+    else hi = mid;
+  }
+  const int64_t first = bound(lo), end = bound(lo + 1);
+  int64_t at = -1;
+  if (first >= 0 && t >= first && t < end) {
+    at = (int64_t)lens[lo] - (end - t);
+    if (prefix >= 0 && lo != prefix) at += lens[prefix] > 0 ? lens[prefix] : 0;
+    at = at < -1 ? -1 : at > 0x7fffffff ? 0x7fffffff : at;
+  }
+  out[t] = (int32_t)at;
+}
+
+}  // namespace
+
+hipError_t run_qk_norm_rope(const QkNormRopeArgs& c, hipStream_t stream) {
+  if (c.head_dim <= 0 || c.head_dim > kMaxDim || c.rot < 0 || c.rot % 2 || c.rot > c.head_dim) return hipErrorInvalidValue;
+  const Args a{c.qkv, c.positions, c.inv_freq, c.q_weight, c.k_weight, c.tokens, c.ld, c.heads, c.heads + c.kv_heads,
+               c.head_dim, c.pitch, c.rot / 2, 0, c.eps};
+  return c.dtype == kF16 ? launch_type<f16>(a, c.interleaved, stream) : launch_type<bf16>(a, c.interleaved, stream);
+}
+
+hipError_t run_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* out, int64_t tokens, int batch,
+                               int prefix, hipStream_t stream) {
+  const dim3 groups((unsigned)((tokens + 255) / 256));
+  return batch < kBounds
+             ? launch_status(cache_positions_kernel<true>, groups, dim3(256), stream, cu, lens, out, tokens, batch, prefix)
+             : launch_status(cache_positions_kernel<false>, groups, dim3(256), stream, cu, lens, out, tokens, batch, prefix);
+}
+
+}  // namespace cobra

@@ -31,9 +31,9 @@
 extern "C" {
 #endif
 
-#define COBRA_ABI_VERSION 13
+#define COBRA_ABI_VERSION 14
 
-enum { COBRA_F16 = 0, COBRA_F32 = 1, COBRA_BF16 = 2 };
+enum { COBRA_F16 = 0, COBRA_F32 = 1, COBRA_BF16 = 2, COBRA_E4M3 = 3 /* with scales: cobra_quantize8 */ };
 
 /*
  * Epilogue / row-mask flags (bit set), applied in this order.  A row mask is
@@ -252,6 +252,80 @@ int cobra_cache_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* c
                          int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_blocks,
                          int64_t block_size, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                          int64_t max_len, float scale, int causal, void* stream);
+
+/*
+ * cobra_cache_attn_fwd for requests that share a prefix: row `prefix` of block_table and lens
+ * is a request like any other, and each new token of another request sees all of its keys in
+ * front of its own request's:
+ *     ctx_i = softmax over the prefix's keys and keys j <= lens[b] - n_b + i (causal) or
+ *     j < lens[b] of its own.
+ * New tokens of row `prefix` itself see only that row's keys.  The prefix's keys are read once
+ * for all requests.  max_prefix: the most keys that the prefix is expected to have (speed only,
+ * as max_new and max_len, which are about the other rows).  Everything else, the workspace's
+ * rules too, as in cobra_cache_attn_fwd.
+ */
+int64_t cobra_cache_prefix_attn_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t max_new, int64_t max_len,
+                                                int64_t max_prefix);
+int cobra_cache_prefix_attn_fwd(const void* q, int dtype, int64_t ldq, const int32_t* cu, const int32_t* lens,
+                                const int32_t* block_table, int64_t table_width, int64_t prefix, const void* k,
+                                const void* v, const float* k_scale, const float* v_scale, int cache, void* ctx,
+                                void* workspace, int64_t workspace_bytes, int64_t tokens, int64_t batch,
+                                int64_t num_blocks, int64_t block_size, int64_t heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t max_new, int64_t max_len, int64_t max_prefix, float scale,
+                                int causal, void* stream);
+
+/*
+ * positions[t] [tokens]: where new token t of request b stands among its request's lens[b] tokens
+ * (cu and lens as for cobra_cache_attn_fwd), behind the lens[prefix] tokens of row `prefix` for
+ * every other row when prefix >= 0 (-1: none); -1 for rows outside [cu[0], cu[batch]).
+ */
+int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* positions, int64_t tokens, int64_t batch,
+                          int64_t prefix, void* stream);
+
+/*
+ * Norms of queries and keys for each head and their rotation by position, in place:
+ *     y = x / sqrt(sum x^2 / head_dim + eps) * w   (w: q_weight or k_weight [head_dim]; both
+ *     NULL: y = x), then of the first rot columns each pair (a, b) becomes
+ *     (a cos t - b sin t, b cos t + a sin t),  t = positions[token] * inv_freq[i],
+ * pairs (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved, i < rot / 2.
+ * qkv: [tokens, ld] in dtype (COBRA_F16 or COBRA_BF16, element alignment suffices): heads query
+ * heads, then kv_heads key heads, each head_dim columns, pitch columns apart (ld >= (heads +
+ * kv_heads) * pitch); other columns are left as they are.  head_dim <= 256, rot even and at most
+ * head_dim, 0 for no rotation (positions and inv_freq may then be NULL).  Tokens with a negative
+ * position are left as they are.  fp32 arithmetic, angles in 64 bits, one rounding.
+ */
+int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, const float* inv_freq, int64_t rot,
+                       int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream);
+
+/*
+ * A matrix held in 8 bits (COBRA_E4M3): codes [M, Kp] with Kp = K rounded up to 128, zeros past K,
+ * and scale [M, S] bytes, S = 4 ceil(K / 512): 2^(byte - 127) for each row and 128 columns, 127
+ * past Kp / 128.  Of a block whose largest finite magnitude is a, the scale is the least power of
+ * two >= 2^-126 with a <= 448 scale, and codes are the nearest e4m3 values of x / scale (ties to
+ * even); what is not finite becomes NaN.  x: [M, K] in any of the three types (element alignment
+ * suffices); K <= 8388352; M ceil(K / 512) < 2^31; no buffer may overlap another.
+ */
+int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_t M, int64_t K, void* stream);
+
+/*
+ * cobra_linear_fwd with both operands in 8 bits:
+ *     v = a . w^T + bias;  then the epi flags GELU, MASK_BRANCH;  v += resid;
+ *     then MASK_RESID;  c = v
+ * a: [M, K] COBRA_F16 or COBRA_BF16, quantised in the call as cobra_quantize8 does, or codes
+ * [M, Kp] (COBRA_E4M3) with a_scale [M, S]; w, w_scale: codes [N, Kp] and scales [N, S] of the
+ * weight in nn.Linear's layout.  bias: [N] fp32 (optional); resid (optional) and c: [M, N] in any
+ * of the three types each (resid may be c itself in c's type; c overlaps nothing else).  Sums are
+ * fp32.  N <= 134217727.  COBRA_EPI_MASK_OUT is rejected.  workspace:
+ * cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0), which
+ * launches that overlap must not share.
+ */
+int64_t cobra_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_dtype);
+int cobra_linear8_fwd(const void* a, int a_dtype, const void* a_scale, const void* w, const void* w_scale,
+                      const float* bias, const void* resid, int resid_dtype, const uint8_t* row_mask, int epi, void* c,
+                      int c_dtype, void* workspace, int64_t workspace_bytes, int64_t M, int64_t N, int64_t K,
+                      void* stream);
 
 /*
  * Fused QKV projection + multi-head attention on a normalised activation:
