@@ -164,8 +164,9 @@ struct Args {
 
 // What a pass over keys is: a call's own (kWhole); of a call with a shared prefix, every row of the
 // call over the prefix's keys, as if they were one request's (kPrefix), or each request's over its
-// own keys (kOwn).  The last two always leave partial results.
-enum : int { kWhole = 0, kPrefix = 1, kOwn = 2 };
+// own keys (kOwn), which both leave partial results; or each request's over the prefix's keys and
+// then its own (kBoth, not split).
+enum : int { kWhole = 0, kPrefix = 1, kOwn = 2, kBoth = 3 };
 
 // A request as the kernels see it, whatever its lengths say: bounds that keep every access
 // inside the tensors.
@@ -748,6 +749,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
   const int bs = 1 << a.shift;
   const Strides st(a, h, bs * HDP);
   Pages pages(a, b, (first * KT) >> a.shift);
+  int len = rq.len;  // of the keys that are passed over
 
   // What this thread brings of a tile: of K 16-code pieces lane, lane + 64, .. of the keys of
   // group `wave`, of V pieces tid, tid + 256, .. (four to a dimension).
@@ -785,7 +787,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
   float sk = 1.f, sv = 1.f;
   bool bad = false;
   auto load_v = [&](int tile, const Ids& ids) {
-    there = rq.len - tile * KT - 16 * (tid & 3);
+    there = len - tile * KT - 16 * (tid & 3);
     if (one) {
       const uint8_t* pv = st.v + st.block(ids.i0) + (uint32_t)((tile * KT) & (bs - 1));
 #pragma unroll
@@ -833,14 +835,27 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
     R w;
     w.init(a, rq, h, (int)row0);
     wait_vmcnt<0>();  // the queries: waited for in the loop, they would take every tile's loads along
+    int own[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) own[r] = w.lim[r];
+#pragma unroll 1
+    for (int pass = MODE == kBoth && b != a.prefix ? 0 : 1; pass < 2; ++pass) {
+    const bool pre = MODE == kBoth && pass == 0;
+    if constexpr (MODE == kBoth) {
+      const int held = request_of<kPrefix>(a, a.prefix).len;
+      pages = Pages(a, pre ? a.prefix : b, 0);
+      len = pre ? held : rq.len;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) w.lim[r] = !pre ? own[r] : row0 + 16 * r + n < rows ? held : 0;
+    }
     // Tiles that any of the workgroup's rows see; keys that all of this wave's do.
-    int full = rq.len, most = rq.len;
-    if (a.causal) {
+    int full = len, most = len;
+    if (a.causal && !pre) {
       full = rq.len - rq.n + (int)(row0 / a.group) + 1;
       most = rq.len - rq.n + (int)((min(at + kRows, rows) - 1) / a.group) + 1;
     }
     most = most > 0 ? (most + KT - 1) / KT : 0;
-    if (most > first + chunk / KT) most = first + chunk / KT;
+    if (MODE != kBoth && most > first + chunk / KT) most = first + chunk / KT;
     __syncthreads();
     Ids ids, next;  // of the tiles two ahead and one ahead
     int begin = first;
@@ -900,11 +915,12 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
         ids = load_ids(tile + 3);
       }
     }
+    }
     if (row0 < rows) {
       w.total_l();
 #pragma unroll
       for (int r = 0; r < NR; ++r)
-        w.store(a, rq, h, (int)row0, r, MODE == kOwn ? a.base + split : split, MODE == kWhole && chunk >= rq.len);
+        w.store(a, rq, h, (int)row0, r, MODE == kOwn ? a.base + split : split, MODE == kBoth || (MODE == kWhole && chunk >= rq.len));
     }
   }
 }

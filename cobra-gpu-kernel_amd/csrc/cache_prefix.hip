@@ -7,8 +7,7 @@
 // With a table of each request that lists the shared blocks too, the prefix would be read and widened
 // once for every request.  Here the rows of all requests pass over it together, as if they were one
 // request's: few rows of each become many, which share tiles in LDS.  Both passes are one launch,
-// the prefix's workgroups first, each leaves partial results (O, M, l), and a second launch joins a
-// row's.  The prefix's own new tokens see only itself.
+// each leaves partial results (O, M, l), and a second launch joins a row's.  The prefix's own new tokens see only itself.
 #include "cache_attn.hpp"
 
 namespace cobra {
@@ -18,7 +17,7 @@ namespace {
 // Both passes of a call: the prefix's workgroups, then the requests' own.
 struct Both {
   Args pre, own;
-  int groups;  // workgroups of the prefix's pass
+  int pre_groups;  // workgroups of the prefix's pass, which come first
 };
 
 template <typename T, int CACHE, int HDP, bool PRE_CHUNK, bool OWN_CHUNK>
@@ -27,115 +26,209 @@ __global__ __launch_bounds__(256, (PRE_CHUNK || OWN_CHUNK) && HDP <= 128 ? 2 : 1
   constexpr int kBytes = kChunk && sizeof(ChunkShared<HDP>) > sizeof(DecodeShared<HDP>) ? (int)sizeof(ChunkShared<HDP>)
                                                                                         : (int)sizeof(DecodeShared<HDP>);
   __shared__ __attribute__((aligned(16))) char smem[kBytes];
-  const int id = blockIdx.x;
-  if (id < c.groups) {
+  if ((int)blockIdx.x < c.pre_groups) {
     if constexpr (PRE_CHUNK)
-      chunk_rows<kPrefix, T, CACHE, HDP, 2>(c.pre, id, *reinterpret_cast<ChunkShared<HDP>*>(smem));
+      chunk_rows<kPrefix, T, CACHE, HDP, 2>(c.pre, blockIdx.x, *reinterpret_cast<ChunkShared<HDP>*>(smem));
     else
-      decode_rows<kPrefix, T, CACHE, HDP, decode_keys(HDP)>(c.pre, id, *reinterpret_cast<DecodeShared<HDP>*>(smem));
+      decode_rows<kPrefix, T, CACHE, HDP, decode_keys(HDP)>(c.pre, blockIdx.x, *reinterpret_cast<DecodeShared<HDP>*>(smem));
   } else {
     if constexpr (OWN_CHUNK)
-      chunk_rows<kOwn, T, CACHE, HDP, 2>(c.own, id - c.groups, *reinterpret_cast<ChunkShared<HDP>*>(smem));
+      chunk_rows<kOwn, T, CACHE, HDP, 2>(c.own, blockIdx.x - c.pre_groups, *reinterpret_cast<ChunkShared<HDP>*>(smem));
     else
-      decode_rows<kOwn, T, CACHE, HDP, decode_keys(HDP)>(c.own, id - c.groups,
-                                                         *reinterpret_cast<DecodeShared<HDP>*>(smem));
+      decode_rows<kOwn, T, CACHE, HDP, decode_keys(HDP)>(c.own, blockIdx.x - c.pre_groups, *reinterpret_cast<DecodeShared<HDP>*>(smem));
   }
 }
 
-// A row's shares joined, the prefix's splits and then its request's own, always in the same order:
-// o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s.  W waves have a row; a wave takes as many splits at a
-// time as it has lanes for.
-template <typename T, int HDP, int W>
-__global__ __launch_bounds__(256) void cache_prefix_join_kernel(Both c, int pre_step, int own_step) {
-  constexpr int kLanes = HDP / 4, kAt = 64 / kLanes;  // lanes of a split, splits of a wave
-  __shared__ f32x4 sh[W > 1 ? W : 1][kLanes];
-  const Args& a = c.own;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = W > 1 ? wave : 0;
-  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const int64_t rows = (int64_t)a.tokens * a.heads;
-  if (row >= rows) return;
-  const int t = (int)(row / a.heads);
-  int lo = 0;  // the last request with cu[b] <= t
+// Requests of many new tokens each: their rows fill tiles of their own, so each tile passes over the
+// prefix's keys and then its request's, and nothing is joined.
+template <typename T, int CACHE, int HDP>
+__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_prefix_chunk_kernel(Args a) {
+  __shared__ ChunkShared<HDP> sh;
+  chunk_rows<kBoth, T, CACHE, HDP, 2>(a, blockIdx.x, sh);
+}
+
+// The request that token t belongs to: the last with cu[b] <= t.
+__device__ __forceinline__ int request_at(const Args& a, int t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
   for (int b0 = 0; b0 < a.batch && a.batch > 1; b0 += 64) {
     const int below = __popcll(__ballot(b0 + lane < a.batch && a.cu[min(b0 + lane, a.batch)] <= t));
     if (below) lo = b0 + below - 1;
     if (below < 64) break;
   }
-  const Request rq = request_of<kOwn>(a, lo), pre = request_of<kPrefix>(c.pre, a.prefix);
-  if (t < rq.t0 || t >= rq.t0 + rq.n) return;
-  const int pre_chunk = chunk_of(c.pre, pre.len, pre_step), own_chunk = chunk_of(a, rq.len, own_step);
-  const int pre_n = lo == a.prefix ? 0 : (int)(((int64_t)pre.len + pre_chunk - 1) / pre_chunk);
-  const int n = pre_n + (int)(((int64_t)rq.len + own_chunk - 1) / own_chunk);
-  // Where a row's share s lies.
-  auto at = [&](int s) { return (int64_t)(s < pre_n ? s : a.base + s - pre_n) * rows + row; };
-  float m = kNegInf;
-  for (int s = lane; s < n; s += 64) m = fmaxf(m, a.part_m[at(s)].x);
+  return lo;
+}
+
+// A row's shares joined, the prefix's splits and then its request's own, always in the same order:
+// o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s.  W waves have a row; for the statistics a lane has every
+// 64th split, for O a wave takes as many splits at a time as it has lanes for.
+//
+// Bound by latency, so what does not depend on the request is asked for first: the statistics of
+// every split that there may be, and the first kEarly rounds of O.
+constexpr int kMaxSplits = 256, kOwnSplits = 64;
+template <typename T, int HDP, int W>
+__global__ __launch_bounds__(256) void cache_prefix_join_kernel(Both c, int pre_step, int own_step) {
+  constexpr int kLanes = HDP / 4, kAt = 64 / kLanes;  // lanes of a split, splits of a wave
+  constexpr int kEarly = W > 1 ? 4 : 8, kStats = W > 1 ? kMaxSplits / 64 : 1;
+  __shared__ float factor[4][64 * kStats];
+  __shared__ f32x4 sh[W > 1 ? W : 1][kLanes];
+  const Args& a = c.own;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = W > 1 ? wave : 0;
+  const int all = c.pre.splits + c.own.splits;
+  const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4, s0 = part * kAt + sub;
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  for (int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave; row < rows;
+       row += (int64_t)gridDim.x * (W > 1 ? 1 : 4)) {
+    float2 ml[kStats];
 #pragma unroll
-  for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  const float base = m == kNegInf ? 0.f : m;
-  float l = 0.f;
-  for (int s = lane; s < n; s += 64) {
-    const float2 ml = a.part_m[at(s)];
-    l += __builtin_amdgcn_exp2f(ml.x - base) * ml.y;
-  }
-  l = group_sum<64>(l);
-  const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (sub < kAt) {
-#pragma unroll 4
-    for (int s = part * kAt + sub; s < n; s += W * kAt) {
-      const float f = __builtin_amdgcn_exp2f(a.part_m[at(s)].x - base);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + at(s) * HDP + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+    for (int k = 0; k < kStats; ++k) {
+      ml[k] = make_float2(kNegInf, 0.f);
+      if (lane + 64 * k < all) ml[k] = a.part_m[(lane + 64 * k) * rows + row];
     }
-  }
+    f32x4 early[kEarly];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v = 0.f;
+    for (int i = 0; i < kEarly; ++i) {
+      const int s = s0 + i * W * kAt;
+      if (sub < kAt && s < all) early[i] = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
+    }
+    const int t = (int)(row / a.heads), b = request_at(a, t);
+    const Request rq = request_of<kOwn>(a, b), pre = request_of<kPrefix>(c.pre, a.prefix);
+    if (t < rq.t0 || t >= rq.t0 + rq.n) continue;
+    const int pre_chunk = chunk_of(c.pre, pre.len, pre_step), own_chunk = chunk_of(a, rq.len, own_step);
+    const int pre_n = b == a.prefix ? 0 : (int)(((int64_t)pre.len + pre_chunk - 1) / pre_chunk);
+    const int own_n = (int)(((int64_t)rq.len + own_chunk - 1) / own_chunk);
+    // Splits that were written: the first pre_n, and own_n from a.base on.
+    auto there = [&](int s) { return s < a.base ? s < pre_n : s - a.base < own_n; };
+    float m = kNegInf;
 #pragma unroll
-    for (int k = 0; k < kAt; ++k) v += __shfl(o[i], lane % kLanes + k * kLanes);
-    o[i] = v;
-  }
-  if constexpr (W > 1) {
-    if (lane < kLanes) sh[part][lane] = o;
-    __syncthreads();
-    if (part) return;
+    for (int k = 0; k < kStats; ++k) {
+      if (!there(lane + 64 * k)) ml[k] = make_float2(kNegInf, 0.f);
+      m = fmaxf(m, ml[k].x);
+    }
 #pragma unroll
-    for (int w = 1; w < W; ++w)
-      if (lane < kLanes) o += sh[w][lane];
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (lane < kLanes && d < a.head_dim) {
-    typename Op16<T>::V4 y;
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    float l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
-    *reinterpret_cast<typename Op16<T>::V4*>(static_cast<T*>(a.out) + row * a.head_dim + d) = y;
+    for (int k = 0; k < kStats; ++k) {
+      const float f = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - m);
+      factor[wave][lane + 64 * k] = f;
+      l += f * ml[k].y;
+    }
+    l = group_sum<64>(l);
+    __builtin_amdgcn_wave_barrier();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    auto take = [&](int s, const f32x4& x) {
+      if (sub < kAt && s < all && there(s)) {
+        const float w = factor[wave][s];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(w, x[i], o[i]);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i) take(s0 + i * W * kAt, early[i]);
+    for (int s = s0 + kEarly * W * kAt; s - sub < all; s += W * kAt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (sub < kAt && s < all) x = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
+      take(s, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) v += __shfl(o[i], lane % kLanes + k * kLanes);
+      o[i] = v;
+    }
+    if constexpr (W > 1) {
+      if (lane < kLanes) sh[part][lane] = o;
+      __syncthreads();
+      if (part) continue;  // (a workgroup has one row)
+#pragma unroll
+      for (int w = 1; w < W; ++w)
+        if (lane < kLanes) o += sh[w][lane];
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (lane < kLanes && d < a.head_dim) {
+      typename Op16<T>::V4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+      *reinterpret_cast<typename Op16<T>::V4*>(static_cast<T*>(a.out) + row * a.head_dim + d) = y;
+    }
   }
 }
 
 struct PrefixPlan {
   CachePlan pre, own;
+  bool both;  // one pass over the prefix and the request's own keys
 };
+
+// How the prefix's pass is cut: as a call of one request with all of the tokens, but for the splits.
+// In tiles of 128 rows as many as give three quarters of the chip's places (two workgroups a CU up to
+// head_dim 128) a workgroup, so that the requests' own keys, which are bound by memory, have
+// the rest from the start: 128 requests of up to 2000 keys behind 30000, 32 heads of 128 on 8, take 140 us with
+// 384 workgroups, 168 and 157 with 256 and 512; alone the passes take 88 (with 512) and 63.  (Own ones evenly
+// between the prefix's: 182 us; behind them in all of these.)  Few keys a split cost the join
+// little: 23 drafts of 2 to 6 tokens behind 4001 keys, 6 heads of 256 on 2, take 79 us with splits of 1024
+// keys, 50 with 512, 37 with 256 and 35 with 128.
+CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_prefix) {
+  CachePlan p = cache_plan(tokens, 1, heads, kv_heads, head_dim, tokens, max_prefix);
+  max_prefix = max_prefix < 1 ? 1 : max_prefix > kMaxKeys ? kMaxKeys : max_prefix;
+  const int64_t units = (p.chunked ? (tokens * (heads / kv_heads) + 127) / 128 : p.row_tiles) * kv_heads;
+  const int64_t least = p.chunked ? 128 : p.step, room = kMaxParts / (tokens * heads);
+  // Few rows (direct loads): a workgroup a CU, 32 requests of one token behind 6000, 16 heads of 64,
+  // 18.6 us against 21.1 with two, 8 behind 4000 with 32 heads of 128 on 8 15.8 and 17.8; two where the splits
+  // are of hardly any rows (one behind 99999, 16 heads of 64 on 2: 16.8 us against 19.4).
+  const int64_t target = !p.chunked ? (units <= 4 ? 512 : 256) : cache_width(head_dim) <= 128 ? 384 : 192;
+  int64_t splits = p.chunked ? (target + units / 2) / units : (target + units - 1) / units;
+  // A little more than a workgroup a CU leaves most CUs with one: thirds fill two rounds.  16 prompts of
+  // 64 to 256 tokens behind 16000, 16 heads of 64 on 4 (320 units): 318 us against 392 in one pass, 4 of
+  // 300 to 1000 behind 9000 (328 units) 301 and 314.
+  if (p.chunked && units > 256 && 3 * units <= 1024) splits = 3;
+  const int64_t most = (max_prefix + least - 1) / least;
+  splits = splits < most ? splits : most;
+  splits = splits < room ? splits : room;
+  splits = splits < kMaxSplits - kOwnSplits ? splits : kMaxSplits - kOwnSplits;
+  splits = splits < 1 ? 1 : splits;
+  const int64_t even = (max_prefix + splits - 1) / splits;
+  p.chunk = (int)((even + p.step - 1) / p.step * p.step);
+  p.splits = (int)((max_prefix + p.chunk - 1) / p.chunk);
+  return p;
+}
+
+// .. and the requests' own keys, in at most kOwnSplits.
+CachePlan own_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
+                   int64_t max_len) {
+  CachePlan p = cache_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  if (p.splits > kOwnSplits) {
+    const int64_t even = ((max_len > kMaxKeys ? kMaxKeys : max_len) + kOwnSplits - 1) / kOwnSplits;
+    p.chunk = (int)((even + p.step - 1) / p.step * p.step);
+    p.splits = kOwnSplits;
+  }
+  return p;
+}
 
 PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                    int64_t max_len, int64_t max_prefix) {
   PrefixPlan p;
-  // The prefix's pass is a call of one request with all of the tokens.
-  p.pre = cache_plan(tokens, 1, heads, kv_heads, head_dim, tokens, max_prefix);
-  p.own = cache_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix);
+  p.own = own_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  // (8 prompts of 1000 to 2000 tokens behind 8000, 32 heads of 128 on 8: 2037 us in one pass, 2380 joined.)
+  p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
   return p;
 }
 
 template <typename T, int CACHE, int HDP>
 hipError_t launch(const Both& c, const PrefixPlan& p, hipStream_t stream) {
+  const dim3 block(256);
   const int64_t own = (int64_t)c.own.batch * c.own.kv_heads * p.own.row_tiles * p.own.splits;
   const int64_t pre = (int64_t)c.own.kv_heads * p.pre.row_tiles * p.pre.splits;
+  if (p.both)
+    return own > kMaxGrid ? hipErrorInvalidValue
+                          : launch_status(cache_prefix_chunk_kernel<T, CACHE, HDP>, dim3((unsigned)own), block, stream, c.own);
   if (own + pre > kMaxGrid) return hipErrorInvalidValue;
   Both b = c;
-  b.groups = (int)pre;
-  const dim3 groups((unsigned)(own + pre)), block(256);
+  b.pre_groups = (int)pre;
+  const dim3 groups((unsigned)(own + pre));
   // Requests of many new tokens are many tokens together.
   auto* kernel = p.own.chunked   ? cache_prefix_kernel<T, CACHE, HDP, true, true>
                  : p.pre.chunked ? cache_prefix_kernel<T, CACHE, HDP, true, false>
@@ -143,10 +236,10 @@ hipError_t launch(const Both& c, const PrefixPlan& p, hipStream_t stream) {
   const hipError_t e = launch_status(kernel, groups, block, stream, b);
   if (e != hipSuccess) return e;
   const int64_t rows = (int64_t)c.own.tokens * c.own.heads;
-  return p.pre.splits + p.own.splits > 16
+  return p.pre.splits + p.own.splits > 64
              ? launch_status(cache_prefix_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, b, p.pre.step,
                              p.own.step)
-             : launch_status(cache_prefix_join_kernel<T, HDP, 1>, dim3((unsigned)((rows + 3) / 4)), block, stream, b,
+             : launch_status(cache_prefix_join_kernel<T, HDP, 1>, dim3((unsigned)((rows + 3) / 4 < kMaxGrid ? (rows + 3) / 4 : kMaxGrid)), block, stream, b,
                              p.pre.step, p.own.step);
 }
 
@@ -168,6 +261,7 @@ hipError_t launch_width(const Both& c, const PrefixPlan& p, int width, hipStream
 int64_t cache_prefix_workspace_bytes(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                      int64_t max_new, int64_t max_len, int64_t max_prefix) {
   const PrefixPlan p = plan_of(tokens, batch, heads, kv_heads, head_dim, max_new, max_len, max_prefix);
+  if (p.both) return 0;
   return (int64_t)(p.pre.splits + p.own.splits) * tokens * heads * (cache_width(head_dim) * 4 + 8);
 }
 
@@ -178,11 +272,13 @@ hipError_t run_cache_prefix(const CachePrefixArgs& c, int64_t workspace_bytes, h
   const PrefixPlan p =
       plan_of(t.tokens, t.batch, t.heads, t.kv_heads, t.head_dim, t.max_new, t.max_len, c.max_prefix);
   const int64_t rows = t.tokens * t.heads, parts = (p.pre.splits + p.own.splits) * rows;
-  if (!t.part || workspace_bytes < parts * (width * 4 + 8)) return hipErrorInvalidValue;
+  if (!p.both && (!t.part || workspace_bytes < parts * (width * 4 + 8))) return hipErrorInvalidValue;
   Both b{};
   b.own = cache_args(t, p.own);
-  b.own.part_o = t.part;
-  b.own.part_m = reinterpret_cast<float2*>(t.part + parts * width);
+  if (!p.both) {
+    b.own.part_o = t.part;
+    b.own.part_m = reinterpret_cast<float2*>(t.part + parts * width);
+  }
   b.own.prefix = c.prefix;
   b.own.base = p.pre.splits;
   b.pre = b.own;

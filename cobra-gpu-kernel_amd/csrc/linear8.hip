@@ -12,10 +12,12 @@
 //   meet in fp32): 4e-5 of a result in the root mean square.  An fp16 result's own rounding is 2e-4, a
 //   bf16's 1.6e-3, an fp32's 3e-8: fp32 results take the exact kind.
 //
-// Two kernels.  Up to 64 rows of A the weights' bytes are all that counts: linear8_few_kernel
+// Two kernels.  Up to 32 rows of A the weights' bytes are all that counts: linear8_few_kernel
 // (exact) has 16 or more rows of W a workgroup, split along K over its waves, and takes 16-bit
 // activations as they are, quantising them in the registers that the product reads.  More rows go
 // through tiles in LDS.
+#include <type_traits>
+
 #include "kernels.hpp"
 #include "lds_dma.hpp"
 #include "quant8.hpp"
@@ -160,9 +162,16 @@ struct RowBlock<uint8_t> {
   }
 };
 
-// MT sets of 16 rows of A, NT of W for a workgroup of eight waves, each with every eighth block of K;
-// UB blocks' loads are asked for together.
-template <typename TA, int MT, int NT, int UB>
+// MT sets of 16 rows of A, NT of W for a workgroup of eight waves, each with every eighth block of K.
+//
+// Bound by memory behind a launch's and a first load's latency: 8192 x 4096 weights take 10.8 us with
+// one row (9.9 as codes), 3.1 TB/s in all, where the bytes alone are 6.6 us at a copy's rate; 12.4 with 16
+// rows.  32 rows of W a workgroup where that still gives every CU one, 16 otherwise: each workgroup reads and
+// quantises all of A (16 rows, 8192 x 4096: 12.4 us against 16.2 with 16; 4096 x 8192: 16.0 against
+// 20.9 with 32).  Several blocks' loads asked for together gained nothing (12.4 to 14.9 us, 16.0 to 16.8),
+// nor did 16 waves (12.6, 16.3).  From 33 rows on quantising once and a tile kernel are faster: 64 rows
+// 19 us against 28.
+template <typename TA, int MT, int NT>
 __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
   constexpr int kWaves = 8;
   __shared__ f32x4 part[kWaves][NT * MT][64];
@@ -182,46 +191,33 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int j0 = wave; j0 < blocks; j0 += kWaves * UB) {
-    i32x4 lo[UB][NT], hi[UB][NT];
-    uint32_t wb[UB][NT];
-    RowBlock<TA> x[UB][MT];
+  for (int j = wave; j < blocks; j += kWaves) {
+    i32x8 c[NT];
+    uint32_t wb[NT];
+    RowBlock<TA> x[MT];
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int j = j0 + u * kWaves;
-      if (j < blocks) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          lo[u][t] = *reinterpret_cast<const i32x4*>(w[t] + 128 * j);
-          hi[u][t] = *reinterpret_cast<const i32x4*>(w[t] + 128 * j + 64);
-          wb[u][t] = ws[t][j];
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) x[u][i].load(a, 16 * i + r, 16 * i + r < a.M, j, g);
-      }
+    for (int t = 0; t < NT; ++t) {
+      c[t] = join8(*reinterpret_cast<const i32x4*>(w[t] + 128 * j), *reinterpret_cast<const i32x4*>(w[t] + 128 * j + 64));
+      wb[t] = ws[t][j];
     }
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      if (j0 + u * kWaves < blocks) {
-        bf16x8 y[MT][4];
+    for (int i = 0; i < MT; ++i) x[i].load(a, 16 * i + r, 16 * i + r < a.M, j, g);
+    bf16x8 y[MT][4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          float scale;
-          const i32x8 c = x[u][i].codes(scale);
+    for (int i = 0; i < MT; ++i) {
+      float scale;
+      const i32x8 q = x[i].codes(scale);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[i][k] = widen(c[2 * k], c[2 * k + 1], scale);
-        }
+      for (int k = 0; k < 4; ++k) y[i][k] = widen(q[2 * k], q[2 * k + 1], scale);
+    }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float scale = scale_of(wb[u][t]);
-          const i32x8 c = join8(lo[u][t], hi[u][t]);
+    for (int t = 0; t < NT; ++t) {
+      const float scale = scale_of(wb[t]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bf16x8 z = widen(c[2 * k], c[2 * k + 1], scale);
+      for (int k = 0; k < 4; ++k) {
+        const bf16x8 z = widen(c[t][2 * k], c[t][2 * k + 1], scale);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[t][i] = mfma16(z, y[i][k], acc[t][i]);
-          }
-        }
+        for (int i = 0; i < MT; ++i) acc[t][i] = mfma16(z, y[i][k], acc[t][i]);
       }
     }
   }
@@ -295,6 +291,7 @@ struct Tile {
   static_assert(WTM % 32 == 0 && WTN % 32 == 0 && BM % 64 == 0 && BN % 64 == 0, "wave tile");
   static_assert(ROWS / 8 % NW == 0, "every wave issues the same number of transfers");
   static_assert(LDS <= 163840, "LDS budget");
+  static_assert(TN <= 4, "slices of the epilogue");
 };
 
 __device__ __forceinline__ int chunk_swz(int row) { return (row >> 1) & 7; }
@@ -323,12 +320,14 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
   const uint8_t* scales = srow < BM ? a.a_scale + min(m0 + srow, a.M - 1) * a.s
                                     : a.w_scale + (int64_t)min(n0 + srow - BM, a.N - 1) * a.s;
   const uint32_t lds0 = lds_addr(smem);
-  auto issue = [&](int stage, int kt) {
-    const uint32_t dst = lds0 + stage * T::STAGE;
-#pragma unroll
-    for (int i = 0; i < LPT; ++i)
+  constexpr int kAll = LPT + 1;  // transfers a wave and k-tile
+  // Transfer i of k-tile kt to its stage.
+  auto transfer = [&](int kt, int i) {
+    const uint32_t dst = lds0 + (kt % ST) * T::STAGE;
+    if (i < LPT)
       dma16_untracked((8 * (wave + i * NW) < BM ? A : W) + 128 * kt, src_off[i], dst + (wave + i * NW) * 1024);
-    dma4_untracked(scales + (kt & ~3), dst + T::ROWS * 128 + (wave % (T::ROWS / 64)) * 256);
+    else
+      dma4_untracked(scales + (kt & ~3), dst + T::ROWS * 128 + (wave % (T::ROWS / 64)) * 256);
   };
 
 #pragma unroll
@@ -341,84 +340,109 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
   const int KT = a.kp >> 7;
 #pragma unroll
   for (int s = 0; s < ST; ++s)
-    if (s < KT) issue(s, s);
+    if (s < KT) {
+#pragma unroll
+      for (int i = 0; i < kAll; ++i) transfer(s, i);
+    }
 
+  // Operands of half a k-tile (64 columns), in two sets: a half's products run while the next
+  // half's reads and the transfers that refill its stage are in flight, one of each between two
+  // products.  In front of them all, a wave's reads kept its matrix core waiting.
   i32x8 af[2][T::TM], wf[2][T::TN];
-  int as[T::TM], ws[T::TN];
-  auto frags = [&](const char* st, int kk, int b) {
+  int as[T::TM], ws[T::TN], an[T::TM], wnx[T::TN];
+  constexpr int kFrags = T::TM + T::TN, kProducts = T::TM * T::TN;
+  auto read = [&](const char* st, int kk, int f) {
     const int c0 = ((4 * kk + g) ^ sw) * 16, c1 = ((4 * kk + 2 + g) ^ sw) * 16;
-#pragma unroll
-    for (int j = 0; j < T::TN; ++j) {
-      const char* p = st + (wrow + j * 32) * 128;
-      wf[b][j] = join8(*reinterpret_cast<const i32x4*>(p + c0), *reinterpret_cast<const i32x4*>(p + c1));
-    }
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-      const char* p = st + (arow + i * 32) * 128;
-      af[b][i] = join8(*reinterpret_cast<const i32x4*>(p + c0), *reinterpret_cast<const i32x4*>(p + c1));
-    }
+    const char* p = st + (f < T::TN ? wrow + f * 32 : arow + (f - T::TN) * 32) * 128;
+    const i32x8 x = join8(*reinterpret_cast<const i32x4*>(p + c0), *reinterpret_cast<const i32x4*>(p + c1));
+    if (f < T::TN) wf[kk][f] = x;
+    else af[kk][f - T::TN] = x;
   };
-  int an[T::TM], wnx[T::TN];
-  auto scale_words = [&](const char* st) {
+  auto read_scales = [&](const char* st) {
     const int* p = reinterpret_cast<const int*>(st + T::ROWS * 128);
 #pragma unroll
     for (int j = 0; j < T::TN; ++j) wnx[j] = p[wrow + j * 32];
 #pragma unroll
     for (int i = 0; i < T::TM; ++i) an[i] = p[arow + i * 32];
   };
+  // Half kk's products; between(x) after product x of kProducts.
+  auto products = [&](int kk, auto&& between) {
+    if constexpr (EXACT) {
+      bf16x8 y[T::TM][4];
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[i][k] = widen(af[kk][i][2 * k], af[kk][i][2 * k + 1], scale_of(as[i] & 255));
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bf16x8 z = widen(wf[kk][j][2 * k], wf[kk][j][2 * k + 1], scale_of(ws[j] & 255));
+#pragma unroll
+          for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma32x32x16(z, y[i][k], acc[j][i]);
+        }
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) between(j * T::TM + i);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          acc[j][i] = mfma8(wf[kk][j], af[kk][i], acc[j][i], ws[j], as[i]);
+          __builtin_amdgcn_sched_barrier(0);
+          between(j * T::TM + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  };
+  // Wait for the oldest k-tile in flight, of which there are n.
   auto wait_oldest = [&](int n) {
-    constexpr int L = LPT + 1;
-    if (ST >= 4 && n >= 4) wait_vmcnt<(ST >= 4 ? 3 : 0) * L>();
-    else if (ST >= 3 && n >= 3) wait_vmcnt<(ST >= 3 ? 2 : 0) * L>();
-    else if (n >= 2) wait_vmcnt<L>();
+    if (ST >= 4 && n >= 4) wait_vmcnt<(ST >= 4 ? 3 : 0) * kAll>();
+    else if (ST >= 3 && n >= 3) wait_vmcnt<(ST >= 3 ? 2 : 0) * kAll>();
+    else if (n >= 2) wait_vmcnt<kAll>();
     else wait_vmcnt<0>();
   };
-  wait_oldest(min(ST, KT));
-  stage_barrier();
-  frags(smem, 0, 0);
-  scale_words(smem);
-  for (int kt = 0; kt < KT; ++kt) {
+  // One k-tile.  MORE: there is a next one, FILL: and one to refill the stage with.  The barrier
+  // stands where a wave has read all of its operands of the k-tile and its own transfers of the
+  // next have landed.
+  auto step = [&](int kt, auto more, auto fill) {
+    constexpr bool MORE = decltype(more)::value, FILL = decltype(fill)::value;
     const char* st = smem + (kt % ST) * T::STAGE;
 #pragma unroll
     for (int j = 0; j < T::TN; ++j) ws[j] = wnx[j] >> (8 * (kt & 3));
 #pragma unroll
     for (int i = 0; i < T::TM; ++i) as[i] = an[i] >> (8 * (kt & 3));
+    products(0, [&](int x) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      if (kk == 0) {
-        frags(st, 1, 1);
-      } else if (kt + 1 < KT) {
-        wait_oldest(min(ST - 1, KT - 1 - kt));
-        lds_barrier();
-        if (kt + ST < KT) issue(kt % ST, kt + ST);
-        const char* next = smem + ((kt + 1) % ST) * T::STAGE;
-        frags(next, 0, 0);
-        scale_words(next);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (EXACT) {
-        bf16x8 y[T::TM][4];
-#pragma unroll
-        for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y[i][k] = widen(af[kk][i][2 * k], af[kk][i][2 * k + 1], scale_of(as[i] & 255));
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bf16x8 z = widen(wf[kk][j][2 * k], wf[kk][j][2 * k + 1], scale_of(ws[j] & 255));
-#pragma unroll
-            for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma32x32x16(z, y[i][k], acc[j][i]);
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-          for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma8(wf[kk][j], af[kk][i], acc[j][i], ws[j], as[i]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      for (int f = x * kFrags / kProducts; f < (x + 1) * kFrags / kProducts; ++f) read(st, 1, f);
+    });
+    if constexpr (MORE) {
+      wait_oldest(FILL ? ST - 1 : min(ST - 1, KT - 1 - kt));
+      lds_barrier();
     }
-  }
+    const char* next = smem + ((kt + 1) % ST) * T::STAGE;
+    if constexpr (MORE) read_scales(next);
+    products(1, [&](int x) {
+      if constexpr (MORE) {
+#pragma unroll
+        for (int f = x * kFrags / kProducts; f < (x + 1) * kFrags / kProducts; ++f) read(next, 0, f);
+      }
+      if constexpr (FILL) {
+#pragma unroll
+        for (int i = x * kAll / kProducts; i < (x + 1) * kAll / kProducts; ++i) transfer(kt + ST, i);
+      }
+    });
+  };
+  wait_oldest(min(ST, KT));
+  stage_barrier();
+#pragma unroll
+  for (int f = 0; f < kFrags; ++f) read(smem, 0, f);
+  read_scales(smem);
+  int kt = 0;
+  for (; kt + ST < KT; ++kt) step(kt, std::true_type(), std::true_type());
+  for (; kt + 1 < KT; ++kt) step(kt, std::true_type(), std::false_type());
+  step(kt, std::false_type(), std::false_type());
 }
 
 template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
@@ -454,9 +478,11 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
   const int cl = (tid % LPR) * CPL;
   const int ccol = (cl / 32) * T::WTN + (cl % 32);
   const bool whole = a.N % 8 == 0;
-  constexpr int cdt = sizeof(TC) == 4 ? (int)kF32 : std::is_same<TC, f16>::value ? (int)kF16 : (int)kBF16;
-#pragma unroll
-  for (int j = 0; j < T::TN; ++j) {
+  const bool masks = a.epi & (kEpiMaskBranch | kEpiMaskResid);
+  // (A template for each slice: as a loop, the accumulators' index stayed a variable, and they went to
+  // scratch.)
+  auto slice = [&](auto jc) {
+    constexpr int j = decltype(jc)::value;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -467,78 +493,100 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
         *reinterpret_cast<f32x4*>(Cs + (wm * T::WTM + i * 32 + li) * T::LDC + wn * 32 + 8 * q + 4 * g) = v;
       }
     const int n = n0 + ccol + j * 32;
-    f32x4 rv[NP][CPL / 4], bv[CPL / 4];
+    f32x4 bv[CPL / 4];
 #pragma unroll
-    for (int h = 0; h < CPL / 4; ++h) {
-      bv[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < CPL / 4; ++h)
+      bv[h] = a.bias && whole && n < a.N ? *reinterpret_cast<const f32x4*>(a.bias + n + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
+    // A row of the slice: its LDS place, product, bias and GELU.
+    auto value = [&](int p, int h) {
+      f32x4 v = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h) + bv[h];
+      if (a.epi & kEpiGelu) {
 #pragma unroll
-      for (int p = 0; p < NP; ++p) rv[p][h] = bv[h];
-    }
-    if (whole && n < a.N) {
+        for (int e = 0; e < 4; ++e) v[e] = gelu_erf(v[e]);
+      }
+      return v;
+    };
+    auto store = [&](int64_t m, const f32x4 (&v)[CPL / 4]) {
+      TC* at = static_cast<TC*>(a.c) + m * a.N + n;
+      if constexpr (sizeof(TC) == 4) {
+        *reinterpret_cast<f32x4*>(at) = v[0];
+      } else {
+        typename Op16<TC>::V8 hv;
 #pragma unroll
-      for (int h = 0; h < CPL / 4; ++h) {
-        if (a.bias) bv[h] = *reinterpret_cast<const f32x4*>(a.bias + n + 4 * h);
-        if (a.resid) {
+        for (int e = 0; e < 8; ++e) hv[e] = (TC)v[e >> 2][e & 3];
+        *reinterpret_cast<typename Op16<TC>::V8*>(at) = hv;
+      }
+    };
+    const int64_t first = m0 + tid / LPR;  // this thread's rows: first, first + RPP, ..
+    // Loads share a counter with the stores: one between two passes would wait for the stores of
+    // the pass before it.  So there are none in the loop without residual and masks (which is no
+    // longer than it is because a tile runs it once, its instructions coming from memory), and with
+    // them all of a slice's are asked for before its first store.
+    if (whole && !a.resid && !masks) {
+      __syncthreads();
+      if (n < a.N) {
+#pragma unroll 2
+        for (int p = 0; p < NP; ++p) {
+          if (first + p * RPP >= a.M) break;
+          f32x4 v[CPL / 4];
 #pragma unroll
-          for (int p = 0; p < NP; ++p)
-            rv[p][h] = get4(a.resid, a.resid_dtype, min(m0 + tid / LPR + p * RPP, a.M - 1) * a.N + n + 4 * h);
+          for (int h = 0; h < CPL / 4; ++h) v[h] = value(p, h);
+          store(first + p * RPP, v);
+        }
+      }
+    } else if (whole) {
+      f32x4 rv[NP][CPL / 4];
+      uint32_t padded = 0;
+      const int nc = min(n, a.N - CPL);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int64_t m = min(first + p * RPP, a.M - 1);
+        if (masks && a.row_mask[m] == 0) padded |= 1u << p;
+#pragma unroll
+        for (int h = 0; h < CPL / 4; ++h)
+          rv[p][h] = a.resid ? get4(a.resid, a.resid_dtype, m * a.N + nc + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        if (n < a.N && first + p * RPP < a.M) {
+          f32x4 v[CPL / 4];
+#pragma unroll
+          for (int h = 0; h < CPL / 4; ++h) {
+            v[h] = value(p, h);
+            if ((padded >> p & 1) && (a.epi & kEpiMaskBranch)) v[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            v[h] += rv[p][h];
+            if ((padded >> p & 1) && (a.epi & kEpiMaskResid)) v[h] *= 0.f;
+          }
+          store(first + p * RPP, v);
         }
       }
     } else {
-#pragma unroll
-      for (int e = 0; e < CPL; ++e)
-        if (a.bias && n + e < a.N) bv[e / 4][e % 4] = a.bias[n + e];
-    }
-    __syncthreads();
-    if (n < a.N) {
-#pragma unroll
+      __syncthreads();
+#pragma unroll 1
       for (int p = 0; p < NP; ++p) {
-        const int64_t m = m0 + tid / LPR + p * RPP;
+        const int64_t m = first + p * RPP;
         if (m >= a.M) break;
-        const bool padded = (a.epi & (kEpiMaskBranch | kEpiMaskResid)) && a.row_mask[m] == 0;
-        const int64_t at = m * a.N + n;
-        float v[CPL];
-#pragma unroll
-        for (int h = 0; h < CPL / 4; ++h) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = t[e] + bv[h][e];
-            if (a.epi & kEpiGelu) x = gelu_erf(x);
-            if (padded && (a.epi & kEpiMaskBranch)) x = 0.f;
-            v[4 * h + e] = x + rv[p][h][e];
-          }
-        }
-        if (whole) {
-          if (padded && (a.epi & kEpiMaskResid)) {
-#pragma unroll
-            for (int e = 0; e < CPL; ++e) v[e] *= 0.f;
-          }
-#pragma unroll
-          for (int h = 0; h < 1; ++h) {
-            if constexpr (sizeof(TC) == 4) {
-              *reinterpret_cast<f32x4*>(static_cast<float*>(a.c) + at) = f32x4{v[0], v[1], v[2], v[3]};
-            } else {
-              typename Op16<TC>::V8 hv;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) hv[e] = (TC)v[e];
-              *reinterpret_cast<typename Op16<TC>::V8*>(static_cast<TC*>(a.c) + at) = hv;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < CPL; ++e)
-            if (n + e < a.N) {
-              float x = v[e];
-              if (a.resid) x += get(a.resid, a.resid_dtype, at + e);
-              if (padded && (a.epi & kEpiMaskResid)) x *= 0.f;
-              put(a.c, cdt, at + e, x);
-            }
+        const bool padded = masks && a.row_mask[m] == 0;
+#pragma unroll 1
+        for (int e = 0; e < CPL && n + e < a.N; ++e) {
+          const int64_t at = m * a.N + n + e;
+          float v = Cs[(tid / LPR + p * RPP) * T::LDC + cl + e];
+          if (a.bias) v += a.bias[n + e];
+          if (a.epi & kEpiGelu) v = gelu_erf(v);
+          if (padded && (a.epi & kEpiMaskBranch)) v = 0.f;
+          if (a.resid) v += get(a.resid, a.resid_dtype, at);
+          if (padded && (a.epi & kEpiMaskResid)) v *= 0.f;
+          static_cast<TC*>(a.c)[at] = (TC)v;
         }
       }
     }
-    __syncthreads();
-  }
+    if (j + 1 < T::TN) __syncthreads();
+  };
+  slice(std::integral_constant<int, 0>());
+  if constexpr (T::TN > 1) slice(std::integral_constant<int, 1>());
+  if constexpr (T::TN > 2) slice(std::integral_constant<int, 2>());
+  if constexpr (T::TN > 3) slice(std::integral_constant<int, 3>());
 }
 
 template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
@@ -549,27 +597,66 @@ hipError_t launch_tile(const Args& a, hipStream_t stream) {
                        stream, a);
 }
 
+// Tile choice: the candidate with the least estimated time, as for the 16-bit kernel.  n workgroups
+// fall to each CU, per_cu at a time; a group of r takes `fixed` (launch, first loads, epilogue) plus
+// per k-tile the larger of `step` (one workgroup's chain) and r x `busy` (its share of the CU).  Fits
+// (us) to timings of every candidate over M 128 .. 16384, N and K 1000 .. 8192, for the scaled
+// kind and the exact one: 8192 x 4096 x 4096 takes 114.8 us in 256 x 256 tiles (2394 TFLOP/s) and 146 in
+// 128 x 128, 8192^3 417 (2635 TFLOP/s; a library product of e4m3 2605 to 2675 on the same cards) and 539,
+// 512 x 4096 x 4096 44.6, 26.6, 16.4 and 19.7 in the four, 128 x 4096 x 4096 37.8, 19.5, 14.8 and 10.6.
+// Exact, fp32 results: 8192 x 4096 x 4096 221 us in 256 x 256 and 241 in 128 x 128, 8192^3 790
+// (1391 TFLOP/s; a library product in bf16 1308 to 1339) and 881.
+struct TileCand {
+  int bm, bn, per_cu;
+  double fixed, step, busy;
+};
+constexpr TileCand kScaled[] = {{256, 256, 1, 11.0, 1.00, 1.45}, {128, 128, 2, 4.4, 0.47, 0.50},
+                                {128, 64, 2, 4.1, 0.36, 0.28},   {64, 64, 2, 3.5, 0.22, 0.21}};
+constexpr TileCand kExact[] = {{256, 256, 1, 21.0, 1.80, 2.75}, {128, 128, 2, 8.7, 0.67, 0.80},
+                               {128, 64, 2, 6.0, 0.58, 0.51},   {64, 64, 2, 4.8, 0.37, 0.39}};
+
+int pick_tile(const TileCand (&tiles)[4], const Args& a) {
+  const int64_t cus = compute_units();
+  const double kt = a.kp / 128;
+  int best = 0;
+  double best_t = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    const TileCand& c = tiles[i];
+    const int64_t all = ((a.M + c.bm - 1) / c.bm) * (int64_t)((a.N + c.bn - 1) / c.bn);
+    const int64_t n = (all + cus - 1) / cus, rest = n % c.per_cu;
+    auto group = [&](double r) { return c.fixed + kt * (r * c.busy > c.step ? r * c.busy : c.step); };
+    const double t = (double)(n / c.per_cu) * group(c.per_cu) + (rest ? group((double)rest) : 0.0);
+    if (t < best_t) {
+      best_t = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
 template <typename TC>
 hipError_t dispatch_tile(const Args& a, hipStream_t stream) {
-  auto tiles = [&](int bm, int bn) { return ((a.M + bm - 1) / bm) * (int64_t)((a.N + bn - 1) / bn); };
-  const int64_t cus = compute_units();
-  if (tiles(128, 128) >= cus) return launch_tile<128, 128, 2, 2, 2, 8, TC>(a, stream);
-  return launch_tile<64, 64, 2, 2, 4, 8, TC>(a, stream);
+  switch (pick_tile(sizeof(TC) == 4 ? kExact : kScaled, a)) {
+    case 0: return launch_tile<256, 256, 4, 2, 2, 4, TC>(a, stream);
+    case 1: return launch_tile<128, 128, 2, 2, 2, 8, TC>(a, stream);
+    case 2: return launch_tile<128, 64, 2, 2, 3, 8, TC>(a, stream);
+    default: return launch_tile<64, 64, 2, 2, 4, 8, TC>(a, stream);
+  }
 }
 
-template <typename TA>
+template <int MT, int NT, typename TA>
 hipError_t launch_few(const Args& a, hipStream_t stream) {
-  const dim3 block(512);
-  auto groups = [&](int nt) { return dim3((unsigned)((a.N + 16 * nt - 1) / (16 * nt))); };
-  if (a.M <= 16)
-    return a.M <= 4 || a.N <= 16 * 2 * compute_units()
-               ? launch_status(linear8_few_kernel<TA, 1, 1, 4>, groups(1), block, stream, a)
-               : launch_status(linear8_few_kernel<TA, 1, 2, 2>, groups(2), block, stream, a);
-  if (a.M <= 32) return launch_status(linear8_few_kernel<TA, 2, 2, 2>, groups(2), block, stream, a);
-  return launch_status(linear8_few_kernel<TA, 4, 2, 1>, groups(2), block, stream, a);
+  return launch_status(linear8_few_kernel<TA, MT, NT>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(512),
+                       stream, a);
+}
+template <typename TA>
+hipError_t dispatch_few(const Args& a, hipStream_t stream) {
+  const bool wide = a.N >= 32 * compute_units();
+  if (a.M <= 16) return wide ? launch_few<1, 2, TA>(a, stream) : launch_few<1, 1, TA>(a, stream);
+  return wide ? launch_few<2, 2, TA>(a, stream) : launch_few<2, 1, TA>(a, stream);
 }
 
-constexpr int64_t kFewRows = 64;
+constexpr int64_t kFewRows = 32;
 
 bool whole_rows(const Linear8Args& c) {
   return c.K % 8 == 0 && (reinterpret_cast<uintptr_t>(c.a) & 15) == 0;
@@ -591,7 +678,7 @@ hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_
          c.resid_dtype, c.c_dtype, c.epi};
   const bool codes = c.a_dtype == kE4M3;
   if (c.M <= kFewRows && !codes && whole_rows(c))
-    return c.a_dtype == kF16 ? launch_few<f16>(a, stream) : launch_few<bf16>(a, stream);
+    return c.a_dtype == kF16 ? dispatch_few<f16>(a, stream) : dispatch_few<bf16>(a, stream);
   if (!codes) {
     if (!c.workspace || workspace_bytes < c.M * (kp + s)) return hipErrorInvalidValue;
     uint8_t* scale = static_cast<uint8_t*>(c.workspace) + c.M * kp;
@@ -601,7 +688,7 @@ hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_
     a.a = c.workspace;
     a.a_scale = scale;
   }
-  if (c.M <= kFewRows) return launch_few<uint8_t>(a, stream);
+  if (c.M <= kFewRows) return dispatch_few<uint8_t>(a, stream);
   switch (c.c_dtype) {
     case kF16: return dispatch_tile<f16>(a, stream);
     case kBF16: return dispatch_tile<bf16>(a, stream);

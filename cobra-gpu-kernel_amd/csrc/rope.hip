@@ -15,12 +15,14 @@
 // half of what turns) have a wave each and their partners from memory.
 #include "common.hpp"
 #include "kernels.hpp"
+#include "lds_dma.hpp"
 
 namespace cobra {
 
 namespace {
 
 constexpr int kMaxDim = 256;
+constexpr int kTurns = 256, kSome = 8;  // angles and tokens of a workgroup, at most
 
 struct Args {
   void* qkv;
@@ -50,14 +52,12 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
-// A token's turns: (cos, sin) of its position times each frequency.
-__device__ __forceinline__ void turns(const Args& a, int pos, float2* turn) {
-  for (int i = threadIdx.x; i < a.half; i += 256) {
-    const double x = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189535);  // 1 / 2 pi
-    float s, c;
-    sincospif(2.f * (float)(x - __builtin_rint(x)), &s, &c);
-    turn[i] = make_float2(c, s);
-  }
+// (cos, sin) of a position times frequency i.
+__device__ __forceinline__ float2 turn_of(const Args& a, int pos, int i) {
+  const double x = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189535);  // 1 / 2 pi
+  float s, c;
+  sincospif(2.f * (float)(x - __builtin_rint(x)), &s, &c);
+  return make_float2(c, s);
 }
 __device__ __forceinline__ void rotate(float& u, float& v, const float2& r) {
   const float x = u;
@@ -66,59 +66,102 @@ __device__ __forceinline__ void rotate(float& u, float& v, const float2& r) {
 }
 __device__ __forceinline__ float norm_of(const Args& a, float sum) { return 1.0f / sqrtf(sum / (float)a.dim + a.eps); }
 
+// A workgroup has `some` tokens; a thread every 256th piece pair of their heads, always the same place
+// in the head, so that it holds that place's weights.  U pairs' loads are asked for before the turns
+// are formed and the first of them is used.  16384 tokens of 32 + 8 heads of 128 (335 MB): 76 us,
+// 4.4 TB/s against a large copy's 5.1; with a token a workgroup 162 (its angles and barriers), with two
+// 100, three 80, six 80; four pairs ahead 83 (registers for three waves of a SIMD).
 template <typename T, int V, bool INTER>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a) {
-  __shared__ float2 turn[kMaxDim / 2];
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
+  constexpr int U = 2;
+  __shared__ float2 turn[kTurns];
+  __shared__ int place[kSome];
   const int tid = threadIdx.x;
   const int p = tid & (a.lanes - 1), per = 256 / a.lanes;
   const bool pair = !INTER && p * V < a.half;  // this lane's pieces are partners
   const int c0 = pair ? p * V : 2 * p * V, c1 = pair ? a.half + p * V : c0 + V;
   const bool on0 = c0 < a.dim, on1 = c1 < a.dim;
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int pos = a.positions ? a.positions[t] : 0;
-    if (pos < 0) continue;
-    __syncthreads();  // the last token's turns are used up
-    turns(a, pos, turn);
-    __syncthreads();
-    T* row = static_cast<T*>(a.qkv) + t * a.ld;
-    for (int h = tid / a.lanes; h < a.all; h += per) {
-      T* x = row + (int64_t)h * a.pitch;
-      Piece<T, V> p0{}, p1{};
-      if (on0) p0 = *reinterpret_cast<const Piece<T, V>*>(x + c0);
-      if (on1) p1 = *reinterpret_cast<const Piece<T, V>*>(x + c1);
+  const int64_t t0 = (int64_t)blockIdx.x * some;
+  const int count = (int)min((int64_t)some, a.tokens - t0);
+  const uint32_t work = (uint32_t)count * a.all;  // heads of these tokens
+  T* base = static_cast<T*>(a.qkv) + t0 * a.ld;
+  Piece<T, V> x[U][2];
+  auto ask = [&](uint32_t first) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t w = first + u * per;
+      x[u][0] = x[u][1] = Piece<T, V>{};
+      if (w < work) {
+        const uint32_t t = w / a.all;
+        const T* at = base + t * a.ld + (int64_t)(w - t * a.all) * a.pitch;
+        if (on0) x[u][0] = *reinterpret_cast<const Piece<T, V>*>(at + c0);
+        if (on1) x[u][1] = *reinterpret_cast<const Piece<T, V>*>(at + c1);
+      }
+    }
+  };
+  const uint32_t mine = tid / a.lanes;
+  // The positions first: loads come back in order, and the angles need nothing else.
+  const int at = tid < count && a.positions ? a.positions[t0 + tid] : 0;
+  ask(mine);
+  if (tid < count) place[tid] = at;
+  float wq[2][V], wk[2][V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    wq[0][e] = a.q_weight && on0 ? a.q_weight[c0 + e] : 1.f;
+    wq[1][e] = a.q_weight && on1 ? a.q_weight[c1 + e] : 1.f;
+    wk[0][e] = a.q_weight && on0 ? a.k_weight[c0 + e] : 1.f;
+    wk[1][e] = a.q_weight && on1 ? a.k_weight[c1 + e] : 1.f;
+  }
+  lds_barrier();
+  for (int i = tid; i < count * a.half; i += 256) {
+    const int t = i / a.half, k = i - t * a.half;
+    turn[i] = turn_of(a, place[t], k);
+  }
+  lds_barrier();
+  for (uint32_t first = mine; first < work; first += U * per) {
+    if (first != mine) ask(first);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t w = first + u * per;
+      if (w >= work) break;
+      const uint32_t t = w / a.all, h = w - t * a.all;
       float y0[V], y1[V], ss = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        y0[e] = (float)p0.e[e];
-        y1[e] = (float)p1.e[e];
+        y0[e] = (float)x[u][0].e[e];
+        y1[e] = (float)x[u][1].e[e];
         ss = fmaf(y0[e], y0[e], fmaf(y1[e], y1[e], ss));
       }
-      const float* w = h < a.heads ? a.q_weight : a.k_weight;
-      if (w) {
+      if (a.q_weight) {
         const float inv = norm_of(a, lanes_sum(ss, a.lanes));
+        const bool query = h < (uint32_t)a.heads;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          if (on0) y0[e] *= inv * w[c0 + e];
-          if (on1) y1[e] *= inv * w[c1 + e];
+          y0[e] *= inv * (query ? wq[0][e] : wk[0][e]);
+          y1[e] *= inv * (query ? wq[1][e] : wk[1][e]);
         }
       }
+      const float2* r = turn + t * a.half;
       if constexpr (INTER) {
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
-          if (c0 + e < 2 * a.half) rotate(y0[e], y0[e + 1], turn[(c0 + e) >> 1]);
-          if (c1 + e < 2 * a.half) rotate(y1[e], y1[e + 1], turn[(c1 + e) >> 1]);
+          if (c0 + e < 2 * a.half) rotate(y0[e], y0[e + 1], r[(c0 + e) >> 1]);
+          if (c1 + e < 2 * a.half) rotate(y1[e], y1[e + 1], r[(c1 + e) >> 1]);
         }
       } else if (pair) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) rotate(y0[e], y1[e], turn[c0 + e]);
+        for (int e = 0; e < V; ++e) rotate(y0[e], y1[e], r[c0 + e]);
       }
+      if (place[t] < 0) continue;
+      Piece<T, V> z0, z1;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        p0.e[e] = (T)y0[e];
-        p1.e[e] = (T)y1[e];
+        z0.e[e] = (T)y0[e];
+        z1.e[e] = (T)y1[e];
       }
-      if (on0) *reinterpret_cast<Piece<T, V>*>(x + c0) = p0;
-      if (on1) *reinterpret_cast<Piece<T, V>*>(x + c1) = p1;
+      T* at = base + t * a.ld + (int64_t)h * a.pitch;
+      if (on0) *reinterpret_cast<Piece<T, V>*>(at + c0) = z0;
+      if (on1) *reinterpret_cast<Piece<T, V>*>(at + c1) = z1;
     }
   }
 }
@@ -134,7 +177,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(Args a, int inter
     const int pos = a.positions ? a.positions[t] : 0;
     if (pos < 0) continue;
     __syncthreads();
-    turns(a, pos, turn);
+    for (int i = threadIdx.x; i < a.half; i += 256) turn[i] = turn_of(a, pos, i);
     __syncthreads();
     T* row = static_cast<T*>(a.qkv) + t * a.ld;
     for (int h = threadIdx.x >> 6; h < a.all; h += 4) {
@@ -178,7 +221,15 @@ template <typename T, int V, bool INTER>
 hipError_t launch(Args a, hipStream_t stream) {
   a.lanes = 1;
   while (a.lanes * 2 * V < a.dim) a.lanes *= 2;
-  return launch_status(qk_norm_rope_kernel<T, V, INTER>, groups_of(a), dim3(256), stream, a);
+  // As many tokens a workgroup as its threads have five pairs and an angle each for, where every CU
+  // still has eight workgroups; a token each for few.
+  const int64_t batch = 5 * 256 / ((int64_t)a.all * a.lanes), angles = a.half ? kTurns / a.half : kSome;
+  int some = (int)(batch < angles ? batch : angles);
+  some = some > kSome ? kSome : some < 1 ? 1 : some;
+  if (a.tokens < (int64_t)some * 8 * compute_units()) some = 1;
+  const int64_t groups = (a.tokens + some - 1) / some;
+  if ((int64_t)some * a.all > 0x7fffffff) return hipErrorInvalidValue;
+  return launch_status(qk_norm_rope_kernel<T, V, INTER>, dim3((unsigned)groups), dim3(256), stream, a, some);
 }
 
 template <typename T>

@@ -110,8 +110,8 @@ def check_linear(m, k, n, dtype, seed, codes=False, bias=True, gelu=False, out=N
         y = ops.linear8(a.to(DEV), *dw, out_dtype=out, **kw)
     torch.cuda.synchronize()
     assert y.dtype == out_type and y.shape == (m, n)
-    # Up to 64 rows and for fp32 results the products are added in fp32 one by one.
-    cut = serve.cut_of_eights(serve.values(aq, ab), serve.values(wq, wb)) if m > 64 and out_type != F32 else 0.0
+    # Up to 32 rows and for fp32 results the products are added in fp32 one by one.
+    cut = serve.cut_of_eights(serve.values(aq, ab), serve.values(wq, wb)) if m > 32 and out_type != F32 else 0.0
     room = bound(want, mag, aq.shape[1], gelu, out_type, cut)
     if rm is not None and resid is not None and not mask_branch:
         want = torch.where(rm[:, None], want, torch.zeros_like(want))
