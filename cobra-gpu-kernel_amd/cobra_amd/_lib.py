@@ -89,7 +89,8 @@ SIGNATURES = {
     "cobra_cache_positions": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp]),
     "cobra_qk_norm_rope": (
         _c_int,
-        [_vp, _c_int, _c_i64, _vp, _vp, _c_i64, _c_int, _vp, _vp, _c_f32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp],
+        [_vp, _c_int, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _vp, _vp, _c_f32, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i64, _vp],
     ),
     "cobra_quantize8": (_c_int, [_vp, _c_int, _vp, _vp, _c_i64, _c_i64, _vp]),
     "cobra_linear8_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),

@@ -2,7 +2,8 @@
 
 ``CobraCache`` owns the pool of blocks of every layer and the tables, lengths and free blocks
 that all layers share, all on the device; its methods are ``ops.cache_reserve``, ``cache_trim``,
-``cache_append`` and ``cache_attn`` on them, and wait for nothing.  ``CobraTransformer.extend``
+``cache_append``, ``cache_positions``, ``cache_attn`` and ``cache_prefix_attn`` on them, and wait for
+nothing.  ``CobraTransformer.extend``
 runs the stack over new tokens with one.  (The reference's attention sees whole sequences,
 torch_transformer_benchmark.py:88-123; it keeps no cache.)
 """
@@ -70,6 +71,10 @@ class CobraCache:
         return ops.cache_trim(self.lens, keep_lens, self.block_table, self.free_list, self.free_count,
                               self.block_size)
 
+    def positions(self, cu: torch.Tensor, tokens: int, prefix: Optional[int] = None) -> torch.Tensor:
+        """Where the new tokens of a reserve stand in their requests (``ops.cache_positions``)."""
+        return ops.cache_positions(cu, self.lens, tokens, prefix)
+
     def append(self, layer: int, qkv: torch.Tensor, slots: torch.Tensor, heads: int) -> None:
         """A layer's new keys and values into their slots (``ops.cache_append``)."""
         ops.cache_append(qkv, slots, heads, self.head_dim, self.k[layer], self.v[layer], self.k_scale[layer],
@@ -77,8 +82,14 @@ class CobraCache:
 
     def attn(self, layer: int, q: torch.Tensor, cu: torch.Tensor, heads: int, scale: float, causal: bool = True,
              max_new: Optional[int] = None, max_len: Optional[int] = None,
-             out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Attention of the new tokens over what a layer's cache holds of their requests (``ops.cache_attn``)."""
+             out: Optional[torch.Tensor] = None, prefix: Optional[int] = None,
+             max_prefix: Optional[int] = None) -> torch.Tensor:
+        """Attention of the new tokens over what a layer's cache holds of their requests (``ops.cache_attn``),
+        or of row ``prefix`` and their requests (``ops.cache_prefix_attn``)."""
+        if prefix is not None:
+            return ops.cache_prefix_attn(q, cu, self.lens, self.block_table, prefix, heads, self.head_dim, scale,
+                                         self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
+                                         causal=causal, max_new=max_new, max_len=max_len, max_prefix=max_prefix, out=out)
         return ops.cache_attn(q, cu, self.lens, self.block_table, heads, self.head_dim, scale, self.k[layer],
                               self.v[layer], self.k_scale[layer], self.v_scale[layer], causal=causal,
                               max_new=max_new, max_len=max_len, out=out)

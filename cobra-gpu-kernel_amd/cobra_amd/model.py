@@ -56,7 +56,10 @@ GRAPH_MAX_INPUT_BYTES = 64 * 1024 * 1024
 
 @dataclass(frozen=True)
 class TransformerConfig:
-    """Fields and validation of the reference's ``TransformerConfig`` (TTB:28-57)."""
+    """Fields and validation of the reference's ``TransformerConfig`` (TTB:28-57), and two options
+    that it has not: ``rope_theta`` rotates queries and keys by position (frequencies
+    ``rope_theta^(-2 i / head_dim)``, pairs of halves), ``qk_norm`` norms them for each head before
+    (``q_norm`` and ``k_norm`` of each block)."""
 
     batch_size: int
     seq_len: int
@@ -65,6 +68,8 @@ class TransformerConfig:
     ffn_dim: int
     num_layers: int
     causal: bool
+    rope_theta: Optional[float] = None
+    qk_norm: bool = False
 
     def validate(self) -> None:
         for name in ("batch_size", "seq_len", "d_model", "num_heads", "ffn_dim", "num_layers"):
@@ -72,30 +77,43 @@ class TransformerConfig:
                 raise ValueError(f"{name} must be positive")
         if self.d_model % self.num_heads != 0:
             raise ValueError(f"d_model ({self.d_model}) must be divisible by num_heads ({self.num_heads})")
+        if self.rope_theta is not None:
+            if not self.rope_theta > 0:
+                raise ValueError(f"rope_theta must be positive, got {self.rope_theta}")
+            if self.d_model // self.num_heads % 2:
+                raise ValueError(f"rotation needs an even head_dim, got {self.d_model // self.num_heads}")
 
 
 class CobraTransformerBlock(nn.Module):
-    """Parameters of ``BaselineTransformerBlock`` (TTB:126-133), same names and draw order."""
+    """Parameters of ``BaselineTransformerBlock`` (TTB:126-133), same names and draw order (the norms
+    of ``qk_norm`` draw nothing)."""
 
-    def __init__(self, d_model: int, num_heads: int, ffn_dim: int) -> None:
+    def __init__(self, d_model: int, num_heads: int, ffn_dim: int, qk_norm: bool = False) -> None:
         super().__init__()
         self.norm1 = nn.LayerNorm(d_model)
         self.attention = CobraSelfAttention(d_model, num_heads)
         self.norm2 = nn.LayerNorm(d_model)
         self.ffn_in = nn.Linear(d_model, ffn_dim)
         self.ffn_out = nn.Linear(ffn_dim, d_model)
+        if qk_norm:
+            self.q_norm = nn.RMSNorm(d_model // num_heads, eps=1e-6)
+            self.k_norm = nn.RMSNorm(d_model // num_heads, eps=1e-6)
 
 
 class _BlockPack:
     """Kernel-ready copies of one block's parameters (plain attributes, so the
     state_dict is unchanged; TTB:857-914), zero-padded when the geometry needs it.  The
     weight matrices are in the MFMA operand type ``op``: fp16, or bf16 for bf16
-    activations."""
+    activations; with ``weights8`` they are ``ops.quantize8`` of the parameters."""
 
-    __slots__ = ("w_qkv", "b_qkv", "w_o", "b_o", "w1", "b1", "w2", "b2", "ln1_w", "ln1_b", "ln2_w", "ln2_b")
+    __slots__ = ("w_qkv", "b_qkv", "w_o", "b_o", "w1", "b1", "w2", "b2", "ln1_w", "ln1_b", "ln2_w", "ln2_b", "q_norm",
+                 "k_norm", "qk_eps")
 
-    def __init__(self, blk: CobraTransformerBlock, geom: PadGeometry, op: torch.dtype = torch.float16) -> None:
+    def __init__(self, blk: CobraTransformerBlock, geom: PadGeometry, op: torch.dtype = torch.float16,
+                 weights8: bool = False) -> None:
         att = blk.attention
+        if weights8:
+            op = att.q_proj.weight.dtype
         with torch.no_grad():
             w = (torch.cat([att.q_proj.weight, att.k_proj.weight, att.v_proj.weight]).to(op),
                  torch.cat([att.q_proj.bias, att.k_proj.bias, att.v_proj.bias]).float(),
@@ -106,21 +124,45 @@ class _BlockPack:
                 w = pad_block_weights(*w, geom)
             (self.w_qkv, self.b_qkv, self.w_o, self.b_o, self.w1, self.b1, self.w2,
              self.b2) = (t.contiguous() for t in w)
+            if weights8:
+                self.w_qkv, self.w_o, self.w1, self.w2 = (ops.quantize8(t) for t in
+                                                          (self.w_qkv, self.w_o, self.w1, self.w2))
             self.ln1_w = blk.norm1.weight.float().contiguous()
             self.ln1_b = blk.norm1.bias.float().contiguous()
             self.ln2_w = blk.norm2.weight.float().contiguous()
             self.ln2_b = blk.norm2.bias.float().contiguous()
+            norms = hasattr(blk, "q_norm")
+            self.q_norm = blk.q_norm.weight.float().contiguous() if norms else None
+            self.k_norm = blk.k_norm.weight.float().contiguous() if norms else None
+            self.qk_eps = float(blk.q_norm.eps) if norms else 0.0
+
+
+def _linear(h: torch.Tensor, w, b: torch.Tensor, gelu: bool = False, out_fp32: bool = False,
+            resid: Optional[torch.Tensor] = None, rmask: Optional[torch.Tensor] = None,
+            mask_branch: bool = False) -> torch.Tensor:
+    """``ops.linear``, or ``ops.linear8`` for a weight held in 8 bits."""
+    if isinstance(w, tuple):
+        return ops.linear8(h, *w, b, gelu=gelu, out_dtype=torch.float32 if out_fp32 else None, resid=resid, rmask=rmask,
+                           mask_branch=mask_branch)
+    return ops.linear(h, w, b, gelu=gelu, out_fp32=out_fp32, resid=resid, rmask=rmask, mask_branch=mask_branch)
 
 
 class CobraTransformer(nn.Module):
-    def __init__(self, config: TransformerConfig, graph: Optional[bool] = None) -> None:
+    """``weights8``: the blocks' weights are held in 8 bits for the kernels (e4m3 codes with a power of
+    two for each row and 128 columns, laid out from the parameters like the 16-bit copies are), and
+    activations are quantised the same way for each product (``ops.linear8``)."""
+
+    def __init__(self, config: TransformerConfig, graph: Optional[bool] = None, weights8: bool = False) -> None:
         super().__init__()
         config.validate()
         self.config = config
+        self.weights8 = bool(weights8)
+        # What only the composed forward has.
+        self._composed = self.weights8 or config.rope_theta is not None or config.qk_norm
         self._geom = PadGeometry(config.d_model, config.num_heads, config.ffn_dim)
         # Construction order = BaselineTransformer's (TTB:153-161).
         self.layers = nn.ModuleList(
-            [CobraTransformerBlock(config.d_model, config.num_heads, config.ffn_dim)
+            [CobraTransformerBlock(config.d_model, config.num_heads, config.ffn_dim, config.qk_norm)
              for _ in range(config.num_layers)]
         )
         self.final_norm = nn.LayerNorm(config.d_model)
@@ -133,6 +175,7 @@ class CobraTransformer(nn.Module):
         self._packs: Optional[List[_BlockPack]] = None
         self._op = torch.float16  # operand type of the packs
         self._final = None
+        self._inv_freq: Optional[torch.Tensor] = None
         self._versions = None
         self._sig = None
         self._graph_ok = False
@@ -163,7 +206,10 @@ class CobraTransformer(nn.Module):
         if not ready:
             if not self.final_norm.weight.is_cuda:
                 raise RuntimeError("CobraTransformer runs on the GPU only: move it with .to('cuda')")
-            self._packs = [_BlockPack(blk, self._geom, op) for blk in self.layers]
+            self._packs = [_BlockPack(blk, self._geom, op, self.weights8) for blk in self.layers]
+            if self.config.rope_theta is not None:
+                turn = torch.arange(0, self._geom.hd, 2, dtype=torch.float64) / self._geom.hd
+                self._inv_freq = (float(self.config.rope_theta) ** -turn).float().to(self.final_norm.weight.device)
             self._op = op
             with torch.no_grad():
                 self._final = (self.final_norm.weight.float().contiguous(), self.final_norm.bias.float().contiguous())
@@ -195,7 +241,7 @@ class CobraTransformer(nn.Module):
             # block); launch the one-kernel-per-block forward directly, which measured
             # faster than its graph replay at B >= 4 (56 vs 62 us at case 1).
             cfg = self.config
-            blocks = x.dtype != torch.bfloat16 and \
+            blocks = x.dtype != torch.bfloat16 and not self._composed and \
                 ops.block_plan(x.shape[0], x.shape[1], cfg.d_model, cfg.num_heads, cfg.ffn_dim) == 1
             self._graph_ok = (self.graph if self.graph is not None else not blocks) and \
                 x.numel() * x.element_size() <= GRAPH_MAX_INPUT_BYTES
@@ -260,10 +306,10 @@ class CobraTransformer(nn.Module):
         out16 = x.dtype == torch.float16
         n = len(packs)
         bf16 = x.dtype == torch.bfloat16
-        if not bf16 and ops.block_plan(B, S, D, H, cfg.ffn_dim) == 1:
+        if not bf16 and not self._composed and ops.block_plan(B, S, D, H, cfg.ffn_dim) == 1:
             return self._run_blocks(x, m, packs).view(B, S, D)
         bits = None if m is None else ops.mask_bits(m.view(B, S))
-        if self._geom.needed or bf16:
+        if self._geom.needed or bf16 or self._composed:
             # bf16: the same per-op composition with bf16 operands (the LayerNorm-epilogue
             # GEMMs, LN1-in-prologue projection and fused kernels are fp16-operand)
             return self._run_padded(x, m, mrow, bits, packs).view(B, S, D)
@@ -330,18 +376,27 @@ class CobraTransformer(nn.Module):
         for i, p in enumerate(packs):
             last = i == n - 1
             nw, nb = self._final if last else (packs[i + 1].ln1_w, packs[i + 1].ln1_b)
-            qkv = ops.linear(h, p.w_qkv, p.b_qkv)
+            qkv = _linear(h, p.w_qkv, p.b_qkv)
+            self._norm_rotate(qkv, p, seq_len=S)
             ctx = ops.attn(qkv, B, S, cfg.num_heads, g.hdp, scale, causal=cfg.causal, key_bits=bits)
-            r = ops.linear(ctx, p.w_o, p.b_o, out_fp32=True, resid=r, rmask=mrow, mask_branch=True)
+            r = _linear(ctx, p.w_o, p.b_o, out_fp32=True, resid=r, rmask=mrow, mask_branch=True)
             h2 = ops.ln_strided(r, D, p.ln2_w, p.ln2_b, out_cols=g.dp, out_dtype=op, eps=eps)
-            hid = ops.linear(h2, p.w1, p.b1, gelu=True)
-            r = ops.linear(hid, p.w2, p.b2, out_fp32=True, resid=r, rmask=mrow)
+            hid = _linear(h2, p.w1, p.b1, gelu=True)
+            r = _linear(hid, p.w2, p.b2, out_fp32=True, resid=r, rmask=mrow)
             if last:
                 h = ops.ln_strided(r, D, nw, nb, out_cols=D, out_dtype=x.dtype, mask_row=mrow,
                                    mask_resid=mrow is not None, mask_out=mrow is not None, eps=eps)
             else:
                 h = ops.ln_strided(r, D, nw, nb, out_cols=g.dp, out_dtype=op, eps=eps)
         return h
+
+    def _norm_rotate(self, qkv: torch.Tensor, p: _BlockPack, positions: Optional[torch.Tensor] = None,
+                     seq_len: Optional[int] = None) -> None:
+        """The norms of queries and keys and their rotation, where the model has them, in place."""
+        if p.q_norm is not None or self._inv_freq is not None:
+            g = self._geom
+            ops.qk_norm_rope(qkv, g.heads, g.heads, g.hd, positions=positions, inv_freq=self._inv_freq, q_weight=p.q_norm,
+                             k_weight=p.k_norm, eps=p.qk_eps, pitch=g.hdp, seq_len=seq_len)
 
     def _run_blocks(self, x: torch.Tensor, m: Optional[torch.Tensor], packs: List[_BlockPack]) -> torch.Tensor:
         """One launch per block (``cobra_block_fwd``) for the shapes the whole-block kernel
@@ -377,7 +432,8 @@ class CobraTransformer(nn.Module):
                           block_size, dtype, max_len, self.final_norm.weight.device)
 
     def extend(self, x: torch.Tensor, cache: CobraCache, new_lens: torch.Tensor, max_new: Optional[int] = None,
-               max_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+               max_len: Optional[int] = None, prefix: Optional[int] = None,
+               max_prefix: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The causal stack over new tokens of the requests in ``cache`` -> ``(y, missing)``.
 
         x: [T, d_model], request b's ``new_lens[b]`` (int32 device tensor) tokens after those of
@@ -389,6 +445,13 @@ class CobraTransformer(nn.Module):
         to the lengths before gives it back.  ``max_new`` / ``max_len``: expected bounds on a request's
         new tokens and length (speed only).  Every launch is the library's own, with the ops of the
         composed forward.
+
+        ``prefix``: the row of a request that all others of this call go on from (a shared prompt, put
+        into its row by an ``extend`` of its own): their tokens stand behind its tokens and attend
+        over them, and it is held and read once (``ops.cache_prefix_attn``).  ``y`` is then what
+        ``forward`` gives for the prefix's tokens and theirs in one sequence.  The prefix has to stay as it is while
+        requests that go on from it live; requests without it need a call without ``prefix``, with 0 in
+        ``new_lens`` for the others.  ``max_prefix``: its expected length (speed only).
 
         A step can be captured in a graph once the model has run with activations of x's type and
         its present parameters (it lays its weights out then, which must not become part of the
@@ -414,14 +477,17 @@ class CobraTransformer(nn.Module):
                                "weights are laid out for the kernels then")
         packs = self._packed(x.dtype)
         if capturing:
-            cache.hold(packs, self._final)
+            cache.hold(packs, self._final, self._inv_freq)
         op = self._op
         x = x.contiguous()
         T, D = x.shape
         H, eps, scale = cfg.num_heads, self.final_norm.eps, g.hd ** -0.5
+        if prefix is not None and not 0 <= prefix < cache.lens.shape[0]:
+            raise ValueError(f"prefix must be a row of the cache, 0 .. {cache.lens.shape[0] - 1}, got {prefix}")
         slots, cu, missing = cache.reserve(new_lens, T)
         if T == 0:
             return torch.empty_like(x), missing
+        positions = cache.positions(cu, T, prefix) if self._inv_freq is not None else None
         r = torch.zeros((T, g.dp), device=x.device, dtype=torch.float32)
         ctx = torch.zeros((T, g.e), device=x.device, dtype=op)  # rows of no request stay zero
         h = ops.ln_strided(x, D, packs[0].ln1_w, packs[0].ln1_b, out_cols=g.dp, out_dtype=op, resid_out=r, eps=eps)
@@ -429,13 +495,15 @@ class CobraTransformer(nn.Module):
         for i, p in enumerate(packs):
             last = i == n - 1
             nw, nb = self._final if last else (packs[i + 1].ln1_w, packs[i + 1].ln1_b)
-            qkv = ops.linear(h, p.w_qkv, p.b_qkv)
+            qkv = _linear(h, p.w_qkv, p.b_qkv)
+            self._norm_rotate(qkv, p, positions=positions)
             cache.append(i, qkv, slots, H)
-            cache.attn(i, qkv, cu, H, scale, max_new=max_new, max_len=max_len, out=ctx)
-            r = ops.linear(ctx, p.w_o, p.b_o, out_fp32=True, resid=r)
+            cache.attn(i, qkv, cu, H, scale, max_new=max_new, max_len=max_len, out=ctx, prefix=prefix,
+                       max_prefix=max_prefix)
+            r = _linear(ctx, p.w_o, p.b_o, out_fp32=True, resid=r)
             h2 = ops.ln_strided(r, D, p.ln2_w, p.ln2_b, out_cols=g.dp, out_dtype=op, eps=eps)
-            hid = ops.linear(h2, p.w1, p.b1, gelu=True)
-            r = ops.linear(hid, p.w2, p.b2, out_fp32=True, resid=r)
+            hid = _linear(h2, p.w1, p.b1, gelu=True)
+            r = _linear(hid, p.w2, p.b2, out_fp32=True, resid=r)
             h = ops.ln_strided(r, D, nw, nb, out_cols=D if last else g.dp, out_dtype=x.dtype if last else op, eps=eps)
         return h, missing
 

@@ -800,6 +800,7 @@ def qk_norm_rope(
     interleaved: bool = False,
     eps: float = 1e-6,
     pitch: Optional[int] = None,
+    seq_len: Optional[int] = None,
 ) -> None:
     """Root-mean-square norms of queries and keys for each head and their rotation by position, in
     place and in one pass.
@@ -809,11 +810,12 @@ def qk_norm_rope(
     keys is left as it is).  ``q_weight`` and ``k_weight`` [head_dim]: ``x / sqrt(mean(x^2) + eps) *
     weight`` for each head; both or neither.  ``inv_freq`` [r]: the first 2 r columns turn by
     ``positions[t] * inv_freq[i]``, pairs (i, i + r) or, ``interleaved``, (2 i, 2 i + 1); ``positions``
-    [T] int32, tokens at negative ones are left as they are.  fp32 arithmetic (angles in 64 bits), one
+    [T] int32, tokens at negative ones are left as they are; or ``seq_len``, for whole sequences one
+    after the other: token t stands at ``t % seq_len``.  fp32 arithmetic (angles in 64 bits), one
     rounding.
     """
     if _lib.host().qk_norm_rope(qkv, heads, kv_heads, head_dim, positions, inv_freq, q_weight, k_weight, interleaved,
-                                eps, pitch):
+                                eps, pitch, seq_len):
         return
     if qkv.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
@@ -831,10 +833,12 @@ def qk_norm_rope(
     if inv_freq is not None:
         if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or 2 * inv_freq.shape[0] > head_dim:
             raise ValueError(f"inv_freq must be float32 [<= {head_dim // 2}], got {inv_freq.dtype} {list(inv_freq.shape)}")
-        if positions is None:
-            raise ValueError("inv_freq needs positions")
+        if positions is None and seq_len is None:
+            raise ValueError("inv_freq needs positions or seq_len")
         rot = 2 * inv_freq.shape[0]
         given["inv_freq"] = inv_freq
+    if seq_len is not None and (positions is not None or not 0 < seq_len <= 0x7FFFFFFF):
+        raise ValueError(f"seq_len must be positive and without positions, got {seq_len}")
     if positions is not None:
         _i32(positions, (T,), "positions")
         given["positions"] = positions
@@ -845,8 +849,8 @@ def qk_norm_rope(
     if q_weight is not None:
         qw, kw = _f32_param(q_weight, head_dim, "q_weight"), _f32_param(k_weight, head_dim, "k_weight")
         _same_dev(dev, q_weight=qw, k_weight=kw)
-    _call_on(dev, "cobra_qk_norm_rope", qkv.data_ptr(), _DT[qkv.dtype], qkv.shape[1], _ptr(positions), _ptr(inv_freq),
-             rot, 1 if interleaved else 0, _ptr(qw), _ptr(kw), float(eps), T, heads, kv_heads, head_dim, pitch)
+    _call_on(dev, "cobra_qk_norm_rope", qkv.data_ptr(), _DT[qkv.dtype], qkv.shape[1], _ptr(positions), seq_len or 0,
+             _ptr(inv_freq), rot, 1 if interleaved else 0, _ptr(qw), _ptr(kw), float(eps), T, heads, kv_heads, head_dim, pitch)
 
 
 def width8(k: int) -> Tuple[int, int]:

@@ -654,20 +654,20 @@ int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* posit
 
 // -- norms and rotation of queries and keys --------------------------------------------------
 
-int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, const float* inv_freq, int64_t rot,
-                       int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
+int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, int64_t seq_len,
+                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
                        int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream) {
   if (!is_op_dtype(dtype) || tokens < 0 || tokens > 0x7fffffff || heads <= 0 || heads > 0x7fffff || kv_heads <= 0 ||
       kv_heads > 0x7fffff || head_dim <= 0 || head_dim > 256 || pitch < head_dim || pitch > 0x7fffff || rot < 0 ||
-      rot % 2 || rot > head_dim || ld < (heads + kv_heads) * pitch || !(eps >= 0.f) ||
+      rot % 2 || rot > head_dim || seq_len < 0 || seq_len > 0x7fffffff || ld < (heads + kv_heads) * pitch || !(eps >= 0.f) ||
       (q_weight == nullptr) != (k_weight == nullptr))
     return kBad;
   if (tokens == 0 || (rot == 0 && !q_weight)) return 0;
-  if (!qkv || !aligned_to(qkv, 2) || (rot && (!positions || !inv_freq)) || !aligned_to(positions, 4) ||
+  if (!qkv || !aligned_to(qkv, 2) || (rot && ((!positions && !seq_len) || !inv_freq)) || !aligned_to(positions, 4) ||
       !aligned_to(inv_freq, 4) || !aligned_to(q_weight, 4) || !aligned_to(k_weight, 4))
     return kBad;
-  const cobra::QkNormRopeArgs a{qkv, positions, inv_freq, q_weight, k_weight, tokens, ld, (int)heads, (int)kv_heads,
-                                (int)head_dim, (int)pitch, (int)rot, interleaved ? 1 : 0, dtype, eps};
+  const cobra::QkNormRopeArgs a{qkv, positions, inv_freq, q_weight, k_weight, tokens, ld, seq_len, (int)heads,
+                                (int)kv_heads, (int)head_dim, (int)pitch, (int)rot, interleaved ? 1 : 0, dtype, eps};
   return code(cobra::run_qk_norm_rope(a, static_cast<hipStream_t>(stream)));
 }
 
@@ -681,11 +681,12 @@ namespace {
 int64_t codes_of(int64_t K) { return (K + 127) & ~int64_t(127); }
 int64_t scales_of(int64_t K) { return (K + 511) / 512 * 4; }
 constexpr int64_t kMaxK = 0x7fff00;
+constexpr int64_t kMaxUnits = 0xffffff0;  // rows times 512 columns: a launch of as many workgroups as there may be
 
 }  // namespace
 
 int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_t M, int64_t K, void* stream) {
-  if (!is_act_dtype(x_dtype) || M < 0 || M > 0x7fffffff || K <= 0 || K > kMaxK || M * scales_of(K) / 4 > 0x7fffffff)
+  if (!is_act_dtype(x_dtype) || M < 0 || M > 0x7fffffff || K <= 0 || K > kMaxK || M * scales_of(K) / 4 > kMaxUnits)
     return kBad;
   if (M == 0) return 0;
   if (!x || !codes || !scale || !aligned_to(x, dtype_bytes(x_dtype)) || !aligned16(codes) || !aligned_to(scale, 4))
@@ -697,8 +698,8 @@ int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_
 }
 
 int64_t cobra_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_dtype) {
-  if (!(is_op_dtype(a_dtype) || a_dtype == COBRA_E4M3) || M < 0 || M > 0x7fffffff || N <= 0 || N > 0x7ffffff || K <= 0 ||
-      K > kMaxK || M * scales_of(K) / 4 > 0x7fffffff)
+  if (!(is_op_dtype(a_dtype) || a_dtype == COBRA_E4M3) || M < 0 || M > 0x7fffffff || N <= 0 || N > 0x7fffff0 || K <= 0 ||
+      K > kMaxK || M * scales_of(K) / 4 > kMaxUnits)
     return -1;
   return M == 0 ? 0 : cobra::linear8_workspace_bytes(M, K, a_dtype);
 }

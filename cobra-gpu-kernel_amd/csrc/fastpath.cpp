@@ -493,17 +493,18 @@ int act_code(at::ScalarType t) {
 }
 
 // (qkv, heads, kv_heads, head_dim, positions | None, inv_freq | None, q_weight | None, k_weight | None,
-// interleaved, eps, pitch | None) -> True | None
+// interleaved, eps, pitch | None, seq_len | None) -> True | None
 PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     int dt;
-    int64_t heads, kv, hd, pitch;
-    const at::Tensor* x = n == 11 ? rows16(a[0], &dt) : nullptr;
+    int64_t heads, kv, hd, pitch, seq = 0;
+    const at::Tensor* x = n == 12 ? rows16(a[0], &dt) : nullptr;
     if (!x || !py_int(a[1], &heads) || !py_int(a[2], &kv) || !py_int(a[3], &hd) || !PyBool_Check(a[8]) ||
         !PyFloat_Check(a[9]))
       return none();
     pitch = hd;
     if (a[10] != Py_None && !py_int(a[10], &pitch)) return none();
+    if (a[11] != Py_None && (!py_int(a[11], &seq) || seq <= 0 || seq > 0x7fffffff || a[4] != Py_None)) return none();
     const int dev = x->device().index();
     const int64_t T = x->size(0);
     const at::Tensor *qw, *kw, *freq = nullptr, *pos = nullptr;
@@ -515,13 +516,13 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (a[5] != Py_None) {
       freq = dev_tensor(a[5], dev, at::kFloat);
-      if (!freq || freq->dim() != 1 || !pos) return none();
+      if (!freq || freq->dim() != 1 || (!pos && !seq)) return none();
       rot = 2 * freq->size(0);
     }
     if (heads <= 0 || kv <= 0 || heads > 0x7fffff || kv > 0x7fffff || pitch < hd || pitch > 0x7fffff || rot > hd ||
         x->size(1) < (heads + kv) * pitch || !(PyFloat_AS_DOUBLE(a[9]) >= 0.0))
       return none();
-    const int code = cobra_qk_norm_rope(x->data_ptr(), dt, x->size(1), pos ? pos->data_ptr<int>() : nullptr,
+    const int code = cobra_qk_norm_rope(x->data_ptr(), dt, x->size(1), pos ? pos->data_ptr<int>() : nullptr, seq,
                                         f32_or_null(freq), rot, a[8] == Py_True ? 1 : 0, f32_or_null(qw),
                                         f32_or_null(kw), static_cast<float>(PyFloat_AS_DOUBLE(a[9])), T, heads, kv, hd,
                                         pitch, c10::hip::getCurrentHIPStream(dev).stream());

@@ -439,10 +439,10 @@ hipError_t run_linear8(const Linear8Args& a, int64_t workspace_bytes, hipStream_
 // Norms and rotation of packed queries and keys in place (rope.hip).
 struct QkNormRopeArgs {
   void* qkv;                 // [tokens, ld], heads `pitch` columns apart
-  const int32_t* positions;  // [tokens], or null without rotation
+  const int32_t* positions;  // [tokens], or null: token t stands at t % seq_len
   const float* inv_freq;     // [rot / 2]
   const float *q_weight, *k_weight;  // [head_dim], or null without norms
-  int64_t tokens, ld;
+  int64_t tokens, ld, seq_len;
   int heads, kv_heads, head_dim, pitch, rot, interleaved, dtype;
   float eps;
 };

@@ -673,7 +673,7 @@ int64_t linear8_workspace_bytes(int64_t M, int64_t K, int a_dtype) {
 hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t kp = (c.K + 127) & ~int64_t(127), s = (c.K + 511) / 512 * 4;
   // Offsets inside a tile's rows are 32 bits wide.
-  if (c.M <= 0 || c.N <= 0 || c.N > 0x7ffffff || kp > 0x7fffff || c.M > 0x7fffffff) return hipErrorInvalidValue;
+  if (c.M <= 0 || c.N <= 0 || c.N > 0x7fffff0 || kp > 0x7fffff || c.M > 0x7fffffff) return hipErrorInvalidValue;
   Args a{c.a, c.a_scale, c.w, c.w_scale, c.bias, c.resid, c.row_mask, c.c, c.M, (int)c.N, (int)c.K, (int)kp, (int)s,
          c.resid_dtype, c.c_dtype, c.epi};
   const bool codes = c.a_dtype == kE4M3;

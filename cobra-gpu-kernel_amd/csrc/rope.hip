@@ -28,7 +28,7 @@ struct Args {
   void* qkv;
   const int32_t* positions;
   const float *inv_freq, *q_weight, *k_weight;
-  int64_t tokens, ld;
+  int64_t tokens, ld, seq_len;
   int heads, all;       // query heads; query and key heads
   int dim, pitch, half; // columns of a head, from a head to the next, and half of those that turn
   int lanes;            // of a head
@@ -52,6 +52,9 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
+__device__ __forceinline__ int position_of(const Args& a, int64_t t) {
+  return a.positions ? a.positions[t] : a.seq_len ? (int)(t % a.seq_len) : 0;
+}
 // (cos, sin) of a position times frequency i.
 __device__ __forceinline__ float2 turn_of(const Args& a, int pos, int i) {
   const double x = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189535);  // 1 / 2 pi
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
   };
   const uint32_t mine = tid / a.lanes;
   // The positions first: loads come back in order, and the angles need nothing else.
-  const int at = tid < count && a.positions ? a.positions[t0 + tid] : 0;
+  const int at = tid < count ? position_of(a, t0 + tid) : 0;
   ask(mine);
   if (tid < count) place[tid] = at;
   float wq[2][V], wk[2][V];
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(Args a, int inter
   __shared__ float2 turn[kMaxDim / 2];
   const int lane = threadIdx.x & 63;
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int pos = a.positions ? a.positions[t] : 0;
+    const int pos = position_of(a, t);
     if (pos < 0) continue;
     __syncthreads();
     for (int i = threadIdx.x; i < a.half; i += 256) turn[i] = turn_of(a, pos, i);
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256) void cache_positions_kernel(const int32_t* __r
 
 hipError_t run_qk_norm_rope(const QkNormRopeArgs& c, hipStream_t stream) {
   if (c.head_dim <= 0 || c.head_dim > kMaxDim || c.rot < 0 || c.rot % 2 || c.rot > c.head_dim) return hipErrorInvalidValue;
-  const Args a{c.qkv, c.positions, c.inv_freq, c.q_weight, c.k_weight, c.tokens, c.ld, c.heads, c.heads + c.kv_heads,
+  const Args a{c.qkv, c.positions, c.inv_freq, c.q_weight, c.k_weight, c.tokens, c.ld, c.seq_len, c.heads, c.heads + c.kv_heads,
                c.head_dim, c.pitch, c.rot / 2, 0, c.eps};
   return c.dtype == kF16 ? launch_type<f16>(a, c.interleaved, stream) : launch_type<bf16>(a, c.interleaved, stream);
 }

@@ -292,11 +292,11 @@ int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* posit
  * qkv: [tokens, ld] in dtype (COBRA_F16 or COBRA_BF16, element alignment suffices): heads query
  * heads, then kv_heads key heads, each head_dim columns, pitch columns apart (ld >= (heads +
  * kv_heads) * pitch); other columns are left as they are.  head_dim <= 256, rot even and at most
- * head_dim, 0 for no rotation (positions and inv_freq may then be NULL).  Tokens with a negative
- * position are left as they are.  fp32 arithmetic, angles in 64 bits, one rounding.
+ * head_dim, 0 for no rotation (inv_freq may then be NULL).  positions NULL: token t stands at t %
+ * seq_len (which rotation needs then).  Tokens with a negative position are left as they are.  fp32 arithmetic, angles in 64 bits, one rounding.
  */
-int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, const float* inv_freq, int64_t rot,
-                       int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
+int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, int64_t seq_len,
+                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
                        int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream);
 
 /*
@@ -305,7 +305,7 @@ int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* position
  * past Kp / 128.  Of a block whose largest finite magnitude is a, the scale is the least power of
  * two >= 2^-126 with a <= 448 scale, and codes are the nearest e4m3 values of x / scale (ties to
  * even); what is not finite becomes NaN.  x: [M, K] in any of the three types (element alignment
- * suffices); K <= 8388352; M ceil(K / 512) < 2^31; no buffer may overlap another.
+ * suffices); K <= 8388352; M ceil(K / 512) <= 268435440; no buffer may overlap another.
  */
 int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_t M, int64_t K, void* stream);
 
@@ -317,7 +317,7 @@ int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_
  * [M, Kp] (COBRA_E4M3) with a_scale [M, S]; w, w_scale: codes [N, Kp] and scales [N, S] of the
  * weight in nn.Linear's layout.  bias: [N] fp32 (optional); resid (optional) and c: [M, N] in any
  * of the three types each (resid may be c itself in c's type; c overlaps nothing else).  Sums are
- * fp32.  N <= 134217727.  COBRA_EPI_MASK_OUT is rejected.  workspace:
+ * fp32.  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is rejected.  workspace:
  * cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0), which
  * launches that overlap must not share.
  */
