@@ -162,23 +162,34 @@ struct PrefixPlan {
   bool both;  // one pass over the prefix and the request's own keys
 };
 
-// How the prefix's pass is cut: as a call of one request with all of the tokens, but for the splits.
-// In tiles of 128 rows as many as give three quarters of the chip's places (two workgroups a CU up to
-// head_dim 128) a workgroup, so that the requests' own keys, which are bound by memory, have
-// the rest from the start: 128 requests of up to 2000 keys behind 30000, 32 heads of 128 on 8, take 140 us with
-// 384 workgroups, 168 and 157 with 256 and 512; alone the passes take 88 (with 512) and 63.  (Own ones evenly
-// between the prefix's: 182 us; behind them in all of these.)  Few keys a split cost the join
-// little: 23 drafts of 2 to 6 tokens behind 4001 keys, 6 heads of 256 on 2, take 79 us with splits of 1024
-// keys, 50 with 512, 37 with 256 and 35 with 128.
-CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_prefix) {
+// How the prefix's pass is cut: as a call of one request with all of the tokens, but for the splits and
+// the kernel.
+// Rows pass over the keys by direct loads, in tiles of 16, while that is little work in all (rows x keys x
+// head_dim of all kv heads): tiles of 128 take long to start and leave the chip empty.  23 drafts
+// of 2 to 6 tokens behind 4001 keys, 6 heads of 256 on 2: 29 us against 39; 64 requests behind 4000, 32
+// heads of 128 on 8, 30 and 36, 128 so 47 and 48 (2^31), 64 behind 16000 61 and 57, 128 behind 30000 205 and
+// 137; 1024 behind 4000, 8 heads of 64, 92 and 118.  A workgroup a CU then: with two 30, 33, 51, 65, 222
+// and 92; two where the splits are of hardly any rows (one request behind 99999, 16 heads of 64 on 2: 16.8 us
+// against 19.4).
+// In tiles of 128 rows as many splits as give three quarters of the chip's places (two workgroups a CU up
+// to head_dim 128) a workgroup, so that the requests' own keys, which are bound by memory, have the rest
+// from the start: 128 requests of up to 2000 keys behind 30000, 32 heads of 128 on 8, take 135 to 147 us with
+// 384 workgroups, 166 and 152 with 256 and 480; alone the passes take 88 (with 512) and 63.  (Own ones evenly
+// between the prefix's: 182 us; behind them in all of these.)
+CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_prefix,
+                   bool own_chunked) {
   CachePlan p = cache_plan(tokens, 1, heads, kv_heads, head_dim, tokens, max_prefix);
+  const int width = cache_width(head_dim);
   max_prefix = max_prefix < 1 ? 1 : max_prefix > kMaxKeys ? kMaxKeys : max_prefix;
-  const int64_t units = (p.chunked ? (tokens * (heads / kv_heads) + 127) / 128 : p.row_tiles) * kv_heads;
+  const int64_t rows = tokens * (heads / kv_heads);
+  if (p.chunked && !own_chunked && rows * kv_heads * width <= ((int64_t)1 << 31) / max_prefix) {
+    p.chunked = false;
+    p.row_tiles = (rows + 15) / 16;
+    p.step = 4 * decode_keys(width);
+  }
+  const int64_t units = (p.chunked ? (rows + 127) / 128 : p.row_tiles) * kv_heads;
   const int64_t least = p.chunked ? 128 : p.step, room = kMaxParts / (tokens * heads);
-  // Few rows (direct loads): a workgroup a CU, 32 requests of one token behind 6000, 16 heads of 64,
-  // 18.6 us against 21.1 with two, 8 behind 4000 with 32 heads of 128 on 8 15.8 and 17.8; two where the splits
-  // are of hardly any rows (one behind 99999, 16 heads of 64 on 2: 16.8 us against 19.4).
-  const int64_t target = !p.chunked ? (units <= 4 ? 512 : 256) : cache_width(head_dim) <= 128 ? 384 : 192;
+  const int64_t target = !p.chunked ? (units <= 4 ? 512 : 256) : width <= 128 ? 384 : 192;
   int64_t splits = p.chunked ? (target + units / 2) / units : (target + units - 1) / units;
   // A little more than a workgroup a CU leaves most CUs with one: thirds fill two rounds.  16 prompts of
   // 64 to 256 tokens behind 16000, 16 heads of 64 on 4 (320 units): 318 us against 392 in one pass, 4 of
@@ -210,8 +221,8 @@ CachePlan own_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
 PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                    int64_t max_len, int64_t max_prefix) {
   PrefixPlan p;
-  p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix);
   p.own = own_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
+  p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own.chunked);
   // (8 prompts of 1000 to 2000 tokens behind 8000, 32 heads of 128 on 8: 2037 us in one pass, 2380 joined.)
   p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
   return p;
