@@ -12,7 +12,7 @@
 //   meet in fp32): 4e-5 of a result in the root mean square.  An fp16 result's own rounding is 2e-4, a
 //   bf16's 1.6e-3, an fp32's 3e-8: fp32 results take the exact kind.
 //
-// Two kernels.  Up to 32 rows of A the weights' bytes are all that counts: linear8_few_kernel
+// Two kernels.  Up to 16 rows of A the weights' bytes are all that counts: linear8_few_kernel
 // (exact) has 16 or more rows of W a workgroup, split along K over its waves, and takes 16-bit
 // activations as they are, quantising them in the registers that the product reads.  More rows go
 // through tiles in LDS.
@@ -162,19 +162,19 @@ struct RowBlock<uint8_t> {
   }
 };
 
-// MT sets of 16 rows of A, NT of W for a workgroup of eight waves, each with every eighth block of K.
+// A workgroup has NT sets of 16 rows of W, its eight waves every eighth block of K each.
 //
 // Bound by memory behind a launch's and a first load's latency: 8192 x 4096 weights take 10.8 us with
 // one row (9.9 as codes), 3.1 TB/s in all, where the bytes alone are 6.6 us at a copy's rate; 12.4 with 16
 // rows.  32 rows of W a workgroup where that still gives every CU one, 16 otherwise: each workgroup reads and
 // quantises all of A (16 rows, 8192 x 4096: 12.4 us against 16.2 with 16; 4096 x 8192: 16.0 against
 // 20.9 with 32).  Several blocks' loads asked for together gained nothing (12.4 to 14.9 us, 16.0 to 16.8),
-// nor did 16 waves (12.6, 16.3).  From 33 rows on quantising once and a tile kernel are faster: 64 rows
-// 19 us against 28.
-template <typename TA, int MT, int NT>
+// nor did 16 waves (12.6, 16.3).  From 17 rows on quantising once and a tile kernel are faster: 32 rows
+// 13 us against 16.8, 64 rows 15 against 28.
+template <typename TA, int NT>
 __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
   constexpr int kWaves = 8;
-  __shared__ f32x4 part[kWaves][NT * MT][64];
+  __shared__ f32x4 part[kWaves][NT][64];
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16 * NT;
@@ -186,51 +186,38 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
     w[t] = a.w + n * a.kp + 16 * g;
     ws[t] = a.w_scale + n * a.s;
   }
-  f32x4 acc[NT][MT];
+  f32x4 acc[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int j = wave; j < blocks; j += kWaves) {
     i32x8 c[NT];
     uint32_t wb[NT];
-    RowBlock<TA> x[MT];
+    RowBlock<TA> x;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       c[t] = join8(*reinterpret_cast<const i32x4*>(w[t] + 128 * j), *reinterpret_cast<const i32x4*>(w[t] + 128 * j + 64));
       wb[t] = ws[t][j];
     }
+    x.load(a, r, r < a.M, j, g);
+    float row_scale;
+    const i32x8 q = x.codes(row_scale);
+    bf16x8 y[4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x[i].load(a, 16 * i + r, 16 * i + r < a.M, j, g);
-    bf16x8 y[MT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float scale;
-      const i32x8 q = x[i].codes(scale);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) y[i][k] = widen(q[2 * k], q[2 * k + 1], scale);
-    }
+    for (int k = 0; k < 4; ++k) y[k] = widen(q[2 * k], q[2 * k + 1], row_scale);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float scale = scale_of(wb[t]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bf16x8 z = widen(c[t][2 * k], c[t][2 * k + 1], scale);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[t][i] = mfma16(z, y[i][k], acc[t][i]);
-      }
+      for (int k = 0; k < 4; ++k) acc[t] = mfma16(widen(c[t][2 * k], c[t][2 * k + 1], scale), y[k], acc[t]);
     }
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) part[wave][t * MT + i][lane] = acc[t][i];
+  for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
   __syncthreads();
   // A thread has four columns of a row: the waves' shares in their order.
-  for (int q = threadIdx.x; q < NT * MT * 64; q += kWaves * 64) {
+  for (int q = threadIdx.x; q < NT * 64; q += kWaves * 64) {
     const int tile = q >> 6, l = q & 63;
-    const int m = 16 * (tile % MT) + (l & 15);
-    const int n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
+    const int m = l & 15, n = n0 + 16 * tile + 4 * (l >> 4);
     if (m >= a.M || n >= a.N) continue;
     f32x4 v = part[0][tile][l];
 #pragma unroll
@@ -277,18 +264,26 @@ __device__ __forceinline__ void dma4_untracked(const void* src, uint32_t lds) {
 
 // A tile of BM x BN by WM x WN waves; a k-tile is one block of 128 columns.  A stage of LDS holds
 // the rows' codes (A's, then W's), 128 bytes each with 16-byte chunks swizzled by row as in the
-// 16-bit kernel, and behind them the rows' words of four scale bytes.
-template <int BM, int BN, int WM, int WN, int ST>
+// 16-bit kernel, and behind them the rows' words of four scale bytes.  KS groups of such waves have a
+// k-tile each at a time, with stages of their own, and are added at the end.
+//
+// Large tiles are bound by the matrix cores (8192^3 2635 TFLOP/s of 4600 that the instruction reaches by
+// itself, with the clock that such a load leaves), small ones by how much a CU has in flight: a CU alone
+// takes in some 21 GB/s from memory, so few rows want as many workgroups as there are CUs, and two groups
+// of waves in each.  64 rows, 4096 x 4096 weights take 8.4 us in tiles of 64 x 32 and two groups, 9.3 with
+// one, 11.7 in 64 x 64, 11.0 there with two groups; 64 rows, 8192 x 4096 12.1, 12.6, 15.9 and 16.2.
+template <int BM, int BN, int WM, int WN, int ST, int KS>
 struct Tile {
-  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int NW = WM * WN, NT = NW * KS * 64;  // waves of a group, threads
   static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
   static constexpr int ROWS = BM + BN;
-  static constexpr int STAGE = ROWS * 132;
+  static constexpr int SCALES = (ROWS + 63) / 64;  // transfers of 64 rows' scale words
+  static constexpr int PART = ROWS * 128 + SCALES * 256, STAGE = PART * KS;
   static constexpr int LPT = ROWS / 8 / NW;     // transfers of 8 rows' codes a wave and k-tile; one more of scales
   static constexpr int EPW = WN * 32, LDC = EPW + 4;
   static constexpr int EPI_LDS = BM * LDC * 4;
   static constexpr int LDS = ST * STAGE > EPI_LDS ? ST * STAGE : EPI_LDS;
-  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && BM % 64 == 0 && BN % 64 == 0, "wave tile");
+  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && BM % 64 == 0 && BN % 32 == 0, "wave tile");
   static_assert(ROWS / 8 % NW == 0, "every wave issues the same number of transfers");
   static_assert(LDS <= 163840, "LDS budget");
   static_assert(TN <= 4, "slices of the epilogue");
@@ -296,15 +291,16 @@ struct Tile {
 
 __device__ __forceinline__ int chunk_swz(int row) { return (row >> 1) & 7; }
 
-template <int BM, int BN, int WM, int WN, int ST, bool EXACT>
+template <int BM, int BN, int WM, int WN, int ST, int KS, bool EXACT>
 __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char* smem,
                                          f32x16 (&acc)[BN / WN / 32][BM / WM / 32]) {
-  using T = Tile<BM, BN, WM, WN, ST>;
+  using T = Tile<BM, BN, WM, WN, ST, KS>;
   constexpr int NW = T::NW, LPT = T::LPT;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW;
   const int wm = wave / WN, wn = wave % WN;
   const int li = lane & 31, g = lane >> 5;
+  smem += group * T::PART;  // of each stage
   const uint8_t* A = static_cast<const uint8_t*>(a.a) + m0 * a.kp;
   const uint8_t* W = a.w + (int64_t)n0 * a.kp;
   // Rows past M or N are the last one: their products are never stored.
@@ -316,18 +312,20 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
     const int64_t at = row < BM ? min(m0 + row, a.M - 1) - m0 : (int64_t)min(n0 + row - BM, a.N - 1) - n0;
     src_off[i] = (unsigned)(at * a.kp + chunk * 16);
   }
-  const int srow = 64 * (wave % (T::ROWS / 64)) + lane;
+  const int srow = min(64 * (wave % T::SCALES) + lane, T::ROWS - 1);
   const uint8_t* scales = srow < BM ? a.a_scale + min(m0 + srow, a.M - 1) * a.s
                                     : a.w_scale + (int64_t)min(n0 + srow - BM, a.N - 1) * a.s;
   const uint32_t lds0 = lds_addr(smem);
   constexpr int kAll = LPT + 1;  // transfers a wave and k-tile
-  // Transfer i of k-tile kt to its stage.
-  auto transfer = [&](int kt, int i) {
-    const uint32_t dst = lds0 + (kt % ST) * T::STAGE;
+  const int KT = a.kp >> 7, steps = (KT + KS - 1) / KS;
+  // Transfer i of this group's k-tile of a step to its stage (where there is none, of the last).
+  auto transfer = [&](int step, int i) {
+    const uint32_t dst = lds0 + (step % ST) * T::STAGE;
+    const int kt = min(step * KS + group, KT - 1);
     if (i < LPT)
       dma16_untracked((8 * (wave + i * NW) < BM ? A : W) + 128 * kt, src_off[i], dst + (wave + i * NW) * 1024);
     else
-      dma4_untracked(scales + (kt & ~3), dst + T::ROWS * 128 + (wave % (T::ROWS / 64)) * 256);
+      dma4_untracked(scales + (kt & ~3), dst + T::ROWS * 128 + (wave % T::SCALES) * 256);
   };
 
 #pragma unroll
@@ -337,10 +335,9 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
 
   const int sw = chunk_swz(li);
   const int arow = wm * T::WTM + li, wrow = BM + wn * T::WTN + li;
-  const int KT = a.kp >> 7;
 #pragma unroll
   for (int s = 0; s < ST; ++s)
-    if (s < KT) {
+    if (s < steps) {
 #pragma unroll
       for (int i = 0; i < kAll; ++i) transfer(s, i);
     }
@@ -403,12 +400,14 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
     else if (n >= 2) wait_vmcnt<kAll>();
     else wait_vmcnt<0>();
   };
-  // One k-tile.  MORE: there is a next one, FILL: and one to refill the stage with.  The barrier
-  // stands where a wave has read all of its operands of the k-tile and its own transfers of the
+  // One step.  MORE: there is a next one, FILL: and one to refill the stage with.  The barrier
+  // stands where a wave has read all of its operands of the step and its own transfers of the
   // next have landed.
-  auto step = [&](int kt, auto more, auto fill) {
+  auto take = [&](int at, auto more, auto fill) {
     constexpr bool MORE = decltype(more)::value, FILL = decltype(fill)::value;
-    const char* st = smem + (kt % ST) * T::STAGE;
+    const char* st = smem + (at % ST) * T::STAGE;
+    const int kt = at * KS + group;
+    if (!MORE && KS > 1 && kt >= KT) return;
 #pragma unroll
     for (int j = 0; j < T::TN; ++j) ws[j] = wnx[j] >> (8 * (kt & 3));
 #pragma unroll
@@ -418,10 +417,10 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
       for (int f = x * kFrags / kProducts; f < (x + 1) * kFrags / kProducts; ++f) read(st, 1, f);
     });
     if constexpr (MORE) {
-      wait_oldest(FILL ? ST - 1 : min(ST - 1, KT - 1 - kt));
+      wait_oldest(FILL ? ST - 1 : min(ST - 1, steps - 1 - at));
       lds_barrier();
     }
-    const char* next = smem + ((kt + 1) % ST) * T::STAGE;
+    const char* next = smem + ((at + 1) % ST) * T::STAGE;
     if constexpr (MORE) read_scales(next);
     products(1, [&](int x) {
       if constexpr (MORE) {
@@ -430,24 +429,24 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
       }
       if constexpr (FILL) {
 #pragma unroll
-        for (int i = x * kAll / kProducts; i < (x + 1) * kAll / kProducts; ++i) transfer(kt + ST, i);
+        for (int i = x * kAll / kProducts; i < (x + 1) * kAll / kProducts; ++i) transfer(at + ST, i);
       }
     });
   };
-  wait_oldest(min(ST, KT));
+  wait_oldest(min(ST, steps));
   stage_barrier();
 #pragma unroll
   for (int f = 0; f < kFrags; ++f) read(smem, 0, f);
   read_scales(smem);
-  int kt = 0;
-  for (; kt + ST < KT; ++kt) step(kt, std::true_type(), std::true_type());
-  for (; kt + 1 < KT; ++kt) step(kt, std::true_type(), std::false_type());
-  step(kt, std::false_type(), std::false_type());
+  int at = 0;
+  for (; at + ST < steps; ++at) take(at, std::true_type(), std::true_type());
+  for (; at + 1 < steps; ++at) take(at, std::true_type(), std::false_type());
+  take(at, std::false_type(), std::false_type());
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
-__global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
-  using T = Tile<BM, BN, WM, WN, ST>;
+template <int BM, int BN, int WM, int WN, int ST, int KS, int GM, typename TC>
+__global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
+  using T = Tile<BM, BN, WM, WN, ST, KS>;
   constexpr int NT = T::NT;
   __shared__ __attribute__((aligned(1024))) char smem[T::LDS];
   // Tile order as in the 16-bit kernel: an XCD runs a contiguous range of ids, which walk GM row
@@ -462,19 +461,19 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
   const int64_t m0 = (int64_t)(first_m + in_group % gm) * BM;
   const int n0 = (in_group / gm) * BN;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = __builtin_amdgcn_readfirstlane(tid >> 6) / T::NW, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % T::NW;
   const int wm = wave / WN, wn = wave % WN;
   const int li = lane & 31, g = lane >> 5;
 
   f32x16 acc[T::TN][T::TM];
-  mainloop<BM, BN, WM, WN, ST, sizeof(TC) == 4>(a, m0, n0, smem, acc);
+  mainloop<BM, BN, WM, WN, ST, KS, sizeof(TC) == 4>(a, m0, n0, smem, acc);
   __syncthreads();  // every wave is done with the operand stages
 
   // In TN slices of 32 columns for each wave column, through LDS as fp32 rows, then written 16
   // bytes a lane with the epilogue's options; N not in groups of 8 element by element.
   float* Cs = reinterpret_cast<float*>(smem);
-  constexpr int CPL = 16 / (int)sizeof(TC), LPR = T::EPW / CPL, RPP = NT / LPR, NP = BM / RPP;
-  static_assert(NT % LPR == 0 && BM % RPP == 0 && 32 % CPL == 0, "epilogue geometry");
+  constexpr int CPL = 16 / (int)sizeof(TC), LPR = T::EPW / CPL, RPP = NT / LPR, NP = BM > RPP ? BM / RPP : 1;
+  static_assert(NT % LPR == 0 && (BM % RPP == 0 || RPP > BM) && 32 % CPL == 0, "epilogue geometry");
   const int cl = (tid % LPR) * CPL;
   const int ccol = (cl / 32) * T::WTN + (cl % 32);
   const bool whole = a.N % 8 == 0;
@@ -483,15 +482,24 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
   // scratch.)
   auto slice = [&](auto jc) {
     constexpr int j = decltype(jc)::value;
+    // The groups' shares one after the other.
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int k = KS - 1; k >= 0; --k) {
+      if (k < KS - 1) __syncthreads();
+      if (KS == 1 || split == k) {
 #pragma unroll
-      for (int i = 0; i < T::TM; ++i) {
-        f32x4 v;
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e];
-        *reinterpret_cast<f32x4*>(Cs + (wm * T::WTM + i * 32 + li) * T::LDC + wn * 32 + 8 * q + 4 * g) = v;
+          for (int i = 0; i < T::TM; ++i) {
+            f32x4* at = reinterpret_cast<f32x4*>(Cs + (wm * T::WTM + i * 32 + li) * T::LDC + wn * 32 + 8 * q + 4 * g);
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e];
+            if (k < KS - 1) v += *at;
+            *at = v;
+          }
       }
+    }
     const int n = n0 + ccol + j * 32;
     f32x4 bv[CPL / 4];
 #pragma unroll
@@ -517,7 +525,8 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
         *reinterpret_cast<typename Op16<TC>::V8*>(at) = hv;
       }
     };
-    const int64_t first = m0 + tid / LPR;  // this thread's rows: first, first + RPP, ..
+    // This thread's rows: first, first + RPP, ..
+    const int64_t first = RPP <= BM || tid / LPR < BM ? m0 + tid / LPR : a.M;
     // Loads share a counter with the stores: one between two passes would wait for the stores of
     // the pass before it.  So there are none in the loop without residual and masks (which is no
     // longer than it is because a tile runs it once, its instructions coming from memory), and with
@@ -589,18 +598,18 @@ __global__ __launch_bounds__(WM* WN * 64) void linear8_tile_kernel(Args a) {
   if constexpr (T::TN > 3) slice(std::integral_constant<int, 3>());
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int GM, typename TC>
+template <int BM, int BN, int WM, int WN, int ST, int KS, int GM, typename TC>
 hipError_t launch_tile(const Args& a, hipStream_t stream) {
   const int64_t tiles = ((a.M + BM - 1) / BM) * (int64_t)((a.N + BN - 1) / BN);
   if (tiles > 0x7fffff) return hipErrorInvalidValue;
-  return launch_status(linear8_tile_kernel<BM, BN, WM, WN, ST, GM, TC>, dim3((unsigned)tiles), dim3(WM * WN * 64),
-                       stream, a);
+  return launch_status(linear8_tile_kernel<BM, BN, WM, WN, ST, KS, GM, TC>, dim3((unsigned)tiles),
+                       dim3(WM * WN * KS * 64), stream, a);
 }
 
 // Tile choice: the candidate with the least estimated time, as for the 16-bit kernel.  n workgroups
 // fall to each CU, per_cu at a time; a group of r takes `fixed` (launch, first loads, epilogue) plus
 // per k-tile the larger of `step` (one workgroup's chain) and r x `busy` (its share of the CU).  Fits
-// (us) to timings of every candidate over M 128 .. 16384, N and K 1000 .. 8192, for the scaled
+// (us) to timings of every candidate over M 64 .. 16384, N and K 1000 .. 8192, for the scaled
 // kind and the exact one: 8192 x 4096 x 4096 takes 114.8 us in 256 x 256 tiles (2394 TFLOP/s) and 146 in
 // 128 x 128, 8192^3 417 (2635 TFLOP/s; a library product of e4m3 2605 to 2675 on the same cards) and 539,
 // 512 x 4096 x 4096 44.6, 26.6, 16.4 and 19.7 in the four, 128 x 4096 x 4096 37.8, 19.5, 14.8 and 10.6.
@@ -610,17 +619,20 @@ struct TileCand {
   int bm, bn, per_cu;
   double fixed, step, busy;
 };
-constexpr TileCand kScaled[] = {{256, 256, 1, 11.0, 1.00, 1.45}, {128, 128, 2, 4.4, 0.47, 0.50},
-                                {128, 64, 2, 4.1, 0.36, 0.28},   {64, 64, 2, 3.5, 0.22, 0.21}};
-constexpr TileCand kExact[] = {{256, 256, 1, 21.0, 1.80, 2.75}, {128, 128, 2, 8.7, 0.67, 0.80},
-                               {128, 64, 2, 6.0, 0.58, 0.51},   {64, 64, 2, 4.8, 0.37, 0.39}};
+constexpr int kTiles = 5;
+constexpr TileCand kScaled[kTiles] = {{256, 256, 1, 11.0, 1.00, 1.45}, {128, 128, 2, 4.4, 0.47, 0.50},
+                                      {128, 64, 2, 4.1, 0.36, 0.28},   {64, 64, 2, 3.5, 0.22, 0.21},
+                                      {64, 32, 1, 2.9, 0.20, 0.23}};
+constexpr TileCand kExact[kTiles] = {{256, 256, 1, 21.0, 1.80, 2.75}, {128, 128, 2, 8.7, 0.67, 0.80},
+                                     {128, 64, 2, 6.0, 0.58, 0.51},   {64, 64, 2, 4.8, 0.37, 0.39},
+                                     {64, 32, 1, 3.6, 0.21, 0.235}};
 
-int pick_tile(const TileCand (&tiles)[4], const Args& a) {
+int pick_tile(const TileCand (&tiles)[kTiles], const Args& a) {
   const int64_t cus = compute_units();
   const double kt = a.kp / 128;
   int best = 0;
   double best_t = 1e300;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kTiles; ++i) {
     const TileCand& c = tiles[i];
     const int64_t all = ((a.M + c.bm - 1) / c.bm) * (int64_t)((a.N + c.bn - 1) / c.bn);
     const int64_t n = (all + cus - 1) / cus, rest = n % c.per_cu;
@@ -637,26 +649,26 @@ int pick_tile(const TileCand (&tiles)[4], const Args& a) {
 template <typename TC>
 hipError_t dispatch_tile(const Args& a, hipStream_t stream) {
   switch (pick_tile(sizeof(TC) == 4 ? kExact : kScaled, a)) {
-    case 0: return launch_tile<256, 256, 4, 2, 2, 4, TC>(a, stream);
-    case 1: return launch_tile<128, 128, 2, 2, 2, 8, TC>(a, stream);
-    case 2: return launch_tile<128, 64, 2, 2, 3, 8, TC>(a, stream);
-    default: return launch_tile<64, 64, 2, 2, 4, 8, TC>(a, stream);
+    case 0: return launch_tile<256, 256, 4, 2, 2, 1, 4, TC>(a, stream);
+    case 1: return launch_tile<128, 128, 2, 2, 2, 1, 8, TC>(a, stream);
+    case 2: return launch_tile<128, 64, 2, 2, 3, 1, 8, TC>(a, stream);
+    case 3: return launch_tile<64, 64, 2, 2, 4, 1, 8, TC>(a, stream);
+    default: return launch_tile<64, 32, 2, 1, 4, 2, 8, TC>(a, stream);
   }
 }
 
-template <int MT, int NT, typename TA>
+template <int NT, typename TA>
 hipError_t launch_few(const Args& a, hipStream_t stream) {
-  return launch_status(linear8_few_kernel<TA, MT, NT>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(512),
+  return launch_status(linear8_few_kernel<TA, NT>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(512),
                        stream, a);
 }
 template <typename TA>
 hipError_t dispatch_few(const Args& a, hipStream_t stream) {
   const bool wide = a.N >= 32 * compute_units();
-  if (a.M <= 16) return wide ? launch_few<1, 2, TA>(a, stream) : launch_few<1, 1, TA>(a, stream);
-  return wide ? launch_few<2, 2, TA>(a, stream) : launch_few<2, 1, TA>(a, stream);
+  return wide ? launch_few<2, TA>(a, stream) : launch_few<1, TA>(a, stream);
 }
 
-constexpr int64_t kFewRows = 32;
+constexpr int64_t kFewRows = 16;
 
 bool whole_rows(const Linear8Args& c) {
   return c.K % 8 == 0 && (reinterpret_cast<uintptr_t>(c.a) & 15) == 0;
