@@ -22,7 +22,7 @@ namespace cobra {
 namespace {
 
 constexpr int kMaxDim = 256;
-constexpr int kTurns = 256, kSome = 8;  // angles and tokens of a workgroup, at most
+constexpr int kTurns = 512, kSome = 8;  // angles and tokens of a workgroup, at most
 
 struct Args {
   void* qkv;
@@ -70,10 +70,12 @@ __device__ __forceinline__ void rotate(float& u, float& v, const float2& r) {
 __device__ __forceinline__ float norm_of(const Args& a, float sum) { return 1.0f / sqrtf(sum / (float)a.dim + a.eps); }
 
 // A workgroup has `some` tokens; a thread every 256th piece pair of their heads, always the same place
-// in the head, so that it holds that place's weights.  U pairs' loads are asked for before the turns
-// are formed and the first of them is used.  16384 tokens of 32 + 8 heads of 128 (335 MB): 76 us,
-// 4.4 TB/s against a large copy's 5.1; with a token a workgroup 162 (its angles and barriers), with two
-// 100, three 80, six 80; four pairs ahead 83 (registers for three waves of a SIMD).
+// in the head, so that it holds that place's weights.  U pairs' loads are asked for before the turns are
+// formed, and always the next U before the last ones are finished.  16384 tokens of 32 + 8 heads of 128
+// (335 MB): 80 to 90 us from memory, 3.7 to 4.2 TB/s against a large copy's 5.1; with a token a workgroup 162
+// (its angles and barriers), with two 117, four 90, eight 85; without the loads ahead 98 where this takes 90;
+// four pairs at a time no faster (registers for three waves of a SIMD either way); stores past the
+// caches 97 to 101.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
   constexpr int U = 2;
@@ -88,8 +90,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
   const int count = (int)min((int64_t)some, a.tokens - t0);
   const uint32_t work = (uint32_t)count * a.all;  // heads of these tokens
   T* base = static_cast<T*>(a.qkv) + t0 * a.ld;
-  Piece<T, V> x[U][2];
-  auto ask = [&](uint32_t first) {
+  Piece<T, V> b0[U][2], b1[U][2];
+  auto ask = [&](Piece<T, V> (&x)[U][2], uint32_t first) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t w = first + u * per;
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
   const uint32_t mine = tid / a.lanes;
   // The positions first: loads come back in order, and the angles need nothing else.
   const int at = tid < count ? position_of(a, t0 + tid) : 0;
-  ask(mine);
+  ask(b0, mine);
   if (tid < count) place[tid] = at;
   float wq[2][V], wk[2][V];
 #pragma unroll
@@ -121,8 +123,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
     turn[i] = turn_of(a, place[t], k);
   }
   lds_barrier();
-  for (uint32_t first = mine; first < work; first += U * per) {
-    if (first != mine) ask(first);
+  auto finish = [&](const Piece<T, V> (&x)[U][2], uint32_t first) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t w = first + u * per;
@@ -166,6 +167,12 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a, int some) {
       if (on0) *reinterpret_cast<Piece<T, V>*>(at + c0) = z0;
       if (on1) *reinterpret_cast<Piece<T, V>*>(at + c1) = z1;
     }
+  };
+  for (uint32_t first = mine; first < work; first += 2 * U * per) {
+    ask(b1, first + U * per);
+    finish(b0, first);
+    ask(b0, first + 2 * U * per);
+    finish(b1, first + U * per);
   }
 }
 
@@ -218,21 +225,26 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(Args a, int inter
   }
 }
 
-dim3 groups_of(const Args& a) { return dim3((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20)); }
+template <typename T>
+hipError_t any(const Args& a, int inter, hipStream_t stream) {
+  const dim3 groups((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20));
+  return launch_status(qk_norm_rope_any_kernel<T>, groups, dim3(256), stream, a, inter);
+}
 
 template <typename T, int V, bool INTER>
 hipError_t launch(Args a, hipStream_t stream) {
   a.lanes = 1;
   while (a.lanes * 2 * V < a.dim) a.lanes *= 2;
-  // As many tokens a workgroup as its threads have five pairs and an angle each for, where every CU
-  // still has eight workgroups; a token each for few.
-  const int64_t batch = 5 * 256 / ((int64_t)a.all * a.lanes), angles = a.half ? kTurns / a.half : kSome;
-  int some = (int)(batch < angles ? batch : angles);
+  // As many tokens a workgroup as its threads have ten pairs and two angles each for, fewer where
+  // every CU would not have eight workgroups then.
+  const int64_t pairs = 10 * 256 / ((int64_t)a.all * a.lanes), angles = a.half ? kTurns / a.half : kSome;
+  const int64_t each = a.tokens / (8 * compute_units());
+  int64_t some = pairs < angles ? pairs : angles;
+  some = some < each ? some : each;
   some = some > kSome ? kSome : some < 1 ? 1 : some;
-  if (a.tokens < (int64_t)some * 8 * compute_units()) some = 1;
   const int64_t groups = (a.tokens + some - 1) / some;
-  if ((int64_t)some * a.all > 0x7fffffff) return hipErrorInvalidValue;
-  return launch_status(qk_norm_rope_kernel<T, V, INTER>, dim3((unsigned)groups), dim3(256), stream, a, some);
+  if (groups > 0xffffff) return any<T>(a, INTER, stream);  // (a launch's workgroups; that kernel goes round)
+  return launch_status(qk_norm_rope_kernel<T, V, INTER>, dim3((unsigned)groups), dim3(256), stream, a, (int)some);
 }
 
 template <typename T>
@@ -243,7 +255,7 @@ hipError_t launch_type(const Args& a, int inter, hipStream_t stream) {
   };
   if (fits(8)) return inter ? launch<T, 8, true>(a, stream) : launch<T, 8, false>(a, stream);
   if (fits(4)) return inter ? launch<T, 4, true>(a, stream) : launch<T, 4, false>(a, stream);
-  return launch_status(qk_norm_rope_any_kernel<T>, groups_of(a), dim3(256), stream, a, inter);
+  return any<T>(a, inter, stream);
 }
 
 // Position of each new token: its request's tokens before it, behind those of the prefix; -1 where

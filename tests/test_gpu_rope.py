@@ -100,8 +100,11 @@ def test_far_positions(far):
     check(9, 2, 2, 40, F16, 20, True, True, far=far)
 
 
-def test_many_tokens():
-    check(3000, 8, 2, 64, BF16, 64, False, True)
+@pytest.mark.parametrize("t,rot,inter,norm", [(3000, 64, False, True), (5001, 64, True, False), (20003, 64, False, True),
+                                              (20003, 16, True, True), (20003, 0, False, True)])
+def test_many_tokens(t, rot, inter, norm):
+    """Several tokens a workgroup, and a last one with fewer."""
+    check(t, 2, 1, 64, BF16, rot, inter, norm)
 
 
 def test_zero_rows_and_large_values():
