@@ -59,7 +59,7 @@ hipError_t launch(const Args& a, const CachePlan& p, hipStream_t stream) {
   if (grid > kMaxGrid) return hipErrorInvalidValue;
   const dim3 groups((unsigned)grid), block(256);
   const hipError_t e =
-      p.chunked ? launch_status(cache_chunk_kernel<T, CACHE, HDP, 2>, groups, block, stream, a)
+      p.chunked ? launch_status(cache_chunk_kernel<kWhole, T, CACHE, HDP, 2>, groups, block, stream, a, NoPass{})
                 : launch_status(cache_decode_kernel<T, CACHE, HDP, decode_keys(HDP)>, groups, block, stream, a);
   if (p.splits <= 1 || e != hipSuccess) return e;
   const int64_t rows = (int64_t)a.tokens * a.heads;

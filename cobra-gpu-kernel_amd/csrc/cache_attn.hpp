@@ -168,6 +168,13 @@ struct Args {
 // then its own (kBoth, not split).
 enum : int { kWhole = 0, kPrefix = 1, kOwn = 2, kBoth = 3 };
 
+// The prefix's pass, where it is of one launch with the requests' own: its workgroups are the first.
+struct PrePass {
+  Args args;
+  int groups;
+};
+struct NoPass {};
+
 // A request as the kernels see it, whatever its lengths say: bounds that keep every access
 // inside the tensors.
 struct Request {
@@ -533,17 +540,12 @@ struct Rows {
 // Eight waves to a workgroup took 24 us for the 64 requests, registers for four waves of a SIMD
 // (with scratch) 23, 32 rows a wave 33.6 us for 18 rows where 16 a wave take 26 twice over the
 // keys.
-template <int HDP>
-struct DecodeShared {
-  f32x4 o[2][HDP / 16][64];
-  float m[2][64], l[2][64];
-};
 template <int MODE, typename T, int CACHE, int HDP, int KT>
-__device__ __forceinline__ void decode_rows(const Args& a, int id, DecodeShared<HDP>& sh) {
+__device__ __forceinline__ void decode_rows(const Args& a, int id) {
   typedef Rows<T, CACHE, HDP, 1, KT> R;
   constexpr int kWaves = 4, kRows = 16;
-  auto &sh_o = sh.o;
-  auto &sh_m = sh.m, &sh_l = sh.l;
+  __shared__ f32x4 sh_o[kWaves / 2][R::kDims][64];
+  __shared__ float sh_m[kWaves / 2][64], sh_l[kWaves / 2][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int h = id % a.kv_heads;
   id /= a.kv_heads;
@@ -598,8 +600,7 @@ __device__ __forceinline__ void decode_rows(const Args& a, int id, DecodeShared<
 }
 template <typename T, int CACHE, int HDP, int KT>
 __global__ __launch_bounds__(256) void cache_decode_kernel(Args a) {
-  __shared__ DecodeShared<HDP> sh;
-  decode_rows<kWhole, T, CACHE, HDP, KT>(a, blockIdx.x, sh);
+  decode_rows<kWhole, T, CACHE, HDP, KT>(a, blockIdx.x);
 }
 
 // The splits of a row joined: o = sum 2^(M_s - M) O_s / sum 2^(M_s - M) l_s, always in the same
@@ -706,19 +707,33 @@ __global__ __launch_bounds__(256) void cache_join_kernel(Args a, int step) {
 // ALU active in 64 % of cycles, the matrix cores in 40 %.  With few requests by the longest one's tiles:
 // 5 of 301 to 1024 new tokens, 16 heads of 64 on 4 (fp16), 159 us, CUs busy for two thirds of it (the
 // vector ALU for 67 %, the matrix cores for 32 % of that) while one request's 105 tiles follow each other.
-template <int HDP>
-struct ChunkShared {
-  u32x4 k[2][64 * (HDP / 16)], v[2][HDP * 4];
-};
-template <int MODE, typename T, int CACHE, int HDP, int NR>
-__device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HDP>& sh) {
+// MODE kPrefix: the workgroups behind the prefix's have the requests' own keys, which they pass over
+// in tiles too (OWN_TILES), or by decode_rows.  The body stands in the kernel itself and has its second
+// pass by a jump: in a device function with a loop, the one-pass kernel of 16 heads of 64 got other
+// registers and took 172 to 178 us in place of 165.
+template <int MODE, typename T, int CACHE, int HDP, int NR, bool OWN_TILES = false, typename P = NoPass>
+__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a, P pre) {
   constexpr int kWaves = 4, kRows = kWaves * NR * 16, KT = 64;
   typedef Rows<T, CACHE, HDP, NR, KT> R;
   constexpr int kC = HDP / 16, kPer = (HDP + 63) / 64;  // 16 codes each: of a K row; a thread's of K, of V
   constexpr bool kAll = HDP % 64 == 0;
   // At head_dim 128 int8's widening leaves no registers for a product's codes at once.
   constexpr bool kBatch = CACHE == kCacheE4M3 || HDP != 128;
-  auto &sh_k = sh.k, &sh_v = sh.v;
+  __shared__ u32x4 sh_k[2][KT * kC], sh_v[2][HDP * 4];
+  int id = blockIdx.x;
+  bool pre_pass = false;  // this workgroup's rows are every request's
+  if constexpr (MODE == kPrefix) {
+    pre_pass = id < pre.groups;
+    if (pre_pass) {
+      a = pre.args;
+    } else {
+      id -= pre.groups;
+      if constexpr (!OWN_TILES) {
+        decode_rows<kOwn, T, CACHE, HDP, decode_keys(HDP)>(a, id);
+        return;
+      }
+    }
+  }
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   auto swz = [](int row) { return kC == 8 || kC == 16 ? row & 7 : kC == 4 || kC == 12 ? (row >> 1) & 3 : (row >> 2) & 1; };
@@ -731,8 +746,8 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
   const int tile0 = a.row_tiles - 1 - id % a.row_tiles;
   id /= a.row_tiles;
   const int split = id % a.splits;
-  int b = MODE == kPrefix ? a.prefix : id / a.splits;
-  if (MODE != kPrefix && a.batch <= 64) {
+  int b = pre_pass ? a.prefix : id / a.splits;
+  if (!pre_pass && a.batch <= 64) {
     const int len = lane < a.batch ? a.lens[lane] : -1;
     int rank = 0;
     for (int k = 0; k < a.batch; ++k) {
@@ -741,7 +756,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
     }
     b = __builtin_ctzll(__ballot(lane < a.batch && rank == b));
   }
-  const Request rq = request_of<MODE>(a, b);
+  const Request rq = pre_pass ? request_of<kPrefix>(a, b) : request_of(a, b);
   const int64_t rows = (int64_t)rq.n * a.group;
   const int chunk = chunk_of(a, rq.len, KT);
   if (split > 0 && (int64_t)split * chunk >= rq.len) return;
@@ -749,7 +764,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
   const int bs = 1 << a.shift;
   const Strides st(a, h, bs * HDP);
   Pages pages(a, b, (first * KT) >> a.shift);
-  int len = rq.len;  // of the keys that are passed over
+  int len = rq.len;  // of the keys that are passed over (kBoth)
 
   // What this thread brings of a tile: of K 16-code pieces lane, lane + 64, .. of the keys of
   // group `wave`, of V pieces tid, tid + 256, .. (four to a dimension).
@@ -787,7 +802,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
   float sk = 1.f, sv = 1.f;
   bool bad = false;
   auto load_v = [&](int tile, const Ids& ids) {
-    there = len - tile * KT - 16 * (tid & 3);
+    there = (MODE == kBoth ? len : rq.len) - tile * KT - 16 * (tid & 3);
     if (one) {
       const uint8_t* pv = st.v + st.block(ids.i0) + (uint32_t)((tile * KT) & (bs - 1));
 #pragma unroll
@@ -835,22 +850,21 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
     R w;
     w.init(a, rq, h, (int)row0);
     wait_vmcnt<0>();  // the queries: waited for in the loop, they would take every tile's loads along
-    int own[NR];
+    // Once over the request's own keys, or over the prefix's and then those.
+    [[maybe_unused]] int pass = b != a.prefix ? 0 : 1, own[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) own[r] = w.lim[r];
-#pragma unroll 1
-    for (int pass = MODE == kBoth && b != a.prefix ? 0 : 1; pass < 2; ++pass) {
-    const bool pre = MODE == kBoth && pass == 0;
+  over:
     if constexpr (MODE == kBoth) {
       const int held = request_of<kPrefix>(a, a.prefix).len;
-      pages = Pages(a, pre ? a.prefix : b, 0);
-      len = pre ? held : rq.len;
+      pages = Pages(a, pass == 0 ? a.prefix : b, 0);
+      len = pass == 0 ? held : rq.len;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) w.lim[r] = !pre ? own[r] : row0 + 16 * r + n < rows ? held : 0;
+      for (int r = 0; r < NR; ++r) w.lim[r] = pass ? own[r] : row0 + 16 * r + n < rows ? held : 0;
     }
     // Tiles that any of the workgroup's rows see; keys that all of this wave's do.
-    int full = len, most = len;
-    if (a.causal && !pre) {
+    int full = MODE == kBoth ? len : rq.len, most = full;
+    if (a.causal && !(MODE == kBoth && pass == 0)) {
       full = rq.len - rq.n + (int)(row0 / a.group) + 1;
       most = rq.len - rq.n + (int)((min(at + kRows, rows) - 1) / a.group) + 1;
     }
@@ -915,19 +929,17 @@ __device__ __forceinline__ void chunk_rows(const Args& a, int id, ChunkShared<HD
         ids = load_ids(tile + 3);
       }
     }
+    if constexpr (MODE == kBoth) {
+      if (pass++ == 0) goto over;
     }
     if (row0 < rows) {
       w.total_l();
 #pragma unroll
       for (int r = 0; r < NR; ++r)
-        w.store(a, rq, h, (int)row0, r, MODE == kOwn ? a.base + split : split, MODE == kBoth || (MODE == kWhole && chunk >= rq.len));
+        w.store(a, rq, h, (int)row0, r, MODE != kPrefix || pre_pass ? split : a.base + split,
+                MODE == kBoth || (MODE == kWhole && chunk >= rq.len));
     }
   }
-}
-template <typename T, int CACHE, int HDP, int NR>
-__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_chunk_kernel(Args a) {
-  __shared__ ChunkShared<HDP> sh;
-  chunk_rows<kWhole, T, CACHE, HDP, NR>(a, blockIdx.x, sh);
 }
 
 // The kernels' arguments of a call; its partial results are set where it has any.

@@ -14,37 +14,13 @@ namespace cobra {
 
 namespace {
 
-// Both passes of a call: the prefix's workgroups, then the requests' own.
-struct Both {
-  Args pre, own;
-  int pre_groups;  // workgroups of the prefix's pass, which come first
-};
-
-template <typename T, int CACHE, int HDP, bool PRE_CHUNK, bool OWN_CHUNK>
-__global__ __launch_bounds__(256, (PRE_CHUNK || OWN_CHUNK) && HDP <= 128 ? 2 : 1) void cache_prefix_kernel(Both c) {
-  constexpr bool kChunk = PRE_CHUNK || OWN_CHUNK;
-  constexpr int kBytes = kChunk && sizeof(ChunkShared<HDP>) > sizeof(DecodeShared<HDP>) ? (int)sizeof(ChunkShared<HDP>)
-                                                                                        : (int)sizeof(DecodeShared<HDP>);
-  __shared__ __attribute__((aligned(16))) char smem[kBytes];
-  if ((int)blockIdx.x < c.pre_groups) {
-    if constexpr (PRE_CHUNK)
-      chunk_rows<kPrefix, T, CACHE, HDP, 2>(c.pre, blockIdx.x, *reinterpret_cast<ChunkShared<HDP>*>(smem));
-    else
-      decode_rows<kPrefix, T, CACHE, HDP, decode_keys(HDP)>(c.pre, blockIdx.x, *reinterpret_cast<DecodeShared<HDP>*>(smem));
-  } else {
-    if constexpr (OWN_CHUNK)
-      chunk_rows<kOwn, T, CACHE, HDP, 2>(c.own, blockIdx.x - c.pre_groups, *reinterpret_cast<ChunkShared<HDP>*>(smem));
-    else
-      decode_rows<kOwn, T, CACHE, HDP, decode_keys(HDP)>(c.own, blockIdx.x - c.pre_groups, *reinterpret_cast<DecodeShared<HDP>*>(smem));
-  }
-}
-
-// Requests of many new tokens each: their rows fill tiles of their own, so each tile passes over the
-// prefix's keys and then its request's, and nothing is joined.
+// Both passes by direct loads.
 template <typename T, int CACHE, int HDP>
-__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void cache_prefix_chunk_kernel(Args a) {
-  __shared__ ChunkShared<HDP> sh;
-  chunk_rows<kBoth, T, CACHE, HDP, 2>(a, blockIdx.x, sh);
+__global__ __launch_bounds__(256) void cache_prefix_decode_kernel(Args own, PrePass pre) {
+  if ((int)blockIdx.x < pre.groups)
+    decode_rows<kPrefix, T, CACHE, HDP, decode_keys(HDP)>(pre.args, blockIdx.x);
+  else
+    decode_rows<kOwn, T, CACHE, HDP, decode_keys(HDP)>(own, blockIdx.x - pre.groups);
 }
 
 // The request that token t belongs to: the last with cu[b] <= t.
@@ -67,15 +43,14 @@ __device__ __forceinline__ int request_at(const Args& a, int t) {
 // every split that there may be, and the first kEarly rounds of O.
 constexpr int kMaxSplits = 256, kOwnSplits = 64;
 template <typename T, int HDP, int W>
-__global__ __launch_bounds__(256) void cache_prefix_join_kernel(Both c, int pre_step, int own_step) {
+__global__ __launch_bounds__(256) void cache_prefix_join_kernel(Args a, PrePass shared, int pre_step, int own_step) {
   constexpr int kLanes = HDP / 4, kAt = 64 / kLanes;  // lanes of a split, splits of a wave
   constexpr int kEarly = W > 1 ? 4 : 8, kStats = W > 1 ? kMaxSplits / 64 : 1;
   __shared__ float factor[4][64 * kStats];
   __shared__ f32x4 sh[W > 1 ? W : 1][kLanes];
-  const Args& a = c.own;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = W > 1 ? wave : 0;
-  const int all = c.pre.splits + c.own.splits;
+  const int all = shared.args.splits + a.splits;
   const int sub = lane / kLanes, d = (lane - sub * kLanes) * 4, s0 = part * kAt + sub;
   const int64_t rows = (int64_t)a.tokens * a.heads;
   for (int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave; row < rows;
@@ -93,9 +68,9 @@ __global__ __launch_bounds__(256) void cache_prefix_join_kernel(Both c, int pre_
       if (sub < kAt && s < all) early[i] = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HDP + d);
     }
     const int t = (int)(row / a.heads), b = request_at(a, t);
-    const Request rq = request_of<kOwn>(a, b), pre = request_of<kPrefix>(c.pre, a.prefix);
+    const Request rq = request_of<kOwn>(a, b), pre = request_of<kPrefix>(a, a.prefix);
     if (t < rq.t0 || t >= rq.t0 + rq.n) continue;
-    const int pre_chunk = chunk_of(c.pre, pre.len, pre_step), own_chunk = chunk_of(a, rq.len, own_step);
+    const int pre_chunk = chunk_of(shared.args, pre.len, pre_step), own_chunk = chunk_of(a, rq.len, own_step);
     const int pre_n = b == a.prefix ? 0 : (int)(((int64_t)pre.len + pre_chunk - 1) / pre_chunk);
     const int own_n = (int)(((int64_t)rq.len + own_chunk - 1) / own_chunk);
     // Splits that were written: the first pre_n, and own_n from a.base on.
@@ -229,40 +204,40 @@ PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
 }
 
 template <typename T, int CACHE, int HDP>
-hipError_t launch(const Both& c, const PrefixPlan& p, hipStream_t stream) {
+hipError_t launch(const Args& a, PrePass shared, const PrefixPlan& p, hipStream_t stream) {
   const dim3 block(256);
-  const int64_t own = (int64_t)c.own.batch * c.own.kv_heads * p.own.row_tiles * p.own.splits;
-  const int64_t pre = (int64_t)c.own.kv_heads * p.pre.row_tiles * p.pre.splits;
+  const int64_t own = (int64_t)a.batch * a.kv_heads * p.own.row_tiles * p.own.splits;
+  const int64_t pre = (int64_t)a.kv_heads * p.pre.row_tiles * p.pre.splits;
   if (p.both)
     return own > kMaxGrid ? hipErrorInvalidValue
-                          : launch_status(cache_prefix_chunk_kernel<T, CACHE, HDP>, dim3((unsigned)own), block, stream, c.own);
+                          : launch_status(cache_chunk_kernel<kBoth, T, CACHE, HDP, 2>, dim3((unsigned)own), block, stream, a, NoPass{});
   if (own + pre > kMaxGrid) return hipErrorInvalidValue;
-  Both b = c;
-  b.pre_groups = (int)pre;
+  shared.groups = (int)pre;
   const dim3 groups((unsigned)(own + pre));
   // Requests of many new tokens are many tokens together.
-  auto* kernel = p.own.chunked   ? cache_prefix_kernel<T, CACHE, HDP, true, true>
-                 : p.pre.chunked ? cache_prefix_kernel<T, CACHE, HDP, true, false>
-                                 : cache_prefix_kernel<T, CACHE, HDP, false, false>;
-  const hipError_t e = launch_status(kernel, groups, block, stream, b);
+  auto* kernel = p.own.chunked   ? cache_chunk_kernel<kPrefix, T, CACHE, HDP, 2, true, PrePass>
+                 : p.pre.chunked ? cache_chunk_kernel<kPrefix, T, CACHE, HDP, 2, false, PrePass>
+                                 : cache_prefix_decode_kernel<T, CACHE, HDP>;
+  const hipError_t e = launch_status(kernel, groups, block, stream, a, shared);
   if (e != hipSuccess) return e;
-  const int64_t rows = (int64_t)c.own.tokens * c.own.heads;
-  return p.pre.splits + p.own.splits > 64
-             ? launch_status(cache_prefix_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, b, p.pre.step,
-                             p.own.step)
-             : launch_status(cache_prefix_join_kernel<T, HDP, 1>, dim3((unsigned)((rows + 3) / 4 < kMaxGrid ? (rows + 3) / 4 : kMaxGrid)), block, stream, b,
-                             p.pre.step, p.own.step);
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  if (p.pre.splits + p.own.splits > 64)
+    return launch_status(cache_prefix_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, a, shared,
+                         p.pre.step, p.own.step);
+  const int64_t quads = (rows + 3) / 4;
+  return launch_status(cache_prefix_join_kernel<T, HDP, 1>, dim3((unsigned)(quads < kMaxGrid ? quads : kMaxGrid)),
+                       block, stream, a, shared, p.pre.step, p.own.step);
 }
 
 template <typename T, int CACHE>
-hipError_t launch_width(const Both& c, const PrefixPlan& p, int width, hipStream_t stream) {
+hipError_t launch_width(const Args& a, const PrePass& shared, const PrefixPlan& p, int width, hipStream_t stream) {
   switch (width) {
-    case 32: return launch<T, CACHE, 32>(c, p, stream);
-    case 64: return launch<T, CACHE, 64>(c, p, stream);
-    case 96: return launch<T, CACHE, 96>(c, p, stream);
-    case 128: return launch<T, CACHE, 128>(c, p, stream);
-    case 192: return launch<T, CACHE, 192>(c, p, stream);
-    case 256: return launch<T, CACHE, 256>(c, p, stream);
+    case 32: return launch<T, CACHE, 32>(a, shared, p, stream);
+    case 64: return launch<T, CACHE, 64>(a, shared, p, stream);
+    case 96: return launch<T, CACHE, 96>(a, shared, p, stream);
+    case 128: return launch<T, CACHE, 128>(a, shared, p, stream);
+    case 192: return launch<T, CACHE, 192>(a, shared, p, stream);
+    case 256: return launch<T, CACHE, 256>(a, shared, p, stream);
   }
   return hipErrorInvalidValue;
 }
@@ -284,24 +259,23 @@ hipError_t run_cache_prefix(const CachePrefixArgs& c, int64_t workspace_bytes, h
       plan_of(t.tokens, t.batch, t.heads, t.kv_heads, t.head_dim, t.max_new, t.max_len, c.max_prefix);
   const int64_t rows = t.tokens * t.heads, parts = (p.pre.splits + p.own.splits) * rows;
   if (!p.both && (!t.part || workspace_bytes < parts * (width * 4 + 8))) return hipErrorInvalidValue;
-  Both b{};
-  b.own = cache_args(t, p.own);
+  Args a = cache_args(t, p.own);
   if (!p.both) {
-    b.own.part_o = t.part;
-    b.own.part_m = reinterpret_cast<float2*>(t.part + parts * width);
+    a.part_o = t.part;
+    a.part_m = reinterpret_cast<float2*>(t.part + parts * width);
   }
-  b.own.prefix = c.prefix;
-  b.own.base = p.pre.splits;
-  b.pre = b.own;
-  b.pre.causal = 0;
-  b.pre.splits = p.pre.splits;
-  b.pre.chunk = p.pre.chunk;
-  b.pre.row_tiles = (int)p.pre.row_tiles;
+  a.prefix = c.prefix;
+  a.base = p.pre.splits;
+  PrePass shared{a, 0};
+  shared.args.causal = 0;
+  shared.args.splits = p.pre.splits;
+  shared.args.chunk = p.pre.chunk;
+  shared.args.row_tiles = (int)p.pre.row_tiles;
   if (t.dtype == kF16)
-    return t.cache == kCacheE4M3 ? launch_width<f16, kCacheE4M3>(b, p, width, stream)
-                                 : launch_width<f16, kCacheI8>(b, p, width, stream);
-  return t.cache == kCacheE4M3 ? launch_width<bf16, kCacheE4M3>(b, p, width, stream)
-                               : launch_width<bf16, kCacheI8>(b, p, width, stream);
+    return t.cache == kCacheE4M3 ? launch_width<f16, kCacheE4M3>(a, shared, p, width, stream)
+                                 : launch_width<f16, kCacheI8>(a, shared, p, width, stream);
+  return t.cache == kCacheE4M3 ? launch_width<bf16, kCacheE4M3>(a, shared, p, width, stream)
+                               : launch_width<bf16, kCacheI8>(a, shared, p, width, stream);
 }
 
 }  // namespace cobra
