@@ -532,6 +532,8 @@ class CobraTransformer(nn.Module):
         fp32 residual, fp16 h / qkv / ctx / h2 / FFN hidden, the input and the output."""
         S, D, F = x.shape[1], self._geom.dp, self._geom.fp
         per_tok = 4 * D + 2 * D + 6 * D + 2 * D + 2 * D + 2 * F + 2 * D * x.element_size() + 4 * D
+        if self.weights8:  # a product's quantised activations
+            per_tok += sum(ops.width8(max(D, F)))
         return S * per_tok
 
     def _stream_needed(self, x: torch.Tensor) -> bool:
