@@ -183,10 +183,16 @@ struct Request {
 template <int MODE = kWhole>
 __device__ __forceinline__ Request request_of(const Args& a, int b) {
   Request r;
-  r.t0 = a.cu[MODE == kPrefix ? 0 : b];
-  const int t1 = a.cu[MODE == kPrefix ? a.batch : b + 1];
-  r.n = t1 - r.t0;
-  if (r.t0 < 0 || t1 > a.tokens || r.n < 0) r.n = 0;
+  if constexpr (MODE == kPrefix) {  // every request's rows: one bad offset is that request's alone
+    r.t0 = max(a.cu[0], 0);
+    const int t1 = (int)min((int64_t)max(a.cu[a.batch], 0), (int64_t)a.tokens);
+    r.n = max(t1 - r.t0, 0);
+  } else {
+    r.t0 = a.cu[b];
+    const int t1 = a.cu[b + 1];
+    r.n = t1 - r.t0;
+    if (r.t0 < 0 || t1 > a.tokens || t1 < r.t0) r.n = 0;
+  }
   const int64_t most = min(a.table_width << a.shift, kMaxKeys);
   const int len = a.lens[b];
   r.len = len < 0 ? 0 : len > most ? (int)most : len;

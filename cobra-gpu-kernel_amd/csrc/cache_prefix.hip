@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void cache_prefix_join_kernel(Args a, PrePass 
     }
     const int t = (int)(row / a.heads), b = request_at(a, t);
     const Request rq = request_of<kOwn>(a, b), pre = request_of<kPrefix>(a, a.prefix);
-    if (t < rq.t0 || t >= rq.t0 + rq.n) continue;
+    if (t < max(rq.t0, pre.t0) || t >= min(rq.t0 + rq.n, pre.t0 + pre.n)) continue;  // (offsets that fall: no shares)
     const int pre_chunk = chunk_of(shared.args, pre.len, pre_step), own_chunk = chunk_of(a, rq.len, own_step);
     const int pre_n = b == a.prefix ? 0 : (int)(((int64_t)pre.len + pre_chunk - 1) / pre_chunk);
     const int own_n = (int)(((int64_t)rq.len + own_chunk - 1) / own_chunk);

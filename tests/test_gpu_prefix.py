@@ -138,6 +138,88 @@ def test_pages_outside_the_pool_are_masked():
     assert ((got.cpu().double() - want).abs() <= room).all()
 
 
+@pytest.mark.parametrize("new,hints", [([0, 2, 3, 1], {}), ([0, 2, 3, 1], dict(max_new=300)),
+                                       ([0, 2, 3, 1], dict(max_new=300, max_len=1, max_prefix=1))])
+def test_bad_offsets_and_lengths_stay_inside(new, hints):
+    """Offsets outside the rows, lengths past the table and negative ones: the other requests' rows are right."""
+    from cobra_amd import ops
+
+    held = [700, 40, 50, 60]
+    table, pool, q, cu = build(held, new, 0, 8, 2, 64, 16, F16, E4M3, 13)
+    k, v, ks, vs = pool
+    dev = [t.to(DEV) for t in pool]
+    for lens, off in (([700, 2 ** 31 - 1, 50, -4], cu), (held, [0, 0, 2, 5, 99]), (held, [-5, -5, 2, 5, 6]),
+                      (held, [0, 0, 2, 5, 4])):
+        out = torch.full((6, 512), 7.0, dtype=F16, device=DEV)
+        ops.cache_prefix_attn(q.to(DEV), i32(off), i32(lens), i32(table), 0, 8, 64, 0.125, *dev, out=out, **hints)
+        want, mag, top, reach = serve.attend(q[:, :512].double(), cu, held, table, 0, 8, 64, 0.125, codes_of(k), codes_of(v),
+                                             ks, vs, True)
+        room = attn_tolerance(want, mag, top, reach, 900, 64, F16, float(vs.max()))
+        rows = slice(2, 4 if off[-1] == 4 else 5)  # falling offsets: the rows before the last
+        assert ((out.cpu().double() - want).abs() <= room)[rows].all()
+
+
+@pytest.mark.parametrize("hints", [{}, dict(max_new=300)])
+def test_offsets_that_fall_to_the_lowest_value(hints):
+    """The last request's rows would be 2^31 - 5 in number; it has none, with a prefix and without."""
+    from cobra_amd import ops
+
+    held, off = [700, 40, 50, 60], [0, 0, 2, 5, -2 ** 31]
+    table, pool, q, cu = build(held, [0, 2, 3, 1], 0, 8, 2, 64, 16, F16, E4M3, 13)
+    rest = [i32(held), i32(table)], [8, 64, 0.125] + [t.to(DEV) for t in pool]
+    for prefix in (False, True):
+        out = torch.full((6, 512), 7.0, dtype=F16, device=DEV)
+        call, row = (ops.cache_prefix_attn, [0]) if prefix else (ops.cache_attn, [])
+        call(q.to(DEV), i32(off), *rest[0], *row, *rest[1], out=out, **hints)
+        if not prefix:
+            want = ops.cache_attn(q.to(DEV), i32(cu), *rest[0], *rest[1], **hints)
+            assert torch.equal(out[:5], want[:5])
+        assert (out[5] == 7).all()
+
+
+@pytest.mark.parametrize("heads,kv,hd,held,new", [(4, 4, 128, [200, 70, 5], [0, 1, 1]),
+                                                  (32, 2, 128, [3000] + [50] * 70, [0] + [1] * 70),
+                                                  (16, 2, 128, [400, 300, 290], [0, 300, 280])])
+def test_offsets_past_32_bits(heads, kv, hd, held, new):
+    """Blocks that stand more than 2^32 bytes into the pool."""
+    from cobra_amd import ops
+
+    table, pool, q, cu = build(held, new, 0, heads, kv, hd, 64, BF16, E4M3, 17)
+    k, v, ks, vs = pool
+    few, all_blocks = k.shape[0], 2 ** 32 // (kv * 64 * hd) + 2 * k.shape[0]
+    dev = []
+    for t in pool:
+        big = torch.zeros((all_blocks, *t.shape[1:]), dtype=t.dtype, device=DEV)
+        big[-few:] = t.to(DEV)
+        dev.append(big)
+    far = [[i + all_blocks - few if 0 <= i < few else i for i in row] for row in table]
+    got = ops.cache_prefix_attn(q.to(DEV), i32(cu), i32(held), i32(far), 0, heads, hd, hd ** -0.5, *dev)
+    near = ops.cache_prefix_attn(q.to(DEV), i32(cu), i32(held), i32(table), 0, heads, hd, hd ** -0.5,
+                                 *[t.to(DEV) for t in pool])
+    assert torch.equal(got, near)
+    check(held, new, 0, heads, kv, hd, 64, BF16, E4M3, seed=17)
+
+
+def test_two_streams_at_once():
+    from cobra_amd import ops
+
+    held, new = [900] + [40] * 30, [0] + [1] * 30
+    table, pool, q, cu = build(held, new, 0, 8, 2, 64, 16, F16, E4M3, 19)
+    dev = [t.to(DEV) for t in pool]
+    rest = [i32(cu), i32(held), i32(table), 0, 8, 64, 0.125, *dev]
+    qs = [q.to(DEV), (-0.5 * q).to(DEV)]
+    want = [ops.cache_prefix_attn(x, *rest) for x in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for s, x, y in zip(streams, qs, got):
+            with torch.cuda.stream(s):
+                y.append(ops.cache_prefix_attn(x, *rest))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+
+
 def test_groups_with_a_prefix_each():
     """Two groups of neighbouring rows, a call each on views, one result."""
     from cobra_amd import ops
