@@ -135,6 +135,8 @@ class _BlockPack:
             self.q_norm = blk.q_norm.weight.float().contiguous() if norms else None
             self.k_norm = blk.k_norm.weight.float().contiguous() if norms else None
             self.qk_eps = float(blk.q_norm.eps) if norms else 0.0
+            if norms and blk.q_norm.eps != blk.k_norm.eps:
+                raise ValueError(f"q_norm and k_norm must have one eps, got {blk.q_norm.eps} and {blk.k_norm.eps}")
 
 
 def _linear(h: torch.Tensor, w, b: torch.Tensor, gelu: bool = False, out_fp32: bool = False,
@@ -199,6 +201,8 @@ class CobraTransformer(nn.Module):
         """(operand type, parameter versions, whether the packs are laid out for them)."""
         op = torch.bfloat16 if x_dtype == torch.bfloat16 else torch.float16
         versions = tuple([p._version if v else p.data_ptr() for p, v in zip(self._params, self._versioned)])
+        if self.config.qk_norm:
+            versions += tuple([n.eps for blk in self.layers for n in (blk.q_norm, blk.k_norm)])
         return op, versions, self._packs is not None and self._versions == versions and self._op == op
 
     def _packed(self, x_dtype: torch.dtype = torch.float16) -> List[_BlockPack]:

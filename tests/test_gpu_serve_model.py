@@ -255,6 +255,26 @@ def test_step_with_prefix_in_a_graph():
     assert one.lens.tolist() == two.lens.tolist() == [20, 45, 20]
 
 
+def test_norms_eps_is_the_modules_own():
+    """A changed eps counts from the next call on, eager and captured; the two norms of a block share it."""
+    cfg = (2, 33, 64, 4, 64, 1, True)
+    _, _, mod = build(cfg, F16, 10000.0, True)
+    x = torch.randn(2, 33, 64, generator=torch.Generator().manual_seed(1)).half().to(DEV)
+    with torch.inference_mode():
+        first = mod(x).clone()
+        blk = mod.layers[0]
+        blk.q_norm.eps = 30.0
+        with pytest.raises(ValueError, match="eps"):
+            mod(x)
+        blk.k_norm.eps = 30.0
+        other = mod(x).clone()
+        fresh = build(cfg, F16, 10000.0, True)[2]
+        fresh.layers[0].q_norm.eps = fresh.layers[0].k_norm.eps = 30.0
+        assert torch.equal(other, fresh(x)) and not torch.equal(other, first)
+        blk.q_norm.eps = blk.k_norm.eps = 1e-6
+        assert torch.equal(mod(x), first)
+
+
 def test_model_refuses():
     from cobra_amd import CobraTransformer, TransformerConfig
 
