@@ -226,3 +226,39 @@ def test_linear8_in_a_graph_and_on_another_stream():
         torch.cuda.synchronize()
         for x, y in zip(a, out):
             assert torch.equal(y, ops.linear8(x, *w))
+
+
+def test_sizes_past_32_bits():
+    """Results, weights and inputs of more than 2^32 bytes: rows that repeat give results that repeat."""
+    from cobra_amd import ops
+
+    base = rows(250, 128, BF16, 1).to(DEV)
+    w = rows(33000, 128, F32, 2, 0.1)
+    y = ops.linear8(base.repeat(264, 1), *ops.quantize8(w.to(DEV))).view(264, 250, 33000)
+    for i in range(1, 264):
+        assert torch.equal(y[i], y[0])
+    at = [0, 1, 63, 16500, 32998, 32999]
+    aq, wq = serve.values(*serve.quantize(base.cpu())), serve.values(*serve.quantize(w[at]))
+    want, mag = serve.linear(aq, wq, None, False, None, None, False)
+    room = bound(want, mag, 128, False, BF16, serve.cut_of_eights(aq, wq))
+    assert ((y[0][:, at].cpu().double() - want).abs() <= room).all()
+    del y
+
+    base = rows(500, 8192, BF16, 3, 0.1).to(DEV)
+    codes, scale = ops.quantize8(base.repeat(1060, 1))
+    want = ops.quantize8(base)
+    for i in range(1060):
+        at = slice(500 * i, 500 * i + 500)
+        assert torch.equal(codes[at].view(torch.uint8), want[0].view(torch.uint8))
+        assert torch.equal(scale[at].view(torch.uint8), want[1].view(torch.uint8))
+    for m in (3, 40):
+        a = rows(m, 8192, F16, m).to(DEV)
+        y = ops.linear8(a, codes, scale).view(m, 1060, 500)
+        assert torch.equal(y, y[:, :1].expand_as(y))
+        aq, wq = serve.values(*serve.quantize(a.cpu())), serve.values(*serve.quantize(base.cpu()[:40]))
+        ref, mag = serve.linear(aq, wq, None, False, None, None, False)
+        room = bound(ref, mag, 8192, False, F16, serve.cut_of_eights(aq, wq) if m > 16 else 0.0)
+        got = y[:, 0, :40].cpu().double()
+        over = got.isinf()  # fp16 rounds what is not below 65520 to infinity
+        assert (ref.abs() + room >= 65520)[over].all() and (got.sign() == ref.sign())[over].all()
+        assert ((got - ref).abs() <= room)[~over].all()

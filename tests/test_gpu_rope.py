@@ -165,3 +165,22 @@ def test_rope_in_a_graph():
         want = src.clone()
         ops.qk_norm_rope(want, 4, 1, 64, pos, freq, w, w)
         assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("hd", [128, 126])
+def test_rows_past_32_bits(hd):
+    """More than 2^32 bytes of rows: those that repeat, at positions that repeat, turn alike."""
+    from cobra_amd import ops
+
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn(250, 60 * hd, generator=g).to(BF16).to(DEV)
+    freq = (10000.0 ** -(torch.arange(hd // 2).double() * 2 / hd)).float().to(DEV)
+    w = torch.ones(hd, device=DEV)
+    x = base.repeat(1200, 1)
+    ops.qk_norm_rope(x, 40, 10, hd, seq_len=250, inv_freq=freq, q_weight=w, k_weight=w)
+    want = base.clone()
+    ops.qk_norm_rope(want, 40, 10, hd, seq_len=250, inv_freq=freq, q_weight=w, k_weight=w)
+    x = x.view(1200, 250, -1)
+    for i in range(1200):
+        assert torch.equal(x[i], want)
+    assert not torch.equal(want, base)
