@@ -655,8 +655,9 @@ int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* posit
 // -- norms and rotation of queries and keys --------------------------------------------------
 
 int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, int64_t seq_len,
-                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
-                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream) {
+                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight,
+                       const float* k_weight, float eps, int64_t tokens, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t pitch, void* stream) {
   if (!is_op_dtype(dtype) || tokens < 0 || tokens > 0x7fffffff || heads <= 0 || heads > 0x7fffff || kv_heads <= 0 ||
       kv_heads > 0x7fffff || head_dim <= 0 || head_dim > 256 || pitch < head_dim || pitch > 0x7fffff || rot < 0 ||
       rot % 2 || rot > head_dim || seq_len < 0 || seq_len > 0x7fffffff || ld < (heads + kv_heads) * pitch || !(eps >= 0.f) ||

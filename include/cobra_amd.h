@@ -293,11 +293,13 @@ int cobra_cache_positions(const int32_t* cu, const int32_t* lens, int32_t* posit
  * heads, then kv_heads key heads, each head_dim columns, pitch columns apart (ld >= (heads +
  * kv_heads) * pitch); other columns are left as they are.  head_dim <= 256, rot even and at most
  * head_dim, 0 for no rotation (inv_freq may then be NULL).  positions NULL: token t stands at t %
- * seq_len (which rotation needs then).  Tokens with a negative position are left as they are.  fp32 arithmetic, angles in 64 bits, one rounding.
+ * seq_len (which rotation needs then).  Tokens with a negative position are left as they are.
+ * fp32 arithmetic, angles in 64 bits, one rounding.
  */
 int cobra_qk_norm_rope(void* qkv, int dtype, int64_t ld, const int32_t* positions, int64_t seq_len,
-                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight, const float* k_weight, float eps, int64_t tokens,
-                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pitch, void* stream);
+                       const float* inv_freq, int64_t rot, int interleaved, const float* q_weight,
+                       const float* k_weight, float eps, int64_t tokens, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t pitch, void* stream);
 
 /*
  * A matrix held in 8 bits (COBRA_E4M3): codes [M, Kp] with Kp = K rounded up to 128, zeros past K,
@@ -317,7 +319,8 @@ int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_
  * [M, Kp] (COBRA_E4M3) with a_scale [M, S]; w, w_scale: codes [N, Kp] and scales [N, S] of the
  * weight in nn.Linear's layout.  bias: [N] fp32 (optional); resid (optional) and c: [M, N] in any
  * of the three types each (resid may be c itself in c's type; c overlaps nothing else).  Sums are
- * fp32.  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is rejected.  workspace:
+ * fp32.  Scale bytes are 1 .. 254, as cobra_quantize8 writes them (0 and 255 give no meaningful
+ * result).  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is rejected.  workspace:
  * cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0), which
  * launches that overlap must not share.
  */
