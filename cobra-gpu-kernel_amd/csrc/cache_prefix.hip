@@ -137,6 +137,32 @@ struct PrefixPlan {
   bool both;  // one pass over the prefix and the request's own keys
 };
 
+// More units of rows than CUs take whole rounds, so 1 to 4 splits by cost: a CU's n workgroups pass two at a
+// time (up to head_dim 128), one alone in 0.7 of that, over their share of the tiles and two tiles' time to
+// start; splits are written and joined, one and a half tiles' time for each 256 units and 64 columns, and as
+// much for the pass of its own that each request's keys are then.  Times with 1 to 4 splits:
+//   388 units behind 9000 (4 prompts of 300 to 1000 tokens, 16 heads of 64 on 4, fp16)   318 330 299 306
+//   680 (8 of them) 569 496 492 504; 388 behind 2000 110 148 150 156
+//   324 behind 16000 (16 of 64 to 256 tokens, bf16)                                       408 399 320 348
+//   384 behind 12000, 632 behind 8000, 1216 (32 heads of 128 on 8)    456 433 448 437, 547 499 500 510, 811 920 943
+//   284 behind 6000 (8 heads of 256 on 2)                                                 497 440 426 445
+int64_t splits_of_many(int64_t units, int64_t keys, int width, bool joined) {
+  const int64_t cus = compute_units();
+  const double tiles = keys / 64.0, join = 1.5 * (double)units / cus * (width / 64.0);
+  int64_t best = 1;
+  double best_t = 1e300;
+  for (int64_t s = 1; s <= 4; ++s) {
+    const int64_t n = (units * s + cus - 1) / cus;
+    const double rounds = width > 128 ? (double)n : (double)(n / 2) + 0.7 * (double)(n % 2);
+    const double t = rounds * (tiles / (double)s + 2.0) + (s > 1 || joined ? join * (double)(1 + s) : 0.0);
+    if (t < best_t) {
+      best_t = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // How the prefix's pass is cut: as a call of one request with all of the tokens, but for the splits and
 // the kernel.
 // Rows pass over the keys by direct loads, in tiles of 16, while that is little work in all (rows x keys x
@@ -152,12 +178,12 @@ struct PrefixPlan {
 // 384 workgroups, 166 and 152 with 256 and 480; alone the passes take 88 (with 512) and 63.  (Own ones evenly
 // between the prefix's: 182 us; behind them in all of these.)
 CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_prefix,
-                   bool own_chunked) {
+                   const CachePlan& own) {
   CachePlan p = cache_plan(tokens, 1, heads, kv_heads, head_dim, tokens, max_prefix);
   const int width = cache_width(head_dim);
   max_prefix = max_prefix < 1 ? 1 : max_prefix > kMaxKeys ? kMaxKeys : max_prefix;
   const int64_t rows = tokens * (heads / kv_heads);
-  if (p.chunked && !own_chunked && rows * kv_heads * width <= ((int64_t)1 << 31) / max_prefix) {
+  if (p.chunked && !own.chunked && rows * kv_heads * width <= ((int64_t)1 << 31) / max_prefix) {
     p.chunked = false;
     p.row_tiles = (rows + 15) / 16;
     p.step = 4 * decode_keys(width);
@@ -166,10 +192,8 @@ CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head
   const int64_t least = p.chunked ? 128 : p.step, room = kMaxParts / (tokens * heads);
   const int64_t target = !p.chunked ? (units <= 4 ? 512 : 256) : width <= 128 ? 384 : 192;
   int64_t splits = p.chunked ? (target + units / 2) / units : (target + units - 1) / units;
-  // A little more than a workgroup a CU leaves most CUs with one: thirds fill two rounds.  16 prompts of
-  // 64 to 256 tokens behind 16000, 16 heads of 64 on 4 (320 units): 318 us against 392 in one pass, 4 of
-  // 300 to 1000 behind 9000 (328 units) 301 and 314.
-  if (p.chunked && units > 256 && 3 * units <= 1024) splits = 3;
+  if (p.chunked && units > compute_units())
+    splits = splits_of_many(units, max_prefix, width, !own.chunked || own.splits > 1);
   const int64_t most = (max_prefix + least - 1) / least;
   splits = splits < most ? splits : most;
   splits = splits < room ? splits : room;
@@ -197,7 +221,7 @@ PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
                    int64_t max_len, int64_t max_prefix) {
   PrefixPlan p;
   p.own = own_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
-  p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own.chunked);
+  p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own);
   // (8 prompts of 1000 to 2000 tokens behind 8000, 32 heads of 128 on 8: 2037 us in one pass, 2380 joined.)
   p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
   return p;
