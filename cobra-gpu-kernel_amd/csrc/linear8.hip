@@ -74,16 +74,21 @@ __device__ __forceinline__ void put(void* p, int dtype, int64_t i, float v) {
   else if (dtype == kF16) static_cast<f16*>(p)[i] = (f16)v;
   else static_cast<bf16*>(p)[i] = (bf16)v;
 }
-// Four consecutive elements from i on (i % 4 == 0).
+// Four elements at any element's address.
+typedef float f32x4e __attribute__((ext_vector_type(4), aligned(4)));
+typedef f16 f16x4e __attribute__((ext_vector_type(4), aligned(2)));
+typedef bf16 bf16x4e __attribute__((ext_vector_type(4), aligned(2)));
+
+// Four consecutive elements from i on.
 __device__ __forceinline__ f32x4 get4(const void* p, int dtype, int64_t i) {
-  if (dtype == kF32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+  if (dtype == kF32) return *reinterpret_cast<const f32x4e*>(static_cast<const float*>(p) + i);
   f32x4 r;
   if (dtype == kF16) {
-    const f16x4 h = *reinterpret_cast<const f16x4*>(static_cast<const f16*>(p) + i);
+    const f16x4 h = *reinterpret_cast<const f16x4e*>(static_cast<const f16*>(p) + i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = (float)h[e];
   } else {
-    const bf16x4 h = *reinterpret_cast<const bf16x4*>(static_cast<const bf16*>(p) + i);
+    const bf16x4 h = *reinterpret_cast<const bf16x4e*>(static_cast<const bf16*>(p) + i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = (float)h[e];
   }
@@ -91,25 +96,26 @@ __device__ __forceinline__ f32x4 get4(const void* p, int dtype, int64_t i) {
 }
 __device__ __forceinline__ void put4(void* p, int dtype, int64_t i, const f32x4& v) {
   if (dtype == kF32) {
-    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    *reinterpret_cast<f32x4e*>(static_cast<float*>(p) + i) = v;
   } else if (dtype == kF16) {
     f16x4 h;
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = (f16)v[e];
-    *reinterpret_cast<f16x4*>(static_cast<f16*>(p) + i) = h;
+    *reinterpret_cast<f16x4e*>(static_cast<f16*>(p) + i) = h;
   } else {
     bf16x4 h;
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = (bf16)v[e];
-    *reinterpret_cast<bf16x4*>(static_cast<bf16*>(p) + i) = h;
+    *reinterpret_cast<bf16x4e*>(static_cast<bf16*>(p) + i) = h;
   }
 }
 
 // -- few rows --------------------------------------------------------------------------
 
-// A lane's 32 columns of a block of one row of activations: codes and the block's scale.  16-bit values are quantised here: a row's block lies in the four
-// lanes l, l + 16, l + 32, l + 48.
-template <typename TA>
+// A lane's 32 columns of a block of one row of activations: codes and the block's scale.  16-bit values
+// are quantised here: a row's block lies in the four lanes l, l + 16, l + 32, l + 48.  ODD: K >= 8 is no
+// multiple of 8 (one row of 1023, 1024 rows of W: 3.8 to 4.5 us, quantised first 6.0 to 7.7).
+template <typename TA, bool ODD>
 struct RowBlock {
   uint32_t w[16];
   __device__ __forceinline__ void load(const Args& a, int64_t m, bool there, int j, int g) {
@@ -120,11 +126,32 @@ struct RowBlock {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (there && c + 8 * q < a.K) v = *reinterpret_cast<const uint4*>(p + c + 8 * q);
+        if (there && c + 8 * q < a.K) {
+          if constexpr (ODD) {
+            const Words x = *reinterpret_cast<const Words*>(p + min(c + 8 * q, a.K - 8));
+            v = make_uint4(x[0], x[1], x[2], x[3]);
+          } else {
+            v = *reinterpret_cast<const uint4*>(p + c + 8 * q);
+          }
+        }
         w[8 * h + 4 * q] = v.x;
         w[8 * h + 4 * q + 1] = v.y;
         w[8 * h + 4 * q + 2] = v.z;
         w[8 * h + 4 * q + 3] = v.w;
+      }
+    }
+    if constexpr (ODD) {
+      if (128 * j + 128 > a.K) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int past = 128 * j + 64 * (k >> 1) + 16 * g + 8 * (k & 1) + 8 - a.K;
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = w[4 * k + e];
+          if (past > 0) drop_first(x, past);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[4 * k + e] = x[e];
+        }
       }
     }
   }
@@ -142,7 +169,7 @@ struct RowBlock {
   }
 };
 template <>
-struct RowBlock<uint8_t> {
+struct RowBlock<uint8_t, false> {
   i32x4 lo, hi;
   uint32_t b;
   __device__ __forceinline__ void load(const Args& a, int64_t m, bool there, int j, int g) {
@@ -171,7 +198,7 @@ struct RowBlock<uint8_t> {
 // 20.9 with 32).  Several blocks' loads asked for together gained nothing (12.4 to 14.9 us, 16.0 to 16.8),
 // nor did 16 waves (12.6, 16.3).  From 17 rows on quantising once and a tile kernel are faster: 32 rows
 // 13 us against 16.8, 64 rows 15 against 28.
-template <typename TA, int NT>
+template <typename TA, bool ODD, int NT>
 __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
   constexpr int kWaves = 8;
   __shared__ f32x4 part[kWaves][NT][64];
@@ -192,7 +219,7 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
   for (int j = wave; j < blocks; j += kWaves) {
     i32x8 c[NT];
     uint32_t wb[NT];
-    RowBlock<TA> x;
+    RowBlock<TA, ODD> x;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       c[t] = join8(*reinterpret_cast<const i32x4*>(w[t] + 128 * j), *reinterpret_cast<const i32x4*>(w[t] + 128 * j + 64));
@@ -223,7 +250,7 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
 #pragma unroll
     for (int k = 1; k < kWaves; ++k) v += part[k][tile][l];
     const bool padded = (a.epi & (kEpiMaskBranch | kEpiMaskResid)) && a.row_mask[m] == 0;
-    const bool four = a.N % 4 == 0;
+    const bool four = n + 4 <= a.N;
     const int64_t at = (int64_t)m * a.N + n;
     f32x4 b = {0.f, 0.f, 0.f, 0.f}, e = b;
     if (four) {
@@ -470,13 +497,14 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
   __syncthreads();  // every wave is done with the operand stages
 
   // In TN slices of 32 columns for each wave column, through LDS as fp32 rows, then written 16
-  // bytes a lane with the epilogue's options; N not in groups of 8 element by element.
+  // bytes a lane with the epilogue's options, at any element's address; the last columns of an N not in
+  // groups of that many element by element (with all of them so 8192 x 4096 x 4091 takes
+  // 217 us in place of 160, quantising with it).
   float* Cs = reinterpret_cast<float*>(smem);
   constexpr int CPL = 16 / (int)sizeof(TC), LPR = T::EPW / CPL, RPP = NT / LPR, NP = BM > RPP ? BM / RPP : 1;
   static_assert(NT % LPR == 0 && (BM % RPP == 0 || RPP > BM) && 32 % CPL == 0, "epilogue geometry");
   const int cl = (tid % LPR) * CPL;
   const int ccol = (cl / 32) * T::WTN + (cl % 32);
-  const bool whole = a.N % 8 == 0;
   const bool masks = a.epi & (kEpiMaskBranch | kEpiMaskResid);
   // (A template for each slice: as a loop, the accumulators' index stayed a variable, and they went to
   // scratch.)
@@ -501,10 +529,18 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
       }
     }
     const int n = n0 + ccol + j * 32;
+    const int live = a.N - n;  // columns that are there
     f32x4 bv[CPL / 4];
 #pragma unroll
-    for (int h = 0; h < CPL / 4; ++h)
-      bv[h] = a.bias && whole && n < a.N ? *reinterpret_cast<const f32x4*>(a.bias + n + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < CPL / 4; ++h) {
+      bv[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (a.bias && live >= CPL) bv[h] = *reinterpret_cast<const f32x4*>(a.bias + n + 4 * h);
+    }
+    if (a.bias && live < CPL) {
+#pragma unroll
+      for (int e = 0; e < CPL; ++e)
+        if (e < live) bv[e >> 2][e & 3] = a.bias[n + e];
+    }
     // A row of the slice: its LDS place, product, bias and GELU.
     auto value = [&](int p, int h) {
       f32x4 v = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h) + bv[h];
@@ -516,13 +552,17 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
     };
     auto store = [&](int64_t m, const f32x4 (&v)[CPL / 4]) {
       TC* at = static_cast<TC*>(a.c) + m * a.N + n;
-      if constexpr (sizeof(TC) == 4) {
-        *reinterpret_cast<f32x4*>(at) = v[0];
+      if (live < CPL) {
+#pragma unroll
+        for (int e = 0; e < CPL; ++e)
+          if (e < live) at[e] = (TC)v[e >> 2][e & 3];
+      } else if constexpr (sizeof(TC) == 4) {
+        *reinterpret_cast<f32x4e*>(at) = v[0];
       } else {
         typename Op16<TC>::V8 hv;
 #pragma unroll
         for (int e = 0; e < 8; ++e) hv[e] = (TC)v[e >> 2][e & 3];
-        *reinterpret_cast<typename Op16<TC>::V8*>(at) = hv;
+        *reinterpret_cast<Words*>(at) = __builtin_bit_cast(Words, hv);
       }
     };
     // This thread's rows: first, first + RPP, ..
@@ -531,9 +571,9 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
     // the pass before it.  So there are none in the loop without residual and masks (which is no
     // longer than it is because a tile runs it once, its instructions coming from memory), and with
     // them all of a slice's are asked for before its first store.
-    if (whole && !a.resid && !masks) {
+    if (!a.resid && !masks) {
       __syncthreads();
-      if (n < a.N) {
+      if (live > 0) {
 #pragma unroll 2
         for (int p = 0; p < NP; ++p) {
           if (first + p * RPP >= a.M) break;
@@ -543,22 +583,28 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
           store(first + p * RPP, v);
         }
       }
-    } else if (whole) {
+    } else {
       f32x4 rv[NP][CPL / 4];
       uint32_t padded = 0;
-      const int nc = min(n, a.N - CPL);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         const int64_t m = min(first + p * RPP, a.M - 1);
         if (masks && a.row_mask[m] == 0) padded |= 1u << p;
 #pragma unroll
-        for (int h = 0; h < CPL / 4; ++h)
-          rv[p][h] = a.resid ? get4(a.resid, a.resid_dtype, m * a.N + nc + 4 * h) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < CPL / 4; ++h) {
+          rv[p][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (a.resid && live >= CPL) rv[p][h] = get4(a.resid, a.resid_dtype, m * a.N + n + 4 * h);
+        }
+        if (a.resid && live < CPL) {
+#pragma unroll
+          for (int e = 0; e < CPL; ++e)
+            if (e < live) rv[p][e >> 2][e & 3] = get(a.resid, a.resid_dtype, m * a.N + n + e);
+        }
       }
       __syncthreads();
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        if (n < a.N && first + p * RPP < a.M) {
+        if (live > 0 && first + p * RPP < a.M) {
           f32x4 v[CPL / 4];
 #pragma unroll
           for (int h = 0; h < CPL / 4; ++h) {
@@ -568,25 +614,6 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
             if ((padded >> p & 1) && (a.epi & kEpiMaskResid)) v[h] *= 0.f;
           }
           store(first + p * RPP, v);
-        }
-      }
-    } else {
-      __syncthreads();
-#pragma unroll 1
-      for (int p = 0; p < NP; ++p) {
-        const int64_t m = first + p * RPP;
-        if (m >= a.M) break;
-        const bool padded = masks && a.row_mask[m] == 0;
-#pragma unroll 1
-        for (int e = 0; e < CPL && n + e < a.N; ++e) {
-          const int64_t at = m * a.N + n + e;
-          float v = Cs[(tid / LPR + p * RPP) * T::LDC + cl + e];
-          if (a.bias) v += a.bias[n + e];
-          if (a.epi & kEpiGelu) v = gelu_erf(v);
-          if (padded && (a.epi & kEpiMaskBranch)) v = 0.f;
-          if (a.resid) v += get(a.resid, a.resid_dtype, at);
-          if (padded && (a.epi & kEpiMaskResid)) v *= 0.f;
-          static_cast<TC*>(a.c)[at] = (TC)v;
         }
       }
     }
@@ -657,27 +684,26 @@ hipError_t dispatch_tile(const Args& a, hipStream_t stream) {
   }
 }
 
-template <int NT, typename TA>
+template <int NT, typename TA, bool ODD>
 hipError_t launch_few(const Args& a, hipStream_t stream) {
-  return launch_status(linear8_few_kernel<TA, NT>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(512),
+  return launch_status(linear8_few_kernel<TA, ODD, NT>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(512),
                        stream, a);
 }
-template <typename TA>
+template <typename TA, bool ODD>
 hipError_t dispatch_few(const Args& a, hipStream_t stream) {
-  const bool wide = a.N >= 32 * compute_units();
-  return wide ? launch_few<2, TA>(a, stream) : launch_few<1, TA>(a, stream);
+  const bool wide = (a.N + 31) / 32 >= compute_units();
+  return wide ? launch_few<2, TA, ODD>(a, stream) : launch_few<1, TA, ODD>(a, stream);
 }
 
 constexpr int64_t kFewRows = 16;
 
-bool whole_rows(const Linear8Args& c) {
-  return c.K % 8 == 0 && (reinterpret_cast<uintptr_t>(c.a) & 15) == 0;
-}
+// Few rows of 16-bit activations that the product itself quantises.
+bool quantised_inside(int64_t M, int64_t K, int a_dtype) { return M <= kFewRows && K >= 8 && a_dtype != kE4M3; }
 
 }  // namespace
 
 int64_t linear8_workspace_bytes(int64_t M, int64_t K, int a_dtype) {
-  if (a_dtype == kE4M3 || (M <= kFewRows && K % 8 == 0)) return 0;
+  if (a_dtype == kE4M3 || quantised_inside(M, K, a_dtype)) return 0;
   const int64_t kp = (K + 127) & ~int64_t(127), s = (K + 511) / 512 * 4;
   return M * (kp + s);
 }
@@ -689,8 +715,11 @@ hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_
   Args a{c.a, c.a_scale, c.w, c.w_scale, c.bias, c.resid, c.row_mask, c.c, c.M, (int)c.N, (int)c.K, (int)kp, (int)s,
          c.resid_dtype, c.c_dtype, c.epi};
   const bool codes = c.a_dtype == kE4M3;
-  if (c.M <= kFewRows && !codes && whole_rows(c))
-    return c.a_dtype == kF16 ? dispatch_few<f16>(a, stream) : dispatch_few<bf16>(a, stream);
+  if (quantised_inside(c.M, c.K, c.a_dtype)) {
+    if (c.K % 8)
+      return c.a_dtype == kF16 ? dispatch_few<f16, true>(a, stream) : dispatch_few<bf16, true>(a, stream);
+    return c.a_dtype == kF16 ? dispatch_few<f16, false>(a, stream) : dispatch_few<bf16, false>(a, stream);
+  }
   if (!codes) {
     if (!c.workspace || workspace_bytes < c.M * (kp + s)) return hipErrorInvalidValue;
     uint8_t* scale = static_cast<uint8_t*>(c.workspace) + c.M * kp;
@@ -700,7 +729,7 @@ hipError_t run_linear8(const Linear8Args& c, int64_t workspace_bytes, hipStream_
     a.a = c.workspace;
     a.a_scale = scale;
   }
-  if (c.M <= kFewRows) return dispatch_few<uint8_t>(a, stream);
+  if (c.M <= kFewRows) return dispatch_few<uint8_t, false>(a, stream);
   switch (c.c_dtype) {
     case kF16: return dispatch_tile<f16>(a, stream);
     case kBF16: return dispatch_tile<bf16>(a, stream);

@@ -2,7 +2,8 @@
 //
 // 16 lanes have a block of 128 columns, 8 each; their largest magnitude meets over four lane
 // exchanges and the codes are converted from the loaded words, two at a time, the scale inside the
-// conversion.  A wave has 512 columns of a row at a time, so that its scales are one word.
+// conversion.  A wave has 512 columns of a row at a time, so that its scales are one word, or several rows
+// of few columns.
 // Bound by memory for many rows, by the launch for few.
 #include "kernels.hpp"
 #include "quant8.hpp"
@@ -17,30 +18,26 @@ struct Eight {
   uint32_t w[sizeof(T) * 2];
 };
 
-// The lane's eight columns from c on of a row of K, zeros past it; whole: K % 8 == 0 and rows aligned.
-template <typename T, bool WHOLE>
+// Eight columns of a row of K for column c, to be settled; SHORT: K < 8.
+template <typename T, bool SHORT>
 __device__ __forceinline__ Eight<T> load8_of(const T* row, int c, int K) {
   Eight<T> r{};
-  if constexpr (WHOLE) {
-    if (c < K) {
+  if constexpr (SHORT) {
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(row + c)[i];
-        r.w[4 * i] = q.x;
-        r.w[4 * i + 1] = q.y;
-        r.w[4 * i + 2] = q.z;
-        r.w[4 * i + 3] = q.w;
+    for (int i = 0; i < 7; ++i)
+      if (c + i < K) {
+        if constexpr (sizeof(T) == 2)
+          r.w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[c + i] << (16 * (i & 1));
+        else
+          r.w[i] = reinterpret_cast<const uint32_t*>(row)[c + i];
       }
-    }
   } else {
+    const T* p = row + min(c, K - 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        const uint32_t v = c + i < K ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + i] : 0u;
-        r.w[i >> 1] |= v << (16 * (i & 1));
-      } else {
-        r.w[i] = c + i < K ? reinterpret_cast<const uint32_t*>(row)[c + i] : 0u;
-      }
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+      const Words q = reinterpret_cast<const Words*>(p)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.w[4 * i + e] = q[e];
     }
   }
   return r;
@@ -94,59 +91,74 @@ __device__ __forceinline__ uint2 codes_of(const Eight<T>& x, float s) {
   }
 }
 
-// U units (512 columns of a row) a wave, all of their loads asked for before the first is used.
-template <typename T, bool WHOLE, int U>
+// U units a wave, all of their loads asked for before the first is used.  A unit is 512 columns of a row,
+// or with few columns R rows of 512 / R: 60 MB in rows of 128 take 16.4 us with four rows a unit and 30.6
+// with one, in rows of 200 columns 18.4 and 21.4 with two and one.  Rows of every length take the same
+// loads, at any element's address: 60 MB in rows of 8190 take 16.2 us, of 8191 18.5 (a value at a time
+// 35.8), of 512 15.8, of 50 25.1 (157).
+template <typename T, bool SHORT, int U, int R>
 __global__ __launch_bounds__(256) void quantize8_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes,
-                                                        uint32_t* __restrict__ scale, int64_t K, uint32_t per_row,
-                                                        uint32_t units) {
-  const uint32_t lane = threadIdx.x & 63;
+                                                        uint32_t* __restrict__ scale, int64_t rows, int64_t K,
+                                                        uint32_t per_row, uint32_t units) {
+  constexpr int kLanes = 64 / R;  // of a row
+  const uint32_t lane = threadIdx.x & 63, sub = lane / kLanes;
   const uint32_t wave = __builtin_amdgcn_readfirstlane((blockIdx.x * 256 + threadIdx.x) >> 6);
   const uint32_t u0 = wave * U;
   const int kp = (int)((K + 127) & ~int64_t(127));
+  auto row_of = [&](uint32_t u) { return R > 1 ? (int64_t)u * R + sub : (int64_t)(u / per_row); };
+  auto col_of = [&](uint32_t u) { return (int)((R > 1 ? 0 : u % per_row) * 512 + (lane % kLanes) * 8); };
   Eight<T> v[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const uint32_t u = u0 + i;
-    if (u < units) {
-      const uint32_t row = u / per_row;
-      v[i] = load8_of<T, WHOLE>(x + (int64_t)row * K, (int)((u - row * per_row) * 512 + lane * 8), (int)K);
-    }
+    if (u < units && (R == 1 || row_of(u) < rows)) v[i] = load8_of<T, SHORT>(x + row_of(u) * K, col_of(u), (int)K);
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const uint32_t u = u0 + i;
     if (u >= units) return;
-    const uint32_t row = u / per_row;
-    const int c = (int)((u - row * per_row) * 512 + lane * 8);
+    const int64_t row = row_of(u);
+    const int c = col_of(u);
+    const bool there = c < kp && (R == 1 || row < rows);
+    if (R > 1 && row >= rows) v[i] = Eight<T>{};
+    if (!SHORT && c + 8 > (int)K) drop_first(v[i].w, c + 8 - (int)K);
     const uint32_t mine = scale_byte(max16(largest_of(v[i])));
-    const uint32_t byte = c < kp ? mine : 127u;
+    const uint32_t byte = there ? mine : 127u;
     const uint2 q = codes_of(v[i], scale_of(byte));
-    if (c < kp) *reinterpret_cast<uint2*>(codes + (int64_t)row * kp + c) = q;
+    if (there) *reinterpret_cast<uint2*>(codes + row * kp + c) = q;
+    // A row's word: its blocks' bytes, 127 past them.
     uint32_t word = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) word |= (uint32_t)__builtin_amdgcn_readlane((int)byte, 16 * j) << (8 * j);
-    if (lane == 0) scale[u] = word;
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)byte, 16 * j);
+      if (R == 1) word |= b << (8 * j);
+      else if ((uint32_t)(16 * j / kLanes) == sub) word |= b << (8 * (j % (4 / R)));
+    }
+    if (R == 2) word |= 0x7f7f0000u;
+    if (R == 4) word |= 0x7f7f7f00u;
+    if (lane % kLanes == 0 && (R == 1 || row < rows)) scale[R == 1 ? u : row] = word;
   }
 }
 
-template <typename T, bool WHOLE>
+template <typename T, bool SHORT, int R>
 hipError_t launch(const Quantize8Args& a, hipStream_t stream) {
-  const int64_t per_row = (a.K + 511) / 512, units = a.M * per_row;
+  const int64_t per_row = (a.K + 511) / 512, units = R > 1 ? (a.M + R - 1) / R : a.M * per_row;
   if (units > 0x7fffffff || a.K > 0x7fffff00) return hipErrorInvalidValue;
   // Four units a wave once every CU has its eight workgroups with one: until then more waves
   // shorten the call, from there on more loads in flight for each do.
   const bool many = units > 4 * 8 * (int64_t)compute_units();
   const int64_t groups = many ? (units + 15) / 16 : (units + 3) / 4;
-  auto* kernel = many ? quantize8_kernel<T, WHOLE, 4> : quantize8_kernel<T, WHOLE, 1>;
+  auto* kernel = many ? quantize8_kernel<T, SHORT, 4, R> : quantize8_kernel<T, SHORT, 1, R>;
   return launch_status(kernel, dim3((unsigned)groups), dim3(256), stream, static_cast<const T*>(a.x),
-                       static_cast<uint8_t*>(a.codes), static_cast<uint32_t*>(a.scale), a.K, (uint32_t)per_row,
+                       static_cast<uint8_t*>(a.codes), static_cast<uint32_t*>(a.scale), a.M, a.K, (uint32_t)per_row,
                        (uint32_t)units);
 }
 
 template <typename T>
 hipError_t launch_rows(const Quantize8Args& a, hipStream_t stream) {
-  const bool whole = a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  return whole ? launch<T, true>(a, stream) : launch<T, false>(a, stream);
+  if (a.K < 8) return launch<T, true, 4>(a, stream);
+  return a.K <= 128 ? launch<T, false, 4>(a, stream) : a.K <= 256 ? launch<T, false, 2>(a, stream)
+                                                                  : launch<T, false, 1>(a, stream);
 }
 
 }  // namespace

@@ -74,4 +74,27 @@ __device__ __forceinline__ uint32_t finite16(uint32_t (&w)[N]) {
   return m;
 }
 
+// Sixteen bytes at any element's address.
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+
+// Eight values from c on of a row of K >= 8 are loaded as those from min(c, K - 8) on, so that rows of any
+// length take the same loads; here the first n > 0 that are not asked for go, zeros follow.
+template <int N>
+__device__ __forceinline__ void drop_first(uint32_t (&w)[N], int n) {
+  constexpr int kPer = 8 / N;  // values of a word
+#pragma unroll
+  for (int k = N / 2; k >= 1; k /= 2)
+    if ((n / kPer) & k) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = i + k < N ? w[i + k] : 0u;
+    }
+  if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = 0u;
+  } else if (kPer == 2 && n & 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = (w[i] >> 16) | (i + 1 < N ? w[i + 1] << 16 : 0u);
+  }
+}
+
 }  // namespace cobra

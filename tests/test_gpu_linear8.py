@@ -45,6 +45,21 @@ def test_quantize_is_the_plain_form(m, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("m,k", [(1, 3), (9, 7), (7, 9), (13, 100), (6, 121), (1, 129), (5, 200), (3, 255), (8, 256), (5, 257),
+                                 (9, 509), (5, 1023), (3, 4091), (33333, 5), (40001, 100), (30001, 129), (20001, 250),
+                                 (9001, 301), (2001, 2049)])
+def test_quantize_narrow_and_odd_rows(m, k, dtype):
+    check_codes(rows(m, k, dtype, m + k))
+
+
+@pytest.mark.parametrize("m", [1, 5, 16])
+@pytest.mark.parametrize("k", [7, 9, 100, 127, 129, 250, 1023, 2050])
+@pytest.mark.parametrize("n", [17, 9000])
+def test_linear8_few_rows_of_odd_lengths(m, k, n):
+    check_linear(m, k, n, F16 if k % 2 else BF16, m + k, gelu=k == 100, out=F32 if m == 5 else None)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_quantize_every_16_bit_pattern(dtype):
     """Every fp16 and bf16 value, subnormals, infinities and NaN among them, each beside a block's
     largest value that puts the border of a scale, and ties, on either side."""

@@ -50,7 +50,8 @@ def test_abi_rejects_bad_products():
         assert linear(M=100, **kw) != 0, kw
     q = lib.cobra_linear8_workspace_bytes
     assert q(0, 64, 256, m.F16) == 0 and q(100, 64, 256, m.E4M3) == 0 and q(16, 64, 256, m.BF16) == 0
-    assert q(16, 64, 250, m.BF16) == 16 * 260  # rows that are not whole vectors are quantised first
+    assert q(16, 64, 250, m.BF16) == 0 and q(17, 64, 250, m.BF16) == 17 * 260
+    assert q(16, 64, 7, m.BF16) == 16 * 132  # rows under a load's length are quantised first
     assert q(1, 64, 256, m.F32) == -1 and q(-1, 64, 256, m.F16) == -1 and q(1, 0, 256, m.F16) == -1
 
 
