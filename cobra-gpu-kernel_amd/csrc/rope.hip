@@ -11,7 +11,7 @@
 // Bound by memory for many tokens (every query and key read and written once), by the launch for few.
 // A token's R / 2 sines and cosines are formed once, in LDS, for all of its heads.  A lane has two
 // pieces of V columns, chosen so that a pair's partners are both its own: V columns from i and V from
-// i + R / 2, or two neighbouring pieces.  Heads that 4 columns do not divide (the whole, its pitch or
+// i + R / 2, or two neighbouring pieces.  Heads that 2 columns do not divide (the whole, its pitch or
 // half of what turns) have a wave each and their partners from memory.
 #include "common.hpp"
 #include "kernels.hpp"
@@ -253,8 +253,11 @@ hipError_t launch_type(const Args& a, int inter, hipStream_t stream) {
     return a.dim % v == 0 && a.pitch % v == 0 && a.ld % v == 0 && (inter || a.half % v == 0) &&
            (reinterpret_cast<uintptr_t>(a.qkv) & (2 * v - 1)) == 0;
   };
+  // (In pieces of 2 columns 30 million values of 6 + 6 heads of 40, halves of 10 turned, take 45 us, of
+  // 5 + 5 of 168, halves of 42, 41; one by one 135 and 80.)
   if (fits(8)) return inter ? launch<T, 8, true>(a, stream) : launch<T, 8, false>(a, stream);
   if (fits(4)) return inter ? launch<T, 4, true>(a, stream) : launch<T, 4, false>(a, stream);
+  if (fits(2)) return inter ? launch<T, 2, true>(a, stream) : launch<T, 2, false>(a, stream);
   return any<T>(a, inter, stream);
 }
 
