@@ -132,12 +132,13 @@ __global__ __launch_bounds__(256) void cache_prefix_join_kernel(Args a, PrePass 
   }
 }
 
-// The same for at most kFewShares splits: a row has as many lanes as its dimensions in fours, which take
+// The same for few splits: a row has as many lanes as its dimensions in fours, which take
 // the splits one after the other, so that a wave has 64 / lanes rows and does the divisions and the search
 // for the request once for all of them.  Bound by instructions with a row a wave: 44800 rows of 64, 4 splits,
-// 15 us in place of 50.
-constexpr int kFewShares = 8;
-template <typename T, int HDP>
+// 15 us in place of 50.  With up to kMoreShares only where a wave has two rows: 8192 of 64 with 9 shares 87 us in
+// all in place of 92, 4096 of 128 with 13 8.5 in place of 9.4, but 276 of 256 with 9 6.6 in place of 5.6.
+constexpr int kFewShares = 8, kMoreShares = 16;
+template <typename T, int HDP, int S>
 __global__ __launch_bounds__(256) void cache_prefix_join_rows_kernel(Args a, PrePass shared, int pre_step, int own_step) {
   constexpr int kLanes = HDP / 4, kRows = 64 / kLanes;
   const int lane = threadIdx.x & 63, sub = lane / kLanes, d = (lane - sub * kLanes) * 4;
@@ -145,10 +146,10 @@ __global__ __launch_bounds__(256) void cache_prefix_join_rows_kernel(Args a, Pre
   const uint32_t rows = (uint32_t)(a.tokens * a.heads), row = wave * kRows + sub;  // (less than 2^31)
   const bool active = sub < kRows && row < rows;
   const int all = shared.args.splits + a.splits;
-  float2 ml[kFewShares];
-  f32x4 x[kFewShares];
+  float2 ml[S];
+  f32x4 x[S];
 #pragma unroll
-  for (int s = 0; s < kFewShares; ++s)
+  for (int s = 0; s < S; ++s)
     if (s < all && active) {
       ml[s] = a.part_m[(int64_t)s * rows + row];
       x[s] = *reinterpret_cast<const f32x4*>(a.part_o + ((int64_t)s * rows + row) * HDP + d);
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void cache_prefix_join_rows_kernel(Args a, Pre
   const int own_n = (int)(((uint32_t)rq.len + own_chunk - 1) / own_chunk);
   float m = kNegInf;
 #pragma unroll
-  for (int s = 0; s < kFewShares; ++s) {
+  for (int s = 0; s < S; ++s) {
     const bool there = s < all && (s < a.base ? s < pre_n : s - a.base < own_n);
     if (!there) {
       ml[s] = make_float2(kNegInf, 0.f);
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256) void cache_prefix_join_rows_kernel(Args a, Pre
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int s = 0; s < kFewShares; ++s) {
+  for (int s = 0; s < S; ++s) {
     const float w = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[s].x - m);
     l = fmaf(w, ml[s].y, l);
 #pragma unroll
@@ -206,11 +207,12 @@ struct PrefixPlan {
 // time (up to head_dim 128), one alone in 0.7 of that, over their share of the tiles and two tiles' time to
 // start; splits are written and joined, one and a half tiles' time for each 256 units and 64 columns, and as
 // much for the pass of its own that each request's keys are then.  Times with 1 to 4 splits:
-//   388 units behind 9000 (4 prompts of 300 to 1000 tokens, 16 heads of 64 on 4, fp16)   318 330 299 306
-//   680 (8 of them) 569 496 492 504; 388 behind 2000 110 148 150 156
-//   324 behind 16000 (16 of 64 to 256 tokens, bf16)                                       408 399 320 348
-//   384 behind 12000, 632 behind 8000, 1216 (32 heads of 128 on 8)    456 433 448 437, 547 499 500 510, 811 920 943
-//   284 behind 6000 (8 heads of 256 on 2)                                                 497 440 426 445
+//   388 units behind 9000 (4 prompts of 300 to 1000 tokens, 16 heads of 64 on 4, fp16)   317 295 266 272
+//   680 (8 of them) 566 435 433 446; 388 behind 2000 110 114 117 123
+//   324 behind 16000 (16 of 64 to 256 tokens, bf16)                                       408 371 294 320
+//   384 behind 12000, 632 behind 8000, 1216 (32 heads of 128 on 8)    453 406 421 411, 548 452 460 471, 809 821 848
+//   284 behind 6000 (8 heads of 256 on 2)                                                 495 432 413 431
+// (5 to 7 splits gain nothing in any of them.)
 int64_t splits_of_many(int64_t units, int64_t keys, int width, bool joined) {
   const int64_t cus = compute_units();
   const double tiles = keys / 64.0, join = 1.5 * (double)units / cus * (width / 64.0);
@@ -287,7 +289,7 @@ PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   PrefixPlan p;
   p.own = own_plan(tokens, batch, heads, kv_heads, head_dim, max_new, max_len);
   p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own);
-  // (8 prompts of 1000 to 2000 tokens behind 8000, 32 heads of 128 on 8: 2037 us in one pass, 2380 joined.)
+  // (4 prompts of 300 to 1000 tokens behind 2000, 16 heads of 64 on 4: 110 us in one pass, 114 joined.)
   p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
   return p;
 }
@@ -314,9 +316,12 @@ hipError_t launch(const Args& a, PrePass shared, const PrefixPlan& p, hipStream_
     return launch_status(cache_prefix_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, a, shared,
                          p.pre.step, p.own.step);
   constexpr int kRows = 4 * (64 / (HDP / 4));  // of a workgroup, with few shares
-  if (p.pre.splits + p.own.splits <= kFewShares && (rows + kRows - 1) / kRows <= kMaxGrid)
-    return launch_status(cache_prefix_join_rows_kernel<T, HDP>, dim3((unsigned)((rows + kRows - 1) / kRows)), block,
-                         stream, a, shared, p.pre.step, p.own.step);
+  const int shares = p.pre.splits + p.own.splits;
+  constexpr int kMost = HDP <= 128 ? kMoreShares : kFewShares;
+  if (shares <= kMost && (rows + kRows - 1) / kRows <= kMaxGrid)
+    return launch_status(shares <= kFewShares ? cache_prefix_join_rows_kernel<T, HDP, kFewShares>
+                                              : cache_prefix_join_rows_kernel<T, HDP, kMost>,
+                         dim3((unsigned)((rows + kRows - 1) / kRows)), block, stream, a, shared, p.pre.step, p.own.step);
   const int64_t quads = (rows + 3) / 4;
   return launch_status(cache_prefix_join_kernel<T, HDP, 1>, dim3((unsigned)(quads < kMaxGrid ? quads : kMaxGrid)),
                        block, stream, a, shared, p.pre.step, p.own.step);

@@ -200,6 +200,20 @@ def test_offsets_past_32_bits(heads, kv, hd, held, new):
     check(held, new, 0, heads, kv, hd, 64, BF16, E4M3, seed=17)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(4, 4, 32), (6, 6, 40), (8, 4, 96), (4, 1, 128), (5, 5, 168), (2, 1, 256)])
+@pytest.mark.parametrize("prefix_len", [90, 700])
+def test_joins_of_many_requests(heads, kv, hd, prefix_len):
+    """Rows of one wave that are of several requests, some without new tokens."""
+    new = [0] + [(0, 1, 1, 2, 0, 0, 3)[i % 7] for i in range(150)]
+    held = [prefix_len] + [1 + n + 7 * i % 60 for i, n in enumerate(new[1:])]
+    check(held, new, 0, heads, kv, hd, 32, BF16, E4M3, seed=hd, lead=5, tail=3)
+
+
+def test_more_row_tiles_than_compute_units():
+    """Prompts whose tiles of rows are more than the chip takes at once, so that the prefix is cut in a few."""
+    check([9000, 700, 730, 720], [0, 700, 701, 720], 0, 18, 18, 32, 64, F16, E4M3, seed=2)
+
+
 def test_two_streams_at_once():
     from cobra_amd import ops
 
