@@ -158,11 +158,14 @@ __global__ __launch_bounds__(256) void cache_prefix_join_rows_kernel(Args a, Pre
   int before = 0;  // requests that begin at t or before it
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int first = b0 + lane < a.batch ? a.cu[b0 + lane] : 0x7fffffff;
+    int most = 0;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int n = __popcll(__ballot(first <= __builtin_amdgcn_readlane(t, i * kLanes)));
       if (sub == i) before += n;
+      most = max(most, n);
     }
+    if (most < 64) break;
   }
   const int b = before > 0 ? before - 1 : 0;
   const Request rq = request_of<kOwn>(a, b), pre = request_of<kPrefix>(a, a.prefix);
