@@ -9,8 +9,11 @@
 //   block give the block's byte, so it does not matter which columns the instruction counts to which
 //   lane.  But it adds eight products at a time and cuts each where it falls under 2^-13 of
 //   the largest one's exponent (measured, as for the instructions without scales; the sums of eight
-//   meet in fp32): 4e-5 of a result in the root mean square.  An fp16 result's own rounding is 2e-4, a
-//   bf16's 1.6e-3, an fp32's 3e-8: fp32 results take the exact kind.
+//   meet in fp32): 4e-5 to 6e-5 of a result in the root mean square, and where large products cancel
+//   what they leave may be gone.  Only bf16 results take this kind: their own rounding is 1.6e-3 in the
+//   root mean square, and half a step of one as large as the largest product, 2^-8, covers the 7 2^-13 of
+//   it that an eight can lose.  An fp16's rounding is 2e-4, an fp32's 3e-8: the exact kind, for any
+//   number of rows.
 //
 // Two kernels.  Up to 16 rows of A the weights' bytes are all that counts: linear8_few_kernel
 // (exact) has 16 or more rows of W a workgroup, split along K over its waves, and takes 16-bit
@@ -471,6 +474,10 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
   take(at, std::false_type(), std::false_type());
 }
 
+// Results whose rounding hides what the scaled instructions cut take them; the others' products are exact.
+template <typename TC>
+constexpr bool kExactSums = !std::is_same<TC, bf16>::value;
+
 template <int BM, int BN, int WM, int WN, int ST, int KS, int GM, typename TC>
 __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
   using T = Tile<BM, BN, WM, WN, ST, KS>;
@@ -493,7 +500,7 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
   const int li = lane & 31, g = lane >> 5;
 
   f32x16 acc[T::TN][T::TM];
-  mainloop<BM, BN, WM, WN, ST, KS, sizeof(TC) == 4>(a, m0, n0, smem, acc);
+  mainloop<BM, BN, WM, WN, ST, KS, kExactSums<TC>>(a, m0, n0, smem, acc);
   __syncthreads();  // every wave is done with the operand stages
 
   // In TN slices of 32 columns for each wave column, through LDS as fp32 rows, then written 16
@@ -641,7 +648,8 @@ hipError_t launch_tile(const Args& a, hipStream_t stream) {
 // 128 x 128, 8192^3 417 (2635 TFLOP/s; a library product of e4m3 2605 to 2675 on the same cards) and 539,
 // 512 x 4096 x 4096 44.6, 26.6, 16.4 and 19.7 in the four, 128 x 4096 x 4096 37.8, 19.5, 14.8 and 10.6.
 // Exact, fp32 results: 8192 x 4096 x 4096 221 us in 256 x 256 and 241 in 128 x 128, 8192^3 790
-// (1391 TFLOP/s; a library product in bf16 1308 to 1339) and 881.
+// (1391 TFLOP/s; a library product in bf16 1308 to 1339) and 881.  Exact, fp16 results, in the tiles chosen: 8192^3
+// 763, 8192 x 4096 x 4096 200 (116 scaled), 512 x 4096 x 4096 24.8 (16.1), 64 x 4096 x 4096 10.6 (7.8).
 struct TileCand {
   int bm, bn, per_cu;
   double fixed, step, busy;
@@ -675,7 +683,7 @@ int pick_tile(const TileCand (&tiles)[kTiles], const Args& a) {
 
 template <typename TC>
 hipError_t dispatch_tile(const Args& a, hipStream_t stream) {
-  switch (pick_tile(sizeof(TC) == 4 ? kExact : kScaled, a)) {
+  switch (pick_tile(kExactSums<TC> ? kExact : kScaled, a)) {
     case 0: return launch_tile<256, 256, 4, 2, 2, 1, 4, TC>(a, stream);
     case 1: return launch_tile<128, 128, 2, 2, 2, 1, 8, TC>(a, stream);
     case 2: return launch_tile<128, 64, 2, 2, 3, 1, 8, TC>(a, stream);

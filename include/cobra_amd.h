@@ -319,7 +319,9 @@ int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_
  * [M, Kp] (COBRA_E4M3) with a_scale [M, S]; w, w_scale: codes [N, Kp] and scales [N, S] of the
  * weight in nn.Linear's layout.  bias: [N] fp32 (optional); resid (optional) and c: [M, N] in any
  * of the three types each (resid may be c itself in c's type; c overlaps nothing else).  Sums are
- * fp32.  Scale bytes are 1 .. 254, as cobra_quantize8 writes them (0 and 255 give no meaningful
+ * fp32 of exact products; but for COBRA_BF16 c of more than 16 rows products are added in eights, each cut
+ * where it falls under 2^-13 of its eight's largest: up to 7 2^-13 of every eight's largest
+ * product, under a result's rounding unless large products cancel.  Scale bytes are 1 .. 254, as cobra_quantize8 writes them (0 and 255 give no meaningful
  * result).  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is rejected.  workspace:
  * cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0), which
  * launches that overlap must not share.
