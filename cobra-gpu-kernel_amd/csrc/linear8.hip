@@ -3,7 +3,10 @@
 //   c = sum_j 2^(ea[m,j] + ew[n,j]) sum_{k in block j} a[m,k] w[n,k]
 // Two kinds of matrix instructions.
 // * Exact: codes become bf16 in registers, with their scale inside the conversion (4 significant bits
-//   and a power of two: nothing is rounded), and v_mfma_*_bf16 adds their products in fp32.
+//   and a power of two), and v_mfma_*_bf16 adds their products in fp32.  Each operand is widened with half of its
+//   scale, since a block's largest value may round to 2^128, which bf16 has not; sums are multiplied by 4.
+//   Nothing is rounded but blocks under 2^-115 (scale bytes 1 to 3), whose least values become whole
+//   multiples of 2^-132, bf16's least step twice.
 // * Scaled: v_mfma_scale_f32_32x32x64_f8f6f4 takes the codes as they are and one scale byte for each
 //   row and 32 columns of an operand, at twice the rate.  All lanes that hold parts of a row's
 //   block give the block's byte, so it does not matter which columns the instruction counts to which
@@ -52,6 +55,9 @@ __device__ __forceinline__ bf16x8 widen(uint32_t x, uint32_t y, float scale) {
 __device__ __forceinline__ f32x16 mfma8(const i32x8& a, const i32x8& b, const f32x16& c, int sa, int sb) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
+
+// What products of operands with half of their scales are short of.
+constexpr float kUnhalve = 4.f;
 
 struct Args {
   const void* a;
@@ -158,13 +164,14 @@ struct RowBlock {
       }
     }
   }
-  __device__ __forceinline__ i32x8 codes(float& scale) {
+  __device__ __forceinline__ i32x8 codes(uint32_t& byte) {
     uint32_t m = largest16(w);
     if (__any(m >= Quant<TA>::kInf)) m = finite16<TA>(w);
     float v = Quant<TA>::wide(m);
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = max_xor32(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-    scale = scale_of(scale_byte(__float_as_uint(v)));
+    byte = scale_byte(__float_as_uint(v));
+    const float scale = scale_of(byte);
     i32x8 r;
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = (int)Quant<TA>::four(w[2 * i], w[2 * i + 1], scale);
@@ -186,8 +193,8 @@ struct RowBlock<uint8_t, false> {
       b = a.a_scale[m * a.s + j];
     }
   }
-  __device__ __forceinline__ i32x8 codes(float& scale) {
-    scale = scale_of(b);
+  __device__ __forceinline__ i32x8 codes(uint32_t& byte) {
+    byte = b;
     return join8(lo, hi);
   }
 };
@@ -229,14 +236,15 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
       wb[t] = ws[t][j];
     }
     x.load(a, r, r < a.M, j, g);
-    float row_scale;
-    const i32x8 q = x.codes(row_scale);
+    uint32_t row_byte;
+    const i32x8 q = x.codes(row_byte);
+    const float row_scale = half_scale_of(row_byte);
     bf16x8 y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = widen(q[2 * k], q[2 * k + 1], row_scale);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float scale = scale_of(wb[t]);
+      const float scale = half_scale_of(wb[t]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[t] = mfma16(widen(c[t][2 * k], c[t][2 * k + 1], scale), y[k], acc[t]);
     }
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Args a) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[i] += b[i];
+      v[i] = fmaf(v[i], kUnhalve, b[i]);
       if (a.epi & kEpiGelu) v[i] = gelu_erf(v[i]);
       if (padded && (a.epi & kEpiMaskBranch)) v[i] = 0.f;
       v[i] += e[i];
@@ -399,12 +407,12 @@ __device__ __forceinline__ void mainloop(const Args& a, int64_t m0, int n0, char
 #pragma unroll
       for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[i][k] = widen(af[kk][i][2 * k], af[kk][i][2 * k + 1], scale_of(as[i] & 255));
+        for (int k = 0; k < 4; ++k) y[i][k] = widen(af[kk][i][2 * k], af[kk][i][2 * k + 1], half_scale_of(as[i] & 255));
 #pragma unroll
       for (int j = 0; j < T::TN; ++j) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const bf16x8 z = widen(wf[kk][j][2 * k], wf[kk][j][2 * k + 1], scale_of(ws[j] & 255));
+          const bf16x8 z = widen(wf[kk][j][2 * k], wf[kk][j][2 * k + 1], half_scale_of(ws[j] & 255));
 #pragma unroll
           for (int i = 0; i < T::TM; ++i) acc[j][i] = mfma32x32x16(z, y[i][k], acc[j][i]);
         }
@@ -550,7 +558,9 @@ __global__ __launch_bounds__(WM* WN* KS * 64) void linear8_tile_kernel(Args a) {
     }
     // A row of the slice: its LDS place, product, bias and GELU.
     auto value = [&](int p, int h) {
-      f32x4 v = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h) + bv[h];
+      f32x4 v = *reinterpret_cast<const f32x4*>(Cs + (tid / LPR + p * RPP) * T::LDC + cl + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = kExactSums<TC> ? fmaf(v[e], kUnhalve, bv[h][e]) : v[e] + bv[h][e];
       if (a.epi & kEpiGelu) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = gelu_erf(v[e]);

@@ -22,6 +22,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t a) {
 }
 // The scale itself, 1 <= byte < 255.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Half of it, for conversions, which take 0 for 2^-127.
+__device__ __forceinline__ float half_scale_of(uint32_t byte) { return __uint_as_float((byte << 23) - 0x800000u); }
 
 // What the conversion needs of a 16- or 32-bit activation type.  A magnitude's bits order like the
 // magnitudes do, so 16-bit values are compared two at a time; past kInf they are not finite.

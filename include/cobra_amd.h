@@ -321,10 +321,11 @@ int cobra_quantize8(const void* x, int x_dtype, void* codes, void* scale, int64_
  * of the three types each (resid may be c itself in c's type; c overlaps nothing else).  Sums are
  * fp32 of exact products; but for COBRA_BF16 c of more than 16 rows products are added in eights, each cut
  * where it falls under 2^-13 of its eight's largest: up to 7 2^-13 of every eight's largest
- * product, under a result's rounding unless large products cancel.  Scale bytes are 1 .. 254, as cobra_quantize8 writes them (0 and 255 give no meaningful
- * result).  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is rejected.  workspace:
- * cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is 0), which
- * launches that overlap must not share.
+ * product, under a result's rounding unless large products cancel.  Scale bytes are 1 .. 247, as
+ * cobra_quantize8 writes them (others give no meaningful result); of blocks with bytes 1 to 3 values may be
+ * rounded to multiples of 2^-132.  N <= 134217712; M and K as for cobra_quantize8.  COBRA_EPI_MASK_OUT is
+ * rejected.  workspace: cobra_linear8_workspace_bytes() bytes (16-byte aligned, may be NULL when that is
+ * 0), which launches that overlap must not share.
  */
 int64_t cobra_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_dtype);
 int cobra_linear8_fwd(const void* a, int a_dtype, const void* a_scale, const void* w, const void* w_scale,
