@@ -287,6 +287,9 @@ CachePlan own_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   return p;
 }
 
+// Row tiles of a pass where a launch has room for so many: at least one.
+int64_t at_most(int64_t row_tiles, int64_t room) { return row_tiles < room ? row_tiles : room > 1 ? room : 1; }
+
 PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                    int64_t max_len, int64_t max_prefix) {
   PrefixPlan p;
@@ -294,6 +297,13 @@ PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own);
   // (4 prompts of 300 to 1000 tokens behind 2000, 16 heads of 64 on 4: 110 us in one pass, 114 joined.)
   p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
+  // Both passes' workgroups are one launch's: the prefix's have what one row tile of each request leaves, the
+  // requests' the rest, and either go round the row tiles that they have fewer for.
+  const int64_t own = batch * kv_heads * p.own.splits, pre = kv_heads * p.pre.splits;
+  if (!p.both) {
+    p.pre.row_tiles = at_most(p.pre.row_tiles, (kMaxGrid - own) / pre);
+    p.own.row_tiles = at_most(p.own.row_tiles, (kMaxGrid - pre * p.pre.row_tiles) / own);
+  }
   return p;
 }
 
