@@ -5,13 +5,13 @@ import torch
 
 from oracle import serve
 
-from _cache_util import E4M3, attn_tolerance, codes_of
+from _cache_util import E4M3, I8, attn_tolerance, codes_of
 from _gpu_util import DEV, log
-from test_gpu_prefix import build, i32
+from test_gpu_prefix import build, check, i32
 
 pytestmark = pytest.mark.gpu
 
-F16 = torch.float16
+F16, BF16 = torch.float16, torch.bfloat16
 
 
 @pytest.mark.parametrize("heads,kv,hd,batch,tokens,own", [(4, 2, 64, 19370, 59377, 3), (16, 16, 32, 2047, 68000, 33),
@@ -46,3 +46,36 @@ def test_as_many_workgroups_as_a_launch_has(heads, kv, hd, batch, tokens, own):
     near = ops.cache_prefix_attn(*args, max_new=max(own, rest), max_len=500, max_prefix=100).cpu().double()
     largest = float((codes_of(v).abs().amax((1, 2, 3)) * vs.double().amax(1)).max())
     assert float((got - near).abs().max()) <= 2.0 ** -8 * largest
+
+
+def shares(tokens, batch, heads, kv, hd, new, length, prefix):
+    """Shares of a row in all, from the workspace."""
+    from cobra_amd import _lib
+
+    width = next(w for w in (32, 64, 96, 128, 192, 256) if w >= hd)
+    return _lib.lib().cobra_cache_prefix_attn_workspace_bytes(tokens, batch, heads, kv, hd, new, length, prefix) // (
+        tokens * heads * (4 * width + 8))
+
+
+@pytest.mark.parametrize("batch", [2, 3, 4])
+@pytest.mark.parametrize("heads,kv,hd,dtype,cache", [(4, 2, 64, F16, E4M3), (4, 1, 256, BF16, I8), (2, 2, 128, BF16, E4M3),
+                                                     (2, 1, 40, F16, I8)])
+def test_few_requests_behind_a_long_prefix_without_hints(batch, heads, kv, hd, dtype, cache):
+    """A table as wide as the prefix's lets the requests' own keys be as many: they are cut in 64 at most,
+    where a call without a prefix would take more."""
+    held = [20000, 300, 1, 77][:batch]
+    new = [0, 3, 1, 1][:batch]
+    T = sum(new)
+    width = 20000
+    assert shares(T, batch, heads, kv, hd, max(1, T - batch + 2), width, width) > 65
+    check(held, new, 0, heads, kv, hd, 32, dtype, cache, seed=batch)
+
+
+@pytest.mark.parametrize("hd,block", [(64, 16), (128, 64), (256, 32)])
+def test_all_shares_that_there_may_be(hd, block):
+    """192 of a prefix and 64 of a request's own keys, few of them written, or most."""
+    assert shares(2, 3, 2, 1, hd, 1, 98304, 98304) == 256
+    for held in ([20000, 17500, 40], [700, 16, 3], [0, 17001, 1]):
+        check(held, [0, 1, 1], 0, 2, 1, hd, block, F16, E4M3, seed=hd, max_new=1, max_len=98304, max_prefix=98304)
+    check([150, 17500, 260], [1, 0, 1], 0, 2, 1, hd, block, BF16, E4M3, seed=hd, max_new=1, max_len=98304, max_prefix=98304)
+    check([17500, 17100], [0, 2], 0, 2, 1, hd, block, BF16, I8, seed=hd)
