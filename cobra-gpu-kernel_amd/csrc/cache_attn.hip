@@ -30,6 +30,9 @@ CachePlan cache_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_he
   // Where max_new is too low for the tokens it is the workspace that has to be bounded.
   const int64_t room = kMaxParts / (tokens * heads);
   splits = splits < room ? splits : room;
+  // Every request has its workgroups, those without new tokens too.
+  const int64_t places = kMaxGrid / (batch * kv_heads);
+  splits = splits < places ? splits : places;
   // Up to 1024 keys one workgroup takes less time than the second launch that joins splits: at 1000
   // 6.6 us against 8.0 for one request of 4 x 32, 10.6 against 14.5 for 64 of 16 x 64 on 4, 12.3 against
   // 15.3 for 16 of 8 x 128 (one of these 10.7 against 10.0), at 300 5.3 to 8.4 against 7.7 to 11.1.
