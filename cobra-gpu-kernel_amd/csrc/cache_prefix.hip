@@ -287,9 +287,6 @@ CachePlan own_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   return p;
 }
 
-// Row tiles of a pass where a launch has room for so many: at least one.
-int64_t at_most(int64_t row_tiles, int64_t room) { return row_tiles < room ? row_tiles : room > 1 ? room : 1; }
-
 PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new,
                    int64_t max_len, int64_t max_prefix) {
   PrefixPlan p;
@@ -297,13 +294,9 @@ PrefixPlan plan_of(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   p.pre = pre_plan(tokens, heads, kv_heads, head_dim, max_prefix, p.own);
   // (4 prompts of 300 to 1000 tokens behind 2000, 16 heads of 64 on 4: 110 us in one pass, 114 joined.)
   p.both = p.own.chunked && p.pre.splits == 1 && p.own.splits == 1;
-  // Both passes' workgroups are one launch's: the prefix's have what one row tile of each request leaves, the
-  // requests' the rest, and either go round the row tiles that they have fewer for.
-  const int64_t own = batch * kv_heads * p.own.splits, pre = kv_heads * p.pre.splits;
-  if (!p.both) {
-    p.pre.row_tiles = at_most(p.pre.row_tiles, (kMaxGrid - own) / pre);
-    p.own.row_tiles = at_most(p.own.row_tiles, (kMaxGrid - pre * p.pre.row_tiles) / own);
-  }
+  // (Either pass goes round the row tiles that a launch has no workgroups for.)
+  const int64_t tiles = kMaxGrid / (kv_heads * p.pre.splits);
+  if (p.pre.row_tiles > tiles) p.pre.row_tiles = tiles > 1 ? tiles : 1;
   return p;
 }
 
@@ -315,15 +308,21 @@ hipError_t launch(const Args& a, PrePass shared, const PrefixPlan& p, hipStream_
   if (p.both)
     return own > kMaxGrid ? hipErrorInvalidValue
                           : launch_status(cache_chunk_kernel<kBoth, T, CACHE, HDP, 2>, dim3((unsigned)own), block, stream, a, NoPass{});
-  if (own + pre > kMaxGrid) return hipErrorInvalidValue;
-  shared.groups = (int)pre;
-  const dim3 groups((unsigned)(own + pre));
+  if (own > kMaxGrid || pre > kMaxGrid) return hipErrorInvalidValue;
   // Requests of many new tokens are many tokens together.
   auto* kernel = p.own.chunked   ? cache_chunk_kernel<kPrefix, T, CACHE, HDP, 2, true, PrePass>
                  : p.pre.chunked ? cache_chunk_kernel<kPrefix, T, CACHE, HDP, 2, false, PrePass>
                                  : cache_prefix_decode_kernel<T, CACHE, HDP>;
-  const hipError_t e = launch_status(kernel, groups, block, stream, a, shared);
+  // Both passes together, or one after the other where they are more workgroups than a launch has.
+  const bool together = own + pre <= kMaxGrid;
+  shared.groups = (int)pre;
+  hipError_t e = launch_status(kernel, dim3((unsigned)(together ? own + pre : pre)), block, stream, a, shared);
   if (e != hipSuccess) return e;
+  if (!together) {
+    shared.groups = 0;
+    e = launch_status(kernel, dim3((unsigned)own), block, stream, a, shared);
+    if (e != hipSuccess) return e;
+  }
   const int64_t rows = (int64_t)a.tokens * a.heads;
   if (p.pre.splits + p.own.splits > 64)
     return launch_status(cache_prefix_join_kernel<T, HDP, 4>, dim3((unsigned)rows), block, stream, a, shared,

@@ -18,7 +18,7 @@ F16, BF16 = torch.float16, torch.bfloat16
                                                           (2, 1, 128, 70000, 140000, 2)])
 def test_as_many_workgroups_as_a_launch_has(heads, kv, hd, batch, tokens, own):
     """Without max_new every request might have nearly all of the tokens: the own keys' workgroups alone are
-    a launch's most, and go round their row tiles where the prefix's come to them."""
+    a launch's most, and the prefix's come to them."""
     from cobra_amd import ops
 
     rest = tokens - own * (batch - 2)
@@ -46,6 +46,30 @@ def test_as_many_workgroups_as_a_launch_has(heads, kv, hd, batch, tokens, own):
     near = ops.cache_prefix_attn(*args, max_new=max(own, rest), max_len=500, max_prefix=100).cpu().double()
     largest = float((codes_of(v).abs().amax((1, 2, 3)) * vs.double().amax(1)).max())
     assert float((got - near).abs().max()) <= 2.0 ** -8 * largest
+
+
+@pytest.mark.parametrize("heads,kv,batch", [(16, 16, 1048575), (32, 2, 8388607)])
+@pytest.mark.parametrize("new", [1, 40])
+def test_as_many_requests_as_a_launch_has_workgroups(heads, kv, batch, new):
+    """batch x kv_heads just under 2^24, a few requests with new tokens among them: as those few alone."""
+    from cobra_amd import ops
+
+    hd, where = 32, [0, 5, batch // 2, batch - 1]
+    held, few = [90, 30 + new, 2 + new, new], [0, new, new, new]
+    table, pool, q, cu = build(held, few, 0, heads, kv, hd, 16, F16, E4M3, 7)
+    dev = [t.to(DEV) for t in pool]
+    rest = [0, heads, hd, hd ** -0.5, *dev]
+    want = ops.cache_prefix_attn(q.to(DEV), i32(cu), i32(held), i32(table), *rest)
+    lens = torch.zeros(batch, dtype=torch.int32)
+    fresh = torch.zeros(batch + 1, dtype=torch.int32)
+    tables = torch.full((batch, len(table[0])), -1, dtype=torch.int32)
+    for b, n, f, row in zip(where, held, few, table):
+        lens[b], fresh[b + 1], tables[b] = n, f, torch.tensor(row)
+    offsets = torch.cumsum(fresh, 0, dtype=torch.int32)
+    for hints in ({}, dict(max_new=new, max_len=100, max_prefix=100), dict(max_new=new, max_len=5000, max_prefix=5000)):
+        got = ops.cache_prefix_attn(q.to(DEV), offsets.to(DEV), lens.to(DEV), tables.to(DEV), *rest, **hints)
+        largest = float((codes_of(pool[1]).abs().amax((1, 2, 3)) * pool[3].double().amax(1)).max())
+        assert float((got.double() - want.double()).abs().max()) <= 2.0 ** -8 * largest
 
 
 def shares(tokens, batch, heads, kv, hd, new, length, prefix):
