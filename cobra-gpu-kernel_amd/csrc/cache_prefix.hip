@@ -246,7 +246,13 @@ int64_t splits_of_many(int64_t units, int64_t keys, int width, bool joined) {
 // to head_dim 128) a workgroup, so that the requests' own keys, which are bound by memory, have the rest
 // from the start: 128 requests of up to 2000 keys behind 30000, 32 heads of 128 on 8, take 135 to 147 us with
 // 384 workgroups, 166 and 152 with 256 and 480; alone the passes take 88 (with 512) and 63.  (Own ones evenly
-// between the prefix's: 182 us; behind them in all of these.)
+// between the prefix's: 182 us; behind them in all of these.)  With 256, 320, 384, 448 and 512 (half as many at 256):
+//   64 requests of up to 2000 behind 60000, 32 heads of 128 on 8   161 151 135 123 136
+//   128 of up to 4000 behind 16000, 32 of 128 on 8                 141 153 165 177 189
+//   128 of up to 500 behind 30000, 16 of 64 on 4                    65  68  61  55  53
+//   128 of up to 2000 behind 30000, 8 of 128 on 1                   52  55  52  52  54
+//   60 of 4 new tokens, up to 2000 behind 30000, 8 of 128 on 2      76  79  71  65  67
+//   100 of up to 300 behind 20000, 6 of 256 on 2, int8              80  72  67  69  71
 CachePlan pre_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_prefix,
                    const CachePlan& own) {
   CachePlan p = cache_plan(tokens, 1, heads, kv_heads, head_dim, tokens, max_prefix);
